@@ -34,6 +34,10 @@ NVCC_FLAGS = [
     "-DNDEBUG",
 ]
 CXX_FLAGS = ["-O3", "-std=c++17", "-DNDEBUG"]
+# The C++ library torch itself runs on.  A compiler whose own search path holds only libstdc++.a
+# would otherwise link a second, static copy of it into the extension, whose stream locales nothing
+# initialises: the first number formatted into an error message then crashes the process.
+LINK_FLAGS = ["-l:libstdc++.so.6"]
 
 
 def kernel_sources():
@@ -53,6 +57,7 @@ ext_modules = [
         kernel_sources(),
         include_dirs=[CSRC],
         extra_compile_args={"cxx": CXX_FLAGS, "nvcc": NVCC_FLAGS},
+        extra_link_args=LINK_FLAGS,
     ),
 ]
 if rewriter_sources():
@@ -62,6 +67,7 @@ if rewriter_sources():
             rewriter_sources(),
             include_dirs=[os.path.join(CSRC, "rewriter")],
             extra_compile_args={"cxx": CXX_FLAGS},
+            extra_link_args=LINK_FLAGS,
         ))
 
 setup(
