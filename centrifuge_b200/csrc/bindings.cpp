@@ -7,7 +7,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <tuple>
+#include <vector>
 
 #include "kernels/launch_api.h"
 
@@ -792,6 +794,252 @@ void zero_unless_error(Tensor& buf, const Tensor& err) {
                "zero_unless_error");
 }
 
+// ---- row operators around the blocks (argument checks of shapes and types: ops/fused.py)
+inline int type_code(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return kBF16;
+    case at::kHalf: return kF16;
+    case at::kFloat: return kF32;
+    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32"); return -1;
+  }
+}
+// A tensor of the operator's device (absent tensors pass).
+inline void same_device(const Tensor& first, const c10::optional<Tensor>& t, const char* name) {
+  if (t.has_value() && t->defined())
+    TORCH_CHECK(t->device() == first.device(), name, " is on ", t->device(), ", not on ",
+                first.device());
+}
+inline int row_count(int64_t rows, const char* what) {
+  TORCH_CHECK(rows < (1ll << 30), what, ": ", rows, " rows");
+  return static_cast<int>(rows);
+}
+
+// out[r] = scale * table[ids[r]]
+void scaled_embedding_fwd(const Tensor& table, const Tensor& ids, Tensor& out, double scale) {
+  check_cuda(table, "table");
+  same_device(table, ids, "ids");
+  same_device(table, out, "out");
+  const c10::cuda::CUDAGuard guard(table.device());
+  CFB_CHECK_RC(cfb_scaled_embedding_fwd(
+                   table.data_ptr(), type_code(table, "table"), table.stride(0), table.size(0),
+                   ids.data_ptr(), ids.scalar_type() == at::kInt, out.data_ptr(),
+                   type_code(out, "out"), out.stride(0),
+                   row_count(ids.numel(), "scaled_embedding_fwd"), table.size(1),
+                   static_cast<float>(scale), err_word(table.get_device()).data_ptr<int>(),
+                   cur_stream()),
+               "scaled_embedding_fwd");
+}
+
+// dtable[v] (+)= scale * sum of the dy rows of token v
+void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids, const c10::optional<Tensor>& id_rows,
+                          Tensor& dtable, double scale, int64_t pad, bool accumulate) {
+  check_cuda(dy, "dy");
+  same_device(dy, ids, "ids");
+  same_device(dy, id_rows, "id_rows");
+  same_device(dy, dtable, "dtable");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const int rows = row_count(dy.size(0), "scaled_embedding_bwd"), H = dy.size(1);
+  Tensor work;
+  if (rows > 0)
+    work = at::empty({cfb_scaled_embedding_bwd_workspace(rows, H)}, dy.options().dtype(at::kByte));
+  CFB_CHECK_RC(cfb_scaled_embedding_bwd(
+                   dy.data_ptr(), type_code(dy, "dy"), dy.stride(0), ids.data_ptr(),
+                   ids.scalar_type() == at::kInt, ids.numel(), opt_ptr<int>(id_rows), pad,
+                   dtable.data_ptr<float>(), dtable.stride(0), dtable.size(0), rows, H,
+                   static_cast<float>(scale), accumulate, rows > 0 ? work.data_ptr() : nullptr,
+                   err_word(dy.get_device()).data_ptr<int>(), cur_stream()),
+               "scaled_embedding_bwd");
+}
+
+CfbBlockNorms block_norms_args(const Tensor& h, const c10::optional<Tensor>& x, int resid_type,
+                               const Tensor& w_post, const c10::optional<Tensor>& w_pre,
+                               const c10::optional<Tensor>& gate, double block_scale,
+                               double resid_scale) {
+  CfbBlockNorms p = {};
+  p.type = type_code(h, "h");
+  p.resid_type = resid_type;
+  p.H = h.size(1);
+  TORCH_CHECK(p.H <= kBlockNormsMaxH, "block norms: hidden size ", p.H, " is over ",
+              kBlockNormsMaxH);
+  p.h = h.data_ptr();
+  p.ld_h = h.stride(0);
+  if (x.has_value() && x->defined()) {
+    p.x = x->data_ptr();
+    p.ld_x = x->stride(0);
+  }
+  p.w_post = w_post.data_ptr();
+  p.w_pre = opt_ptr<void>(w_pre);
+  if (gate.has_value() && gate->defined()) {
+    p.gate = gate->data_ptr();
+    p.ld_gate = gate->dim() == 2 ? gate->stride(0) : 0;
+    p.gate_kind = gate->dim() == 1 ? kGateChannel
+                  : gate->scalar_type() == at::kFloat && gate->size(1) == 1 ? kGateToken
+                                                                             : kGateElement;
+  }
+  p.block_scale = static_cast<float>(block_scale);
+  p.resid_scale = static_cast<float>(resid_scale);
+  check_cuda(h, "h");
+  same_device(h, x, "x");
+  same_device(h, w_post, "w_post");
+  same_device(h, w_pre, "w_pre");
+  same_device(h, gate, "gate");
+  return p;
+}
+
+// (y, n, rstd_post, rstd_pre); n and rstd_pre are undefined without w_pre
+std::tuple<Tensor, c10::optional<Tensor>, Tensor, c10::optional<Tensor>> block_norms_fwd(
+    const Tensor& h, const Tensor& x, const Tensor& w_post, const c10::optional<Tensor>& w_pre,
+    double eps, const c10::optional<Tensor>& gate, double block_scale, double resid_scale) {
+  const CfbBlockNorms p = block_norms_args(h, x, type_code(x, "x"), w_post, w_pre, gate,
+                                           block_scale, resid_scale);
+  const c10::cuda::CUDAGuard guard(h.device());
+  const int rows = row_count(h.size(0), "block_norms_fwd");
+  const auto f32 = h.options().dtype(at::kFloat);
+  Tensor y = at::empty({rows, p.H}, x.options()), rstd_post = at::empty({rows}, f32);
+  c10::optional<Tensor> n, rstd_pre;
+  if (p.w_pre) {
+    n = at::empty({rows, p.H}, h.options());
+    rstd_pre = at::empty({rows}, f32);
+  }
+  CFB_CHECK_RC(cfb_block_norms_fwd(&p, static_cast<float>(eps), y.data_ptr(),
+                                   p.w_pre ? n->data_ptr() : nullptr, rstd_post.data_ptr<float>(),
+                                   p.w_pre ? rstd_pre->data_ptr<float>() : nullptr, rows,
+                                   cur_stream()),
+               "block_norms_fwd");
+  return {y, n, rstd_post, rstd_pre};
+}
+
+// (dx, dh, dgate); a channel gate's dgate is `dgate` itself
+std::tuple<Tensor, Tensor, c10::optional<Tensor>> block_norms_bwd(
+    const c10::optional<Tensor>& dy, const c10::optional<Tensor>& dn, const Tensor& h,
+    const c10::optional<Tensor>& y, const Tensor& rstd_post, const c10::optional<Tensor>& rstd_pre,
+    const Tensor& w_post, const c10::optional<Tensor>& w_pre, Tensor& dw_post,
+    const c10::optional<Tensor>& dw_pre, const c10::optional<Tensor>& gate,
+    const c10::optional<Tensor>& dgate, double block_scale, double resid_scale,
+    const c10::optional<Tensor>& rows, bool accumulate) {
+  const Tensor& up = dy.has_value() ? *dy : *dn;
+  const Tensor& resid = y.has_value() ? *y : *dy;
+  const CfbBlockNorms p = block_norms_args(h, y, type_code(resid, "y"), w_post, w_pre, gate,
+                                           block_scale, resid_scale);
+  same_device(h, dy, "dy");
+  same_device(h, dn, "dn");
+  same_device(h, rstd_post, "rstd_post");
+  same_device(h, rstd_pre, "rstd_pre");
+  same_device(h, dw_post, "dw_post");
+  same_device(h, dw_pre, "dw_pre");
+  same_device(h, dgate, "dgate");
+  same_device(h, rows, "rows");
+  const c10::cuda::CUDAGuard guard(h.device());
+  const int R = row_count(up.size(0), "block_norms_bwd");
+  Tensor dx = at::empty({R, p.H}, resid.options()), dh = at::empty({R, p.H}, h.options());
+  c10::optional<Tensor> dg = dgate;
+  if (p.gate_kind == kGateToken) dg = at::empty({R, 1}, gate->options());
+  if (p.gate_kind == kGateElement) dg = at::empty({R, p.H}, h.options());
+  Tensor work;
+  if (R > 0)
+    work = at::empty({cfb_block_norms_bwd_workspace(R, p.H)}, h.options().dtype(at::kByte));
+  CFB_CHECK_RC(
+      cfb_block_norms_bwd(&p, opt_ptr<void>(dy), dy.has_value() ? dy->stride(0) : 0,
+                          opt_ptr<void>(dn), dn.has_value() ? dn->stride(0) : 0,
+                          rstd_post.data_ptr<float>(), opt_ptr<float>(rstd_pre), opt_ptr<int>(rows),
+                          h.size(0), dx.data_ptr(), dh.data_ptr(),
+                          p.gate_kind != kGateNone ? dg->data_ptr() : nullptr,
+                          dw_post.data_ptr<float>(),
+                          dw_pre.has_value() ? dw_pre->data_ptr<float>() : nullptr, accumulate,
+                          R > 0 ? work.data_ptr() : nullptr, R,
+                          err_word(h.get_device()).data_ptr<int>(), cur_stream()),
+      "block_norms_bwd");
+  return {dx, dh, dg};
+}
+
+// The non-empty tensors of a gradient list and where their scaled values go.  Checks that no output
+// overlaps another output or another tensor of the list.
+std::vector<CfbTensorRef> tensor_refs(const std::vector<Tensor>& grads,
+                                      const std::vector<Tensor>& outs, bool* in_place) {
+  struct Span {
+    uintptr_t lo, hi;
+    size_t index;
+    bool written;
+  };
+  std::vector<CfbTensorRef> refs;
+  std::vector<Span> spans;
+  refs.reserve(grads.size());
+  bool same = true;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& g = grads[i];
+    TORCH_CHECK(g.layout() == at::kStrided && g.is_cuda() && g.device() == grads[0].device(),
+                "gradient ", i, " must be a dense tensor on ", grads[0].device());
+    TORCH_CHECK(g.is_non_overlapping_and_dense(), "gradient ", i, " has gaps or overlaps itself");
+    CfbTensorRef r = {g.data_ptr(), nullptr, g.numel(), type_code(g, "a gradient"), 0};
+    if (!outs.empty()) {
+      const Tensor& o = outs[i];
+      TORCH_CHECK(o.device() == g.device() && o.sizes() == g.sizes() &&
+                      (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
+                  "output ", i, " must have the device, sizes and strides of gradient ", i);
+      r.out = o.data_ptr();
+      r.out_type = type_code(o, "an output");
+      const uintptr_t a = reinterpret_cast<uintptr_t>(r.ptr), b = reinterpret_cast<uintptr_t>(r.out);
+      const bool own = r.out == r.ptr && r.out_type == r.type;
+      same = same && own;
+      if (r.numel > 0) {
+        if (!own) spans.push_back({a, a + g.nbytes(), i, false});
+        spans.push_back({b, b + o.nbytes(), i, true});
+      }
+    }
+    if (r.numel > 0) refs.push_back(r);
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  uintptr_t end = 0, end_written = 0;  // of all spans so far, and of the written ones
+  for (const Span& s : spans) {
+    TORCH_CHECK(s.lo >= (s.written ? end : end_written), "tensor ", s.index,
+                " of the list overlaps another that is written");
+    end = std::max(end, s.hi);
+    if (s.written) end_written = std::max(end_written, s.hi);
+  }
+  if (in_place) *in_place = same;
+  return refs;
+}
+
+// Sum of squares of the list in the elements of `partial` (fp32): their sum is the list's.
+void grad_list_sumsq(const std::vector<Tensor>& grads, Tensor& partial) {
+  TORCH_CHECK(!grads.empty(), "grad_list_sumsq: empty list");
+  const std::vector<CfbTensorRef> refs = tensor_refs(grads, {}, nullptr);
+  TORCH_CHECK(partial.scalar_type() == at::kFloat && partial.is_contiguous() &&
+                  partial.device() == grads[0].device(),
+              "grad_list_sumsq: partial must be contiguous fp32 on the gradients' device");
+  const c10::cuda::CUDAGuard guard(partial.device());
+  const int count = static_cast<int>(refs.size()), groups = cfb_grad_list_groups(count);
+  const int64_t per = partial.numel() / groups;
+  TORCH_CHECK(per > 0, "grad_list_sumsq: partial needs ", groups, " elements");
+  if (count == 0 || per * groups < partial.numel()) partial.zero_();
+  if (count == 0) return;
+  CFB_CHECK_RC(cfb_grad_list_sumsq(refs.data(), count, partial.data_ptr<float>(),
+                                   static_cast<int>(per), cur_stream()),
+               "grad_list_sumsq");
+}
+
+// out_i = g_i * extra_scale * min(1, max_norm / (norm + 1e-6)), norm = extra_scale * sqrt(sum of
+// partial)
+void grad_list_scale(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs,
+                     const Tensor& partial, double max_norm, double extra_scale, Tensor& norm) {
+  TORCH_CHECK(!grads.empty() && outs.size() == grads.size(), "grad_list_scale: ", grads.size(),
+              " gradients, ", outs.size(), " outputs");
+  TORCH_CHECK(partial.scalar_type() == at::kFloat && partial.is_contiguous() &&
+                  partial.numel() > 0 && partial.device() == grads[0].device() &&
+                  norm.scalar_type() == at::kFloat && norm.numel() == 1 &&
+                  norm.device() == grads[0].device(),
+              "grad_list_scale: partial and norm must be fp32 on the gradients' device");
+  bool in_place = false;
+  std::vector<CfbTensorRef> refs = tensor_refs(grads, outs, &in_place);
+  if (refs.empty()) refs.push_back({nullptr, nullptr, 0, kF32, kF32});  // the norm is still due
+  const c10::cuda::CUDAGuard guard(partial.device());
+  CFB_CHECK_RC(cfb_grad_list_scale(refs.data(), static_cast<int>(refs.size()),
+                                   partial.data_ptr<float>(), static_cast<int>(partial.numel()),
+                                   static_cast<float>(max_norm), static_cast<float>(extra_scale),
+                                   norm.data_ptr<float>(), in_place, cur_stream()),
+               "grad_list_scale");
+}
+
 // Dispatcher-visible attention ops on token-major rows, used by the graph rewriter's filtered
 // attention node (centrifuge_b200._filter_C) for SDPA graphs of arbitrary models.
 std::tuple<Tensor, Tensor> attn_fwd_rows(const Tensor& qkv, int64_t B, int64_t S, int64_t nh,
@@ -867,6 +1115,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ex2_poly", &ex2_poly);
   m.def("embedding_bwd", &embedding_bwd, py::arg("dy"), py::arg("ids"), py::arg("id_rows"),
         py::arg("dtable"), py::arg("deterministic") = true);
+  m.def("scaled_embedding_fwd", &scaled_embedding_fwd);
+  m.def("scaled_embedding_bwd", &scaled_embedding_bwd);
+  m.def("block_norms_fwd", &block_norms_fwd);
+  m.def("block_norms_bwd", &block_norms_bwd);
+  m.def("grad_list_sumsq", &grad_list_sumsq);
+  m.def("grad_list_scale", &grad_list_scale);
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd", &ce_bwd, py::arg("logits"), py::arg("rows"), py::arg("labels"),
         py::arg("lse"), py::arg("dloss"), py::arg("dlogits"), py::arg("vocab_start") = 0);

@@ -1,0 +1,428 @@
+// The norms after and before a block with the block's gate and the residual scale (sm_100a).
+//
+// With h a block's output, x the residual stream, w1 / w2 the weights of the norm after the block
+// and of the norm before the next one, g the gate, a / b the residual and block scales:
+//
+//   r1 = (mean(h^2) + eps)^-1/2      y = a x + b g (h r1 w1)
+//   r2 = (mean(y^2) + eps)^-1/2      n = y r2 w2
+//
+// and with dy, dn the gradients of y and n, on the kept rows:
+//
+//   dY  = dy + r2 (w2 dn) - y r2^3 mean(w2 dn y)              dx  = a dY
+//   v   = b dY g w1         dh = r1 v - h r1^3 mean(v h)
+//   dw2 = sum dn y r2       dw1 = sum b dY g h r1             dg  = b dY w1 h r1
+//
+// (dg summed over what the gate is broadcast along).  Everything is bound by memory: each row is
+// read once, its sums are formed in fp32 and n is computed from y before y is rounded.
+//
+// The gate is absent, one value for each channel [H], for each token [T, 1] (fp32), or for each
+// element [T, H].
+#include "row_types.cuh"
+
+namespace cfb {
+
+struct NormRows {
+  const void* h;
+  long long ld_h;
+  const void* x;  // forward: the residual stream; backward: the saved y
+  long long ld_x;
+  const void* w_post;
+  const void* w_pre;  // null: no norm before the next block
+  const void* gate;
+  long long ld_gate;
+  int gate_kind;
+  float block_scale, resid_scale;
+  int H;
+};
+
+// ---------------------------------------------------------------- forward
+// Sum of v over the `warps` warps of the row team this thread belongs to.
+template <int WPR>
+__device__ __forceinline__ float team_sum(float v, float* red) {
+  v = warp_add(v);
+  if (WPR == 1) return v;
+  const int wp = warp_id();
+  __syncthreads();  // red may still be read
+  if (lane_id() == 0) red[wp] = v;
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < WPR; ++i) s += red[wp / WPR * WPR + i];
+  return s;
+}
+
+// A team of WPR warps holds one row in registers, NV groups of W columns in each thread.
+template <typename TH, typename TX, int W, int WPR, int NV>
+__global__ void __launch_bounds__(WPR < 8 ? 256 : WPR * 32) block_norms_fwd_kernel(
+    NormRows a, float eps, TX* __restrict__ y, TH* __restrict__ n, float* __restrict__ rstd_post,
+    float* __restrict__ rstd_pre, int rows) {
+  constexpr int kRows = WPR < 8 ? 8 / WPR : 1;
+  __shared__ float red[WPR < 8 ? 8 : WPR];
+  const int row = blockIdx.x * kRows + warp_id() / WPR;
+  const bool live = row < rows;
+  const int t0 = (warp_id() % WPR) * 32 + lane_id();
+  const int H = a.H;
+  const TH* h = static_cast<const TH*>(a.h) + row * a.ld_h;
+  const TX* x = static_cast<const TX*>(a.x) + row * a.ld_x;
+  float hv[NV][W], xv[NV][W];
+  float ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (t0 + k * WPR * 32) * W;
+    if (live && c < H) {
+      load_f32<TH, W>(h + c, hv[k]);
+      load_f32<TX, W>(x + c, xv[k]);
+#pragma unroll
+      for (int i = 0; i < W; ++i) ss += hv[k][i] * hv[k][i];
+    }
+  }
+  ss = team_sum<WPR>(ss, red);
+  const float inv_h = 1.f / static_cast<float>(H);
+  const float r1 = rsqrtf(ss * inv_h + eps);
+  float row_scale = a.block_scale * r1;
+  if (a.gate_kind == kGateToken && live) row_scale *= static_cast<const float*>(a.gate)[row * a.ld_gate];
+  const TH* gate = static_cast<const TH*>(a.gate);
+  if (a.gate_kind == kGateElement) gate += row * a.ld_gate;
+  ss = 0.f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (t0 + k * WPR * 32) * W;
+    if (live && c < H) {
+      float w[W];
+      load_f32<TH, W>(static_cast<const TH*>(a.w_post) + c, w);
+      if (a.gate_kind == kGateChannel || a.gate_kind == kGateElement) {
+        float g[W];
+        load_f32<TH, W>(gate + c, g);
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] *= g[i];
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        xv[k][i] = a.resid_scale * xv[k][i] + hv[k][i] * row_scale * w[i];
+        ss += xv[k][i] * xv[k][i];
+      }
+      store_f32<TX, W>(y + static_cast<long long>(row) * H + c, xv[k]);
+    }
+  }
+  if (live && t0 == 0) rstd_post[row] = r1;
+  if (a.w_pre == nullptr) return;
+  ss = team_sum<WPR>(ss, red);
+  const float r2 = rsqrtf(ss * inv_h + eps);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (t0 + k * WPR * 32) * W;
+    if (live && c < H) {
+      float w[W];
+      load_f32<TH, W>(static_cast<const TH*>(a.w_pre) + c, w);
+#pragma unroll
+      for (int i = 0; i < W; ++i) w[i] *= xv[k][i] * r2;
+      store_f32<TH, W>(n + static_cast<long long>(row) * H + c, w);
+    }
+  }
+  if (live && t0 == 0) rstd_pre[row] = r2;
+}
+
+// ---------------------------------------------------------------- backward
+// Sum of v over the block.  One barrier: the next call takes another `red`, and comes back to this
+// one only after a further barrier.
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = warp_add(v);
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
+  if (lane_id() == 0) red[warp_id()] = v;
+  __syncthreads();
+  float s = lane_id() < warps ? red[lane_id()] : 0.f;
+  return warp_add(s);
+}
+
+// One block walks the rows blockIdx.x, + gridDim.x, ...; each thread owns NV groups of W columns of
+// every row and keeps the column sums of the weights' gradients in registers:
+//   part[block][0] = sum dn y r2,  part[block][1] = sum b dY h r1 (times the token's or element's
+// gate; a channel's gate is applied once, when the sums are joined).
+template <typename TH, typename TX, int W, int NV>
+__global__ void __launch_bounds__(1024) block_norms_bwd_kernel(
+    NormRows a, const TX* __restrict__ dy, long long ld_dy, const TH* __restrict__ dn,
+    long long ld_dn, const float* __restrict__ rstd_post, const float* __restrict__ rstd_pre,
+    const int* __restrict__ row_ids, long long n_rows, TX* __restrict__ dx, TH* __restrict__ dh,
+    void* __restrict__ dgate, float* __restrict__ part, int rows, int* err) {
+  __shared__ float red[4][32];
+  const int H = a.H, tid = threadIdx.x, nt = blockDim.x;
+  const bool pre = a.w_pre != nullptr;
+  const float inv_h = 1.f / static_cast<float>(H);
+  float s_pre[NV][W], s_post[NV][W];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < W; ++i) s_pre[k][i] = s_post[k][i] = 0.f;
+
+  int turn = 0;
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const long long src = row_ids ? row_ids[r] : r;
+    const long long out = static_cast<long long>(r) * H;
+    if (!index_in(src, n_rows, err)) {  // out-of-range row id: zero gradients
+      float z[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) z[i] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * nt) * W;
+        if (c < H) {
+          store_f32<TX, W>(dx + out + c, z);
+          store_f32<TH, W>(dh + out + c, z);
+          if (a.gate_kind == kGateElement) store_f32<TH, W>(static_cast<TH*>(dgate) + out + c, z);
+        }
+      }
+      if (a.gate_kind == kGateToken && tid == 0) static_cast<float*>(dgate)[r] = 0.f;
+      continue;
+    }
+    const TH* h = static_cast<const TH*>(a.h) + src * a.ld_h;
+    float d[NV][W], hv[NV][W];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (tid + k * nt) * W;
+      if (c < H) {
+        load_f32<TH, W>(h + c, hv[k]);
+        if (dy) {
+          load_f32<TX, W>(dy + r * ld_dy + c, d[k]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < W; ++i) d[k][i] = 0.f;
+        }
+      }
+    }
+    if (pre) {
+      const TX* y = static_cast<const TX*>(a.x) + src * a.ld_x;
+      const float r2 = rstd_pre[src];
+      float yv[NV][W];
+      float dot = 0.f;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * nt) * W;
+        if (c < H) {
+          float q[W], w[W];
+          load_f32<TX, W>(y + c, yv[k]);
+          load_f32<TH, W>(dn + r * ld_dn + c, q);
+          load_f32<TH, W>(static_cast<const TH*>(a.w_pre) + c, w);
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            s_pre[k][i] += q[i] * (yv[k][i] * r2);
+            w[i] *= q[i];
+            dot += w[i] * yv[k][i];
+            d[k][i] += r2 * w[i];
+          }
+        }
+      }
+      const float coef = block_sum(dot, red[turn]) * inv_h * r2 * r2 * r2;
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < W; ++i) d[k][i] -= yv[k][i] * coef;
+    }
+    const float r1 = rstd_post[src];
+    const float tg = a.gate_kind == kGateToken
+                         ? static_cast<const float*>(a.gate)[src * a.ld_gate] : 1.f;
+    const TH* gate = static_cast<const TH*>(a.gate);
+    if (a.gate_kind == kGateElement) gate += src * a.ld_gate;
+    float v[NV][W];
+    float dot = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (tid + k * nt) * W;
+      if (c < H) {
+        float w[W], g[W], e[W];
+        load_f32<TH, W>(static_cast<const TH*>(a.w_post) + c, w);
+        const bool by_column = a.gate_kind == kGateChannel || a.gate_kind == kGateElement;
+        if (by_column) load_f32<TH, W>(gate + c, g);
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          e[i] = a.resid_scale * d[k][i];
+          const float t = a.block_scale * d[k][i];
+          const float th = t * (hv[k][i] * r1);
+          v[k][i] = t * w[i];  // without the token's gate
+          if (a.gate_kind == kGateElement) {
+            s_post[k][i] += th * g[i];
+            w[i] *= th;  // dgate of the element
+          } else {
+            s_post[k][i] += th * tg;
+          }
+          if (by_column) v[k][i] *= g[i];
+          dot += v[k][i] * hv[k][i];
+        }
+        store_f32<TX, W>(dx + out + c, e);
+        if (a.gate_kind == kGateElement) store_f32<TH, W>(static_cast<TH*>(dgate) + out + c, w);
+      }
+    }
+    dot = block_sum(dot, red[turn + 1]);
+    if (a.gate_kind == kGateToken && tid == 0) static_cast<float*>(dgate)[r] = dot * r1;
+    const float coef = dot * inv_h * r1 * r1;
+    const float scale = tg * r1;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (tid + k * nt) * W;
+      if (c < H) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[k][i] = scale * (v[k][i] - hv[k][i] * coef);
+        store_f32<TH, W>(dh + out + c, v[k]);
+      }
+    }
+    turn ^= 2;
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (tid + k * nt) * W;
+    if (c < H) {
+      float* p = part + 2ll * blockIdx.x * H + c;
+      if (pre) store_f32<float, W>(p, s_pre[k]);
+      store_f32<float, W>(p + H, s_post[k]);
+    }
+  }
+}
+
+// dw_pre, dw_post and a channel gate's gradient from the blocks' column sums, in block order.
+// Block: 32 columns x 8 slices of the blocks.
+template <typename TH>
+__global__ void __launch_bounds__(256) block_norms_join_kernel(
+    const float* __restrict__ part, int blocks, int H, const TH* __restrict__ w_post,
+    const TH* __restrict__ gate, float* __restrict__ dw_pre, float* __restrict__ dw_post,
+    float* __restrict__ dgate, int add) {
+  __shared__ float red[2][8][33];
+  const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + cx;
+  float s0 = 0.f, s1 = 0.f;
+  if (c < H)
+    for (int b = ry; b < blocks; b += 8) {
+      if (dw_pre) s0 += part[2ll * b * H + c];
+      s1 += part[(2ll * b + 1) * H + c];
+    }
+  red[0][ry][cx] = s0;
+  red[1][ry][cx] = s1;
+  __syncthreads();
+  if (ry != 0 || c >= H) return;
+  s0 = s1 = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    s0 += red[0][k][cx];
+    s1 += red[1][k][cx];
+  }
+  if (dw_pre) dw_pre[c] = (add ? dw_pre[c] : 0.f) + s0;
+  const float g = gate ? to_f32(gate[c]) : 1.f;
+  dw_post[c] = (add ? dw_post[c] : 0.f) + s1 * g;
+  if (dgate) dgate[c] = (add ? dgate[c] : 0.f) + s1 * to_f32(w_post[c]);
+}
+
+// f(TypeTag<TH>, TypeTag<TX>): the residual stream has the block's type or fp32.
+template <typename F>
+int with_types(int type, int resid_type, F&& f) {
+  return with_type(type, [&](auto th) {
+    using TH = typename decltype(th)::type;
+    if (resid_type == type) return f(TypeTag<TH>(), TypeTag<TH>());
+    if (resid_type == kF32) return f(TypeTag<TH>(), TypeTag<float>());
+    return -12;
+  });
+}
+
+}  // namespace cfb
+
+using namespace cfb;
+
+namespace {
+template <typename TH, typename TX, int W, int WPR, int NV>
+int launch_fwd(const NormRows& a, float eps, void* y, void* n, float* rstd_post, float* rstd_pre,
+               int rows, cudaStream_t st) {
+  constexpr int kRows = WPR < 8 ? 8 / WPR : 1;
+  block_norms_fwd_kernel<TH, TX, W, WPR, NV>
+      <<<(rows + kRows - 1) / kRows, WPR < 8 ? 256 : WPR * 32, 0, st>>>(
+          a, eps, static_cast<TX*>(y), static_cast<TH*>(n), rstd_post, rstd_pre, rows);
+  return launch_status();
+}
+}  // namespace
+
+int cfb_block_norms_fwd(const CfbBlockNorms* p, float eps, void* y, void* n, float* rstd_post,
+                        float* rstd_pre, int rows, cudaStream_t st) {
+  const NormRows a = {p->h, p->ld_h, p->x, p->ld_x, p->w_post, p->w_pre, p->gate, p->ld_gate,
+                      p->gate_kind, p->block_scale, p->resid_scale, p->H};
+  if (rows == 0 || a.H == 0) return 0;
+  if (a.H > kBlockNormsMaxH) return -11;
+  const bool wide = a.H % 8 == 0 && rows_of_8(a.h, a.ld_h, p->type) &&
+                    rows_of_8(a.x, a.ld_x, p->resid_type) && rows_of_8(a.w_post, 0, p->type) &&
+                    rows_of_8(a.w_pre, 0, p->type) && rows_of_8(y, a.H, p->resid_type) &&
+                    rows_of_8(n, a.H, p->type) &&
+                    (a.gate_kind == kGateNone || a.gate_kind == kGateToken ||
+                     rows_of_8(a.gate, a.ld_gate, p->type));
+  return with_types(p->type, p->resid_type, [&](auto th, auto tx) {
+    using TH = typename decltype(th)::type;
+    using TX = typename decltype(tx)::type;
+#define CFB_FWD(W, WPR, NV) \
+  return launch_fwd<TH, TX, W, WPR, NV>(a, eps, y, n, rstd_post, rstd_pre, rows, st)
+    if (wide) {
+      if (a.H <= 256) CFB_FWD(8, 1, 1);
+      if (a.H <= 512) CFB_FWD(8, 1, 2);
+      if (a.H <= 1024) CFB_FWD(8, 1, 4);
+      if (a.H <= 2048) CFB_FWD(8, 2, 4);
+      if (a.H <= 4096) CFB_FWD(8, 4, 4);
+      if (a.H <= 8192) CFB_FWD(8, 8, 4);
+      CFB_FWD(8, 16, 4);
+    }
+    if (a.H <= 512) CFB_FWD(1, 1, 16);
+    if (a.H <= 2048) CFB_FWD(1, 4, 16);
+    if (a.H <= 8192) CFB_FWD(1, 16, 16);
+    CFB_FWD(1, 32, 16);
+#undef CFB_FWD
+  });
+}
+
+long long cfb_block_norms_bwd_workspace(int rows, int H) {
+  const long long blocks = rows < 148 * 8 ? rows : 148 * 8;
+  return 4ll * 2 * blocks * H;  // bytes
+}
+
+int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy, const void* dn,
+                        long long ld_dn, const float* rstd_post, const float* rstd_pre,
+                        const int* row_ids, long long n_rows, void* dx, void* dh, void* dgate,
+                        float* dw_post, float* dw_pre, int add, void* work, int rows, int* err,
+                        cudaStream_t st) {
+  const NormRows a = {p->h, p->ld_h, p->x, p->ld_x, p->w_post, p->w_pre, p->gate, p->ld_gate,
+                      p->gate_kind, p->block_scale, p->resid_scale, p->H};
+  const int H = a.H;
+  if (H == 0) return 0;
+  if (H > kBlockNormsMaxH) return -11;
+  const bool by_row = a.gate_kind == kGateToken || a.gate_kind == kGateElement;
+  const bool wide = H % 8 == 0 && rows_of_8(a.h, a.ld_h, p->type) &&
+                    rows_of_8(a.x, a.ld_x, p->resid_type) && rows_of_8(dy, ld_dy, p->resid_type) &&
+                    rows_of_8(dn, ld_dn, p->type) && rows_of_8(a.w_post, 0, p->type) &&
+                    rows_of_8(a.w_pre, 0, p->type) && rows_of_8(dx, H, p->resid_type) &&
+                    rows_of_8(dh, H, p->type) &&
+                    (a.gate_kind == kGateNone || a.gate_kind == kGateToken ||
+                     rows_of_8(a.gate, a.ld_gate, p->type)) &&
+                    (a.gate_kind != kGateElement || rows_of_8(dgate, H, p->type));
+  float* part = static_cast<float*>(work);
+  return with_types(p->type, p->resid_type, [&](auto th, auto tx) {
+    using TH = typename decltype(th)::type;
+    using TX = typename decltype(tx)::type;
+    int blocks = 0;
+    if (rows > 0) {
+      const int W = wide ? 8 : 1;
+      const int nv = wide ? (H <= 8192 ? 1 : 2) : (H <= 4096 ? 4 : 16);
+      const int threads = ((H + W * nv - 1) / (W * nv) + 31) / 32 * 32;
+      auto* kernel = wide ? (nv == 1 ? block_norms_bwd_kernel<TH, TX, 8, 1>
+                                     : block_norms_bwd_kernel<TH, TX, 8, 2>)
+                          : (nv == 4 ? block_norms_bwd_kernel<TH, TX, 1, 4>
+                                     : block_norms_bwd_kernel<TH, TX, 1, 16>);
+      const int per_sm = threads >= 1024 ? 1 : threads >= 512 ? 2 : threads >= 256 ? 4 : 8;
+      blocks = rows < 148 * per_sm ? rows : 148 * per_sm;
+      kernel<<<blocks, threads, 0, st>>>(
+          a, static_cast<const TX*>(dy), ld_dy, static_cast<const TH*>(dn), ld_dn, rstd_post,
+          rstd_pre, row_ids, n_rows, static_cast<TX*>(dx), static_cast<TH*>(dh),
+          by_row ? dgate : nullptr, part, rows, err);
+      if (const int rc = launch_status()) return rc;
+    } else if (add) {
+      return 0;
+    }
+    const bool channel = a.gate_kind == kGateChannel;
+    block_norms_join_kernel<TH><<<(H + 31) / 32, 256, 0, st>>>(
+        part, blocks, H, static_cast<const TH*>(a.w_post),
+        channel ? static_cast<const TH*>(a.gate) : nullptr, a.w_pre ? dw_pre : nullptr, dw_post,
+        channel ? static_cast<float*>(dgate) : nullptr, add);
+    return launch_status();
+  });
+}

@@ -21,6 +21,9 @@ enum {
 // 128 / 256 select a single-CTA tile of that width, 0 lets the planner choose
 enum { kGemmTilePair = 512 };
 
+// Element types of the row operators (block_norms.cu, scaled_embedding.cu, grad_list.cu)
+enum { kBF16 = 0, kF16 = 1, kF32 = 2 };
+
 // GEMM (gemm_sm100.cu): D = alpha * op(A) op(B) with the epilogue `epi`.
 int cfb_gemm_bf16(const void* A, long long lda, int a_mn, const void* B, long long ldb, int b_mn,
                   void* D, long long ldd, int epi, const void* R, long long ldr, int M, int N,
@@ -222,3 +225,67 @@ int cfb_symm_pull_reduce(const float* mc_base, const float* const* peer_base_dev
                          cudaStream_t st);
 // buf[0, n) = 0 unless err[0] != 0 (buf 16-byte aligned)
 int cfb_zero_unless_error(float* buf, long long n, const int* err, cudaStream_t st);
+
+// ---- row operators around the blocks (row counts below 2^30; ld: elements between rows)
+// out[r] = scale * table[ids[r]]; ids int64, or int32 with ids32.  An id outside [0, V) records
+// kErrBounds and gives a zero row.
+int cfb_scaled_embedding_fwd(const void* table, int type, long long ld, long long V,
+                             const void* ids, int ids32, void* out, int out_type,
+                             long long ld_out, int rows, int H, float scale, int* err,
+                             cudaStream_t st);
+// dtable[v] = (add ? dtable[v] : 0) + scale * sum of dy[r] over the rows r with ids[id_rows[r]] = v
+// (ids[r] without id_rows), v != pad (pad < 0: none).  `work`: scratch of
+// cfb_scaled_embedding_bwd_workspace bytes, 16-byte aligned.
+long long cfb_scaled_embedding_bwd_workspace(int rows, int H);
+int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void* ids, int ids32,
+                             long long n_ids, const int* id_rows, long long pad, float* dtable,
+                             long long ld_t, long long V, int rows, int H, float scale, int add,
+                             void* work, int* err, cudaStream_t st);
+
+// The norms after and before a block (formulas in block_norms.cu).  Types: h, n, the weights and a
+// channel's or element's gate have `type`, the residual stream `resid_type` (the same or fp32), a
+// token's gate is fp32.  Contiguous outputs [rows, H]; H up to kBlockNormsMaxH.
+enum { kGateNone = 0, kGateChannel = 1, kGateToken = 2, kGateElement = 3 };
+constexpr int kBlockNormsMaxH = 16384;
+struct CfbBlockNorms {
+  int type, resid_type, gate_kind, H;
+  const void* h;
+  long long ld_h;
+  const void* x;  // forward: the residual stream; backward: the saved y
+  long long ld_x;
+  const void* w_post;
+  const void* w_pre;  // null: no norm before the next block
+  const void* gate;
+  long long ld_gate;
+  float block_scale, resid_scale;
+};
+int cfb_block_norms_fwd(const CfbBlockNorms* p, float eps, void* y, void* n, float* rstd_post,
+                        float* rstd_pre, int rows, cudaStream_t st);
+// Gradient on the rows row_ids[0, rows) (or 0 .. rows) of h and y; a row id outside [0, n_rows)
+// records kErrBounds and gives zero rows.  dgate: [rows, 1] fp32 or [rows, H] for a token's or
+// element's gate, [H] fp32 for a channel's.  dw_post, dw_pre and a channel's dgate are added to
+// with `add`.
+long long cfb_block_norms_bwd_workspace(int rows, int H);
+int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy, const void* dn,
+                        long long ld_dn, const float* rstd_post, const float* rstd_pre,
+                        const int* row_ids, long long n_rows, void* dx, void* dh, void* dgate,
+                        float* dw_post, float* dw_pre, int add, void* work, int rows, int* err,
+                        cudaStream_t st);
+
+// Gradient lists: tensors of numel > 0 dense elements.  sumsq writes `per_group` partial sums for
+// each of cfb_grad_list_groups(count) launches; scale joins all n_partial of them and writes
+// out = g * extra_scale * min(1, max_norm / (norm + 1e-6)) (max_norm <= 0: no limit), norm =
+// extra_scale * sqrt(sum); with in_place (out = ptr everywhere) nothing is written when that factor
+// is one.
+struct CfbTensorRef {
+  const void* ptr;
+  void* out;
+  long long numel;
+  int type, out_type;
+};
+int cfb_grad_list_groups(int count);
+int cfb_grad_list_sumsq(const CfbTensorRef* refs, int count, float* partial, int per_group,
+                        cudaStream_t st);
+int cfb_grad_list_scale(const CfbTensorRef* refs, int count, const float* partial, int n_partial,
+                        float max_norm, float extra_scale, float* norm, int in_place,
+                        cudaStream_t st);

@@ -7,7 +7,7 @@ in :mod:`centrifuge_b200.ops.reference`.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import List, Optional, Sequence
 
 import torch
 
@@ -128,6 +128,204 @@ def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tensor,
     return dtable
 
 
+_ROW_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _need(ok: bool, what: str, *args) -> None:
+    if not ok:
+        raise ValueError(what.format(*args))
+
+
+def _rows2d(t: torch.Tensor, H: int) -> bool:
+    """``t`` is ``[*, H]`` with columns next to each other and rows that do not overlap."""
+    return t.dim() == 2 and t.shape[1] == H and (t.stride(1) == 1 or H <= 1) and (
+        t.stride(0) >= H or t.shape[0] <= 1)
+
+
+def _vector(t: torch.Tensor, H: int, dtype: torch.dtype) -> bool:
+    return t.dim() == 1 and t.shape[0] == H and t.dtype == dtype and t.is_contiguous()
+
+
+def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``out[r] = scale * table[ids[r]]``, rounded once.
+
+    ``table [V, H]`` and ``out [ids.numel(), H]`` are bf16, fp16 or fp32 (``out`` may have another
+    type than the table, e.g. an fp32 residual stream) with unit column stride and any row stride;
+    ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
+    the status block and gives a zero row."""
+    _need(table.dim() == 2 and _rows2d(table, table.shape[1]) and table.dtype in _ROW_TYPES,
+          "scaled_embedding_fwd: table must be a row-major bf16, fp16 or fp32 [V, H]")
+    _need(ids.dtype in (torch.int64, torch.int32), "scaled_embedding_fwd: ids must be int64 or int32")
+    ids = ids.reshape(-1)
+    H = table.shape[1]
+    if out is None:
+        out = torch.empty(ids.shape[0], H, dtype=table.dtype, device=table.device)
+    else:
+        _need(_rows2d(out, H) and out.shape[0] == ids.shape[0] and out.dtype in _ROW_TYPES,
+              "scaled_embedding_fwd: out must be a row-major bf16, fp16 or fp32 [{}, {}]",
+              ids.shape[0], H)
+    if not table.is_cuda:
+        out.copy_(table[ids.long()].float() * scale)
+        return out
+    kernels().scaled_embedding_fwd(table, ids.contiguous(), out, scale)
+    return out
+
+
+def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tensor,
+                         scale: float = 1.0, id_rows: Optional[torch.Tensor] = None,
+                         padding_idx: Optional[int] = None,
+                         accumulate: bool = True) -> torch.Tensor:
+    """``dtable[v] (+)= scale * sum of dy[r] over the rows r of token v``, in fp32 and in one fixed
+    order (same bits on every run).
+
+    Row ``r`` has token ``ids[id_rows[r]]`` (``ids[r]`` without ``id_rows``).  ``dy [R, H]`` is
+    bf16, fp16 or fp32 and ``dtable [V, H]`` fp32, both with unit column stride and any row stride.
+    Rows of token ``padding_idx`` add nothing.  Without ``accumulate`` the gradient replaces what
+    ``dtable`` held: rows of tokens that do not occur become zero.  On the GPU a token outside the
+    table or a row id outside ``ids`` records an error in the status block and adds nothing."""
+    _need(dy.dim() == 2 and _rows2d(dy, dy.shape[1]) and dy.dtype in _ROW_TYPES,
+          "scaled_embedding_bwd: dy must be a row-major bf16, fp16 or fp32 [R, H]")
+    _need(ids.dtype in (torch.int64, torch.int32), "scaled_embedding_bwd: ids must be int64 or int32")
+    _need(_rows2d(dtable, dy.shape[1]) and dtable.dtype == torch.float32,
+          "scaled_embedding_bwd: dtable must be a row-major fp32 [V, {}]", dy.shape[1])
+    ids = ids.reshape(-1)
+    if id_rows is None:
+        _need(ids.shape[0] == dy.shape[0], "scaled_embedding_bwd: {} ids for {} rows",
+              ids.shape[0], dy.shape[0])
+    else:
+        _need(id_rows.dtype == torch.int32 and id_rows.dim() == 1 and id_rows.is_contiguous()
+              and id_rows.shape[0] == dy.shape[0],
+              "scaled_embedding_bwd: id_rows must be contiguous int32 [{}]", dy.shape[0])
+    if not dy.is_cuda:
+        tok = (ids if id_rows is None else ids[id_rows.long()]).long()
+        g = dy.float() * scale
+        if padding_idx is not None:
+            g, tok = g[tok != padding_idx], tok[tok != padding_idx]
+        if not accumulate:
+            dtable.zero_()
+        return dtable.index_add_(0, tok, g)
+    kernels().scaled_embedding_bwd(dy, ids.contiguous(), id_rows, dtable, scale,
+                                   -1 if padding_idx is None else padding_idx, accumulate)
+    return dtable
+
+
+# ---------------------------------------------------------------- norms around a block
+def _check_gate(name: str, gate: torch.Tensor, T: int, H: int, dtype: torch.dtype) -> None:
+    if gate.dim() == 1:
+        _need(_vector(gate, H, dtype), "{}: a channel's gate must be contiguous {} [{}]", name,
+              dtype, H)
+    elif gate.dim() == 2 and gate.shape[1] == 1 and gate.dtype == torch.float32:
+        _need(gate.shape[0] == T, "{}: a token's gate must be fp32 [{}, 1]", name, T)
+    else:
+        _need(_rows2d(gate, H) and gate.shape[0] == T and gate.dtype == dtype,
+              "{}: the gate must be [{}], fp32 [{}, 1] or {} [{}, {}]", name, H, T, dtype, T, H)
+
+
+def block_norms_fwd(h: torch.Tensor, x: torch.Tensor, w_post: torch.Tensor,
+                    w_pre: Optional[torch.Tensor], eps: float,
+                    gate: Optional[torch.Tensor] = None, block_scale: float = 1.0,
+                    resid_scale: float = 1.0):
+    """The norm after a block, its gate, the residual sum and the norm before the next block::
+
+        y = resid_scale * x + block_scale * gate * rmsnorm(h, w_post)
+        n = rmsnorm(y, w_pre)
+
+    in one pass (``n`` from the unrounded ``y``).  Returns ``(y, n, rstd_post, rstd_pre)``; without
+    ``w_pre`` (the last block of a pipeline stage) ``n`` and ``rstd_pre`` are ``None``.
+
+    ``h [T, H]`` (a block's output), ``n`` and the weights are bf16, fp16 or fp32; the residual
+    stream ``x``, ``y`` has that type or fp32.  ``gate``: ``None``, a learned ``[H]``, a weight for
+    each token (fp32 ``[T, 1]``), or ``[T, H]``.  ``h``, ``x`` and ``gate`` may have any row stride.
+    ``H`` up to 16384."""
+    T, H = h.shape if h.dim() == 2 else (-1, -1)
+    _need(T >= 0 and _rows2d(h, H) and h.dtype in _ROW_TYPES,
+          "block_norms_fwd: h must be a row-major bf16, fp16 or fp32 [T, H]")
+    _need(_rows2d(x, H) and x.shape[0] == T and x.dtype in (h.dtype, torch.float32),
+          "block_norms_fwd: x must be a row-major {} or fp32 [{}, {}]", h.dtype, T, H)
+    _need(_vector(w_post, H, h.dtype) and (w_pre is None or _vector(w_pre, H, h.dtype)),
+          "block_norms_fwd: the weights must be contiguous {} [{}]", h.dtype, H)
+    _need(H <= 16384, "block_norms_fwd: hidden size {} is over 16384", H)
+    if gate is not None:
+        _check_gate("block_norms_fwd", gate, T, H, h.dtype)
+    if not h.is_cuda:
+        y, n, rp, rq = ref.block_norms(h, x, w_post, w_pre, eps, gate, block_scale, resid_scale)
+        return y.to(x.dtype), None if n is None else n.to(h.dtype), rp, rq
+    return kernels().block_norms_fwd(h, x, w_post, w_pre, eps, gate, block_scale, resid_scale)
+
+
+def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: torch.Tensor,
+                    y: Optional[torch.Tensor], rstd_post: torch.Tensor,
+                    rstd_pre: Optional[torch.Tensor], w_post: torch.Tensor,
+                    w_pre: Optional[torch.Tensor], dw_post: torch.Tensor,
+                    dw_pre: Optional[torch.Tensor], gate: Optional[torch.Tensor] = None,
+                    dgate: Optional[torch.Tensor] = None, block_scale: float = 1.0,
+                    resid_scale: float = 1.0, rows: Optional[torch.Tensor] = None,
+                    accumulate: bool = True):
+    """Gradient of :func:`block_norms_fwd` on the rows ``rows`` of ``h``, ``y`` and the saved
+    statistics (all when ``None``): ``(dx, dh, dgate)``.
+
+    ``dy [R, H]`` is the gradient that reaches ``y`` past the next block (``None``: none does) and
+    ``dn [R, H]`` that of ``n``; without ``w_pre``, ``dn``, ``y``, ``rstd_pre`` and ``dw_pre`` are
+    ``None``.  ``dw_post``, ``dw_pre`` and, for a learned gate, ``dgate`` are fp32 ``[H]`` buffers,
+    added to (written without ``accumulate``); a token's or element's gate returns its gradient
+    for the ``R`` rows.  On the GPU a row id outside ``h`` records an error in the status block and
+    gives zero rows."""
+    name = "block_norms_bwd"
+    T, H = h.shape if h.dim() == 2 else (-1, -1)
+    _need(T >= 0 and _rows2d(h, H) and h.dtype in _ROW_TYPES,
+          "{}: h must be a row-major bf16, fp16 or fp32 [T, H]", name)
+    pre = w_pre is not None
+    _need((dn is not None) == pre and (y is not None) == pre and (rstd_pre is not None) == pre
+          and (dw_pre is not None) == pre and (pre or dy is not None),
+          "{}: dn, y, rstd_pre and dw_pre go with w_pre, and one of dy and dn is needed", name)
+    R = (dy if dn is None else dn).shape[0]
+    resid = (y if pre else dy).dtype
+    _need(resid in (h.dtype, torch.float32), "{}: y and dy must be {} or fp32", name, h.dtype)
+    if dy is not None:
+        _need(_rows2d(dy, H) and dy.shape[0] == R and dy.dtype == resid,
+              "{}: dy must be a row-major {} [{}, {}]", name, resid, R, H)
+    if pre:
+        _need(_rows2d(dn, H) and dn.dtype == h.dtype and _rows2d(y, H) and y.shape[0] == T,
+              "{}: dn must be a row-major {} [R, {}] and y a row-major [{}, {}]", name, h.dtype, H,
+              T, H)
+        _need(_vector(rstd_pre, T, torch.float32) and _vector(w_pre, H, h.dtype)
+              and _vector(dw_pre, H, torch.float32),
+              "{}: rstd_pre must be fp32 [{}], w_pre {} [{}], dw_pre fp32 [{}]", name, T, h.dtype,
+              H, H)
+    _need(_vector(rstd_post, T, torch.float32) and _vector(w_post, H, h.dtype)
+          and _vector(dw_post, H, torch.float32),
+          "{}: rstd_post must be fp32 [{}], w_post {} [{}], dw_post fp32 [{}]", name, T, h.dtype, H,
+          H)
+    _need(H <= 16384, "{}: hidden size {} is over 16384", name, H)
+    if rows is None:
+        _need(R == T, "{}: {} gradient rows for {} rows", name, R, T)
+    else:
+        _need(rows.dtype == torch.int32 and rows.dim() == 1 and rows.shape[0] == R
+              and rows.is_contiguous(), "{}: rows must be contiguous int32 [{}]", name, R)
+    if gate is not None:
+        _check_gate(name, gate, T, H, h.dtype)
+    learned = gate is not None and gate.dim() == 1
+    _need((dgate is not None) == learned and (not learned or _vector(dgate, H, torch.float32)),
+          "{}: dgate is the fp32 [{}] buffer of a learned gate", name, H)
+    if not h.is_cuda:
+        if rows is not None:
+            at = rows.long()
+            h, rstd_post = h[at], rstd_post[at]
+            y, rstd_pre = (y[at], rstd_pre[at]) if pre else (None, None)
+            gate = gate if gate is None or learned else gate[at]
+        dx, dh, dp, dq, dg = ref.block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre,
+                                                 gate, block_scale, resid_scale)
+        for acc, d in ((dw_post, dp), (dw_pre, dq), (dgate, dg if learned else None)):
+            if acc is not None:
+                acc.copy_(acc + d if accumulate else d)
+        return (dx.to(resid), dh.to(h.dtype),
+                dgate if gate is None or learned else dg.to(gate.dtype))
+    return kernels().block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre, dw_post,
+                                     dw_pre, gate, dgate, block_scale, resid_scale, rows,
+                                     accumulate)
+
+
 # ---------------------------------------------------------------- cross entropy
 def ce_fwd(logits: torch.Tensor, labels: torch.Tensor, loss: Optional[torch.Tensor] = None,
            lse: Optional[torch.Tensor] = None):
@@ -234,6 +432,111 @@ def grad_norm_clip_coef(grad: torch.Tensor, max_norm: float, extra_scale: float,
         extra_sumsq = partial
     k.clip_coef(extra_sumsq, max_norm, extra_scale, coef, norm)
     return coef
+
+
+def grad_list_sumsq(grads: Sequence[torch.Tensor],
+                    partial: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Sum of squares of all elements of a list of tensors, as fp32 partial sums whose total it is
+    (``partial``, one for each block).  Ranks that hold different parameters add their totals (an
+    all-reduce of ``partial.sum()``) and give the result to :func:`grad_list_clip_` as
+    ``extra_sumsq``."""
+    grads = list(grads)
+    _need(len(grads) > 0, "grad_list_sumsq: empty list")
+    _check_grads("grad_list_sumsq", grads)
+    if not grads[0].is_cuda:
+        total = sum(g.double().pow(2).sum() for g in grads).float().view(1)
+        if partial is None:
+            return total
+        partial.zero_()
+        partial[:1] = total
+        return partial
+    if partial is None:
+        partial = torch.empty(148 * 8, dtype=torch.float32, device=grads[0].device)
+    kernels().grad_list_sumsq(grads, partial)
+    return partial
+
+
+def _check_grads(name: str, grads: List[torch.Tensor]) -> None:
+    dev = grads[0].device
+    for i, g in enumerate(grads):
+        if g.dtype not in _ROW_TYPES or g.device != dev or g.layout != torch.strided:
+            raise ValueError(f"{name}: tensor {i} must be a dense bf16, fp16 or fp32 tensor on {dev}")
+
+
+def _check_spans(grads: List[torch.Tensor], outs: List[torch.Tensor]) -> None:
+    """Outputs shaped like their gradients, dense, and apart from every other tensor."""
+    spans, end, end_written = [], 0, 0
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        _need(o.shape == g.shape and (o.stride() == g.stride()
+                                      or o.is_contiguous() and g.is_contiguous()),
+              "grad_list_clip_: output {} must have the sizes and strides of its gradient", i)
+        _need(torch.ops.aten.is_non_overlapping_and_dense.default(g),
+              "grad_list_clip_: tensor {} has gaps or overlaps itself", i)
+        own = o.data_ptr() == g.data_ptr() and o.dtype == g.dtype
+        for t in (o,) if own else (g, o):
+            lo = t.data_ptr()
+            if t.numel():
+                spans.append((lo, lo + t.numel() * t.element_size(), i, t is o))
+    for lo, hi, i, written in sorted(spans):
+        _need(lo >= (end if written else end_written),
+              "grad_list_clip_: tensor {} overlaps another that is written", i)
+        end, end_written = max(end, hi), max(end_written, hi) if written else end_written
+
+
+def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale: float = 1.0,
+                    out: Optional[Sequence[torch.Tensor]] = None,
+                    norm: Optional[torch.Tensor] = None,
+                    extra_sumsq: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Clip a list of gradients by their global norm, without a host synchronisation::
+
+        norm   = extra_scale * sqrt(sum of all squares)
+        out[i] = grads[i] * extra_scale * min(1, max_norm / (norm + 1e-6))
+
+    in place, or into the tensors ``out`` (which may have other types: bf16 gradients into the
+    optimizer's fp32 buffer).  Returns ``norm`` (fp32 ``[1]``).  ``max_norm <= 0`` sets no limit.
+    A norm that is infinite or no number is returned as such, and carries over to the gradients as
+    the formula says.  ``extra_sumsq``: fp32 partial sums of squares to use instead of the list's
+    own (see :func:`grad_list_sumsq`).
+
+    Tensors are bf16, fp16 or fp32, of any size and alignment, in any dense layout (``out[i]``
+    in that of ``grads[i]``); the list may mix types.  Tensors that overlap another one that is
+    written, and tensors with gaps, are refused.  The squares are fp32 (an element above 1.8e19
+    makes the norm infinite)."""
+    grads = list(grads)
+    if not extra_scale > 0:
+        raise ValueError(f"grad_list_clip_: extra_scale = {extra_scale} is not positive")
+    if not grads:
+        return torch.zeros(1) if norm is None else norm.zero_()
+    _check_grads("grad_list_clip_", grads)
+    outs = grads if out is None else list(out)
+    if out is not None:
+        _need(len(outs) == len(grads), "grad_list_clip_: {} gradients, {} outputs", len(grads),
+              len(outs))
+        _check_grads("grad_list_clip_", outs)
+    if norm is None:
+        norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
+    if not grads[0].is_cuda:
+        _check_spans(grads, outs)  # the kernels' binding checks the same
+    if extra_sumsq is None:
+        extra_sumsq = grad_list_sumsq(grads)
+    if not grads[0].is_cuda:
+        norm.copy_((extra_sumsq.double().sum().sqrt() * extra_scale).view(1))
+        k = extra_scale
+        if max_norm > 0:
+            k = (max_norm / (norm.view(()) + 1e-6)).clamp(max=1.0) * extra_scale
+        for g, o in zip(grads, outs):
+            o.copy_(g.float() * k)
+        return norm
+    kernels().grad_list_scale(grads, outs, extra_sumsq, max_norm, extra_scale, norm)
+    return norm
+
+
+def grad_list_clip_coef(grads: Sequence[torch.Tensor], max_norm: float, extra_scale: float,
+                        coef: torch.Tensor, norm: torch.Tensor) -> torch.Tensor:
+    """:func:`grad_norm_clip_coef` of a list of tensors: ``coef`` and ``norm`` for an optimizer that
+    takes the factor itself (:func:`adamw_`'s ``grad_scale``); the gradients are only read."""
+    return grad_norm_clip_coef(grads[0], max_norm, extra_scale, coef, norm,
+                               extra_sumsq=grad_list_sumsq(grads))
 
 
 # ---------------------------------------------------------------- attention

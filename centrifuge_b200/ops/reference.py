@@ -29,6 +29,38 @@ def rmsnorm_bwd(dy, x, rstd, w, dres=None):
     return dx, dw
 
 
+def block_norms(h, x, w_post, w_pre, eps, gate=None, block_scale=1.0, resid_scale=1.0):
+    """Norm after a block, gate, residual sum and the norm before the next block (fp32):
+    ``(y, n, rstd_post, rstd_pre)``, the last two ``None`` without ``w_pre``."""
+    b, rstd_post = rmsnorm(h, w_post, eps)
+    if gate is not None:
+        b = b * gate.float()
+    y = resid_scale * x.float() + block_scale * b
+    if w_pre is None:
+        return y, None, rstd_post, None
+    n, rstd_pre = rmsnorm(y, w_pre, eps)
+    return y, n, rstd_post, rstd_pre
+
+
+def block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre, gate=None, block_scale=1.0,
+                    resid_scale=1.0):
+    """Gradient of :func:`block_norms` (fp32): ``(dx, dh, dw_post, dw_pre, dgate)``."""
+    dY, dw_pre = (None if dy is None else dy.float()), None
+    if w_pre is not None:
+        dY, dw_pre = rmsnorm_bwd(dn, y, rstd_pre, w_pre, dY)
+    t = block_scale * dY
+    db = t if gate is None else t * gate.float()
+    dh, dw_post = rmsnorm_bwd(db, h, rstd_post, w_post)
+    dgate = None
+    if gate is not None:
+        dgate = t * h.float() * rstd_post.unsqueeze(-1) * w_post.float()
+        if gate.dim() == 1:
+            dgate = dgate.sum(0)
+        elif gate.shape[1] == 1 and gate.dtype == torch.float32:
+            dgate = dgate.sum(-1, keepdim=True)
+    return resid_scale * dY, dh, dw_post, dw_pre, dgate
+
+
 def rope_table(max_pos: int, head_dim: int, theta: float, device=None) -> torch.Tensor:
     """``[max_pos, head_dim/2, 2]`` fp32 (cos, sin) of ``pos * theta^(-2i/d)`` (HF convention)."""
     inv_freq = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.int64).float() / head_dim))

@@ -1,0 +1,567 @@
+"""The row operators around the blocks: scaled embedding and its gradient, the norms after and before
+a block, and clipping of a gradient list, against their formulas in 64 bits.
+
+Tolerances are bounds on the rounding errors of the arithmetic, element by element: u = 2^-24 for an
+fp32 operation, k u sum|x| for a sum whose longest chain has k additions, and half a step of the
+output's type for its one rounding.
+"""
+import math
+
+import pytest
+import torch
+
+from centrifuge_b200.ops import fused
+
+U = 2.0 ** -24
+EPS = 1e-5
+CPU_GPU = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def half_step(t):
+    """Half a step of type t relative to the value, and its smallest absolute half step."""
+    return torch.finfo(t).eps / 2, torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def close(got, want, tol, what):
+    """|got - want| <= tol everywhere, after the rounding to got's type."""
+    rel, tiny = half_step(got.dtype)
+    bound = tol + rel * (want.abs() + tol) + tiny
+    bad = ~((got.double() - want).abs() <= bound)
+    if bad.any():
+        i = tuple(bad.nonzero()[0].tolist())
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} off, at {i}: got "
+                             f"{float(got[i])}, want {float(want[i])}, bound {float(bound[i])}")
+
+
+def gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def rand(g, *shape, dtype=F32, scale=1.0, shift=0.0, pad=0, skew=0):
+    """Normal values; the rows `pad` elements longer than asked for and begun at element `skew`."""
+    if len(shape) == 2 and (pad or skew):
+        t = torch.randn(shape[0], shape[1] + pad + skew, generator=g, device=g.device)
+        return (t * scale + shift).to(dtype)[:, skew:skew + shape[1]]
+    return (torch.randn(*shape, generator=g, device=g.device) * scale + shift).to(dtype)
+
+
+# ---------------------------------------------------------------- scaled embedding
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("V,H,R,dtype,out,ids32,pad", [
+    (50, 256, 300, BF, BF, False, 0), (50, 8, 1, HF, HF, True, 0), (7, 1, 33, F32, F32, False, 0),
+    (1, 250, 5, BF, F32, True, 0), (300, 1000, 77, HF, F32, False, 8), (90, 255, 40, BF, BF, True, 3),
+    (33, 2048, 64, F32, BF, False, 0), (20, 4104, 9, BF, HF, False, 8), (20, 64, 0, BF, BF, False, 0),
+])
+def test_scaled_embedding_fwd(dev, V, H, R, dtype, out, ids32, pad):
+    g = gen(dev, V + H)
+    table = rand(g, V, H, dtype=dtype, pad=pad)
+    ids = torch.randint(0, V, (R,), generator=g, device=dev)
+    ids = ids.int() if ids32 else ids
+    o = None if out == dtype and not pad else torch.empty(R, H + pad, dtype=out, device=dev)[:, :H]
+    got = fused.scaled_embedding_fwd(table, ids, math.sqrt(H), out=o)
+    assert got.dtype == out and got.shape == (R, H) and (o is None or got is o)
+    want = table[ids.long()].double() * math.sqrt(H)
+    close(got, want, 2 * U * want.abs(), "out")  # the scale and the product are rounded to fp32
+
+
+def grad_of_table(dy, tok, V, scale):
+    """The gradient and the bound of an fp32 sum of each token's rows, in 64 bits."""
+    z = torch.zeros(V, dy.shape[1], dtype=torch.float64, device=dy.device)
+    count = torch.bincount(tok, minlength=V).double().unsqueeze(1)
+    mass = z.clone().index_add_(0, tok, dy.double().abs()) * scale
+    return z.clone().index_add_(0, tok, dy.double()) * scale, (count + 3) * U * mass
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("V,H,T,R,dtype,ids32,kind", [
+    (1024, 256, 256, 128, BF, False, "uniform"), (1024, 256, 1, 1, BF, True, "uniform"),
+    (5, 8, 400, 400, HF, False, "uniform"), (1, 64, 333, 200, F32, False, "uniform"),
+    (3000, 1000, 3000, 3000, BF, False, "text"), (3000, 250, 1000, 999, BF, True, "text"),
+    (70000, 64, 5000, 4097, BF, False, "text"), (200000, 8, 700, 700, F32, False, "uniform"),
+    (2000, 2056, 900, 900, HF, False, "one"), (500, 96, 4000, 3333, BF, False, "half"),
+    (32, 33, 64, 64, F32, False, "runs"), (32, 7, 33, 32, BF, True, "runs"),
+    (40, 2048, 70, 65, F32, False, "text"), (40, 2500, 70, 65, BF, False, "text"),
+    (64, 16, 100, 0, BF, False, "uniform"),
+])
+@pytest.mark.parametrize("accumulate,pad", [(True, None), (False, 3), (False, None)])
+def test_scaled_embedding_bwd(dev, V, H, T, R, dtype, ids32, kind, accumulate, pad):
+    g = gen(dev, V + H + T)
+    if kind == "uniform":
+        ids = torch.randint(0, V, (T,), generator=g, device=dev)
+    elif kind == "text":
+        u = torch.rand(T, generator=g, device=dev, dtype=torch.float64)
+        ids = (torch.exp(u * math.log(V)) - 1).long().clamp(0, V - 1)
+    elif kind == "one":
+        ids = torch.full((T,), V - 1, device=dev)
+    elif kind == "half":
+        ids = torch.randint(0, V, (T,), generator=g, device=dev)
+        ids[torch.rand(T, generator=g, device=dev) < 0.5] = 3
+    else:  # sorted runs whose borders fall on and beside multiples of 32
+        ids = (torch.arange(T, device=dev) + 1) // 31 % V
+    ids = ids.int() if ids32 else ids
+    rows = None
+    if R != T:
+        rows = torch.randperm(T, generator=g, device=dev)[:R].sort().values.int()
+    dy = rand(g, R, H, dtype=dtype)
+    before = rand(g, V, H)
+    got = before.clone()
+    res = fused.scaled_embedding_bwd(dy, ids, got, 1.7, id_rows=rows, padding_idx=pad,
+                                     accumulate=accumulate)
+    assert res is got
+    tok = (ids if rows is None else ids[rows.long()]).long()
+    keep = tok != (-1 if pad is None else pad)
+    want, tol = grad_of_table(dy[keep], tok[keep], V, 1.7)
+    if accumulate:
+        want = want + before.double()
+        tol = tol + 2 * U * want.abs()
+    close(got, want, tol, "dtable")
+    if not accumulate:  # nothing of what the table held is left
+        assert not got[torch.bincount(tok[keep], minlength=V) == 0].any()
+
+
+@pytest.mark.gpu
+def test_scaled_embedding_bwd_is_repeatable_and_takes_strides():
+    g = gen("cuda", 5)
+    ids = torch.randint(0, 300, (2, 3000), generator=g, device="cuda")
+    ids[:, ::3] = 17
+    dy = rand(g, 6000, 512, dtype=BF, pad=24)
+    base = torch.zeros(300, 520, device="cuda")
+    for a in (base[:, :512], torch.empty(300, 512, device="cuda")):
+        runs = []
+        for _ in range(3):
+            a.zero_()
+            runs.append(fused.scaled_embedding_bwd(dy, ids, a, 0.5).clone())
+        assert torch.equal(runs[0], runs[1]) and torch.equal(runs[0], runs[2])
+        want, tol = grad_of_table(dy, ids.reshape(-1), 300, 0.5)
+        close(runs[0], want, tol, "dtable")
+    assert not base[:, 512:].any()  # behind the rows nothing is written
+    base.fill_(7.0)
+    fused.scaled_embedding_bwd(dy, ids, base[:, :512], 0.5, accumulate=False)
+    assert torch.equal(base[:, :512], runs[0]) and bool((base[:, 512:] == 7.0).all())
+    # rows that begin off the vector borders
+    off = torch.zeros(300, 515, device="cuda")[:, 1:514]
+    fused.scaled_embedding_bwd(rand(g, 6000, 513, dtype=BF, skew=3), ids, off)
+    assert bool(off.any())
+
+
+@pytest.mark.gpu
+def test_scaled_embedding_reports_bad_indices():
+    from centrifuge_b200.ops._ext import kernels
+    status = kernels().status_block(0)
+    status.zero_()
+    g = gen("cuda", 6)
+    table = rand(g, 64, 128, dtype=BF)
+    ids = torch.tensor([3, 64, 5, -1, 1 << 40], device="cuda")
+    out = fused.scaled_embedding_fwd(table, ids, 2.0)
+    assert int(status[0]) == 128 and not out[[1, 3, 4]].any()
+    assert torch.equal(out[[0, 2]], table[[3, 5]] * 2)
+    status.zero_()
+    dy = rand(g, 3, 128, dtype=BF)
+    for rows in ([0, 1, 2], [0, 3, 9], [0, 4, -5]):
+        dt = torch.zeros(64, 128, device="cuda")
+        rid = torch.tensor(rows, dtype=torch.int32, device="cuda")
+        fused.scaled_embedding_bwd(dy, ids, dt, id_rows=rid)
+        assert int(status[0]) == 128
+        status.zero_()
+        assert torch.equal(dt[3], dy[0].float())
+        used = [3] + ([5] if rows[2] == 2 else [])
+        dt[used] = 0
+        assert not dt.any()
+
+
+# ---------------------------------------------------------------- norms around a block
+def norms_case(dev, T, H, dtype, resid, gate, pre, pad=0, skew=0, seed=0):
+    g = gen(dev, 1000 * T + H + seed)
+    c = {"h": rand(g, T, H, dtype=dtype, pad=pad, skew=skew),
+         "x": rand(g, T, H, dtype=resid, scale=2.0, pad=pad, skew=skew),
+         "w_post": rand(g, H, dtype=dtype, scale=0.1, shift=1.0),
+         "w_pre": rand(g, H, dtype=dtype, scale=0.1, shift=1.0) if pre else None}
+    c["gate"] = {"none": lambda: None,
+                 "channel": lambda: rand(g, H, dtype=dtype, scale=0.3, shift=0.5),
+                 "token": lambda: rand(g, T, 1, pad=pad),
+                 "element": lambda: rand(g, T, H, dtype=dtype, pad=pad, skew=skew)}[gate]()
+    return g, c
+
+
+def norms_formula(c, a, b):
+    """Forward in 64 bits from fp64 leaves."""
+    h = c["h"]
+    rp = (h.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    br = b * h * rp * c["w_post"]
+    if c["gate"] is not None:
+        br = br * c["gate"]
+    y = a * c["x"] + br
+    if c["w_pre"] is None:
+        return y, None, rp, None, br
+    rq = (y.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    return y, y * rq * c["w_pre"], rp, rq, br
+
+
+def doubles(c):
+    return {k: None if v is None else v.double() for k, v in c.items()}
+
+
+NORM_CASES = [
+    (256, 256, BF, BF, "none", True), (1, 8, BF, BF, "channel", True), (3, 1, F32, F32, "token", True),
+    (17, 33, HF, HF, "element", True), (300, 250, BF, F32, "channel", True),
+    (200, 1000, HF, HF, "none", False), (65, 512, BF, F32, "token", True),
+    (129, 768, F32, F32, "element", True), (77, 2048, BF, BF, "channel", True),
+    (300, 2048, BF, BF, "token", False), (40, 2049, BF, BF, "element", True),
+    (33, 4096, BF, F32, "element", True), (19, 5632, HF, F32, "channel", False),
+    (12, 8192, BF, BF, "token", True), (9, 8200, BF, BF, "channel", True),
+    (5, 16384, F32, F32, "element", True), (4, 16383, BF, BF, "channel", True),
+    (2500, 64, BF, BF, "channel", True), (2, 24, BF, BF, "channel", True),
+]
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,H,dtype,resid,gate,pre", NORM_CASES)
+@pytest.mark.parametrize("pad,skew", [(0, 0), (8, 0), (5, 1)])
+def test_block_norms_fwd(dev, T, H, dtype, resid, gate, pre, pad, skew):
+    _, c = norms_case(dev, T, H, dtype, resid, gate, pre, pad, skew)
+    a, b = 0.75, 0.5  # exact in fp32
+    y, n, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS,
+                                         gate=c["gate"], block_scale=b, resid_scale=a)
+    assert y.dtype == resid and rp.dtype == F32 and (n is None) == (rq is None) == (not pre)
+    wy, wn, wp, wq, br = norms_formula(doubles(c), a, b)
+    # a mean of squares: a chain of at most 128 additions and 10 exchanges, half of it in the root,
+    # whose own error is at most two steps
+    dr = 70 * U + 4 * U
+    close(rp, wp.squeeze(1), dr * wp.squeeze(1), "rstd_post")
+    dy = (dr + 6 * U) * br.abs() + 3 * U * (a * c["x"].double()).abs()
+    close(y, wy, dy, "y")
+    if pre:
+        assert n.dtype == dtype
+        moved = dy.norm(dim=1, keepdim=True) * wq / math.sqrt(H)  # what dy does to the root
+        close(rq, wq.squeeze(1), ((dr + moved) * wq).squeeze(1), "rstd_pre")
+        close(n, wn, (wq * c["w_pre"].double()).abs() * dy + wn.abs() * (dr + moved + 3 * U), "n")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,H,dtype,resid,gate,pre", NORM_CASES)
+@pytest.mark.parametrize("kept,accumulate,with_dy,pad,skew", [
+    (False, False, True, 0, 0), (True, True, True, 8, 0), (True, False, False, 5, 1)])
+def test_block_norms_bwd(dev, T, H, dtype, resid, gate, pre, kept, accumulate, with_dy, pad, skew):
+    g, c = norms_case(dev, T, H, dtype, resid, gate, pre, pad, skew, seed=7)
+    a, b = 0.75, 0.5
+    y, _, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS,
+                                         gate=c["gate"], block_scale=b, resid_scale=a)
+    with_dy = with_dy or not pre
+    R = max(1, T // 2) if kept else T
+    rows = torch.randperm(T, generator=g, device=dev)[:R].sort().values.int() if kept else None
+    at = torch.arange(T, device=dev) if rows is None else rows.long()
+    dn = rand(g, R, H, dtype=dtype, pad=pad, skew=skew) if pre else None
+    dy = rand(g, R, H, dtype=resid, pad=pad, skew=skew) if with_dy else None
+    base = rand(g, 3, H)
+    acc = base.clone()
+    learned = c["gate"] is not None and c["gate"].dim() == 1
+    dx, dh, dg = fused.block_norms_bwd(
+        dy, dn, c["h"], y if pre else None, rp, rq, c["w_post"], c["w_pre"], acc[0],
+        acc[1] if pre else None, gate=c["gate"], dgate=acc[2] if learned else None, block_scale=b,
+        resid_scale=a, rows=rows, accumulate=accumulate)
+    assert dx.dtype == resid and dh.dtype == dtype and dx.shape == dh.shape == (R, H)
+
+    # the formulas at the saved statistics, in 64 bits, and the bounds
+    d = doubles(c)
+    h, r1, w1 = d["h"][at], rp[at].double().unsqueeze(1), d["w_post"]
+    gt = torch.ones(1, 1, dtype=torch.float64, device=dev)
+    if c["gate"] is not None:
+        gt = d["gate"] if learned else d["gate"][at]
+    up = torch.zeros(R, H, dtype=torch.float64, device=dev) if dy is None else dy.double()
+    t_up = 4 * U * up.abs()
+    K = 48 * U  # a chain of at most 16 products and 10 exchanges, and their roundings, twice over
+    if pre:
+        yy, r2 = y[at].double(), rq[at].double().unsqueeze(1)
+        q = dn.double() * d["w_pre"]
+        dot, mass = (q * yy).sum(1, keepdim=True), (q * yy).abs().sum(1, keepdim=True)
+        part = yy * r2 ** 3 / H
+        up = up + r2 * q - part * dot
+        t_up = t_up + 4 * U * r2 * q.abs() + part.abs() * K * mass + 8 * U * (part * dot).abs()
+        t_up = t_up + 2 * U * up.abs()
+        s = dn.double() * yy * r2
+        want = s.sum(0)
+        tol = (R + 24) * U * s.abs().sum(0)
+        if accumulate:
+            want, tol = want + base[1].double(), tol + 2 * U * (want + base[1].double()).abs()
+        close(acc[1], want, tol, "dw_pre")
+    close(dx, a * up, a * t_up + 2 * U * up.abs(), "dx")
+    v = b * up * gt * w1
+    t_v = (b * gt * w1).abs() * t_up + 4 * U * v.abs()
+    dot, mass = (v * h).sum(1, keepdim=True), (v * h).abs().sum(1, keepdim=True)
+    t_dot = (t_v * h.abs()).sum(1, keepdim=True) + K * mass
+    part = h * r1 ** 3 / H
+    close(dh, r1 * v - part * dot,
+          r1 * t_v + part.abs() * t_dot + 8 * U * (r1 * v.abs() + (part * dot).abs()), "dh")
+    per = b * up * h * r1  # the gradient of gate times weight
+    t_per = (b * h * r1).abs() * t_up + 4 * U * per.abs()
+
+    def summed(got, want, tol, old, what):
+        if accumulate:
+            want, tol = want + old, tol + 2 * U * (want + old).abs()
+        close(got, want, tol, what)
+
+    summed(acc[0], (per * gt).sum(0),
+           ((t_per * gt.abs()).sum(0) + (R + 24) * U * (per * gt).abs().sum(0)), base[0].double(),
+           "dw_post")
+    if learned:
+        assert dg.data_ptr() == acc[2].data_ptr()
+        summed(acc[2], (per * w1).sum(0),
+               (t_per * w1.abs()).sum(0) + (R + 24) * U * (per * w1).abs().sum(0), base[2].double(),
+               "dgate")
+    elif c["gate"] is None:
+        assert dg is None
+    elif gate == "token" or H == 1 and dtype == F32:
+        close(dg, (per * w1).sum(1, keepdim=True),
+              (t_per * w1.abs()).sum(1, keepdim=True) + K * (per * w1).abs().sum(1, keepdim=True),
+              "dgate")
+    else:
+        close(dg, per * w1, t_per * w1.abs() + 2 * U * (per * w1).abs(), "dgate")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
+def test_block_norms_gradient_against_differences(dev, gate):
+    """Central differences of the 64-bit formula along random directions."""
+    g, c = norms_case(dev, 6, 40, F32, F32, gate, True, seed=3)
+    a, b = 0.75, 0.5
+    y, _, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS,
+                                         gate=c["gate"], block_scale=b, resid_scale=a)
+    dy, dn = rand(g, 6, 40), rand(g, 6, 40)
+    acc = torch.zeros(3, 40, device=dev)
+    dx, dh, dg = fused.block_norms_bwd(dy, dn, c["h"], y, rp, rq, c["w_post"], c["w_pre"], acc[0],
+                                       acc[1], gate=c["gate"],
+                                       dgate=acc[2] if gate == "channel" else None, block_scale=b,
+                                       resid_scale=a)
+    grads = {"h": dh, "x": dx, "w_post": acc[0], "w_pre": acc[1], "gate": dg}
+    d = doubles(c)
+
+    def loss(k, step):
+        p = dict(d)
+        p[k] = p[k] + step
+        y_, n_, _, _, _ = norms_formula(p, a, b)
+        return float((y_ * dy).sum() + (n_ * dn).sum())
+
+    for k, grad in grads.items():
+        if d[k] is None:
+            continue
+        way = torch.randn(d[k].shape, generator=g, device=dev, dtype=torch.float64)
+        e = 1e-5
+        diff = (loss(k, e * way) - loss(k, -e * way)) / (2 * e)
+        # differences: e^2 of the third derivative and 1e-16 / e of the loss; the gradient: fp32
+        mass = float((grad.double() * way).abs().sum())
+        assert abs(float((grad.double() * way).sum()) - diff) < 1e-5 * (mass + 1), k
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_block_norms_odd_values(dev):
+    """Rows of zeros stay finite; what is no number in one row stays in its row; no rows at all."""
+    _, c = norms_case(dev, 5, 64, BF, BF, "channel", True)
+    c["h"][1] = 0
+    c["x"][1] = 0
+    c["h"][3, 5] = float("nan")
+    c["x"][4, 6] = float("inf")
+    y, n, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS, c["gate"])
+    assert not y[1].any() and not n[1].any()
+    for t in (y, n):
+        assert bool(torch.isfinite(t[:3]).all()) and bool(t[3].isnan().any())
+    assert bool(y[4].isinf().any()) and bool(torch.isfinite(rp[[0, 1, 2, 4]]).all())
+    acc = torch.ones(3, 64, device=dev)
+    d = torch.zeros(0, 64, dtype=BF, device=dev)
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    for accumulate in (True, False):
+        dx, dh, _ = fused.block_norms_bwd(d, d, c["h"], y, rp, rq, c["w_post"], c["w_pre"], acc[0],
+                                          acc[1], c["gate"], acc[2], rows=none,
+                                          accumulate=accumulate)
+        assert dx.shape == dh.shape == (0, 64)
+        assert bool((acc == (1.0 if accumulate else 0.0)).all())
+    y, n, _, _ = fused.block_norms_fwd(d, d, c["w_post"], c["w_pre"], EPS)
+    assert y.shape == n.shape == (0, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate", ["none", "token", "element"])
+@pytest.mark.parametrize("pre", [True, False])
+def test_block_norms_bwd_reports_bad_rows(gate, pre):
+    from centrifuge_b200.ops._ext import kernels
+    status = kernels().status_block(0)
+    status.zero_()
+    g, c = norms_case("cuda", 2000, 512, BF, BF, gate, pre)
+    y, _, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS, c["gate"])
+    rows = torch.arange(2000, dtype=torch.int32, device="cuda")
+    good = rows % 3 != 0
+    bad = torch.where(good, rows, torch.where(rows % 2 == 0, -1 - rows, 2000 + rows))
+    dy = rand(g, 2000, 512, dtype=BF)
+    res = []
+    for ids, w in ((bad, 1.0), (rows, good.unsqueeze(1).to(BF))):
+        acc = torch.zeros(2, 512, device="cuda")
+        d = dy * w
+        dx, dh, dg = fused.block_norms_bwd(d, d if pre else None, c["h"], y if pre else None, rp, rq,
+                                           c["w_post"], c["w_pre"], acc[0], acc[1] if pre else None,
+                                           gate=c["gate"], rows=ids)
+        res.append((dx, dh, acc, *([] if dg is None else [dg])))
+        assert int(status[0]) == (128 if ids is bad else 0)
+        status.zero_()
+    for p, q in zip(*res):
+        assert torch.equal(p, q)  # the bad rows add nothing and come back as zeros
+
+
+# ---------------------------------------------------------------- gradient lists
+def grad_list(dev, sizes, types, seed=0, skew=0):
+    g = gen(dev, seed)
+    got = []
+    for i, n in enumerate(sizes):
+        t = rand(g, n + skew, dtype=types[i % len(types)], scale=0.01)
+        got.append(t[skew:])
+    return got
+
+
+LISTS = {
+    "one": [1], "tiny": [1, 2, 3, 0, 7, 8, 9], "borders": [32767, 32768, 32769, 65536, 65537, 1],
+    "mixed": [100000, 17, 0, 70001, 5, 256, 33000], "many": [13] * 300, "groups": [3, 40] * 700,
+    "large": [5_000_001, 12],
+}
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("name", list(LISTS))
+@pytest.mark.parametrize("types", [(F32,), (BF,), (F32, BF, HF)])
+@pytest.mark.parametrize("out_type", [None, F32, BF])
+@pytest.mark.parametrize("over,skew", [(3.0, 0), (3.0, 1), (0.5, 0)])
+def test_grad_list_clip(dev, name, types, out_type, over, skew):
+    grads = grad_list(dev, LISTS[name], types, seed=len(name), skew=skew)
+    want = [g.double() for g in grads]
+    norm = math.sqrt(sum(float(g.square().sum()) for g in want)) * 0.25
+    max_norm = norm / over
+    outs = None if out_type is None else [torch.empty(g.numel() + skew, dtype=out_type, device=dev)[skew:]
+                                          for g in grads]
+    got_norm = fused.grad_list_clip_(grads, max_norm, extra_scale=0.25, out=outs)
+    # squares: a thread's chain of 128 additions in fp32, half of it in the root; the partial sums
+    # and the norm are rounded once each
+    dn = (70 + 4) * U
+    assert got_norm.shape == (1,) and abs(float(got_norm) - norm) <= dn * norm
+    k = 0.25 * min(1.0, max_norm / (norm + 1e-6))
+    for i, (g, w) in enumerate(zip(grads if outs is None else outs, want)):
+        close(g, w * k, (w * k).abs() * (dn + 4 * U), f"tensor {i}")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_grad_list_in_place_and_dense_layouts(dev):
+    grads = [torch.randn(30, 50, device=dev).t(), torch.randn(2, 3, 4, 5, device=dev).permute(0, 2, 3, 1),
+             torch.randn((), device=dev)]
+    keep = [g.clone() for g in grads]
+    ptrs = [g.data_ptr() for g in grads]
+    big = float(sum(g.double().square().sum() for g in keep).sqrt()) * 2
+    fused.grad_list_clip_(grads, big)  # under the limit: not a bit changes
+    assert all(torch.equal(g, k) for g, k in zip(grads, keep))
+    n1 = fused.grad_list_clip_(grads, 1.0)
+    n2 = fused.grad_list_clip_(grads, 0.0)  # no limit
+    assert [g.data_ptr() for g in grads] == ptrs
+    assert abs(float(n2) - 1.0) < 1e-5 and float(n1) == pytest.approx(big / 2, rel=1e-5)
+    for g, k in zip(grads, keep):
+        assert torch.allclose(g, k / float(n1), rtol=1e-5, atol=0)
+    # one output is its gradient, the other another tensor
+    other = torch.empty_like(grads[1])
+    fused.grad_list_clip_([grads[0], grads[1]], 0.5, out=[grads[0], other])
+    assert float(sum(t.double().square().sum() for t in (grads[0], other)).sqrt()) == pytest.approx(
+        0.5, rel=1e-4)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_grad_list_norm_of_odd_values(dev):
+    for bad in (float("inf"), float("nan")):
+        grads = [torch.ones(100, device=dev), torch.ones(5, device=dev)]
+        grads[1][2] = bad
+        norm = fused.grad_list_clip_(grads, 1.0)
+        if math.isinf(bad):  # a limit of zero: what was finite is zero, infinity is no number
+            assert math.isinf(float(norm)) and not grads[0].any() and bool(grads[1][2].isnan())
+        else:
+            assert math.isnan(float(norm)) and bool(grads[0].isnan().all())
+    zeros = [torch.zeros(10, device=dev)]
+    assert float(fused.grad_list_clip_(zeros, 1.0)) == 0.0 and not zeros[0].any()
+    empty = [torch.empty(0, device=dev)]
+    assert float(fused.grad_list_clip_(empty, 1.0)) == 0.0
+    assert float(fused.grad_list_clip_([], 1.0)) == 0.0
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_grad_list_over_ranks_and_coef(dev):
+    """Two lists whose sums of squares are added, as ranks with different parameters do it."""
+    a, b = grad_list(dev, [1000, 77], (F32,), 1), grad_list(dev, [500], (BF,), 2)
+    want = [g.double() for g in a + b]
+    norm = math.sqrt(sum(float(g.square().sum()) for g in want))
+    total = fused.grad_list_sumsq(a).sum() + fused.grad_list_sumsq(b).sum()
+    for part in (a, b):
+        n = fused.grad_list_clip_(part, norm / 2, extra_sumsq=total.view(1))
+        assert float(n) == pytest.approx(norm, rel=1e-5)
+    for g, w in zip(a + b, want):
+        k = (norm / 2) / (norm + 1e-6)
+        close(g, w * k, (w * k).abs() * 80 * U, "clipped")
+    c = grad_list(dev, [1000, 77], (F32, BF), 1)
+    ref = math.sqrt(sum(float(g.double().square().sum()) for g in c))
+    coef, nrm = torch.empty(1, device=dev), torch.empty(1, device=dev)
+    fused.grad_list_clip_coef(c, ref / 4, 0.5, coef, nrm)
+    assert float(nrm) == pytest.approx(ref / 2, rel=1e-5)
+    assert float(coef) == pytest.approx(0.25, rel=1e-4)
+
+
+# ---------------------------------------------------------------- refusals
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_refusals(dev):
+    def t(*shape, dtype=F32):
+        return torch.zeros(*shape, dtype=dtype, device=dev)
+
+    def no(f, *args, **kw):
+        with pytest.raises((ValueError, RuntimeError)):
+            f(*args, **kw)
+
+    ids = torch.zeros(4, dtype=torch.long, device=dev)
+    no(fused.scaled_embedding_fwd, t(8, 16, dtype=torch.float64), ids)
+    no(fused.scaled_embedding_fwd, t(16, 8).t(), ids)
+    no(fused.scaled_embedding_fwd, t(8, 16), ids.float())
+    no(fused.scaled_embedding_fwd, t(8, 16), ids, out=t(3, 16))
+    no(fused.scaled_embedding_fwd, t(8, 16), ids, out=t(1, 16).expand(4, 16))
+    dy, dt = t(4, 16), t(8, 16)
+    no(fused.scaled_embedding_bwd, dy, ids[:3], dt)
+    no(fused.scaled_embedding_bwd, dy, ids, t(8, 16, dtype=BF))
+    no(fused.scaled_embedding_bwd, dy, ids, t(8, 15))
+    no(fused.scaled_embedding_bwd, dy, ids, t(1, 16).expand(8, 16))
+    no(fused.scaled_embedding_bwd, dy, ids, dt, id_rows=ids)
+    no(fused.scaled_embedding_bwd, dy, ids, dt, id_rows=ids[:3].int())
+
+    h, x, w, r, z = t(4, 16, dtype=BF), t(4, 16, dtype=BF), t(16, dtype=BF), t(4), t(16)
+    ok = dict(eps=EPS)
+    no(fused.block_norms_fwd, h, t(4, 16, dtype=HF), w, w, **ok)
+    no(fused.block_norms_fwd, h, t(3, 16, dtype=BF), w, w, **ok)
+    no(fused.block_norms_fwd, h, x, t(15, dtype=BF), w, **ok)
+    no(fused.block_norms_fwd, h, x, w.float(), w, **ok)
+    no(fused.block_norms_fwd, h[0], x, w, w, **ok)
+    no(fused.block_norms_fwd, h, x, w, w, gate=t(4, 1, dtype=BF), **ok)
+    no(fused.block_norms_fwd, h, x, w, w, gate=t(3, 1), **ok)
+    no(fused.block_norms_fwd, h, x, w, w, gate=t(1, 16, dtype=BF), **ok)
+    big = t(1, 16392, dtype=BF)
+    no(fused.block_norms_fwd, big, big, big[0], big[0], **ok)
+    bwd = dict(dy=x, dn=h, h=h, y=x, rstd_post=r, rstd_pre=r, w_post=w, w_pre=w, dw_post=z.clone(),
+               dw_pre=z.clone())
+    fused.block_norms_bwd(**bwd)
+    for change in (dict(dn=None), dict(w_pre=None), dict(y=None), dict(dw_pre=None),
+                   dict(dy=x.float()), dict(dn=h.float()), dict(rstd_post=r[:3]),
+                   dict(dw_post=w), dict(dgate=z), dict(gate=w), dict(gate=w, dgate=w),
+                   dict(gate=t(4, 1), dgate=z), dict(rows=torch.zeros(4, device=dev)),
+                   dict(rows=torch.zeros(3, dtype=torch.int32, device=dev)), dict(dy=x[:3])):
+        no(fused.block_norms_bwd, **{**bwd, **change})
+    no(fused.block_norms_bwd, **{**bwd, "dy": None, "dn": None, "w_pre": None, "y": None,
+                                 "rstd_pre": None, "dw_pre": None})
+
+    g = t(100)
+    no(fused.grad_list_clip_, [g.double()], 1.0)
+    no(fused.grad_list_clip_, [g], 1.0, extra_scale=0.0)
+    no(fused.grad_list_clip_, [g], 1.0, out=[])
+    no(fused.grad_list_clip_, [g], 1.0, out=[t(99)])
+    no(fused.grad_list_sumsq, [])
+    no(fused.grad_list_clip_, [g, g], 1.0)  # the same tensor twice
+    no(fused.grad_list_clip_, [g[:60], g[50:]], 1.0)
+    no(fused.grad_list_clip_, [t(100), t(100)], 1.0, out=[g[:], g[:]])
+    no(fused.grad_list_clip_, [g[:50], t(50)], 1.0, out=[t(50), g[25:75]])
+    no(fused.grad_list_clip_, [g[::2]], 1.0)
+    no(fused.grad_list_clip_, [t(1).expand(10)], 1.0)
