@@ -100,15 +100,24 @@ template <typename TI, typename TO>
 __device__ __forceinline__ void chunk_scale(const TI* p, TO* o, int n, float k) {
   const int tid = threadIdx.x;
   int done = 0;
-  if (((reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
+  if (reinterpret_cast<uintptr_t>(p) % (8 * sizeof(TI)) == 0 &&
+      reinterpret_cast<uintptr_t>(o) % (8 * sizeof(TO)) == 0) {
+    constexpr int U = 4;  // packs in flight
     const int vecs = n / 8;
-#pragma unroll 4
-    for (int i = tid; i < vecs; i += 256) {
-      float f[8];
-      load_f32<TI, 8>(p + i * 8, f);
+    for (int i = tid; i < vecs; i += 256 * U) {
+      Pack<TI, 8> v[U];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= k;
-      store_f32<TO, 8>(o + i * 8, f);
+      for (int u = 0; u < U; ++u)
+        if (i + u * 256 < vecs) v[u] = load_pack<TI, 8>(p + (i + u * 256) * 8);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + u * 256 >= vecs) break;
+        float f[8];
+        unpack<TI, 8>(v[u], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= k;
+        store_f32<TO, 8>(o + (i + u * 256) * 8, f);
+      }
     }
     done = vecs * 8;
   }

@@ -280,7 +280,7 @@ int cfb_scaled_embedding_fwd(const void* table, int type, long long ld, long lon
 
 long long cfb_scaled_embedding_bwd_workspace(int rows, int H) {
   const long long chunks = (rows + kChunk - 1) / kChunk;
-  return 4ll * (4 + 2ll * ((rows + 3) / 4 * 4) + 2 * chunks * H);  // bytes
+  return 4ll * (8 + 2ll * ((rows + 3) / 4 * 4) + 2 * chunks * H);  // bytes
 }
 
 int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void* ids, int ids32,
@@ -300,7 +300,7 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
   if (rows == 0) return launch_status();
   const int padded = (rows + 3) / 4 * 4;
   int* n_valid = static_cast<int*>(work);
-  int* order = n_valid + 4;
+  int* order = n_valid + 8;  // the partial sums behind it begin on a 32-byte border
   int* stok = order + padded;
   float* part = reinterpret_cast<float*>(stok + padded);
   // one block for each SM where the vocabulary allows, ranges of whole warps
