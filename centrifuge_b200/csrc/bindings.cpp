@@ -1033,10 +1033,12 @@ void grad_list_scale(const std::vector<Tensor>& grads, const std::vector<Tensor>
   std::vector<CfbTensorRef> refs = tensor_refs(grads, outs, &in_place);
   if (refs.empty()) refs.push_back({nullptr, nullptr, 0, kF32, kF32});  // the norm is still due
   const c10::cuda::CUDAGuard guard(partial.device());
+  Tensor factor = at::empty({1}, norm.options());
   CFB_CHECK_RC(cfb_grad_list_scale(refs.data(), static_cast<int>(refs.size()),
                                    partial.data_ptr<float>(), static_cast<int>(partial.numel()),
                                    static_cast<float>(max_norm), static_cast<float>(extra_scale),
-                                   norm.data_ptr<float>(), in_place, cur_stream()),
+                                   norm.data_ptr<float>(), factor.data_ptr<float>(), in_place,
+                                   cur_stream()),
                "grad_list_scale");
 }
 
