@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "launch_api.h"
 #include "sm100_common.cuh"
 
@@ -73,10 +75,148 @@ __device__ __forceinline__ void store_f32(T* p, const float* f) {
   store_pack<T, W>(p, k);
 }
 
+// Asks the L2 cache for the whole 16-byte pieces of the `bytes` from p.
+__device__ __forceinline__ void prefetch_l2(const void* p, int bytes) {
+  const uintptr_t at = (reinterpret_cast<uintptr_t>(p) + 15) & ~static_cast<uintptr_t>(15);
+  const int n = (bytes - static_cast<int>(at - reinterpret_cast<uintptr_t>(p))) & ~15;
+  if (n > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(at), "r"(n) : "memory");
+}
+
 __device__ __forceinline__ float warp_add(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
+}
+
+// ---------------------------------------------------------------- pairs of fp32
+// sm_100 multiplies and adds two fp32 in one instruction on a 64-bit register pair.  The row
+// kernels' arithmetic is a large part of their issue slots, so the wide ones work on pairs.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float s) { return f2(s, s); }
+__device__ __forceinline__ float2 halves(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ float sum2(F2 a) {
+  const float2 t = halves(a);
+  return t.x + t.y;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// The W elements of a pack as W / 2 pairs (one pair with a zero for W = 1), and back.
+template <int W>
+constexpr int kPairs = (W + 1) / 2;
+template <typename T, int W>
+__device__ __forceinline__ void unpack_f2(const Pack<T, W>& k, F2* f) {
+  if constexpr (W == 1) {
+    f[0] = f2(to_f32(k.v[0]), 0.f);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(&k);
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i)
+      f[i] = f2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+  } else {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) f[i] = f2(to_f32(k.v[2 * i]), to_f32(k.v[2 * i + 1]));
+  }
+}
+template <typename T, int W>
+__device__ __forceinline__ void load_f2(const T* p, F2* f) {
+  unpack_f2<T, W>(load_pack<T, W>(p), f);
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_f2(T* p, const F2* f) {
+  Pack<T, W> k;
+  if constexpr (W == 1) {
+    k.v[0] = from_f32<T>(halves(f[0]).x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const float2 t = halves(f[i]);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        reinterpret_cast<uint32_t*>(&k)[i] = pack_bf16x2(t.x, t.y);
+      } else {
+        k.v[2 * i] = from_f32<T>(t.x);
+        k.v[2 * i + 1] = from_f32<T>(t.y);
+      }
+    }
+  }
+  store_pack<T, W>(p, k);
+}
+template <typename T, int W>
+__device__ __forceinline__ Pack<T, W> zero_pack() {
+  Pack<T, W> k;
+#pragma unroll
+  for (int i = 0; i < W; ++i) k.v[i] = from_f32<T>(0.f);
+  return k;
+}
+
+// ---------------------------------------------------------------- sums of several rows
+// v[r], summed over the warp, for R rows at once: each exchange halves the number of rows that a
+// lane still holds, so that R = 4 takes 6 exchanges instead of 20.  Lane l returns the sum of row
+// (l >> (5 - log2 R)).
+template <int R>
+__device__ __forceinline__ float warp_sums(float* v) {
+  const int lane = lane_id();
+  int o = 16;
+#pragma unroll
+  for (int n = R / 2; n > 0; n /= 2, o /= 2) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float keep = up ? v[n + i] : v[i];
+      const float give = up ? v[i] : v[n + i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+    }
+  }
+  float s = v[0];
+#pragma unroll
+  for (; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return s;
+}
+// The same over a team of up to NW warps (a power of two, R * NW <= 32), which is the block: every
+// thread gets all R sums.  red: R * NW floats of shared memory; the caller sees to it that a barrier
+// lies between two uses of it.
+template <int R, int NW>
+__device__ __forceinline__ void team_sums(float* v, float* red) {
+  constexpr int kShift = R == 4 ? 3 : R == 2 ? 4 : 5;  // lanes of one row after warp_sums
+  const int lane = lane_id();
+  float s = warp_sums<R>(v);
+  if constexpr (NW > 1) {
+    if ((lane & ((1 << kShift) - 1)) == 0) red[(lane >> kShift) * NW + warp_id()] = s;
+    __syncthreads();
+    const int at = lane % (R * NW);
+    s = at % NW < static_cast<int>(blockDim.x >> 5) ? red[at] : 0.f;
+#pragma unroll
+    for (int o = NW / 2; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = __shfl_sync(0xffffffffu, s, r * NW);
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = __shfl_sync(0xffffffffu, s, r << kShift);
+  }
 }
 
 // An index outside [0, n) records kErrBounds in the status block; the caller skips the access.
@@ -101,11 +241,11 @@ int with_type(int code, F&& f) {
   }
 }
 inline int type_bytes(int code) { return code == kF32 ? 4 : 2; }
-// Whether rows that start at p, ld elements apart, can be read eight elements at a time.
-inline bool rows_of_8(const void* p, long long ld, int code) {
-  const int pack = 8 * type_bytes(code);
-  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % pack == 0 && ld % 8 == 0);
+// Whether rows that start at p, ld elements apart, can be read W elements at a time.
+inline bool rows_of(int W, const void* p, long long ld, int code) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) % (W * type_bytes(code)) == 0 && ld % W == 0);
 }
+inline bool rows_of_8(const void* p, long long ld, int code) { return rows_of(8, p, ld, code); }
 
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : -3; }
 
