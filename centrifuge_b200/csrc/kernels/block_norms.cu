@@ -45,11 +45,11 @@ struct NormRows {
 // sums are already under way.  Measured for 16384 x 2048 bf16 with a channel's gate (floor 41.1 us):
 // 44.1 us (46.4 without the request ahead, 86 with one row in registers for two warps, 54 with
 // R = 4 rows and eight columns a thread); 8192 x 4096: 46.1 us (51.5); 4096 x 8192: 50.9 us (61.1).
-template <typename TH, typename TX, int W, int NW, int NV, int R>
+template <typename TH, typename TX, int NW, int NV, int R>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_kernel(
     NormRows a, float eps, TX* __restrict__ y, TH* __restrict__ n, float* __restrict__ rstd_post,
     float* __restrict__ rstd_pre, int rows) {
-  constexpr int P = kPairs<W>;
+  constexpr int W = 8, P = W / 2;
   constexpr int kAhead = 148 * R;  // rows of the blocks in between, at one block an SM
   __shared__ float red[2][R * NW];
   const int team = NW == 1 ? blockIdx.x * 4 + warp_id() : blockIdx.x;
@@ -162,6 +162,61 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_kerne
       if (row0 + r < rows) store_f2<TH, W>(n + static_cast<long long>(row0 + r) * H + c, o);
     }
   }
+}
+
+// Rows of other widths and alignments: one row a team, a pair of columns at a time.
+template <typename TH, typename TX, int W, int NW, int NV>
+__global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_pairs_kernel(
+    NormRows a, float eps, TX* __restrict__ y, TH* __restrict__ n, float* __restrict__ rstd_post,
+    float* __restrict__ rstd_pre, int rows) {
+  constexpr int NT = NW * 32;
+  using C = PairCols<W, NT>;
+  __shared__ float red[2][NW];
+  const int row = NW == 1 ? blockIdx.x * 4 + warp_id() : blockIdx.x;
+  const int tid = NW == 1 ? lane_id() : threadIdx.x;
+  if (NW == 1 && row >= rows) return;
+  const int H = a.H;
+  const TH* h = static_cast<const TH*>(a.h) + row * a.ld_h;
+  const TX* x = static_cast<const TX*>(a.x) + row * a.ld_x;
+  const TH* gate = static_cast<const TH*>(a.gate);
+  if (a.gate_kind == kGateElement) gate += row * a.ld_gate;
+  const bool by_column = a.gate_kind == kGateChannel || a.gate_kind == kGateElement;
+  F2 hv[NV], xv[NV], s = f2(0.f);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    hv[k] = C::load(h, tid * W + k * 2 * NT, H);
+    xv[k] = C::load(x, tid * W + k * 2 * NT, H);
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k) s = fma2(hv[k], hv[k], s);
+  float ss = sum2(s);
+  team_sums<1, NW>(&ss, red[0]);
+  const float inv_h = 1.f / static_cast<float>(H);
+  const float r1 = rsqrtf(ss * inv_h + eps);
+  float scale = a.block_scale * r1;
+  if (a.gate_kind == kGateToken) scale *= static_cast<const float*>(a.gate)[row * a.ld_gate];
+  s = f2(0.f);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = tid * W + k * 2 * NT;
+    F2 v = hv[k] * C::load(static_cast<const TH*>(a.w_post), c, H);
+    if (by_column) v = v * C::load(gate, c, H);
+    xv[k] = fma2(v, f2(scale), xv[k] * f2(a.resid_scale));
+    s = fma2(xv[k], xv[k], s);
+    C::store(y + static_cast<long long>(row) * H, c, H, xv[k]);
+  }
+  if (tid == 0) rstd_post[row] = r1;
+  if (a.w_pre == nullptr) return;
+  ss = sum2(s);
+  team_sums<1, NW>(&ss, red[1]);
+  const float r2 = rsqrtf(ss * inv_h + eps);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = tid * W + k * 2 * NT;
+    C::store(n + static_cast<long long>(row) * H, c, H,
+             xv[k] * f2(r2) * C::load(static_cast<const TH*>(a.w_pre), c, H));
+  }
+  if (tid == 0) rstd_pre[row] = r2;
 }
 
 // ---------------------------------------------------------------- backward
@@ -368,13 +423,21 @@ int with_types(int type, int resid_type, F&& f) {
 using namespace cfb;
 
 namespace {
-template <typename TH, typename TX, int W, int NW, int NV, int R>
+template <typename TH, typename TX, int NW, int NV, int R>
 int launch_fwd(const NormRows& a, float eps, void* y, void* n, float* rstd_post, float* rstd_pre,
                int rows, cudaStream_t st) {
   const int teams = (rows + R - 1) / R;
-  const int threads = NW == 1 ? 128 : ((a.H + W * NV - 1) / (W * NV) + 31) / 32 * 32;
-  block_norms_fwd_kernel<TH, TX, W, NW, NV, R>
+  const int threads = NW == 1 ? 128 : ((a.H + 8 * NV - 1) / (8 * NV) + 31) / 32 * 32;
+  block_norms_fwd_kernel<TH, TX, NW, NV, R>
       <<<NW == 1 ? (teams + 3) / 4 : teams, threads, 0, st>>>(
+          a, eps, static_cast<TX*>(y), static_cast<TH*>(n), rstd_post, rstd_pre, rows);
+  return launch_status();
+}
+template <typename TH, typename TX, int W, int NW, int NV>
+int launch_fwd_pairs(const NormRows& a, float eps, void* y, void* n, float* rstd_post,
+                     float* rstd_pre, int rows, cudaStream_t st) {
+  block_norms_fwd_pairs_kernel<TH, TX, W, NW, NV>
+      <<<NW == 1 ? (rows + 3) / 4 : rows, NW == 1 ? 128 : NW * 32, 0, st>>>(
           a, eps, static_cast<TX*>(y), static_cast<TH*>(n), rstd_post, rstd_pre, rows);
   return launch_status();
 }
@@ -403,36 +466,38 @@ int cfb_block_norms_fwd(const CfbBlockNorms* p, float eps, void* y, void* n, flo
     using TH = typename decltype(th)::type;
     using TX = typename decltype(tx)::type;
     const int H = a.H;
-#define CFB_FWD(W, NW, NV, R) \
-  return launch_fwd<TH, TX, W, NW, NV, R>(a, eps, y, n, rstd_post, rstd_pre, rows, st)
+#define CFB_FWD(NW, NV, R) \
+  return launch_fwd<TH, TX, NW, NV, R>(a, eps, y, n, rstd_post, rstd_pre, rows, st)
     if (W == 8) {
       // Several rows a team pay while there are blocks enough, and where a row is 2 bytes an element
       // (an fp32 stream at 8190 x 4096: 63.2 us with one, 64.6 with two).
       if (rows >= 148 * 8 && sizeof(TX) == 2) {
-        if (H <= 256) CFB_FWD(8, 1, 1, 4);
-        if (H <= 512) CFB_FWD(8, 1, 2, 2);
-        if (H <= 1024) CFB_FWD(8, 4, 1, 4);
-        if (H <= 2048) CFB_FWD(8, 4, 2, 2);
-        if (H <= 4096) CFB_FWD(8, 8, 2, 2);
+        if (H <= 256) CFB_FWD(1, 1, 4);
+        if (H <= 512) CFB_FWD(1, 2, 2);
+        if (H <= 1024) CFB_FWD(4, 1, 4);
+        if (H <= 2048) CFB_FWD(4, 2, 2);
+        if (H <= 4096) CFB_FWD(8, 2, 2);
       }
-      if (H <= 256) CFB_FWD(8, 1, 1, 1);
-      if (H <= 512) CFB_FWD(8, 1, 2, 1);
-      if (H <= 1024) CFB_FWD(8, 4, 1, 1);
-      if (H <= 2048) CFB_FWD(8, 4, 2, 1);
-      if (H <= 4096) CFB_FWD(8, 8, 2, 1);
-      if (H <= 8192) CFB_FWD(8, 16, 2, 1);
-      CFB_FWD(8, 32, 2, 1);
+      if (H <= 256) CFB_FWD(1, 1, 1);
+      if (H <= 512) CFB_FWD(1, 2, 1);
+      if (H <= 1024) CFB_FWD(4, 1, 1);
+      if (H <= 2048) CFB_FWD(4, 2, 1);
+      if (H <= 4096) CFB_FWD(8, 2, 1);
+      if (H <= 8192) CFB_FWD(16, 2, 1);
+      CFB_FWD(32, 2, 1);
     }
-    if (W == 2) {
-      if (H <= 512) CFB_FWD(2, 1, 8, 1);
-      if (H <= 2048) CFB_FWD(2, 4, 8, 1);
-      if (H <= 8192) CFB_FWD(2, 16, 8, 1);
-      CFB_FWD(2, 32, 8, 1);
-    }
-    if (H <= 256) CFB_FWD(1, 1, 8, 1);
-    if (H <= 1024) CFB_FWD(1, 4, 8, 1);
-    if (H <= 4096) CFB_FWD(1, 16, 8, 1);
-    CFB_FWD(1, 32, 16, 1);
+#undef CFB_FWD
+#define CFB_FWD(NW, NV)                                                                          \
+  return W == 2 ? launch_fwd_pairs<TH, TX, 2, NW, NV>(a, eps, y, n, rstd_post, rstd_pre, rows, st) \
+                : launch_fwd_pairs<TH, TX, 1, NW, NV>(a, eps, y, n, rstd_post, rstd_pre, rows, st)
+    if (H <= 256) CFB_FWD(1, 4);
+    if (H <= 512) CFB_FWD(1, 8);
+    if (H <= 1024) CFB_FWD(4, 4);
+    if (H <= 2048) CFB_FWD(4, 8);
+    if (H <= 2560) CFB_FWD(8, 5);
+    if (H <= 4096) CFB_FWD(8, 8);
+    if (H <= 8192) CFB_FWD(16, 8);
+    CFB_FWD(32, 8);
 #undef CFB_FWD
   });
 }

@@ -125,53 +125,75 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   return r;
 }
 
-// The W elements of a pack as W / 2 pairs (one pair with a zero for W = 1), and back.
-template <int W>
-constexpr int kPairs = (W + 1) / 2;
-template <typename T, int W>
-__device__ __forceinline__ void unpack_f2(const Pack<T, W>& k, F2* f) {
-  if constexpr (W == 1) {
-    f[0] = f2(to_f32(k.v[0]), 0.f);
-  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+// The N elements of a pack (N even) as N / 2 pairs, and back.
+template <typename T, int N>
+__device__ __forceinline__ void unpack_f2(const Pack<T, N>& k, F2* f) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
     const uint32_t* u = reinterpret_cast<const uint32_t*>(&k);
 #pragma unroll
-    for (int i = 0; i < W / 2; ++i)
+    for (int i = 0; i < N / 2; ++i)
       f[i] = f2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
   } else {
 #pragma unroll
-    for (int i = 0; i < W / 2; ++i) f[i] = f2(to_f32(k.v[2 * i]), to_f32(k.v[2 * i + 1]));
+    for (int i = 0; i < N / 2; ++i) f[i] = f2(to_f32(k.v[2 * i]), to_f32(k.v[2 * i + 1]));
   }
 }
-template <typename T, int W>
-__device__ __forceinline__ void load_f2(const T* p, F2* f) {
-  unpack_f2<T, W>(load_pack<T, W>(p), f);
-}
-template <typename T, int W>
-__device__ __forceinline__ void store_f2(T* p, const F2* f) {
-  Pack<T, W> k;
-  if constexpr (W == 1) {
-    k.v[0] = from_f32<T>(halves(f[0]).x);
-  } else {
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> pack_f2(const F2* f) {
+  Pack<T, N> k;
 #pragma unroll
-    for (int i = 0; i < W / 2; ++i) {
-      const float2 t = halves(f[i]);
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        reinterpret_cast<uint32_t*>(&k)[i] = pack_bf16x2(t.x, t.y);
-      } else {
-        k.v[2 * i] = from_f32<T>(t.x);
-        k.v[2 * i + 1] = from_f32<T>(t.y);
-      }
+  for (int i = 0; i < N / 2; ++i) {
+    const float2 t = halves(f[i]);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      reinterpret_cast<uint32_t*>(&k)[i] = pack_bf16x2(t.x, t.y);
+    } else {
+      k.v[2 * i] = from_f32<T>(t.x);
+      k.v[2 * i + 1] = from_f32<T>(t.y);
     }
   }
-  store_pack<T, W>(p, k);
-}
-template <typename T, int W>
-__device__ __forceinline__ Pack<T, W> zero_pack() {
-  Pack<T, W> k;
-#pragma unroll
-  for (int i = 0; i < W; ++i) k.v[i] = from_f32<T>(0.f);
   return k;
 }
+template <typename T, int N>
+__device__ __forceinline__ void load_f2(const T* p, F2* f) {
+  unpack_f2<T, N>(load_pack<T, N>(p), f);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f2(T* p, const F2* f) {
+  store_pack<T, N>(p, pack_f2<T, N>(f));
+}
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> zero_pack() {
+  Pack<T, N> k;
+#pragma unroll
+  for (int i = 0; i < N; ++i) k.v[i] = from_f32<T>(0.f);
+  return k;
+}
+
+// Pairs of columns of rows that are no whole aligned groups of eight, for teams of NT threads:
+// neighbours (W = 2), or, where not even two elements are aligned (W = 1), the columns c and
+// c + NT, so that the arithmetic works on pairs all the same.  Pair k of thread t begins at column
+// t * W + k * 2 * NT.  Columns from H on are zeros, and are not stored.
+template <int W, int NT>
+struct PairCols {
+  template <typename T>
+  static __device__ __forceinline__ F2 load(const T* row, int c, int H) {
+    if constexpr (W == 1)
+      return f2(c < H ? to_f32(row[c]) : 0.f, c + NT < H ? to_f32(row[c + NT]) : 0.f);
+    F2 f = f2(0.f);
+    if (c < H) load_f2<T, 2>(row + c, &f);
+    return f;
+  }
+  template <typename T>
+  static __device__ __forceinline__ void store(T* row, int c, int H, F2 f) {
+    if constexpr (W == 1) {
+      const float2 t = halves(f);
+      if (c < H) row[c] = from_f32<T>(t.x);
+      if (c + NT < H) row[c + NT] = from_f32<T>(t.y);
+    } else if (c < H) {
+      store_f2<T, 2>(row + c, &f);
+    }
+  }
+};
 
 // ---------------------------------------------------------------- sums of several rows
 // v[r], summed over the warp, for R rows at once: each exchange halves the number of rows that a
