@@ -18,6 +18,7 @@
 // The gate is absent, one value for each channel [H], for each token [T, 1] (fp32), or for each
 // element [T, H].
 #include "row_types.cuh"
+#include <cstdlib>
 
 namespace cfb {
 
@@ -184,8 +185,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_pairs
   F2 hv[NV], xv[NV], s = f2(0.f);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    hv[k] = C::load(h, tid * W + k * 2 * NT, H);
-    xv[k] = C::load(x, tid * W + k * 2 * NT, H);
+    hv[k] = C::load(h, C::column(tid, k), H);
+    xv[k] = C::load(x, C::column(tid, k), H);
   }
 #pragma unroll
   for (int k = 0; k < NV; ++k) s = fma2(hv[k], hv[k], s);
@@ -198,12 +199,12 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_pairs
   s = f2(0.f);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = tid * W + k * 2 * NT;
+    const int c = C::column(tid, k);
     F2 v = hv[k] * C::load(static_cast<const TH*>(a.w_post), c, H);
     if (by_column) v = v * C::load(gate, c, H);
     xv[k] = fma2(v, f2(scale), xv[k] * f2(a.resid_scale));
     s = fma2(xv[k], xv[k], s);
-    C::store(y + static_cast<long long>(row) * H, c, H, xv[k]);
+    C::store(y + static_cast<long long>(row) * H, c, H, &xv[k]);
   }
   if (tid == 0) rstd_post[row] = r1;
   if (a.w_pre == nullptr) return;
@@ -212,199 +213,265 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_pairs
   const float r2 = rsqrtf(ss * inv_h + eps);
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
-    const int c = tid * W + k * 2 * NT;
-    C::store(n + static_cast<long long>(row) * H, c, H,
-             xv[k] * f2(r2) * C::load(static_cast<const TH*>(a.w_pre), c, H));
+    const int c = C::column(tid, k);
+    const F2 v = xv[k] * f2(r2) * C::load(static_cast<const TH*>(a.w_pre), c, H);
+    C::store(n + static_cast<long long>(row) * H, c, H, &v);
   }
   if (tid == 0) rstd_pre[row] = r2;
 }
 
 // ---------------------------------------------------------------- backward
-// Sum of v over the block.  One barrier: the next call takes another `red`, and comes back to this
-// one only after a further barrier.
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = warp_add(v);
-  const int warps = blockDim.x >> 5;
-  if (warps == 1) return v;
-  if (lane_id() == 0) red[warp_id()] = v;
-  __syncthreads();
-  float s = lane_id() < warps ? red[lane_id()] : 0.f;
-  return warp_add(s);
-}
-
-// One block walks the rows blockIdx.x, + gridDim.x, ...; each thread owns NV groups of W columns of
-// every row and keeps the column sums of the weights' gradients in registers:
+// Blocks walk the rows, R at a time; a team of NW warps (the block, or, where NW < 8, one of 8 / NW
+// in it) has a row, and each thread the same NV groups of columns of every row, whose sums for the
+// weights' gradients it keeps in registers:
 //   part[block][0] = sum dn y r2,  part[block][1] = sum b dY h r1 (times the token's or element's
 // gate; a channel's gate is applied once, when the sums are joined).
-template <typename TH, typename TX, int W, int NV>
-__global__ void __launch_bounds__(1024) block_norms_bwd_kernel(
+// With p = dn y and q = dY h the row sums and the column sums share their products.  While a block
+// works, the rows of its next turn are on their way to the L2 cache.
+template <typename C, typename TH, typename TX, int NW, int NV, int R>
+__global__ void __launch_bounds__(NW < 8 ? 256 : NW * 32) block_norms_bwd_kernel(
     NormRows a, const TX* __restrict__ dy, long long ld_dy, const TH* __restrict__ dn,
     long long ld_dn, const float* __restrict__ rstd_post, const float* __restrict__ rstd_pre,
     const int* __restrict__ row_ids, long long n_rows, TX* __restrict__ dx, TH* __restrict__ dh,
     void* __restrict__ dgate, float* __restrict__ part, int rows, int* err) {
-  __shared__ float red[4][32];
-  const int H = a.H, tid = threadIdx.x, nt = blockDim.x;
+  constexpr int P = C::P;
+  constexpr int kTeams = NW < 8 ? 8 / NW : 1;
+  static_assert(!std::is_same<C, WideCols>::value || kTeams == 1 || NV == 1,
+                "wide columns step by the block");
+  __shared__ float red[kTeams][2][R * NW];
+  const int H = a.H;
+  const int team = kTeams > 1 ? warp_id() / NW : 0;
+  const int tid = kTeams > 1 ? threadIdx.x % (NW * 32) : threadIdx.x;
+  const int named = kTeams > 1 ? team : -1;
   const bool pre = a.w_pre != nullptr;
   const float inv_h = 1.f / static_cast<float>(H);
-  float s_pre[NV][W], s_post[NV][W];
+  F2 s_pre[NV][P], s_post[NV][P];
 #pragma unroll
   for (int k = 0; k < NV; ++k)
 #pragma unroll
-    for (int i = 0; i < W; ++i) s_pre[k][i] = s_post[k][i] = 0.f;
+    for (int i = 0; i < P; ++i) s_pre[k][i] = s_post[k][i] = f2(0.f);
 
-  int turn = 0;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-    const long long src = row_ids ? row_ids[r] : r;
-    const long long out = static_cast<long long>(r) * H;
-    if (!index_in(src, n_rows, err)) {  // out-of-range row id: zero gradients
-      float z[W];
+  const int step = gridDim.x * kTeams * R;
+  for (int r0 = (blockIdx.x * kTeams + team) * R; r0 < rows; r0 += step) {
+    if (tid < R && r0 + step + tid < rows) {  // the next turn's rows
+      const long long r = r0 + step + tid;
+      const long long src = row_ids ? row_ids[r] : r;
+      if (src >= 0 && src < n_rows) {
+        prefetch_l2(static_cast<const TH*>(a.h) + src * a.ld_h, H * static_cast<int>(sizeof(TH)));
+        if (pre) {
+          prefetch_l2(static_cast<const TX*>(a.x) + src * a.ld_x, H * static_cast<int>(sizeof(TX)));
+          prefetch_l2(dn + r * ld_dn, H * static_cast<int>(sizeof(TH)));
+        }
+        if (dy) prefetch_l2(dy + r * ld_dy, H * static_cast<int>(sizeof(TX)));
+      }
+    }
+    long long src[R];
+    int width[R];  // H, or 0 where there is no row: everything of it is zero
 #pragma unroll
-      for (int i = 0; i < W; ++i) z[i] = 0.f;
+    for (int r = 0; r < R; ++r) {
+      src[r] = 0;
+      width[r] = 0;
+      if (r0 + r < rows) {
+        src[r] = row_ids ? row_ids[r0 + r] : r0 + r;
+        if (index_in(src[r], n_rows, err)) width[r] = H; else src[r] = 0;
+      }
+    }
+    typename C::template Raw<TH> hp[NV][R];
+    typename C::template Raw<TX> yp[NV][R];
+    F2 d[NV][R][P];
+    float dot[R];
+    // dY without the part along y, and the sums for it
+#pragma unroll
+    for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (tid + k * nt) * W;
-        if (c < H) {
-          store_f32<TX, W>(dx + out + c, z);
-          store_f32<TH, W>(dh + out + c, z);
-          if (a.gate_kind == kGateElement) store_f32<TH, W>(static_cast<TH*>(dgate) + out + c, z);
-        }
-      }
-      if (a.gate_kind == kGateToken && tid == 0) static_cast<float*>(dgate)[r] = 0.f;
-      continue;
-    }
-    const TH* h = static_cast<const TH*>(a.h) + src * a.ld_h;
-    float d[NV][W], hv[NV][W];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (tid + k * nt) * W;
-      if (c < H) {
-        load_f32<TH, W>(h + c, hv[k]);
+        const int c = C::column(tid, k);
+        hp[k][r] = C::load(static_cast<const TH*>(a.h) + src[r] * a.ld_h, c, width[r]);
+        if (pre) yp[k][r] = C::load(static_cast<const TX*>(a.x) + src[r] * a.ld_x, c, width[r]);
         if (dy) {
-          load_f32<TX, W>(dy + r * ld_dy + c, d[k]);
+          C::template unpack<TX>(C::load(dy + (r0 + r) * ld_dy, c, width[r]), d[k][r]);
         } else {
 #pragma unroll
-          for (int i = 0; i < W; ++i) d[k][i] = 0.f;
+          for (int i = 0; i < P; ++i) d[k][r][i] = f2(0.f);
         }
       }
-    }
     if (pre) {
-      const TX* y = static_cast<const TX*>(a.x) + src * a.ld_x;
-      const float r2 = rstd_pre[src];
-      float yv[NV][W];
-      float dot = 0.f;
+      F2 sum[R];
+      float r2[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        sum[r] = f2(0.f);
+        r2[r] = width[r] ? rstd_pre[src[r]] : 0.f;
+      }
 #pragma unroll
       for (int k = 0; k < NV; ++k) {
-        const int c = (tid + k * nt) * W;
-        if (c < H) {
-          float q[W], w[W];
-          load_f32<TX, W>(y + c, yv[k]);
-          load_f32<TH, W>(dn + r * ld_dn + c, q);
-          load_f32<TH, W>(static_cast<const TH*>(a.w_pre) + c, w);
+        const int c = C::column(tid, k);
+        F2 w[P];
+        C::template unpack<TH>(C::load(static_cast<const TH*>(a.w_pre), c, H), w);
 #pragma unroll
-          for (int i = 0; i < W; ++i) {
-            s_pre[k][i] += q[i] * (yv[k][i] * r2);
-            w[i] *= q[i];
-            dot += w[i] * yv[k][i];
-            d[k][i] += r2 * w[i];
+        for (int r = 0; r < R; ++r) {
+          F2 g[P], y[P];
+          C::template unpack<TH>(C::load(dn + (r0 + r) * ld_dn, c, width[r]), g);
+          C::template unpack<TX>(yp[k][r], y);
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            const F2 p = g[i] * y[i];
+            s_pre[k][i] = fma2(p, f2(r2[r]), s_pre[k][i]);
+            sum[r] = fma2(p, w[i], sum[r]);
+            d[k][r][i] = fma2(g[i] * w[i], f2(r2[r]), d[k][r][i]);
           }
         }
       }
-      const float coef = block_sum(dot, red[turn]) * inv_h * r2 * r2 * r2;
+#pragma unroll
+      for (int r = 0; r < R; ++r) dot[r] = sum2(sum[r]);
+      team_sums<R, NW>(dot, red[team][0], named);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float coef = -dot[r] * inv_h * r2[r] * r2[r] * r2[r];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          F2 y[P];
+          C::template unpack<TX>(yp[k][r], y);
+#pragma unroll
+          for (int i = 0; i < P; ++i) d[k][r][i] = fma2(y[i], f2(coef), d[k][r][i]);
+        }
+      }
+    }
+    float r1[R], tg[R];
+    F2 sum[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      sum[r] = f2(0.f);
+      r1[r] = width[r] ? rstd_post[src[r]] : 0.f;
+      tg[r] = a.gate_kind == kGateToken && width[r]
+                  ? static_cast<const float*>(a.gate)[src[r] * a.ld_gate] : 1.f;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = C::column(tid, k);
+      F2 w[P];
+      C::template unpack<TH>(C::load(static_cast<const TH*>(a.w_post), c, H), w);
+      if (a.gate_kind == kGateChannel) {
+        F2 g[P];
+        C::template unpack<TH>(C::load(static_cast<const TH*>(a.gate), c, H), g);
+#pragma unroll
+        for (int i = 0; i < P; ++i) w[i] = w[i] * g[i];
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const long long out = static_cast<long long>(r0 + r) * H;
+        const int live = r0 + r < rows ? H : 0;  // rows without a source are written as zeros
+        F2 e[P], h[P];
+        C::template unpack<TH>(hp[k][r], h);
+#pragma unroll
+        for (int i = 0; i < P; ++i) e[i] = d[k][r][i] * f2(a.resid_scale);
+        C::store(dx + out, c, live, e);
+        const float br = a.block_scale * r1[r];
+        if (a.gate_kind == kGateElement) {
+          F2 g[P];
+          C::template unpack<TH>(
+              C::load(static_cast<const TH*>(a.gate) + src[r] * a.ld_gate, c, width[r]), g);
+#pragma unroll
+          for (int i = 0; i < P; ++i) e[i] = d[k][r][i] * h[i] * f2(br) * w[i];
+          C::store(static_cast<TH*>(dgate) + out, c, live, e);
+#pragma unroll
+          for (int i = 0; i < P; ++i) d[k][r][i] = d[k][r][i] * g[i];
+        }
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const F2 q = d[k][r][i] * h[i];
+          s_post[k][i] = fma2(q, f2(br * tg[r]), s_post[k][i]);
+          sum[r] = fma2(q, w[i], sum[r]);
+          d[k][r][i] = d[k][r][i] * w[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) dot[r] = sum2(sum[r]);
+    team_sums<R, NW>(dot, red[team][1], named);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const long long out = static_cast<long long>(r0 + r) * H;
+      const int live = r0 + r < rows ? H : 0;
+      const float br = a.block_scale * r1[r];
+      if (a.gate_kind == kGateToken && tid == 0 && live)
+        static_cast<float*>(dgate)[r0 + r] = dot[r] * br;
+      const float coef = -dot[r] * inv_h * r1[r] * r1[r];
+      const F2 scale = f2(br * tg[r]);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        F2 h[P];
+        C::template unpack<TH>(hp[k][r], h);
+#pragma unroll
+        for (int i = 0; i < P; ++i) h[i] = fma2(h[i], f2(coef), d[k][r][i]) * scale;
+        C::store(dh + out, C::column(tid, k), live, h);
+      }
+    }
+    // without the norm before the next block one barrier a turn is left: red[1] would be written
+    // again before the slowest warp has read it
+    if (!pre && NW > 1) {
+      if (kTeams > 1)
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(NW * 32) : "memory");
+      else
+        __syncthreads();
+    }
+  }
+
+  float* mine = part + 2ll * blockIdx.x * H;
+  if constexpr (kTeams > 1) {  // the teams' sums, in the order of the teams
+    extern __shared__ float sums[];  // [kTeams][H]
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      if (which == 0 && !pre) continue;
+      __syncthreads();
 #pragma unroll
       for (int k = 0; k < NV; ++k)
+        C::put(sums + team * H, C::column(tid, k), H, which ? s_post[k] : s_pre[k]);
+      __syncthreads();
+      for (int c = threadIdx.x; c < H; c += 256) {
+        float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) d[k][i] -= yv[k][i] * coef;
-    }
-    const float r1 = rstd_post[src];
-    const float tg = a.gate_kind == kGateToken
-                         ? static_cast<const float*>(a.gate)[src * a.ld_gate] : 1.f;
-    const TH* gate = static_cast<const TH*>(a.gate);
-    if (a.gate_kind == kGateElement) gate += src * a.ld_gate;
-    float v[NV][W];
-    float dot = 0.f;
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      const int c = (tid + k * nt) * W;
-      if (c < H) {
-        float w[W], g[W], e[W];
-        load_f32<TH, W>(static_cast<const TH*>(a.w_post) + c, w);
-        const bool by_column = a.gate_kind == kGateChannel || a.gate_kind == kGateElement;
-        if (by_column) load_f32<TH, W>(gate + c, g);
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          e[i] = a.resid_scale * d[k][i];
-          const float t = a.block_scale * d[k][i];
-          const float th = t * (hv[k][i] * r1);
-          v[k][i] = t * w[i];  // without the token's gate
-          if (a.gate_kind == kGateElement) {
-            s_post[k][i] += th * g[i];
-            w[i] *= th;  // dgate of the element
-          } else {
-            s_post[k][i] += th * tg;
-          }
-          if (by_column) v[k][i] *= g[i];
-          dot += v[k][i] * hv[k][i];
-        }
-        store_f32<TX, W>(dx + out + c, e);
-        if (a.gate_kind == kGateElement) store_f32<TH, W>(static_cast<TH*>(dgate) + out + c, w);
+        for (int t = 0; t < kTeams; ++t) s += sums[t * H + c];
+        mine[which * H + c] = s;
       }
     }
-    dot = block_sum(dot, red[turn + 1]);
-    if (a.gate_kind == kGateToken && tid == 0) static_cast<float*>(dgate)[r] = dot * r1;
-    const float coef = dot * inv_h * r1 * r1;
-    const float scale = tg * r1;
+  } else {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      const int c = (tid + k * nt) * W;
-      if (c < H) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[k][i] = scale * (v[k][i] - hv[k][i] * coef);
-        store_f32<TH, W>(dh + out + c, v[k]);
-      }
-    }
-    turn ^= 2;
-  }
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (tid + k * nt) * W;
-    if (c < H) {
-      float* p = part + 2ll * blockIdx.x * H + c;
-      if (pre) store_f32<float, W>(p, s_pre[k]);
-      store_f32<float, W>(p + H, s_post[k]);
+      if (pre) C::store(mine, C::column(tid, k), H, s_pre[k]);
+      C::store(mine + H, C::column(tid, k), H, s_post[k]);
     }
   }
 }
 
-// dw_pre, dw_post and a channel gate's gradient from the blocks' column sums, in block order.
-// Block: 32 columns x 8 slices of the blocks.
+// dw_pre (blockIdx.y = 0), dw_post and a channel gate's gradient (1) from the blocks' column sums,
+// in block order.  Block: 32 columns x 32 slices of the blocks.
 template <typename TH>
-__global__ void __launch_bounds__(256) block_norms_join_kernel(
+__global__ void __launch_bounds__(1024) block_norms_join_kernel(
     const float* __restrict__ part, int blocks, int H, const TH* __restrict__ w_post,
     const TH* __restrict__ gate, float* __restrict__ dw_pre, float* __restrict__ dw_post,
     float* __restrict__ dgate, int add) {
-  __shared__ float red[2][8][33];
+  __shared__ float red[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
-  float s0 = 0.f, s1 = 0.f;
-  if (c < H)
-    for (int b = ry; b < blocks; b += 8) {
-      if (dw_pre) s0 += part[2ll * b * H + c];
-      s1 += part[(2ll * b + 1) * H + c];
-    }
-  red[0][ry][cx] = s0;
-  red[1][ry][cx] = s1;
-  __syncthreads();
-  if (ry != 0 || c >= H) return;
-  s0 = s1 = 0.f;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    s0 += red[0][k][cx];
-    s1 += red[1][k][cx];
+  const int which = blockIdx.y;
+  if (which == 0 && dw_pre == nullptr) return;
+  float s = 0.f;
+  if (c < H) {
+#pragma unroll 8
+    for (int b = ry; b < blocks; b += 32) s += part[(2ll * b + which) * H + c];
   }
-  if (dw_pre) dw_pre[c] = (add ? dw_pre[c] : 0.f) + s0;
-  const float g = gate ? to_f32(gate[c]) : 1.f;
-  dw_post[c] = (add ? dw_post[c] : 0.f) + s1 * g;
-  if (dgate) dgate[c] = (add ? dgate[c] : 0.f) + s1 * to_f32(w_post[c]);
+  red[ry][cx] = s;
+  __syncthreads();
+  s = warp_add(red[cx][ry]);  // warp ry: the 32 slices of column blockIdx.x * 32 + ry
+  const int col = blockIdx.x * 32 + ry;
+  if (cx != 0 || col >= H) return;
+  if (which == 0) {
+    dw_pre[col] = (add ? dw_pre[col] : 0.f) + s;
+    return;
+  }
+  dw_post[col] = (add ? dw_post[col] : 0.f) + (gate ? s * to_f32(gate[col]) : s);
+  if (dgate) dgate[col] = (add ? dgate[col] : 0.f) + s * to_f32(w_post[col]);
 }
 
 // f(TypeTag<TH>, TypeTag<TX>): the residual stream has the block's type or fp32.
@@ -507,6 +574,49 @@ long long cfb_block_norms_bwd_workspace(int rows, int H) {
   return 4ll * 2 * blocks * H;  // bytes
 }
 
+namespace {
+struct BwdArgs {
+  NormRows a;
+  const void* dy;
+  long long ld_dy;
+  const void* dn;
+  long long ld_dn;
+  const float *rstd_post, *rstd_pre;
+  const int* row_ids;
+  long long n_rows;
+  void *dx, *dh, *dgate;
+  float* part;
+  int rows;
+  int* err;
+};
+// Launches the kernel and returns the number of its blocks, or a negative status.
+template <typename C, typename TH, typename TX, int NW, int NV, int R>
+int launch_bwd(const BwdArgs& b, cudaStream_t st) {
+  constexpr int kTeams = NW < 8 ? 8 / NW : 1;
+  auto* kernel = block_norms_bwd_kernel<C, TH, TX, NW, NV, R>;
+  int threads = NW < 8 ? 256 : NW * 32;
+  if (std::is_same<C, WideCols>::value && NW >= 8)  // no more warps than the row needs
+    threads = ((b.a.H + 8 * NV - 1) / (8 * NV) + 31) / 32 * 32;
+  const int smem = kTeams > 1 ? kTeams * b.a.H * 4 : 0;
+  static int per_sm = 0;  // resident blocks of this kernel: the same on every device of this type
+  if (per_sm == 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, NW < 8 ? 256 : NW * 32,
+                                                      kTeams > 1 ? 16384 : 0) != cudaSuccess)
+      return -3;
+    per_sm = n < 1 ? 1 : n > 8 ? 8 : n;
+  }
+  const int turns = (b.rows + R * kTeams - 1) / (R * kTeams);
+  const int blocks = turns < 148 * per_sm ? turns : 148 * per_sm;
+  kernel<<<blocks, threads, smem, st>>>(
+      b.a, static_cast<const TX*>(b.dy), b.ld_dy, static_cast<const TH*>(b.dn), b.ld_dn,
+      b.rstd_post, b.rstd_pre, b.row_ids, b.n_rows, static_cast<TX*>(b.dx),
+      static_cast<TH*>(b.dh), b.dgate, b.part, b.rows, b.err);
+  const int rc = launch_status();
+  return rc ? rc : blocks;
+}
+}  // namespace
+
 int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy, const void* dn,
                         long long ld_dn, const float* rstd_post, const float* rstd_pre,
                         const int* row_ids, long long n_rows, void* dx, void* dh, void* dgate,
@@ -518,39 +628,66 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
   if (H == 0) return 0;
   if (H > kBlockNormsMaxH) return -11;
   const bool by_row = a.gate_kind == kGateToken || a.gate_kind == kGateElement;
-  const bool wide = H % 8 == 0 && rows_of_8(a.h, a.ld_h, p->type) &&
-                    rows_of_8(a.x, a.ld_x, p->resid_type) && rows_of_8(dy, ld_dy, p->resid_type) &&
-                    rows_of_8(dn, ld_dn, p->type) && rows_of_8(a.w_post, 0, p->type) &&
-                    rows_of_8(a.w_pre, 0, p->type) && rows_of_8(dx, H, p->resid_type) &&
-                    rows_of_8(dh, H, p->type) &&
-                    (a.gate_kind == kGateNone || a.gate_kind == kGateToken ||
-                     rows_of_8(a.gate, a.ld_gate, p->type)) &&
-                    (a.gate_kind != kGateElement || rows_of_8(dgate, H, p->type));
+  const int W = widest([&](int w) {
+    return H % w == 0 && rows_of(w, a.h, a.ld_h, p->type) &&
+           rows_of(w, a.x, a.ld_x, p->resid_type) && rows_of(w, dy, ld_dy, p->resid_type) &&
+           rows_of(w, dn, ld_dn, p->type) && rows_of(w, a.w_post, 0, p->type) &&
+           rows_of(w, a.w_pre, 0, p->type) && rows_of(w, dx, H, p->resid_type) &&
+           rows_of(w, dh, H, p->type) &&
+           (a.gate_kind == kGateNone || a.gate_kind == kGateToken ||
+            rows_of(w, a.gate, a.ld_gate, p->type)) &&
+           (a.gate_kind != kGateElement || rows_of(w, dgate, H, p->type));
+  });
   float* part = static_cast<float*>(work);
+  const BwdArgs b = {a, dy, ld_dy, dn, ld_dn, rstd_post, rstd_pre, row_ids, n_rows, dx, dh,
+                     by_row ? dgate : nullptr, part, rows, err};
   return with_types(p->type, p->resid_type, [&](auto th, auto tx) {
     using TH = typename decltype(th)::type;
     using TX = typename decltype(tx)::type;
+    const auto launch = [&]() -> int {
+#define CFB_BWD(NW, NV, R) return launch_bwd<WideCols, TH, TX, NW, NV, R>(b, st)
+      if (W == 8) {
+        const int ex = getenv("CFB_EXP") ? atoi(getenv("CFB_EXP")) : 0;
+        if (ex == 1) {
+        if (H <= 256) CFB_BWD(1, 1, 2);
+        if (H <= 512) CFB_BWD(2, 1, 2);
+        if (H <= 1024) CFB_BWD(4, 1, 2);
+        if (H <= 2048) CFB_BWD(8, 1, 2);
+        if (H <= 4096) CFB_BWD(16, 1, 2);
+        }
+        if (H <= 256) CFB_BWD(1, 1, 1);
+        if (H <= 512) CFB_BWD(2, 1, 1);
+        if (H <= 1024) CFB_BWD(4, 1, 1);
+        if (H <= 2048) CFB_BWD(8, 1, 1);
+        if (ex == 2) {
+        if (H <= 4096) CFB_BWD(8, 2, 1);
+        if (H <= 8192) CFB_BWD(16, 2, 1);
+        }
+        if (H <= 4096) CFB_BWD(16, 1, 1);
+        if (H <= 8192) CFB_BWD(32, 1, 1);
+        CFB_BWD(32, 2, 1);
+      }
+#undef CFB_BWD
+#define CFB_BWD(NW, NV)                                                                    \
+  return W == 2 ? launch_bwd<PairCols<2, NW * 32>, TH, TX, NW, NV, 1>(b, st)               \
+                : launch_bwd<PairCols<1, NW * 32>, TH, TX, NW, NV, 1>(b, st)
+      if (H <= 256) CFB_BWD(1, 4);
+      if (H <= 1024) CFB_BWD(4, 4);
+      if (H <= 2048) CFB_BWD(8, 4);
+      if (H <= 4096) CFB_BWD(16, 4);
+      if (H <= 8192) CFB_BWD(32, 4);
+      CFB_BWD(32, 8);
+#undef CFB_BWD
+    };
     int blocks = 0;
     if (rows > 0) {
-      const int W = wide ? 8 : 1;
-      const int nv = wide ? (H <= 8192 ? 1 : 2) : (H <= 4096 ? 4 : 16);
-      const int threads = ((H + W * nv - 1) / (W * nv) + 31) / 32 * 32;
-      auto* kernel = wide ? (nv == 1 ? block_norms_bwd_kernel<TH, TX, 8, 1>
-                                     : block_norms_bwd_kernel<TH, TX, 8, 2>)
-                          : (nv == 4 ? block_norms_bwd_kernel<TH, TX, 1, 4>
-                                     : block_norms_bwd_kernel<TH, TX, 1, 16>);
-      const int per_sm = threads >= 1024 ? 1 : threads >= 512 ? 2 : threads >= 256 ? 4 : 8;
-      blocks = rows < 148 * per_sm ? rows : 148 * per_sm;
-      kernel<<<blocks, threads, 0, st>>>(
-          a, static_cast<const TX*>(dy), ld_dy, static_cast<const TH*>(dn), ld_dn, rstd_post,
-          rstd_pre, row_ids, n_rows, static_cast<TX*>(dx), static_cast<TH*>(dh),
-          by_row ? dgate : nullptr, part, rows, err);
-      if (const int rc = launch_status()) return rc;
+      blocks = launch();
+      if (blocks < 0) return blocks;
     } else if (add) {
       return 0;
     }
     const bool channel = a.gate_kind == kGateChannel;
-    block_norms_join_kernel<TH><<<(H + 31) / 32, 256, 0, st>>>(
+    block_norms_join_kernel<TH><<<dim3((H + 31) / 32, 2), 1024, 0, st>>>(
         part, blocks, H, static_cast<const TH*>(a.w_post),
         channel ? static_cast<const TH*>(a.gate) : nullptr, a.w_pre ? dw_pre : nullptr, dw_post,
         channel ? static_cast<float*>(dgate) : nullptr, add);

@@ -169,12 +169,43 @@ __device__ __forceinline__ Pack<T, N> zero_pack() {
   return k;
 }
 
-// Pairs of columns of rows that are no whole aligned groups of eight, for teams of NT threads:
-// neighbours (W = 2), or, where not even two elements are aligned (W = 1), the columns c and
-// c + NT, so that the arithmetic works on pairs all the same.  Pair k of thread t begins at column
-// t * W + k * 2 * NT.  Columns from H on are zeros, and are not stored.
+// How a team of threads walks the columns of a row: group k of thread t begins at column(t, k) and
+// is 2 P columns wide.  Columns from H on are zeros, and are not stored.
+//
+// WideCols: eight neighbours, for rows of whole aligned groups of eight.
+struct WideCols {
+  static constexpr int P = 4;
+  template <typename T>
+  using Raw = Pack<T, 8>;
+  static __device__ __forceinline__ int column(int t, int k) { return (t + k * blockDim.x) * 8; }
+  template <typename T>
+  static __device__ __forceinline__ Raw<T> load(const T* row, int c, int H) {
+    return c < H ? load_pack<T, 8>(row + c) : zero_pack<T, 8>();
+  }
+  template <typename T>
+  static __device__ __forceinline__ void unpack(const Raw<T>& k, F2* f) {
+    unpack_f2<T, 8>(k, f);
+  }
+  template <typename T>
+  static __device__ __forceinline__ void store(T* row, int c, int H, const F2* f) {
+    if (c < H) store_f2<T, 8>(row + c, f);
+  }
+  // a row in shared memory (the accesses above are of global memory)
+  static __device__ __forceinline__ void put(float* row, int c, int H, const F2* f) {
+    if (c >= H) return;
+#pragma unroll
+    for (int i = 0; i < P; ++i) reinterpret_cast<float2*>(row + c)[i] = halves(f[i]);
+  }
+};
+// PairCols: one pair, for teams of NT threads and rows of any width and alignment: neighbours
+// (W = 2), or, where not even two elements are aligned (W = 1), the columns c and c + NT, so that
+// the arithmetic works on pairs all the same.
 template <int W, int NT>
 struct PairCols {
+  static constexpr int P = 1;
+  template <typename T>
+  using Raw = F2;
+  static __device__ __forceinline__ int column(int t, int k) { return t * W + k * 2 * NT; }
   template <typename T>
   static __device__ __forceinline__ F2 load(const T* row, int c, int H) {
     if constexpr (W == 1)
@@ -184,14 +215,21 @@ struct PairCols {
     return f;
   }
   template <typename T>
-  static __device__ __forceinline__ void store(T* row, int c, int H, F2 f) {
+  static __device__ __forceinline__ void unpack(const F2& k, F2* f) {
+    f[0] = k;
+  }
+  template <typename T>
+  static __device__ __forceinline__ void store(T* row, int c, int H, const F2* f) {
     if constexpr (W == 1) {
-      const float2 t = halves(f);
+      const float2 t = halves(f[0]);
       if (c < H) row[c] = from_f32<T>(t.x);
       if (c + NT < H) row[c + NT] = from_f32<T>(t.y);
     } else if (c < H) {
-      store_f2<T, 2>(row + c, &f);
+      store_f2<T, 2>(row + c, f);
     }
+  }
+  static __device__ __forceinline__ void put(float* row, int c, int H, const F2* f) {
+    store(row, c, H, f);
   }
 };
 
@@ -218,19 +256,24 @@ __device__ __forceinline__ float warp_sums(float* v) {
   for (; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
   return s;
 }
-// The same over a team of up to NW warps (a power of two, R * NW <= 32), which is the block: every
-// thread gets all R sums.  red: R * NW floats of shared memory; the caller sees to it that a barrier
-// lies between two uses of it.
+// The same over a team of up to NW warps (a power of two, R * NW <= 32): every thread of the team
+// gets all R sums.  red: R * NW floats of shared memory; the caller sees to it that a barrier lies
+// between two uses of it.  The team is the block, or, with its number `team` >= 0 in the block,
+// exactly NW warps that meet at the block's named barrier 1 + team.
 template <int R, int NW>
-__device__ __forceinline__ void team_sums(float* v, float* red) {
+__device__ __forceinline__ void team_sums(float* v, float* red, int team = -1) {
   constexpr int kShift = R == 4 ? 3 : R == 2 ? 4 : 5;  // lanes of one row after warp_sums
   const int lane = lane_id();
   float s = warp_sums<R>(v);
   if constexpr (NW > 1) {
-    if ((lane & ((1 << kShift) - 1)) == 0) red[(lane >> kShift) * NW + warp_id()] = s;
-    __syncthreads();
+    const int wp = team >= 0 ? warp_id() % NW : warp_id();
+    if ((lane & ((1 << kShift) - 1)) == 0) red[(lane >> kShift) * NW + wp] = s;
+    if (team >= 0)
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(NW * 32) : "memory");
+    else
+      __syncthreads();
     const int at = lane % (R * NW);
-    s = at % NW < static_cast<int>(blockDim.x >> 5) ? red[at] : 0.f;
+    s = team >= 0 || at % NW < static_cast<int>(blockDim.x >> 5) ? red[at] : 0.f;
 #pragma unroll
     for (int o = NW / 2; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
 #pragma unroll
