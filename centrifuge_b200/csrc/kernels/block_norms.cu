@@ -444,6 +444,297 @@ __global__ void __launch_bounds__(NW < 8 ? 256 : NW * 32) block_norms_bwd_kernel
   }
 }
 
+// The same for rows of whole aligned groups of eight, of which two at least fit in shared memory:
+// each team keeps a ring of kStages rows (h, dn, y, dy) there, filled by bulk copies that its first
+// thread issues, so that the loads of the next rows run while a row waits for its sums.  A row's
+// stage is free again once every thread has its columns in registers, which the barrier of the
+// row's first sum tells.  The weights (the one behind the block times a channel's gate) lie in shared
+// memory in fp32, in two planes of the four low and the four high columns of each group of eight,
+// so that a thread's two 16-byte reads have no bank conflicts.
+template <typename TH, typename TX, int NW, int NV>
+__global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 ? 16 / NW : 1)
+    block_norms_bwd_ring_kernel(NormRows a, const TX* __restrict__ dy, long long ld_dy,
+                                const TH* __restrict__ dn, long long ld_dn,
+                                const float* __restrict__ rstd_post,
+                                const float* __restrict__ rstd_pre,
+                                const int* __restrict__ row_ids, long long n_rows,
+                                TX* __restrict__ dx, TH* __restrict__ dh,
+                                void* __restrict__ dgate, float* __restrict__ part, int rows,
+                                int stages, int* err) {
+  constexpr int P = 4, NT = NW * 32;
+  constexpr int kTeams = NW < 4 ? 4 / NW : 1;
+  constexpr int kMaxStages = 4;
+  extern __shared__ __align__(128) uint8_t ring_all[];
+  __shared__ uint64_t full[kTeams][kMaxStages];
+  __shared__ float red[kTeams][3][NW];
+  __shared__ int abort_flag;
+  const int H = a.H;
+  const int team = threadIdx.x / NT, tid = threadIdx.x % NT;
+  const bool pre = a.w_pre != nullptr;
+  const float inv_h = 1.f / static_cast<float>(H);
+  // a stage: h, dn, y, dy
+  const int at_dn = H * static_cast<int>(sizeof(TH)), at_y = 2 * at_dn;
+  const int at_dy = at_y + H * static_cast<int>(sizeof(TX));
+  const int stage_bytes = at_dy + H * static_cast<int>(sizeof(TX));
+  uint8_t* ring = ring_all + static_cast<size_t>(team) * stages * stage_bytes;
+  float* w_pre = reinterpret_cast<float*>(ring_all + static_cast<size_t>(kTeams) * stages * stage_bytes);
+  float* w_post = w_pre + H;
+  for (int c = threadIdx.x; c < H; c += blockDim.x) {
+    const int at = c / 8 * 4 + (c & 3) + ((c & 4) ? H / 2 : 0);
+    if (pre) w_pre[at] = to_f32(static_cast<const TH*>(a.w_pre)[c]);
+    w_post[at] = to_f32(static_cast<const TH*>(a.w_post)[c]) *
+                 (a.gate_kind == kGateChannel ? to_f32(static_cast<const TH*>(a.gate)[c]) : 1.f);
+  }
+  const auto weights = [&](const float* w, int c, F2* f) {
+    const float4 lo = *reinterpret_cast<const float4*>(w + c / 2);
+    const float4 hi = *reinterpret_cast<const float4*>(w + H / 2 + c / 2);
+    f[0] = f2(lo.x, lo.y);
+    f[1] = f2(lo.z, lo.w);
+    f[2] = f2(hi.x, hi.y);
+    f[3] = f2(hi.z, hi.w);
+  };
+  if (tid < stages) mbar_init(smem_u32(&full[team][tid]), 1);
+  if (threadIdx.x == 0) abort_flag = 0;
+  fence_mbar_init();
+  __syncthreads();
+
+  const int step = gridDim.x * kTeams;
+  const int first = blockIdx.x * kTeams + team;
+  const auto id_of = [&](int r) { return r < rows ? (row_ids ? row_ids[r] : r) : 0; };
+  const auto fetch = [&](int r, int src, int s) {  // row r into stage s (thread 0 of the team)
+    const uint32_t bar = smem_u32(&full[team][s]);
+    const uint32_t dst = smem_u32(ring + static_cast<size_t>(s) * stage_bytes);
+    const uint32_t bytes_h = H * sizeof(TH), bytes_x = H * sizeof(TX);
+    if (!index_in(src, n_rows, err)) {  // nothing of it is read
+      mbar_arrive(bar);
+      return;
+    }
+    mbar_arrive_expect_tx(bar, bytes_h + (pre ? bytes_h + bytes_x : 0) + (dy ? bytes_x : 0));
+    bulk_load(dst, static_cast<const TH*>(a.h) + src * a.ld_h, bytes_h, bar);
+    if (pre) {
+      bulk_load(dst + at_dn, dn + r * ld_dn, bytes_h, bar);
+      bulk_load(dst + at_y, static_cast<const TX*>(a.x) + src * a.ld_x, bytes_x, bar);
+    }
+    if (dy) bulk_load(dst + at_dy, dy + r * ld_dy, bytes_x, bar);
+  };
+  int fetch_id = 0;  // thread 0: the id of the next row to be fetched, read one row ahead
+  if (tid == 0) {
+    int ids[kMaxStages + 1];
+#pragma unroll
+    for (int i = 0; i <= kMaxStages; ++i) ids[i] = id_of(first + i * step);
+#pragma unroll
+    for (int i = 0; i < kMaxStages; ++i)
+      if (i < stages && first + i * step < rows) fetch(first + i * step, ids[i], i);
+#pragma unroll
+    for (int i = 0; i <= kMaxStages; ++i)
+      if (i == stages) fetch_id = ids[i];
+  }
+
+  F2 s_pre[NV][P], s_post[NV][P];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int i = 0; i < P; ++i) s_pre[k][i] = s_post[k][i] = f2(0.f);
+  // The sum of v over the team, and whether a thread of it gave up a wait.
+  const auto team_sum = [&](float v, float* slot, bool& failed) {
+    v = warp_add(v);
+    if constexpr (NW == 1) {
+      failed = __any_sync(0xffffffffu, failed);
+      __syncwarp();
+      return v;
+    } else {
+      if (lane_id() == 0) slot[tid / 32] = v;
+      int any;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+          "bar.red.or.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+          : "=r"(any)
+          : "r"(static_cast<int>(failed)), "r"(1 + team), "n"(NT)
+          : "memory");
+      failed = any != 0;
+      if constexpr (NW <= 8) {
+        float s = slot[0];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) s += slot[w];
+        return s;
+      } else {
+        return warp_add(lane_id() < NW ? slot[lane_id()] : 0.f);
+      }
+    }
+  };
+
+  // the row at hand, read one row ahead: its id (-1: out of range), statistics and gate
+  int next = -1;
+  float r1 = 0.f, r2 = 0.f, tg = 1.f;
+  const auto read_row = [&](int id) {
+    next = id >= 0 && id < n_rows ? id : -1;
+    r1 = r2 = 0.f;
+    tg = 1.f;
+    if (next < 0) return;
+    r1 = rstd_post[next];
+    if (pre) r2 = rstd_pre[next];
+    if (a.gate_kind == kGateToken) tg = static_cast<const float*>(a.gate)[next * a.ld_gate];
+  };
+  read_row(id_of(first));
+
+  const auto refill = [&](int r, int s) {
+    if (tid != 0 || r >= rows) return;
+    fetch(r, fetch_id, s);
+    fetch_id = id_of(r + step);
+  };
+
+  int s = 0, phase = 0, turn = 0;
+  bool failed = false;
+  for (int r = first; r < rows; r += step, ++turn) {
+    const int ahead = id_of(r + step);
+    failed = !mbar_wait(smem_u32(&full[team][s]), phase, &abort_flag, err, kErrWaitProducer);
+    const int src = next;
+    const uint8_t* st = ring + static_cast<size_t>(s) * stage_bytes;
+    const int done = s;
+    if (++s == stages) {
+      s = 0;
+      phase ^= 1;
+    }
+    const long long out = static_cast<long long>(r) * H;
+    if (src < 0) {  // out-of-range row id: zero gradients (the whole team is here)
+      F2 zero[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) zero[i] = f2(0.f);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * NT) * 8;
+        if (c >= H) continue;
+        store_f2<TX, 8>(dx + out + c, zero);
+        store_f2<TH, 8>(dh + out + c, zero);
+        if (a.gate_kind == kGateElement) store_f2<TH, 8>(static_cast<TH*>(dgate) + out + c, zero);
+      }
+      if (a.gate_kind == kGateToken && tid == 0) static_cast<float*>(dgate)[r] = 0.f;
+      team_sum(0.f, red[team][2], failed);  // its barrier alone
+      if (failed) break;
+      refill(r + stages * step, done);
+      read_row(ahead);
+      continue;
+    }
+    F2 h[NV][P], d[NV][P];
+    F2 sum = f2(0.f);
+    const float br = a.block_scale * r1, scale = br * tg, c1 = inv_h * r1 * r1;
+    if (pre) {
+      F2 y[NV][P];
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * NT) * 8;
+        if (c >= H) continue;
+        F2 g[P], w[P];
+        unpack_f2<TH, 8>(shared_pack(reinterpret_cast<const TH*>(st) + c), h[k]);
+        unpack_f2<TX, 8>(shared_pack(reinterpret_cast<const TX*>(st + at_y) + c), y[k]);
+        unpack_f2<TH, 8>(shared_pack(reinterpret_cast<const TH*>(st + at_dn) + c), g);
+        if (dy) unpack_f2<TX, 8>(shared_pack(reinterpret_cast<const TX*>(st + at_dy) + c), d[k]);
+        weights(w_pre, c, w);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const F2 p = g[i] * y[k][i];
+          s_pre[k][i] = fma2(p, f2(r2), s_pre[k][i]);
+          sum = fma2(p, w[i], sum);
+          d[k][i] = fma2(g[i] * w[i], f2(r2), dy ? d[k][i] : f2(0.f));
+        }
+      }
+      const float dot = team_sum(sum2(sum), red[team][0], failed);
+      if (failed) break;
+      refill(r + stages * step, done);
+      const F2 coef = f2(-dot * inv_h * r2 * r2 * r2);
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int i = 0; i < P; ++i) d[k][i] = fma2(y[k][i], coef, d[k][i]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * NT) * 8;
+        if (c >= H) continue;
+        unpack_f2<TH, 8>(shared_pack(reinterpret_cast<const TH*>(st) + c), h[k]);
+        unpack_f2<TX, 8>(shared_pack(reinterpret_cast<const TX*>(st + at_dy) + c), d[k]);
+      }
+    }
+    read_row(ahead);
+    sum = f2(0.f);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (tid + k * NT) * 8;
+      if (c >= H) continue;
+      F2 w[P], e[P];
+      weights(w_post, c, w);
+#pragma unroll
+      for (int i = 0; i < P; ++i) e[i] = d[k][i] * f2(a.resid_scale);
+      store_f2<TX, 8>(dx + out + c, e);
+      if (a.gate_kind == kGateElement) {
+#pragma unroll
+        for (int i = 0; i < P; ++i) e[i] = d[k][i] * h[k][i] * f2(br) * w[i];
+        store_f2<TH, 8>(static_cast<TH*>(dgate) + out + c, e);
+        load_f2<TH, 8>(static_cast<const TH*>(a.gate) + src * a.ld_gate + c, e);
+#pragma unroll
+        for (int i = 0; i < P; ++i) d[k][i] = d[k][i] * e[i];
+      }
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const F2 q = d[k][i] * h[k][i];
+        s_post[k][i] = fma2(q, f2(scale), s_post[k][i]);
+        sum = fma2(q, w[i], sum);
+        d[k][i] = d[k][i] * w[i];
+      }
+    }
+    // without the norm before the next block this is the row's only barrier: two slots in turn
+    const float dot = team_sum(sum2(sum), red[team][pre ? 1 : turn & 1], failed);
+    if (!pre) {
+      if (failed) break;
+      refill(r + stages * step, done);
+    }
+    if (a.gate_kind == kGateToken && tid == 0) static_cast<float*>(dgate)[r] = dot * br;
+    const F2 coef = f2(-dot * c1);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (tid + k * NT) * 8;
+      if (c >= H) continue;
+#pragma unroll
+      for (int i = 0; i < P; ++i) h[k][i] = fma2(h[k][i], coef, d[k][i]) * f2(scale);
+      store_f2<TH, 8>(dh + out + c, h[k]);
+    }
+  }
+  if (failed && tid == 0) {  // no copy may land in this memory after the block has ended
+    volatile int never = 0;
+    for (int i = 0; i < stages; ++i)
+      if (first + (turn + i) * step < rows)
+        mbar_wait(smem_u32(&full[team][(turn + i) % stages]), ((turn + i) / stages) & 1, &never,
+                  nullptr, 0);
+  }
+
+  float* mine = part + 2ll * blockIdx.x * H;
+  if constexpr (kTeams > 1) {  // the teams' sums, in the order of the teams
+    float* sums = reinterpret_cast<float*>(ring_all);  // [kTeams][H], in the place of the rows
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      if (which == 0 && !pre) continue;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        WideCols::put(sums + team * H, (tid + k * NT) * 8, H, which ? s_post[k] : s_pre[k]);
+      __syncthreads();
+      for (int c = threadIdx.x; c < H; c += 128) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < kTeams; ++i) t += sums[i * H + c];
+        mine[which * H + c] = t;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (tid + k * NT) * 8;
+      if (pre) WideCols::store(mine, c, H, s_pre[k]);
+      WideCols::store(mine + H, c, H, s_post[k]);
+    }
+  }
+}
+
 // dw_pre (blockIdx.y = 0), dw_post and a channel gate's gradient (1) from the blocks' column sums,
 // in block order.  Block: 32 columns x 32 slices of the blocks.
 template <typename TH>
@@ -615,6 +906,44 @@ int launch_bwd(const BwdArgs& b, cudaStream_t st) {
   const int rc = launch_status();
   return rc ? rc : blocks;
 }
+
+constexpr int kRingBytes = 220 * 1024;  // shared memory of an SM that the rings may take
+
+// The ring kernel where two rows a team fit; 0 where they do not.
+template <typename TH, typename TX, int NW, int NV>
+int launch_ring(const BwdArgs& b, cudaStream_t st) {
+  constexpr int kTeams = NW < 4 ? 4 / NW : 1;
+  constexpr int kResident = NW < 4 ? 4 : NW <= 16 ? 16 / NW : 1;  // the kernel's launch bounds
+  auto* kernel = block_norms_bwd_ring_kernel<TH, TX, NW, NV>;
+  const int row = 2 * b.a.H * static_cast<int>(sizeof(TH) + sizeof(TX)) * kTeams;
+  const int weights = 8 * b.a.H;
+  int per_sm = kResident, stages = 0;
+  for (; per_sm > 0; per_sm = per_sm / 2) {
+    stages = (kRingBytes / per_sm - weights) / row;
+    if (stages >= 2) break;
+  }
+  if (per_sm == 0) return 0;
+  if (stages > 4) stages = 4;
+  if (getenv("STAGES") && stages > atoi(getenv("STAGES"))) stages = atoi(getenv("STAGES"));
+  const int smem = stages * row + weights;
+  static bool allowed[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) !=
+        cudaSuccess)
+      return -3;
+    allowed[dev] = true;
+  }
+  const int turns = (b.rows + kTeams - 1) / kTeams;
+  const int blocks = turns < 148 * per_sm ? turns : 148 * per_sm;
+  kernel<<<blocks, NW < 4 ? 128 : NW * 32, smem, st>>>(
+      b.a, static_cast<const TX*>(b.dy), b.ld_dy, static_cast<const TH*>(b.dn), b.ld_dn,
+      b.rstd_post, b.rstd_pre, b.row_ids, b.n_rows, static_cast<TX*>(b.dx),
+      static_cast<TH*>(b.dh), b.dgate, b.part, b.rows, stages, b.err);
+  const int rc = launch_status();
+  return rc ? rc : blocks;
+}
 }  // namespace
 
 int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy, const void* dn,
@@ -648,6 +977,16 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
 #define CFB_BWD(NW, NV, R) return launch_bwd<WideCols, TH, TX, NW, NV, R>(b, st)
       if (W == 8) {
         const int ex = getenv("CFB_EXP") ? atoi(getenv("CFB_EXP")) : 0;
+        int blocks = 0;
+        if (ex == 0) {
+        if (H <= 256) blocks = launch_ring<TH, TX, 1, 1>(b, st);
+        else if (H <= 512) blocks = launch_ring<TH, TX, 1, 2>(b, st);
+        else if (H <= 1024) blocks = launch_ring<TH, TX, 2, 2>(b, st);
+        else if (H <= 2048) blocks = launch_ring<TH, TX, 4, 2>(b, st);
+        else if (H <= 4096) blocks = launch_ring<TH, TX, 8, 2>(b, st);
+        else if (H <= 8192) blocks = launch_ring<TH, TX, 16, 2>(b, st);
+        }
+        if (blocks != 0) return blocks;
         if (ex == 1) {
         if (H <= 256) CFB_BWD(1, 1, 2);
         if (H <= 512) CFB_BWD(2, 1, 2);

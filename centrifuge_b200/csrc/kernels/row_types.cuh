@@ -75,6 +75,16 @@ __device__ __forceinline__ void store_f32(T* p, const float* f) {
   store_pack<T, W>(p, k);
 }
 
+// Eight elements of a row in shared memory.
+template <typename T>
+__device__ __forceinline__ Pack<T, 8> shared_pack(const T* p) {
+  Pack<T, 8> k;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i)
+    reinterpret_cast<uint4*>(&k)[i] = reinterpret_cast<const uint4*>(p)[i];
+  return k;
+}
+
 // Asks the L2 cache for the whole 16-byte pieces of the `bytes` from p.
 __device__ __forceinline__ void prefetch_l2(const void* p, int bytes) {
   const uintptr_t at = (reinterpret_cast<uintptr_t>(p) + 15) & ~static_cast<uintptr_t>(15);
