@@ -18,7 +18,6 @@
 // The gate is absent, one value for each channel [H], for each token [T, 1] (fp32), or for each
 // element [T, H].
 #include "row_types.cuh"
-#include <cstdlib>
 
 namespace cfb {
 
@@ -472,19 +471,15 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
   const int team = threadIdx.x / NT, tid = threadIdx.x % NT;
   const bool pre = a.w_pre != nullptr;
   const float inv_h = 1.f / static_cast<float>(H);
-  // a stage: h, dn, y, dy
+  // a stage: h, dn, y, dy, the element's gate
   const int at_dn = H * static_cast<int>(sizeof(TH)), at_y = 2 * at_dn;
   const int at_dy = at_y + H * static_cast<int>(sizeof(TX));
-  const int stage_bytes = at_dy + H * static_cast<int>(sizeof(TX));
+  const bool element = a.gate_kind == kGateElement;
+  const int at_gate = at_dy + H * static_cast<int>(sizeof(TX));
+  const int stage_bytes = at_gate + (element ? at_dn : 0);
   uint8_t* ring = ring_all + static_cast<size_t>(team) * stages * stage_bytes;
   float* w_pre = reinterpret_cast<float*>(ring_all + static_cast<size_t>(kTeams) * stages * stage_bytes);
   float* w_post = w_pre + H;
-  for (int c = threadIdx.x; c < H; c += blockDim.x) {
-    const int at = c / 8 * 4 + (c & 3) + ((c & 4) ? H / 2 : 0);
-    if (pre) w_pre[at] = to_f32(static_cast<const TH*>(a.w_pre)[c]);
-    w_post[at] = to_f32(static_cast<const TH*>(a.w_post)[c]) *
-                 (a.gate_kind == kGateChannel ? to_f32(static_cast<const TH*>(a.gate)[c]) : 1.f);
-  }
   const auto weights = [&](const float* w, int c, F2* f) {
     const float4 lo = *reinterpret_cast<const float4*>(w + c / 2);
     const float4 hi = *reinterpret_cast<const float4*>(w + H / 2 + c / 2);
@@ -501,24 +496,49 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
   const int step = gridDim.x * kTeams;
   const int first = blockIdx.x * kTeams + team;
   const auto id_of = [&](int r) { return r < rows ? (row_ids ? row_ids[r] : r) : 0; };
-  const auto fetch = [&](int r, int src, int s) {  // row r into stage s (thread 0 of the team)
+  // Row r, whose row of h and y is src, into stage s.  Of the team's first warp lane 0 copies h,
+  // 1 dn, 2 y, 3 dy and 4 the gate, all by the same few instructions.
+  const uint8_t* lane_base = static_cast<const uint8_t*>(a.h);
+  long long lane_ld = a.ld_h * static_cast<int>(sizeof(TH));
+  int lane_at = 0;
+  if (tid == 1) {
+    lane_base = reinterpret_cast<const uint8_t*>(dn);
+    lane_ld = ld_dn * static_cast<int>(sizeof(TH));
+    lane_at = at_dn;
+  } else if (tid == 2) {
+    lane_base = pre ? static_cast<const uint8_t*>(a.x) : nullptr;
+    lane_ld = a.ld_x * static_cast<int>(sizeof(TX));
+    lane_at = at_y;
+  } else if (tid == 3) {
+    lane_base = reinterpret_cast<const uint8_t*>(dy);
+    lane_ld = ld_dy * static_cast<int>(sizeof(TX));
+    lane_at = at_dy;
+  } else if (tid == 4) {
+    lane_base = element ? static_cast<const uint8_t*>(a.gate) : nullptr;
+    lane_ld = a.ld_gate * static_cast<int>(sizeof(TH));
+    lane_at = at_gate;
+  }
+  const int lane_bytes = H * static_cast<int>(tid == 2 || tid == 3 ? sizeof(TX) : sizeof(TH));
+  const int row_bytes =
+      H * static_cast<int>(sizeof(TH)) * (1 + (pre ? 1 : 0) + (element ? 1 : 0)) +
+      H * static_cast<int>(sizeof(TX)) * ((pre ? 1 : 0) + (dy ? 1 : 0));
+  const auto fetch = [&](int r, int src, int s) {  // lanes 0 to 4 of the team's first warp
     const uint32_t bar = smem_u32(&full[team][s]);
-    const uint32_t dst = smem_u32(ring + static_cast<size_t>(s) * stage_bytes);
-    const uint32_t bytes_h = H * sizeof(TH), bytes_x = H * sizeof(TX);
-    if (!index_in(src, n_rows, err)) {  // nothing of it is read
-      mbar_arrive(bar);
-      return;
+    const bool ok = src >= 0 && src < n_rows;
+    if (tid == 0) {
+      if (ok) {
+        mbar_arrive_expect_tx(bar, row_bytes);
+      } else {  // nothing of it is read
+        mbar_arrive(bar);
+        if (err) atomicCAS(err, 0, kErrBounds);
+      }
     }
-    mbar_arrive_expect_tx(bar, bytes_h + (pre ? bytes_h + bytes_x : 0) + (dy ? bytes_x : 0));
-    bulk_load(dst, static_cast<const TH*>(a.h) + src * a.ld_h, bytes_h, bar);
-    if (pre) {
-      bulk_load(dst + at_dn, dn + r * ld_dn, bytes_h, bar);
-      bulk_load(dst + at_y, static_cast<const TX*>(a.x) + src * a.ld_x, bytes_x, bar);
-    }
-    if (dy) bulk_load(dst + at_dy, dy + r * ld_dy, bytes_x, bar);
+    if (ok && lane_base)
+      bulk_load(smem_u32(ring + static_cast<size_t>(s) * stage_bytes + lane_at),
+                lane_base + ((tid & 1) ? r : src) * lane_ld, lane_bytes, bar);
   };
-  int fetch_id = 0;  // thread 0: the id of the next row to be fetched, read one row ahead
-  if (tid == 0) {
+  int fetch_id = 0;  // the id of the next row to be fetched, read one row ahead
+  if (tid < 5) {
     int ids[kMaxStages + 1];
 #pragma unroll
     for (int i = 0; i <= kMaxStages; ++i) ids[i] = id_of(first + i * step);
@@ -529,6 +549,20 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
     for (int i = 0; i <= kMaxStages; ++i)
       if (i == stages) fetch_id = ids[i];
   }
+  // the weights, while the first rows are on their way
+  for (int c = threadIdx.x * 8; c < H; c += blockDim.x * 8) {
+    const Pack<TH, 8> post = load_pack<TH, 8>(static_cast<const TH*>(a.w_post) + c);
+    Pack<TH, 8> gate = post, before = post;
+    if (a.gate_kind == kGateChannel) gate = load_pack<TH, 8>(static_cast<const TH*>(a.gate) + c);
+    if (pre) before = load_pack<TH, 8>(static_cast<const TH*>(a.w_pre) + c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = c / 2 + (i & 3) + ((i & 4) ? H / 2 : 0);
+      w_post[at] = to_f32(post.v[i]) * (a.gate_kind == kGateChannel ? to_f32(gate.v[i]) : 1.f);
+      if (pre) w_pre[at] = to_f32(before.v[i]);
+    }
+  }
+  __syncthreads();
 
   F2 s_pre[NV][P], s_post[NV][P];
 #pragma unroll
@@ -575,10 +609,12 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
     if (pre) r2 = rstd_pre[next];
     if (a.gate_kind == kGateToken) tg = static_cast<const float*>(a.gate)[next * a.ld_gate];
   };
-  read_row(id_of(first));
+  const int first_id = id_of(first);
+  int ahead = id_of(first + step);  // the id of the row after that
+  read_row(first_id);
 
   const auto refill = [&](int r, int s) {
-    if (tid != 0 || r >= rows) return;
+    if (tid >= 5 || r >= rows) return;
     fetch(r, fetch_id, s);
     fetch_id = id_of(r + step);
   };
@@ -586,9 +622,11 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
   int s = 0, phase = 0, turn = 0;
   bool failed = false;
   for (int r = first; r < rows; r += step, ++turn) {
-    const int ahead = id_of(r + step);
     failed = !mbar_wait(smem_u32(&full[team][s]), phase, &abort_flag, err, kErrWaitProducer);
     const int src = next;
+    const float row_r2 = r2, br = a.block_scale * r1, scale = br * tg, c1 = inv_h * r1 * r1;
+    read_row(ahead);
+    ahead = id_of(r + 2 * step);
     const uint8_t* st = ring + static_cast<size_t>(s) * stage_bytes;
     const int done = s;
     if (++s == stages) {
@@ -606,18 +644,24 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
         if (c >= H) continue;
         store_f2<TX, 8>(dx + out + c, zero);
         store_f2<TH, 8>(dh + out + c, zero);
-        if (a.gate_kind == kGateElement) store_f2<TH, 8>(static_cast<TH*>(dgate) + out + c, zero);
+        if (element) store_f2<TH, 8>(static_cast<TH*>(dgate) + out + c, zero);
       }
       if (a.gate_kind == kGateToken && tid == 0) static_cast<float*>(dgate)[r] = 0.f;
       team_sum(0.f, red[team][2], failed);  // its barrier alone
       if (failed) break;
       refill(r + stages * step, done);
-      read_row(ahead);
       continue;
     }
     F2 h[NV][P], d[NV][P];
     F2 sum = f2(0.f);
-    const float br = a.block_scale * r1, scale = br * tg, c1 = inv_h * r1 * r1;
+    Pack<TH, 8> gate[NV];
+    if (element) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        const int c = (tid + k * NT) * 8;
+        if (c < H) gate[k] = shared_pack(reinterpret_cast<const TH*>(st + at_gate) + c);
+      }
+    }
     if (pre) {
       F2 y[NV][P];
 #pragma unroll
@@ -633,15 +677,15 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
 #pragma unroll
         for (int i = 0; i < P; ++i) {
           const F2 p = g[i] * y[k][i];
-          s_pre[k][i] = fma2(p, f2(r2), s_pre[k][i]);
+          s_pre[k][i] = fma2(p, f2(row_r2), s_pre[k][i]);
           sum = fma2(p, w[i], sum);
-          d[k][i] = fma2(g[i] * w[i], f2(r2), dy ? d[k][i] : f2(0.f));
+          d[k][i] = fma2(g[i] * w[i], f2(row_r2), dy ? d[k][i] : f2(0.f));
         }
       }
       const float dot = team_sum(sum2(sum), red[team][0], failed);
       if (failed) break;
       refill(r + stages * step, done);
-      const F2 coef = f2(-dot * inv_h * r2 * r2 * r2);
+      const F2 coef = f2(-dot * inv_h * row_r2 * row_r2 * row_r2);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -655,7 +699,6 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
         unpack_f2<TX, 8>(shared_pack(reinterpret_cast<const TX*>(st + at_dy) + c), d[k]);
       }
     }
-    read_row(ahead);
     sum = f2(0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -666,11 +709,11 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
 #pragma unroll
       for (int i = 0; i < P; ++i) e[i] = d[k][i] * f2(a.resid_scale);
       store_f2<TX, 8>(dx + out + c, e);
-      if (a.gate_kind == kGateElement) {
+      if (element) {
 #pragma unroll
         for (int i = 0; i < P; ++i) e[i] = d[k][i] * h[k][i] * f2(br) * w[i];
         store_f2<TH, 8>(static_cast<TH*>(dgate) + out + c, e);
-        load_f2<TH, 8>(static_cast<const TH*>(a.gate) + src * a.ld_gate + c, e);
+        unpack_f2<TH, 8>(gate[k], e);
 #pragma unroll
         for (int i = 0; i < P; ++i) d[k][i] = d[k][i] * e[i];
       }
@@ -913,18 +956,20 @@ constexpr int kRingBytes = 220 * 1024;  // shared memory of an SM that the rings
 template <typename TH, typename TX, int NW, int NV>
 int launch_ring(const BwdArgs& b, cudaStream_t st) {
   constexpr int kTeams = NW < 4 ? 4 / NW : 1;
-  constexpr int kResident = NW < 4 ? 4 : NW <= 16 ? 16 / NW : 1;  // the kernel's launch bounds
+  // 16 warps of 128 registers are resident on an SM
+  constexpr int threads = NW < 4 ? 128 : NW * 32;
   auto* kernel = block_norms_bwd_ring_kernel<TH, TX, NW, NV>;
-  const int row = 2 * b.a.H * static_cast<int>(sizeof(TH) + sizeof(TX)) * kTeams;
+  const bool element = b.a.gate_kind == kGateElement;
+  const int row = b.a.H * static_cast<int>(2 * (sizeof(TH) + sizeof(TX)) +
+                                           (element ? sizeof(TH) : 0)) * kTeams;
   const int weights = 8 * b.a.H;
-  int per_sm = kResident, stages = 0;
-  for (; per_sm > 0; per_sm = per_sm / 2) {
+  int per_sm = 512 / threads, stages = 0;
+  for (; per_sm > 0; --per_sm) {
     stages = (kRingBytes / per_sm - weights) / row;
     if (stages >= 2) break;
   }
   if (per_sm == 0) return 0;
   if (stages > 4) stages = 4;
-  if (getenv("STAGES") && stages > atoi(getenv("STAGES"))) stages = atoi(getenv("STAGES"));
   const int smem = stages * row + weights;
   static bool allowed[64] = {};
   int dev = 0;
@@ -937,7 +982,7 @@ int launch_ring(const BwdArgs& b, cudaStream_t st) {
   }
   const int turns = (b.rows + kTeams - 1) / kTeams;
   const int blocks = turns < 148 * per_sm ? turns : 148 * per_sm;
-  kernel<<<blocks, NW < 4 ? 128 : NW * 32, smem, st>>>(
+  kernel<<<blocks, threads, smem, st>>>(
       b.a, static_cast<const TX*>(b.dy), b.ld_dy, static_cast<const TH*>(b.dn), b.ld_dn,
       b.rstd_post, b.rstd_pre, b.row_ids, b.n_rows, static_cast<TX*>(b.dx),
       static_cast<TH*>(b.dh), b.dgate, b.part, b.rows, stages, b.err);
@@ -976,33 +1021,25 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
     const auto launch = [&]() -> int {
 #define CFB_BWD(NW, NV, R) return launch_bwd<WideCols, TH, TX, NW, NV, R>(b, st)
       if (W == 8) {
-        const int ex = getenv("CFB_EXP") ? atoi(getenv("CFB_EXP")) : 0;
+        // fp32 rows of over 1024 columns: a ring of them leaves room for too few blocks (8192 x 2048:
+        // 77.5 us without, 81.0 with; 8192 x 4096: 156, 173)
         int blocks = 0;
-        if (ex == 0) {
-        if (H <= 256) blocks = launch_ring<TH, TX, 1, 1>(b, st);
-        else if (H <= 512) blocks = launch_ring<TH, TX, 1, 2>(b, st);
-        else if (H <= 1024) blocks = launch_ring<TH, TX, 2, 2>(b, st);
+        if (sizeof(TH) == 4 && H > 1024) blocks = 0;
+        else if (H <= 256) blocks = launch_ring<TH, TX, 1, 1>(b, st);
+        else if (H <= 512) blocks = launch_ring<TH, TX, 2, 1>(b, st);
+        else if (H <= 1024) blocks = launch_ring<TH, TX, 4, 1>(b, st);
         else if (H <= 2048) blocks = launch_ring<TH, TX, 4, 2>(b, st);
+        else if (H <= 2560) blocks = launch_ring<TH, TX, 5, 2>(b, st);
+        else if (sizeof(TX) == 4 && H <= 4096) blocks = launch_ring<TH, TX, 16, 1>(b, st);
+        else if (H <= 3584) blocks = launch_ring<TH, TX, 7, 2>(b, st);
         else if (H <= 4096) blocks = launch_ring<TH, TX, 8, 2>(b, st);
         else if (H <= 8192) blocks = launch_ring<TH, TX, 16, 2>(b, st);
-        }
         if (blocks != 0) return blocks;
-        if (ex == 1) {
-        if (H <= 256) CFB_BWD(1, 1, 2);
-        if (H <= 512) CFB_BWD(2, 1, 2);
-        if (H <= 1024) CFB_BWD(4, 1, 2);
-        if (H <= 2048) CFB_BWD(8, 1, 2);
-        if (H <= 4096) CFB_BWD(16, 1, 2);
-        }
         if (H <= 256) CFB_BWD(1, 1, 1);
         if (H <= 512) CFB_BWD(2, 1, 1);
         if (H <= 1024) CFB_BWD(4, 1, 1);
         if (H <= 2048) CFB_BWD(8, 1, 1);
-        if (ex == 2) {
         if (H <= 4096) CFB_BWD(8, 2, 1);
-        if (H <= 8192) CFB_BWD(16, 2, 1);
-        }
-        if (H <= 4096) CFB_BWD(16, 1, 1);
         if (H <= 8192) CFB_BWD(32, 1, 1);
         CFB_BWD(32, 2, 1);
       }
@@ -1013,6 +1050,7 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
       if (H <= 256) CFB_BWD(1, 4);
       if (H <= 1024) CFB_BWD(4, 4);
       if (H <= 2048) CFB_BWD(8, 4);
+      if (H <= 2560) CFB_BWD(8, 5);
       if (H <= 4096) CFB_BWD(16, 4);
       if (H <= 8192) CFB_BWD(32, 4);
       CFB_BWD(32, 8);
