@@ -840,13 +840,13 @@ void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids, const c10::option
   const c10::cuda::CUDAGuard guard(dy.device());
   const int rows = row_count(dy.size(0), "scaled_embedding_bwd"), H = dy.size(1);
   Tensor work;
-  if (rows > 0)
-    work = at::empty({cfb_scaled_embedding_bwd_workspace(rows, H)}, dy.options().dtype(at::kByte));
+  const int64_t bytes = cfb_scaled_embedding_bwd_workspace(dtable.size(0), rows, H);
+  if (bytes > 0) work = at::empty({bytes}, dy.options().dtype(at::kByte));
   CFB_CHECK_RC(cfb_scaled_embedding_bwd(
                    dy.data_ptr(), type_code(dy, "dy"), dy.stride(0), ids.data_ptr(),
                    ids.scalar_type() == at::kInt, ids.numel(), opt_ptr<int>(id_rows), pad,
                    dtable.data_ptr<float>(), dtable.stride(0), dtable.size(0), rows, H,
-                   static_cast<float>(scale), accumulate, rows > 0 ? work.data_ptr() : nullptr,
+                   static_cast<float>(scale), accumulate, bytes > 0 ? work.data_ptr() : nullptr,
                    err_word(dy.get_device()).data_ptr<int>(), cur_stream()),
                "scaled_embedding_bwd");
 }

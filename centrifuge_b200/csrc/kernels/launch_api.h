@@ -236,7 +236,7 @@ int cfb_scaled_embedding_fwd(const void* table, int type, long long ld, long lon
 // dtable[v] = (add ? dtable[v] : 0) + scale * sum of dy[r] over the rows r with ids[id_rows[r]] = v
 // (ids[r] without id_rows), v != pad (pad < 0: none).  `work`: scratch of
 // cfb_scaled_embedding_bwd_workspace bytes, 32-byte aligned.
-long long cfb_scaled_embedding_bwd_workspace(int rows, int H);
+long long cfb_scaled_embedding_bwd_workspace(long long V, int rows, int H);
 int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void* ids, int ids32,
                              long long n_ids, const int* id_rows, long long pad, float* dtable,
                              long long ld_t, long long V, int rows, int H, float scale, int add,

@@ -322,6 +322,31 @@ inline bool rows_of(int W, const void* p, long long ld, int code) {
 }
 inline bool rows_of_8(const void* p, long long ld, int code) { return rows_of(8, p, ld, code); }
 
+// A kernel that is launched behind another one of the same operator: it may start while that one
+// ends, and waits for its results itself (after_previous() before it reads them).
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// In the first kernel: the next one may be put on the SMs from here on.
+__device__ __forceinline__ void let_next_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... P, typename... A>
+int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t st,
+                  A&&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) == cudaSuccess ? 0 : -3;
+}
+
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : -3; }
 
 }  // namespace cfb

@@ -11,21 +11,27 @@
 //                           tokens, reads all the tokens, and so knows both where its range begins
 //                           in the sorted order and which rows are in it: one launch, no exchange
 //                           between blocks.
-//   2. embed_grad_kernel    chunks of kChunk sorted positions, one block each (and per slab of
-//                           columns): a run of equal tokens that lies inside a chunk is summed and
-//                           written by that block alone; a run that crosses a chunk's border leaves
-//                           a partial sum.  A token in half of the rows is so spread over as many
-//                           blocks as any other rows.
+//   2. embed_grad_kernel    chunks of sorted positions, a warp each (and per slab of columns): a run
+//                           of equal tokens that lies inside a chunk is summed and written by that
+//                           warp alone; a run that crosses a chunk's border leaves a partial sum.
+//                           A token in half of the rows is so spread over as many warps as any
+//                           other rows.  Where the gradient replaces the table, further blocks
+//                           clear the rows of the tokens that do not occur meanwhile.
 //   3. embed_join_kernel    the chunk in which a crossing run begins adds the partial sums up in
 //                           chunk order and writes the table row.
 //
-// No atomics on floating values anywhere: two runs give the same bits.
+// A handful of rows takes one launch instead (embed_grad_few_kernel).  No atomics on floating values
+// anywhere: two runs give the same bits.
 #include "row_types.cuh"
 
 namespace cfb {
 
-constexpr int kChunk = 32;      // sorted positions of one block of the gradient
 constexpr int kMaxSpan = 1024;  // tokens of one block of the sort
+constexpr int kFewRows = 128;   // up to here one launch does it all
+
+// Sorted positions of one warp of the gradient: few where few rows would leave SMs idle, more where
+// there are enough, since every chunk border costs a partial sum.
+inline int chunk_rows(int rows) { return rows >= 32768 ? 32 : rows >= 2048 ? 16 : 8; }
 
 template <typename TI, typename TO, int W>
 __global__ void __launch_bounds__(256) scaled_embed_fwd_kernel(
@@ -65,45 +71,91 @@ __device__ __forceinline__ int row_token(int r, const void* ids, int ids32, long
   return index_in(tok, V, err) ? static_cast<int>(tok) : -1;
 }
 
+// t[c .. c + W) of a table row of H columns.
+template <int W>
+__device__ __forceinline__ void clear_row(float* t, int H) {
+  float z[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) z[i] = 0.f;
+#pragma unroll 4
+  for (int c = lane_id() * W; c < H; c += 32 * W) store_f32<float, W>(t + c, z);
+}
+
 // Block b places the rows of tokens [b * span, (b + 1) * span) at their sorted positions.  Each of
 // the 32 warps takes a contiguous part of the rows; hist[w][t] first counts the rows of token t in
-// part w and then, after the scan, is the next position of such a row.
+// part w and then, after the scan, is the next position of such a row.  A thread has eight tokens in
+// flight, and keeps them for the second pass where that is all of its part (up to 8192 rows).
 __global__ void __launch_bounds__(1024) sort_tokens_kernel(
     const void* __restrict__ ids, int ids32, long long n_ids, const int* __restrict__ id_rows,
     int rows, long long V, long long pad, int span, int* __restrict__ order,
-    int* __restrict__ stok, int* __restrict__ n_valid, int* err) {
+    int* __restrict__ stok, int* __restrict__ n_valid, uint32_t* __restrict__ absent, int* err) {
+  constexpr int U = 8;
   extern __shared__ int hist[];  // [32][span]
   __shared__ int warp_sums[32];
   __shared__ int below;
+  let_next_start();
   const int tid = threadIdx.x, lane = lane_id(), wp = warp_id();
   const long long lo = static_cast<long long>(blockIdx.x) * span;
   const long long hi = min(V, lo + span);
   if (blockIdx.x != 0) err = nullptr;  // one block reports
-  for (int i = tid; i < 32 * span; i += 1024) hist[i] = 0;
+  const int part = (rows + 1023) / 1024 * 32;
+  const int r0 = min(rows, wp * part), r1 = min(rows, r0 + part);
+  int tok[U];
+  const auto read = [&](int base, int* e) {
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = base + u * 32 + lane;
+      id[u] = r < r1 ? (id_rows ? id_rows[r] : r) : -1;
+    }
+    long long t[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool ok = id[u] >= 0 && id[u] < n_ids;
+      t[u] = !ok ? -1 : ids32 ? static_cast<const int*>(ids)[id[u]]
+                              : static_cast<const long long*>(ids)[id[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool any = base + u * 32 + lane < r1;
+      const bool padding = pad >= 0 && t[u] == pad;
+      const bool ok = t[u] >= 0 && t[u] < V;  // -1 above for a row id outside ids
+      if (e && any && !ok && !padding) atomicCAS(e, 0, kErrBounds);
+      tok[u] = any && ok && !padding ? static_cast<int>(t[u]) : -1;
+    }
+  };
+  read(r0, err);  // under way while the counts are cleared
+  for (int i = tid * 4; i < 32 * span; i += 4096)
+    *reinterpret_cast<int4*>(hist + i) = make_int4(0, 0, 0, 0);
   if (tid == 0) below = 0;
   __syncthreads();
 
-  const int part = (rows + 1023) / 1024 * 32;
-  const int r0 = min(rows, wp * part), r1 = min(rows, r0 + part);
   int less = 0;
-#pragma unroll 4
-  for (int r = r0 + lane; r < r1; r += 32) {
-    const int tok = row_token(r, ids, ids32, n_ids, id_rows, V, pad, err);
-    less += (tok >= 0 && tok < lo);
-    if (tok >= lo && tok < hi) atomicAdd(&hist[wp * span + static_cast<int>(tok - lo)], 1);
+  for (int base = r0; base < r1; base += 32 * U) {
+    if (base != r0) read(base, err);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      less += (tok[u] >= 0 && tok[u] < lo);
+      if (tok[u] >= lo && tok[u] < hi) atomicAdd(&hist[wp * span + static_cast<int>(tok[u] - lo)], 1);
+    }
   }
   less = __reduce_add_sync(0xffffffffu, less);
-  if (lane == 0) atomicAdd(&below, less);
+  if (lane == 0 && less) atomicAdd(&below, less);
   __syncthreads();
 
   // exclusive scan over (token, warp); thread t owns token lo + t (span <= 1024)
+  int count[32];
   int tot = 0;
-  if (tid < span)
-    for (int w = 0; w < 32; ++w) {
-      const int c = hist[w * span + tid];
-      hist[w * span + tid] = tot;
-      tot += c;
-    }
+  if (tid < span) {
+#pragma unroll
+    for (int w = 0; w < 32; ++w) count[w] = hist[w * span + tid];
+#pragma unroll
+    for (int w = 0; w < 32; ++w) tot += count[w];
+  }
+  if (tid < span) {  // tokens without a row, a bit each
+    const uint32_t none = __ballot_sync(0xffffffffu, tot == 0 && lo + tid < hi);
+    if (lane == 0 && lo + tid < hi) absent[(lo + tid) / 32] = none;
+  }
   int inc = tot;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -124,106 +176,162 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
     if (lane == 31 && blockIdx.x == gridDim.x - 1) *n_valid = below + x;
   }
   __syncthreads();
-  const int first = below + warp_sums[wp] + inc - tot;
-  if (tid < span)
-    for (int w = 0; w < 32; ++w) hist[w * span + tid] += first;
+  if (tid < span) {
+    int at = below + warp_sums[wp] + inc - tot;
+#pragma unroll
+    for (int w = 0; w < 32; ++w) {
+      hist[w * span + tid] = at;
+      at += count[w];
+    }
+  }
   __syncthreads();
 
-  for (int r = r0 + lane; r - lane < r1; r += 32) {
-    int key = -1;
-    if (r < r1) {
-      const int tok = row_token(r, ids, ids32, n_ids, id_rows, V, pad, nullptr);
-      if (tok >= lo && tok < hi) key = static_cast<int>(tok - lo);
+  for (int base = r0; base < r1; base += 32 * U) {
+    if (r1 - r0 > 32 * U) read(base, nullptr);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = tok[u] >= lo && tok[u] < hi ? static_cast<int>(tok[u] - lo) : -1;
+      if (__ballot_sync(0xffffffffu, key >= 0) == 0) continue;
+      const unsigned same = __match_any_sync(0xffffffffu, key);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      int* next = &hist[wp * span + max(key, 0)];
+      const int at = *next + rank;
+      __syncwarp();
+      if (key >= 0) {
+        order[at] = base + u * 32 + lane;
+        stok[at] = static_cast<int>(lo) + key;
+        if (rank == 0) *next = at + __popc(same);
+      }
+      __syncwarp();
     }
-    if (__ballot_sync(0xffffffffu, key >= 0) == 0) continue;
-    const unsigned same = __match_any_sync(0xffffffffu, key);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    int* next = &hist[wp * span + max(key, 0)];
-    const int at = *next + rank;
-    __syncwarp();
-    if (key >= 0) {
-      order[at] = r;
-      stok[at] = static_cast<int>(lo) + key;
-      if (rank == 0) *next = at + __popc(same);
-    }
-    __syncwarp();
   }
 }
 
-// Adds (or, without ACC, writes) W columns of a run's sum to its table row.
+// A lane's columns of a slab of rows: eight neighbours (W = 8), or four columns 32 apart (W = 1).
 template <int W>
-__device__ __forceinline__ void write_run(float* dst, const float* acc, float scale, int add) {
-  float o[W];
-  if (add) load_f32<float, W>(dst, o);
+struct SlabCols {
+  static constexpr int N = W == 8 ? 8 : 4;
+  static constexpr int kSlab = 32 * N;
+  int c, H;
+  __device__ __forceinline__ SlabCols(int slab, int H_) : c(slab * kSlab + lane_id() * W), H(H_) {}
+  template <typename T>
+  __device__ __forceinline__ void load(const T* row, Pack<T, N>& k) const {
+    if constexpr (W == 8) {
+      if (c < H) k = load_pack<T, 8>(row + c);
+    } else {
 #pragma unroll
-  for (int i = 0; i < W; ++i) o[i] = (add ? o[i] : 0.f) + scale * acc[i];
-  store_f32<float, W>(dst, o);
-}
+      for (int i = 0; i < N; ++i)
+        if (c + 32 * i < H) k.v[i] = row[c + 32 * i];
+    }
+  }
+  __device__ __forceinline__ void load(const float* row, float* f) const {
+    Pack<float, N> k;
+    load<float>(row, k);
+    unpack<float, N>(k, f);
+  }
+  __device__ __forceinline__ void store(float* row, const float* f) const {
+    if constexpr (W == 8) {
+      if (c < H) store_f32<float, 8>(row + c, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c + 32 * i < H) row[c + 32 * i] = f[i];
+    }
+  }
+  // Adds a run's sum to its table row, or writes it there.
+  __device__ __forceinline__ void write_run(float* row, const float* acc, float scale,
+                                            int add) const {
+    float o[N];
+    if (add) load(row, o);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = (add ? o[i] : 0.f) + scale * acc[i];
+    store(row, o);
+  }
+};
 
-// Chunk blockIdx.x of the sorted rows, columns (blockIdx.y * blockDim.x + thread) * W.
+// One warp: sorted positions [chunk * per, + per) (per <= 32), one slab of columns.
 // part[chunk][0]: the sum of the rows of a run that began in an earlier chunk;
 // part[chunk][1]: of a run that begins here and goes on in the next chunk.
 template <typename T, int W>
-__global__ void __launch_bounds__(256) embed_grad_kernel(
+__global__ void __launch_bounds__(128, 8) embed_grad_kernel(
     const T* __restrict__ dy, long long ld, const int* __restrict__ order,
-    const int* __restrict__ stok, const int* __restrict__ n_valid, float* __restrict__ dtable,
-    long long ld_t, float* __restrict__ part, int H, float scale, int add) {
-  constexpr int U = sizeof(T) == 4 && W == 8 ? 4 : 8;  // rows in flight
-  __shared__ int s_row[kChunk];
-  __shared__ int s_tok[kChunk + 2];  // with the tokens before and behind the chunk (-1: none)
-  const int n = *n_valid;
-  const int p0 = blockIdx.x * kChunk;
-  if (p0 >= n) return;
-  const int m = min(kChunk, n - p0);
-  if (threadIdx.x < m) s_row[threadIdx.x] = order[p0 + threadIdx.x];
-  for (int i = threadIdx.x; i < m + 2; i += blockDim.x) {
-    const int p = p0 + i - 1;
-    s_tok[i] = p >= 0 && p < n ? stok[p] : -1;
+    const int* __restrict__ stok, const int* __restrict__ n_valid,
+    const uint32_t* __restrict__ absent, float* __restrict__ dtable, long long ld_t,
+    float* __restrict__ part, int H, int slabs, int per, int sum_blocks, float scale, int add) {
+  using S = SlabCols<W>;
+  constexpr int N = S::N;
+  constexpr int U = 4;  // rows in flight
+  after_previous();
+  let_next_start();
+  if (static_cast<int>(blockIdx.x) >= sum_blocks) {  // clear what does not occur of 32 tokens
+    const long long word = static_cast<long long>(blockIdx.x) - sum_blocks;
+    const uint32_t none = absent[word];
+    for (int t = warp_id(); t < 32; t += 4)
+      if (none >> t & 1) clear_row<W>(dtable + (word * 32 + t) * ld_t, H);
+    return;
   }
-  __syncthreads();
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * W;
-  if (c >= H) return;
-  const bool from_before = s_tok[0] == s_tok[1];
-  float acc[W];
+  const int n = *n_valid;
+  const int item = blockIdx.x * 4 + warp_id();
+  const int chunk = item / slabs;
+  const int p0 = chunk * per;
+  if (p0 >= n) return;
+  const int lane = lane_id();
+  const int m = min(per, n - p0);
+  const int my_row = lane < m ? order[p0 + lane] : 0;
+  const int my_tok = lane < m ? stok[p0 + lane] : -1;
+  const int before = p0 > 0 ? stok[p0 - 1] : -1;
+  const int behind = p0 + m < n ? stok[p0 + m] : -1;
+  const bool from_before = before == __shfl_sync(0xffffffffu, my_tok, 0);
+  const S cols(item % slabs, H);
+  float acc[N];
 #pragma unroll
-  for (int i = 0; i < W; ++i) acc[i] = 0.f;
-  int begin = 0;  // first row of the run that acc sums
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  bool head = from_before;  // acc sums the run that began before the chunk
+#pragma unroll 1
   for (int j = 0; j < m; j += U) {
-    Pack<T, W> k[U];
+    Pack<T, N> k[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (j + u < m) k[u] = load_pack<T, W>(dy + s_row[j + u] * ld + c);
+    for (int u = 0; u < U; ++u) {
+      const int row = __shfl_sync(0xffffffffu, my_row, (j + u) & 31);
+      if (j + u < m) cols.load(dy + row * ld, k[u]);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (j + u >= m) break;
-      float f[W];
-      unpack<T, W>(k[u], f);
+      float f[N];
+      unpack<T, N>(k[u], f);
 #pragma unroll
-      for (int i = 0; i < W; ++i) acc[i] += f[i];
-      const int tok = s_tok[j + u + 1];
-      const bool goes_on = s_tok[j + u + 2] == tok;
-      if (goes_on && j + u + 1 < m) continue;
-      const bool head = begin == 0 && from_before;
+      for (int i = 0; i < N; ++i) acc[i] += f[i];
+      const int tok = __shfl_sync(0xffffffffu, my_tok, j + u);
+      const bool last = j + u + 1 == m;
+      const int next = __shfl_sync(0xffffffffu, my_tok, (j + u + 1) & 31);
+      const bool goes_on = (last ? behind : next) == tok;
+      if (goes_on && !last) continue;
       if (head || goes_on) {
-        const long long slot = 2ll * blockIdx.x + (head ? 0 : 1);
-        store_f32<float, W>(part + slot * H + c, acc);
+        cols.store(part + (2ll * chunk + (head ? 0 : 1)) * H, acc);
       } else {
-        write_run<W>(dtable + tok * ld_t + c, acc, scale, add);
+        cols.write_run(dtable + tok * ld_t, acc, scale, add);
       }
 #pragma unroll
-      for (int i = 0; i < W; ++i) acc[i] = 0.f;
-      begin = j + u + 1;
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      head = false;
     }
   }
 }
 
 // The run that begins in chunk blockIdx.x and goes on behind it: its partial sums in chunk order.
+// Eight warps take a contiguous share of the chunks each; the shares are added in their order.
 template <int W>
 __global__ void __launch_bounds__(256) embed_join_kernel(
     const int* __restrict__ stok, const int* __restrict__ n_valid, float* __restrict__ dtable,
-    long long ld_t, const float* __restrict__ part, int H, float scale, int add) {
+    long long ld_t, const float* __restrict__ part, int H, int per, float scale, int add) {
+  using S = SlabCols<W>;
+  constexpr int N = S::N;
+  constexpr int U = 4;
+  __shared__ float share[8][32 * N];
+  after_previous();
   const int n = *n_valid;
-  const int p0 = blockIdx.x * kChunk, p1 = p0 + kChunk;
+  const int p0 = blockIdx.x * per, p1 = p0 + per;
   if (p1 >= n) return;
   const int tok = stok[p1 - 1];
   if (stok[p1] != tok || (p0 > 0 && stok[p0 - 1] == tok)) return;
@@ -232,28 +340,106 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
     const int mid = lo + (hi - lo) / 2;
     if (stok[mid] == tok) lo = mid + 1; else hi = mid;
   }
-  const int last = (lo - 1) / kChunk;
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * W;
-  if (c >= H) return;
-  float acc[W], f[W];
-  load_f32<float, W>(part + (2ll * blockIdx.x + 1) * H + c, acc);
-#pragma unroll 4
-  for (int k = blockIdx.x + 1; k <= last; ++k) {
-    load_f32<float, W>(part + 2ll * k * H + c, f);
+  const int chunks = (lo - 1) / per - blockIdx.x;  // behind the first
+  const int each = (chunks + 7) / 8, wp = warp_id(), lane = lane_id();
+  const int k0 = blockIdx.x + 1 + wp * each, k1 = blockIdx.x + 1 + min(chunks, (wp + 1) * each);
+  const S cols(blockIdx.y, H);
+  float acc[N];
 #pragma unroll
-    for (int i = 0; i < W; ++i) acc[i] += f[i];
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  if (wp == 0) cols.load(part + (2ll * blockIdx.x + 1) * H, acc);
+  for (int k = k0; k < k1; k += U) {
+    Pack<float, N> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k + u < k1) cols.template load<float>(part + 2ll * (k + u) * H, v[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (k + u >= k1) break;
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] += v[u].v[i];
+    }
   }
-  write_run<W>(dtable + tok * ld_t + c, acc, scale, add);
+#pragma unroll
+  for (int i = 0; i < N; ++i) share[wp][i * 32 + lane] = acc[i];
+  __syncthreads();
+  if (wp != 0) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w)
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] += share[w][i * 32 + lane];
+  cols.write_run(dtable + tok * ld_t, acc, scale, add);
+}
+
+// Up to kFewRows rows.  Blocks [0, row_blocks): a warp for each row and slab, which does nothing
+// unless the row is the first of its token, and then sums that token's rows in row order.  The
+// blocks behind them clear the table rows of tokens that do not occur, 32 each.
+template <typename T, int W>
+__global__ void __launch_bounds__(128) embed_grad_few_kernel(
+    const T* __restrict__ dy, long long ld, const void* __restrict__ ids, int ids32,
+    long long n_ids, const int* __restrict__ id_rows, long long pad, float* __restrict__ dtable,
+    long long ld_t, long long V, int rows, int H, int slabs, int row_blocks, float scale, int add,
+    int* err) {
+  using S = SlabCols<W>;
+  constexpr int N = S::N;
+  constexpr int U = sizeof(T) == 4 && W == 8 ? 4 : 8;
+  __shared__ int tok[kFewRows];
+  __shared__ uint32_t present;
+  const int tid = threadIdx.x, wp = warp_id();
+  if (tid == 0) present = 0;
+  for (int r = tid; r < rows; r += 128)
+    tok[r] = row_token(r, ids, ids32, n_ids, id_rows, V, pad, blockIdx.x == 0 ? err : nullptr);
+  __syncthreads();
+  if (static_cast<int>(blockIdx.x) >= row_blocks) {
+    const long long lo = (static_cast<long long>(blockIdx.x) - row_blocks) * 32;
+    for (int r = tid; r < rows; r += 128)
+      if (tok[r] >= lo && tok[r] < lo + 32) atomicOr(&present, 1u << (tok[r] - lo));
+    __syncthreads();
+    for (int t = wp; t < 32; t += 4)
+      if (lo + t < V && !(present >> t & 1)) clear_row<W>(dtable + (lo + t) * ld_t, H);
+    return;
+  }
+  const int item = blockIdx.x * 4 + wp;
+  const int r = item / slabs;
+  if (r >= rows || tok[r] < 0) return;
+  const int mine = tok[r];
+  bool first = true;
+  for (int q = lane_id(); q < r; q += 32) first = first && tok[q] != mine;
+  if (!__all_sync(0xffffffffu, first)) return;
+  const S cols(item % slabs, H);
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int base = r / 32 * 32; base < rows; base += 32) {
+    const int q = base + lane_id();
+    unsigned todo = __ballot_sync(0xffffffffu, q >= r && q < rows && tok[q] == mine);
+    while (todo) {
+      Pack<T, N> k[U];
+      const int n = min(U, __popc(todo));
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < n) {
+          cols.load(dy + (base + __ffs(todo) - 1) * ld, k[u]);
+          todo &= todo - 1;
+        }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (u >= n) break;
+        float f[N];
+        unpack<T, N>(k[u], f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += f[i];
+      }
+    }
+  }
+  cols.write_run(dtable + mine * ld_t, acc, scale, add);
 }
 
 template <int W>
-__global__ void __launch_bounds__(256) zero_rows_kernel(float* __restrict__ t, long long ld,
-                                                        long long V, int H) {
-  float z[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) z[i] = 0.f;
+__global__ void __launch_bounds__(256) clear_table_kernel(float* __restrict__ t, long long ld,
+                                                          long long V, int H) {
   for (long long r = blockIdx.x * 8ll + warp_id(); r < V; r += gridDim.x * 8ll)
-    for (int c = lane_id() * W; c < H; c += 32 * W) store_f32<float, W>(t + r * ld + c, z);
+    clear_row<W>(t + r * ld, H);
 }
 
 }  // namespace cfb
@@ -278,9 +464,15 @@ int cfb_scaled_embedding_fwd(const void* table, int type, long long ld, long lon
   });
 }
 
-long long cfb_scaled_embedding_bwd_workspace(int rows, int H) {
-  const long long chunks = (rows + kChunk - 1) / kChunk;
-  return 4ll * (8 + 2ll * ((rows + 3) / 4 * 4) + 2 * chunks * H);  // bytes
+// 32-bit words: the number of sorted rows, their order, their tokens, the bits of absent tokens, and
+// the partial sums, each from a 32-byte border on
+static long long words_of_8(long long n) { return (n + 7) / 8 * 8; }
+
+long long cfb_scaled_embedding_bwd_workspace(long long V, int rows, int H) {
+  if (rows <= kFewRows) return 0;
+  const int per = chunk_rows(rows);
+  const long long chunks = (rows + per - 1) / per;
+  return 4 * (8 + 2 * words_of_8(rows) + words_of_8((V + 31) / 32) + 2 * chunks * H);
 }
 
 int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void* ids, int ids32,
@@ -290,39 +482,60 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
   if (V <= 0 || V > INT32_MAX) return -11;
   if (H == 0) return 0;
   const bool wide = H % 8 == 0 && rows_of_8(dy, ld, type) && rows_of_8(dtable, ld_t, kF32);
-  if (!add) {
-    const long long blocks = (V + 7) / 8 < 148 * 16 ? (V + 7) / 8 : 148 * 16;
-    if (wide)
-      zero_rows_kernel<8><<<blocks, 256, 0, st>>>(dtable, ld_t, V, H);
-    else
-      zero_rows_kernel<1><<<blocks, 256, 0, st>>>(dtable, ld_t, V, H);
+  if (rows == 0) {
+    if (add) return 0;
+    auto* clear = wide ? clear_table_kernel<8> : clear_table_kernel<1>;
+    clear<<<static_cast<unsigned>((V + 7) / 8), 256, 0, st>>>(dtable, ld_t, V, H);
+    return launch_status();
   }
-  if (rows == 0) return launch_status();
-  const int padded = (rows + 3) / 4 * 4;
+  const int slab = wide ? SlabCols<8>::kSlab : SlabCols<1>::kSlab;
+  const int slabs = (H + slab - 1) / slab;
+  if (rows <= kFewRows) {
+    const int row_blocks = (rows * slabs + 3) / 4;
+    const unsigned blocks = row_blocks + (add ? 0 : static_cast<unsigned>((V + 31) / 32));
+    return with_type(type, [&](auto t) {
+      using T = typename decltype(t)::type;
+      auto* kernel = wide ? embed_grad_few_kernel<T, 8> : embed_grad_few_kernel<T, 1>;
+      kernel<<<blocks, 128, 0, st>>>(static_cast<const T*>(dy), ld, ids, ids32, n_ids, id_rows,
+                                     pad, dtable, ld_t, V, rows, H, slabs, row_blocks, scale, add,
+                                     err);
+      return launch_status();
+    });
+  }
   int* n_valid = static_cast<int*>(work);
-  int* order = n_valid + 8;  // the partial sums behind it begin on a 32-byte border
-  int* stok = order + padded;
-  float* part = reinterpret_cast<float*>(stok + padded);
+  int* order = n_valid + 8;
+  int* stok = order + words_of_8(rows);
+  uint32_t* absent = reinterpret_cast<uint32_t*>(stok + words_of_8(rows));
+  float* part = reinterpret_cast<float*>(absent + words_of_8((V + 31) / 32));
   // one block for each SM where the vocabulary allows, ranges of whole warps
   long long span = ((V + 147) / 148 + 31) / 32 * 32;
   if (span > kMaxSpan) span = kMaxSpan;
   const int smem = static_cast<int>(32 * span * sizeof(int));
-  if (cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           32 * kMaxSpan * static_cast<int>(sizeof(int))) != cudaSuccess)
-    return -3;
+  static bool allowed[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             32 * kMaxSpan * static_cast<int>(sizeof(int))) != cudaSuccess)
+      return -3;
+    allowed[dev] = true;
+  }
   sort_tokens_kernel<<<static_cast<unsigned>((V + span - 1) / span), 1024, smem, st>>>(
-      ids, ids32, n_ids, id_rows, rows, V, pad, static_cast<int>(span), order, stok, n_valid, err);
-  const int W = wide ? 8 : 1;
-  const int need = (H + W - 1) / W;
-  const int threads = need >= 256 ? 256 : (need + 31) / 32 * 32;
-  const dim3 grid((rows + kChunk - 1) / kChunk, (need + threads - 1) / threads);
+      ids, ids32, n_ids, id_rows, rows, V, pad, static_cast<int>(span), order, stok, n_valid,
+      absent, err);
+  if (const int rc = launch_status()) return rc;
+  const int per = chunk_rows(rows);
+  const int chunks = (rows + per - 1) / per;
   return with_type(type, [&](auto t) {
     using T = typename decltype(t)::type;
-    auto* grad = wide ? embed_grad_kernel<T, 8> : embed_grad_kernel<T, 1>;
-    grad<<<grid, threads, 0, st>>>(static_cast<const T*>(dy), ld, order, stok, n_valid, dtable,
-                                   ld_t, part, H, scale, add);
-    auto* join = wide ? embed_join_kernel<8> : embed_join_kernel<1>;
-    join<<<grid, threads, 0, st>>>(stok, n_valid, dtable, ld_t, part, H, scale, add);
-    return launch_status();
+    const int sums = static_cast<int>((static_cast<long long>(chunks) * slabs + 3) / 4);
+    const int clears = add ? 0 : static_cast<int>((V + 31) / 32);
+    if (const int rc = launch_behind(wide ? embed_grad_kernel<T, 8> : embed_grad_kernel<T, 1>,
+                                     dim3(sums + clears), dim3(128), 0, st,
+                                     static_cast<const T*>(dy), ld, order, stok, n_valid, absent,
+                                     dtable, ld_t, part, H, slabs, per, sums, scale, add))
+      return rc;
+    return launch_behind(wide ? embed_join_kernel<8> : embed_join_kernel<1>, dim3(chunks, slabs),
+                         dim3(256), 0, st, stok, n_valid, dtable, ld_t, part, H, per, scale, add);
   });
 }
