@@ -20,13 +20,14 @@
 //   3. embed_join_kernel    the chunk in which a crossing run begins adds the partial sums up in
 //                           chunk order and writes the table row.
 //
-// A handful of rows takes one launch instead (embed_grad_few_kernel).  No atomics on floating values
-// anywhere: two runs give the same bits.
+// A handful of rows takes one launch instead (embed_grad_few_kernel).  Every element of the table is
+// written by one thread, once: two runs give the same bits.
 #include "row_types.cuh"
 
 namespace cfb {
 
 constexpr int kMaxSpan = 1024;  // tokens of one block of the sort
+constexpr int kKeyRows = 32768; // rows whose keys a block of the sort holds in shared memory
 constexpr int kFewRows = 128;   // up to here one launch does it all
 
 // Sorted positions of one warp of the gradient: few where few rows would leave SMs idle, more where
@@ -84,13 +85,15 @@ __device__ __forceinline__ void clear_row(float* t, int H) {
 // Block b places the rows of tokens [b * span, (b + 1) * span) at their sorted positions.  Each of
 // the 32 warps takes a contiguous part of the rows; hist[w][t] first counts the rows of token t in
 // part w and then, after the scan, is the next position of such a row.  A thread has eight tokens in
-// flight, and keeps them for the second pass where that is all of its part (up to 8192 rows).
+// flight; up to kKeyRows rows the second pass finds which of them are of the block in shared memory.
 __global__ void __launch_bounds__(1024) sort_tokens_kernel(
     const void* __restrict__ ids, int ids32, long long n_ids, const int* __restrict__ id_rows,
     int rows, long long V, long long pad, int span, int* __restrict__ order,
     int* __restrict__ stok, int* __restrict__ n_valid, uint32_t* __restrict__ absent, int* err) {
   constexpr int U = 8;
-  extern __shared__ int hist[];  // [32][span]
+  extern __shared__ int hist[];  // [32][span], and a 16-bit key for each of up to kKeyRows rows
+  uint16_t* keys = reinterpret_cast<uint16_t*>(hist + 32 * span);  // 1 + token - lo, 0: not ours
+  const bool keep = rows <= kKeyRows;
   __shared__ int warp_sums[32];
   __shared__ int below;
   let_next_start();
@@ -136,7 +139,10 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       less += (tok[u] >= 0 && tok[u] < lo);
-      if (tok[u] >= lo && tok[u] < hi) atomicAdd(&hist[wp * span + static_cast<int>(tok[u] - lo)], 1);
+      const int key = tok[u] >= lo && tok[u] < hi ? static_cast<int>(tok[u] - lo) : -1;
+      if (key >= 0) atomicAdd(&hist[wp * span + key], 1);
+      const int r = base + u * 32 + lane;
+      if (keep && r < r1) keys[r] = static_cast<uint16_t>(key + 1);
     }
   }
   less = __reduce_add_sync(0xffffffffu, less);
@@ -187,10 +193,15 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
   __syncthreads();
 
   for (int base = r0; base < r1; base += 32 * U) {
-    if (r1 - r0 > 32 * U) read(base, nullptr);
+    if (!keep) read(base, nullptr);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int key = tok[u] >= lo && tok[u] < hi ? static_cast<int>(tok[u] - lo) : -1;
+      const int r = base + u * 32 + lane;
+      int key = -1;
+      if (keep)
+        key = r < r1 ? static_cast<int>(keys[r]) - 1 : -1;
+      else if (tok[u] >= lo && tok[u] < hi)
+        key = static_cast<int>(tok[u] - lo);
       if (__ballot_sync(0xffffffffu, key >= 0) == 0) continue;
       const unsigned same = __match_any_sync(0xffffffffu, key);
       const int rank = __popc(same & ((1u << lane) - 1));
@@ -198,7 +209,7 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
       const int at = *next + rank;
       __syncwarp();
       if (key >= 0) {
-        order[at] = base + u * 32 + lane;
+        order[at] = r;
         stok[at] = static_cast<int>(lo) + key;
         if (rank == 0) *next = at + __popc(same);
       }
@@ -238,14 +249,28 @@ struct SlabCols {
         if (c + 32 * i < H) row[c + 32 * i] = f[i];
     }
   }
-  // Adds a run's sum to its table row, or writes it there.
+  // Adds a run's sum to its table row, or writes it there.  No other thread has these elements, so
+  // the additions of the reduction instructions happen once each and in no order that could vary;
+  // unlike a load and a store they do not make the warp wait for the table.
   __device__ __forceinline__ void write_run(float* row, const float* acc, float scale,
                                             int add) const {
     float o[N];
-    if (add) load(row, o);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = (add ? o[i] : 0.f) + scale * acc[i];
-    store(row, o);
+    for (int i = 0; i < N; ++i) o[i] = scale * acc[i];
+    if (!add) {
+      store(row, o);
+    } else if constexpr (W == 8) {
+      if (c < H)
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+          asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(row + c + i),
+                       "f"(o[i]), "f"(o[i + 1]), "f"(o[i + 2]), "f"(o[i + 3])
+                       : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c + 32 * i < H) atomicAdd(row + c + 32 * i, o[i]);
+    }
   }
 };
 
@@ -253,11 +278,12 @@ struct SlabCols {
 // part[chunk][0]: the sum of the rows of a run that began in an earlier chunk;
 // part[chunk][1]: of a run that begins here and goes on in the next chunk.
 template <typename T, int W>
-__global__ void __launch_bounds__(128, 8) embed_grad_kernel(
+__global__ void __launch_bounds__(128, 6) embed_grad_kernel(
     const T* __restrict__ dy, long long ld, const int* __restrict__ order,
     const int* __restrict__ stok, const int* __restrict__ n_valid,
     const uint32_t* __restrict__ absent, float* __restrict__ dtable, long long ld_t,
-    float* __restrict__ part, int H, int slabs, int per, int sum_blocks, float scale, int add) {
+    float* __restrict__ part, int rows, int H, int slabs, int per, int sum_blocks, float scale,
+    int add) {
   using S = SlabCols<W>;
   constexpr int N = S::N;
   constexpr int U = 4;  // rows in flight
@@ -270,17 +296,19 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
       if (none >> t & 1) clear_row<W>(dtable + (word * 32 + t) * ld_t, H);
     return;
   }
-  const int n = *n_valid;
   const int item = blockIdx.x * 4 + warp_id();
   const int chunk = item / slabs;
   const int p0 = chunk * per;
-  if (p0 >= n) return;
   const int lane = lane_id();
+  // all loads at once; what lies behind the last valid row is not used
+  const int n = *n_valid;
+  const int my_row = lane < per && p0 + lane < rows ? order[p0 + lane] : 0;
+  const int my_tok = lane < per && p0 + lane < rows ? stok[p0 + lane] : -1;
+  const int before = p0 > 0 && p0 <= rows ? stok[p0 - 1] : -1;
+  const int after = p0 + per < rows ? stok[p0 + per] : -1;
+  if (p0 >= n) return;
   const int m = min(per, n - p0);
-  const int my_row = lane < m ? order[p0 + lane] : 0;
-  const int my_tok = lane < m ? stok[p0 + lane] : -1;
-  const int before = p0 > 0 ? stok[p0 - 1] : -1;
-  const int behind = p0 + m < n ? stok[p0 + m] : -1;
+  const int behind = p0 + per < n ? after : -1;
   const bool from_before = before == __shfl_sync(0xffffffffu, my_tok, 0);
   const S cols(item % slabs, H);
   float acc[N];
@@ -324,23 +352,26 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
 template <int W>
 __global__ void __launch_bounds__(256) embed_join_kernel(
     const int* __restrict__ stok, const int* __restrict__ n_valid, float* __restrict__ dtable,
-    long long ld_t, const float* __restrict__ part, int H, int per, float scale, int add) {
+    long long ld_t, const float* __restrict__ part, int rows, int H, int per, float scale,
+    int add) {
   using S = SlabCols<W>;
   constexpr int N = S::N;
   constexpr int U = 4;
   __shared__ float share[8][32 * N];
   after_previous();
-  const int n = *n_valid;
   const int p0 = blockIdx.x * per, p1 = p0 + per;
-  if (p1 >= n) return;
-  const int tok = stok[p1 - 1];
-  if (stok[p1] != tok || (p0 > 0 && stok[p0 - 1] == tok)) return;
-  int lo = p1, hi = n;  // the first position behind the run
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if (stok[mid] == tok) lo = mid + 1; else hi = mid;
+  if (p1 >= rows) return;
+  const int n = *n_valid;
+  const int tok = stok[p1 - 1], here = stok[p1], before = p0 > 0 ? stok[p0 - 1] : -1;
+  if (p1 >= n || here != tok || before == tok) return;
+  // the chunks behind this one whose first row is of the run: 256 looked at at once
+  int chunks = 0;
+  for (int k = blockIdx.x + 1;; k += 256) {
+    const int p = (k + static_cast<int>(threadIdx.x)) * per;
+    const int more = __syncthreads_count(p < n && stok[p] == tok);
+    chunks += more;
+    if (more < 256) break;
   }
-  const int chunks = (lo - 1) / per - blockIdx.x;  // behind the first
   const int each = (chunks + 7) / 8, wp = warp_id(), lane = lane_id();
   const int k0 = blockIdx.x + 1 + wp * each, k1 = blockIdx.x + 1 + min(chunks, (wp + 1) * each);
   const S cols(blockIdx.y, H);
@@ -510,13 +541,14 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
   // one block for each SM where the vocabulary allows, ranges of whole warps
   long long span = ((V + 147) / 148 + 31) / 32 * 32;
   if (span > kMaxSpan) span = kMaxSpan;
-  const int smem = static_cast<int>(32 * span * sizeof(int));
+  const int smem = static_cast<int>(32 * span * sizeof(int)) +
+                   (rows <= kKeyRows ? (rows + 1) / 2 * 4 : 0);
   static bool allowed[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64) return -3;
   if (!allowed[dev]) {
     if (cudaFuncSetAttribute(sort_tokens_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             32 * kMaxSpan * static_cast<int>(sizeof(int))) != cudaSuccess)
+                             32 * kMaxSpan * 4 + kKeyRows * 2) != cudaSuccess)
       return -3;
     allowed[dev] = true;
   }
@@ -533,9 +565,10 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
     if (const int rc = launch_behind(wide ? embed_grad_kernel<T, 8> : embed_grad_kernel<T, 1>,
                                      dim3(sums + clears), dim3(128), 0, st,
                                      static_cast<const T*>(dy), ld, order, stok, n_valid, absent,
-                                     dtable, ld_t, part, H, slabs, per, sums, scale, add))
+                                     dtable, ld_t, part, rows, H, slabs, per, sums, scale, add))
       return rc;
     return launch_behind(wide ? embed_join_kernel<8> : embed_join_kernel<1>, dim3(chunks, slabs),
-                         dim3(256), 0, st, stok, n_valid, dtable, ld_t, part, H, per, scale, add);
+                         dim3(256), 0, st, stok, n_valid, dtable, ld_t, part, rows, H, per, scale,
+                         add);
   });
 }
