@@ -7,10 +7,11 @@
 // of equal tokens in one fixed order, whatever the scheduling and however uneven the tokens are
 // (text repeats a few tokens very often, a padded batch has one token in a third of its rows):
 //
-//   1. sort_tokens_kernel   a stable counting sort of the rows by token.  Each block owns a range of
-//                           tokens, reads all the tokens, and so knows both where its range begins
-//                           in the sorted order and which rows are in it: one launch, no exchange
-//                           between blocks.
+//   1. sort_tokens_kernel   a stable counting sort of the rows by token.  Each block owns the tokens
+//                           with one remainder, reads all the tokens, and so knows both where its
+//                           tokens begin in the sorted order and which rows they are in: one launch,
+//                           no exchange between blocks.  (A text's frequent tokens have neighbouring
+//                           ids; by ranges one block would have had half of all rows.)
 //   2. embed_grad_kernel    chunks of sorted positions, a warp each (and per slab of columns): a run
 //                           of equal tokens that lies inside a chunk is summed and written by that
 //                           warp alone; a run that crosses a chunk's border leaves a partial sum.
@@ -28,6 +29,7 @@ namespace cfb {
 
 constexpr int kMaxSpan = 1024;  // tokens of one block of the sort
 constexpr int kKeyRows = 32768; // rows whose keys a block of the sort holds in shared memory
+constexpr int kClear = 8;       // table rows that one block clears
 constexpr int kFewRows = 128;   // up to here one launch does it all
 
 // Sorted positions of one warp of the gradient: few where few rows would leave SMs idle, more where
@@ -82,52 +84,57 @@ __device__ __forceinline__ void clear_row(float* t, int H) {
   for (int c = lane_id() * W; c < H; c += 32 * W) store_f32<float, W>(t + c, z);
 }
 
-// Block b places the rows of tokens [b * span, (b + 1) * span) at their sorted positions.  Each of
-// the 32 warps takes a contiguous part of the rows; hist[w][t] first counts the rows of token t in
-// part w and then, after the scan, is the next position of such a row.  A thread has eight tokens in
+// Block b of 2^shift places the rows of the tokens t 2^shift + b at their sorted positions, which are
+// by block and t.  Each of the 32 warps takes a contiguous part of the rows; hist[w][t] first counts
+// the rows of the block's token t in part w and then, after the scan, is the next position of such a
+// row.  A thread has eight tokens in
 // flight; up to kKeyRows rows the second pass finds which of them are of the block in shared memory.
 __global__ void __launch_bounds__(1024) sort_tokens_kernel(
-    const void* __restrict__ ids, int ids32, long long n_ids, const int* __restrict__ id_rows,
-    int rows, long long V, long long pad, int span, int* __restrict__ order,
+    const void* __restrict__ ids, int ids32, unsigned n_ids, const int* __restrict__ id_rows,
+    int rows, int V, int pad, int shift, int span, int* __restrict__ order,
     int* __restrict__ stok, int* __restrict__ n_valid, uint32_t* __restrict__ absent, int* err) {
   constexpr int U = 8;
   extern __shared__ int hist[];  // [32][span], and a 16-bit key for each of up to kKeyRows rows
-  uint16_t* keys = reinterpret_cast<uint16_t*>(hist + 32 * span);  // 1 + token - lo, 0: not ours
+  uint16_t* keys = reinterpret_cast<uint16_t*>(hist + 32 * span);  // 1 + t, 0: not ours
   const bool keep = rows <= kKeyRows;
   __shared__ int warp_sums[32];
   __shared__ int below;
   let_next_start();
   const int tid = threadIdx.x, lane = lane_id(), wp = warp_id();
-  const long long lo = static_cast<long long>(blockIdx.x) * span;
-  const long long hi = min(V, lo + span);
-  if (blockIdx.x != 0) err = nullptr;  // one block reports
+  const int me = blockIdx.x, mask = (1 << shift) - 1;
+  const int mine = (V - me + mask) >> shift;  // tokens of this block
   const int part = (rows + 1023) / 1024 * 32;
   const int r0 = min(rows, wp * part), r1 = min(rows, r0 + part);
   int tok[U];
-  const auto read = [&](int base, int* e) {
+  // Tokens as 32-bit numbers, -1 for a row without one: every comparison below is unsigned.
+  const auto read = [&](int base, bool report) {
     int id[U];
+    int2 t[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int r = base + u * 32 + lane;
       id[u] = r < r1 ? (id_rows ? id_rows[r] : r) : -1;
     }
-    long long t[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool ok = id[u] >= 0 && id[u] < n_ids;
-      t[u] = !ok ? -1 : ids32 ? static_cast<const int*>(ids)[id[u]]
-                              : static_cast<const long long*>(ids)[id[u]];
+      t[u] = make_int2(-1, 0);
+      if (static_cast<unsigned>(id[u]) < n_ids) {
+        if (ids32)
+          t[u].x = static_cast<const int*>(ids)[id[u]];
+        else
+          t[u] = static_cast<const int2*>(ids)[id[u]];
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const bool any = base + u * 32 + lane < r1;
-      const bool padding = pad >= 0 && t[u] == pad;
-      const bool ok = t[u] >= 0 && t[u] < V;  // -1 above for a row id outside ids
-      if (e && any && !ok && !padding) atomicCAS(e, 0, kErrBounds);
-      tok[u] = any && ok && !padding ? static_cast<int>(t[u]) : -1;
+      const bool ok = t[u].y == 0 && static_cast<unsigned>(t[u].x) < static_cast<unsigned>(V);
+      const bool padding = pad >= 0 && t[u].y == 0 && t[u].x == pad;
+      tok[u] = ok && !padding ? t[u].x : -1;
+      if (report && base + u * 32 + lane < r1 && !ok && !padding) atomicCAS(err, 0, kErrBounds);
     }
   };
-  read(r0, err);  // under way while the counts are cleared
+  const bool report = blockIdx.x == 0 && err;  // one block does
+  read(r0, report);  // under way while the counts are cleared
   for (int i = tid * 4; i < 32 * span; i += 4096)
     *reinterpret_cast<int4*>(hist + i) = make_int4(0, 0, 0, 0);
   if (tid == 0) below = 0;
@@ -135,21 +142,21 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
 
   int less = 0;
   for (int base = r0; base < r1; base += 32 * U) {
-    if (base != r0) read(base, err);
+    if (base != r0) read(base, report);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      less += (tok[u] >= 0 && tok[u] < lo);
-      const int key = tok[u] >= lo && tok[u] < hi ? static_cast<int>(tok[u] - lo) : -1;
-      if (key >= 0) atomicAdd(&hist[wp * span + key], 1);
+      const int owner = tok[u] >= 0 ? tok[u] & mask : INT32_MAX;
+      less += owner < me;
+      if (owner == me) atomicAdd(&hist[wp * span + (tok[u] >> shift)], 1);
       const int r = base + u * 32 + lane;
-      if (keep && r < r1) keys[r] = static_cast<uint16_t>(key + 1);
+      if (keep && r < r1) keys[r] = static_cast<uint16_t>(owner == me ? (tok[u] >> shift) + 1 : 0);
     }
   }
   less = __reduce_add_sync(0xffffffffu, less);
   if (lane == 0 && less) atomicAdd(&below, less);
   __syncthreads();
 
-  // exclusive scan over (token, warp); thread t owns token lo + t (span <= 1024)
+  // exclusive scan over (token, warp); thread t has the block's token t (span <= 1024)
   int count[32];
   int tot = 0;
   if (tid < span) {
@@ -159,8 +166,8 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
     for (int w = 0; w < 32; ++w) tot += count[w];
   }
   if (tid < span) {  // tokens without a row, a bit each
-    const uint32_t none = __ballot_sync(0xffffffffu, tot == 0 && lo + tid < hi);
-    if (lane == 0 && lo + tid < hi) absent[(lo + tid) / 32] = none;
+    const uint32_t none = __ballot_sync(0xffffffffu, tot == 0 && tid < mine);
+    if (lane == 0) absent[(me * span + tid) / 32] = none;
   }
   int inc = tot;
 #pragma unroll
@@ -193,15 +200,15 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
   __syncthreads();
 
   for (int base = r0; base < r1; base += 32 * U) {
-    if (!keep) read(base, nullptr);
+    if (!keep) read(base, false);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int r = base + u * 32 + lane;
       int key = -1;
       if (keep)
         key = r < r1 ? static_cast<int>(keys[r]) - 1 : -1;
-      else if (tok[u] >= lo && tok[u] < hi)
-        key = static_cast<int>(tok[u] - lo);
+      else if (tok[u] >= 0 && (tok[u] & mask) == me)
+        key = tok[u] >> shift;
       if (__ballot_sync(0xffffffffu, key >= 0) == 0) continue;
       const unsigned same = __match_any_sync(0xffffffffu, key);
       const int rank = __popc(same & ((1u << lane) - 1));
@@ -210,7 +217,7 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
       __syncwarp();
       if (key >= 0) {
         order[at] = r;
-        stok[at] = static_cast<int>(lo) + key;
+        stok[at] = (key << shift) + me;
         if (rank == 0) *next = at + __popc(same);
       }
       __syncwarp();
@@ -282,21 +289,31 @@ __global__ void __launch_bounds__(128, 6) embed_grad_kernel(
     const T* __restrict__ dy, long long ld, const int* __restrict__ order,
     const int* __restrict__ stok, const int* __restrict__ n_valid,
     const uint32_t* __restrict__ absent, float* __restrict__ dtable, long long ld_t,
-    float* __restrict__ part, int rows, int H, int slabs, int per, int sum_blocks, float scale,
-    int add) {
+    float* __restrict__ part, int rows, int H, int slabs, int per, int sum_blocks, int shift,
+    int span, int vocab, float scale, int add) {
   using S = SlabCols<W>;
   constexpr int N = S::N;
   constexpr int U = 4;  // rows in flight
   after_previous();
   let_next_start();
-  if (static_cast<int>(blockIdx.x) >= sum_blocks) {  // clear what does not occur of 32 tokens
-    const long long word = static_cast<long long>(blockIdx.x) - sum_blocks;
-    const uint32_t none = absent[word];
-    for (int t = warp_id(); t < 32; t += 4)
-      if (none >> t & 1) clear_row<W>(dtable + (word * 32 + t) * ld_t, H);
+  // blocks that sum and blocks that clear in turn, as long as there are both: the ones wait for
+  // their rows, the others keep the memory busy
+  const int clear_blocks = static_cast<int>(gridDim.x) - sum_blocks;
+  const int both = 2 * min(sum_blocks, clear_blocks);
+  const int b = blockIdx.x;
+  const bool sums = b < both ? b % 2 == 0 : sum_blocks > clear_blocks;
+  const int block = b < both ? b / 2 : b - both / 2;
+  if (!sums) {  // clear what does not occur of kClear neighbouring tokens
+#pragma unroll
+    for (int i = 0; i < kClear / 4; ++i) {
+      const int token = block * kClear + i * 4 + warp_id();
+      const int place = (token & ((1 << shift) - 1)) * span + (token >> shift);
+      if (token < vocab && (absent[place / 32] >> (place % 32) & 1))
+        clear_row<W>(dtable + token * ld_t, H);
+    }
     return;
   }
-  const int item = blockIdx.x * 4 + warp_id();
+  const int item = block * 4 + warp_id();
   const int chunk = item / slabs;
   const int p0 = chunk * per;
   const int lane = lane_id();
@@ -347,8 +364,10 @@ __global__ void __launch_bounds__(128, 6) embed_grad_kernel(
   }
 }
 
-// The run that begins in chunk blockIdx.x and goes on behind it: its partial sums in chunk order.
-// Eight warps take a contiguous share of the chunks each; the shares are added in their order.
+// The runs that begin in chunks 8 blockIdx.x .. + 8 and go on behind their chunk: their partial sums
+// in chunk order.  A warp has a chunk, and sums a run of up to eight more chunks by itself; of a
+// longer run, of which a block can only have one, eight warps take a contiguous share of the chunks
+// each, and the shares are added in their order.
 template <int W>
 __global__ void __launch_bounds__(256) embed_join_kernel(
     const int* __restrict__ stok, const int* __restrict__ n_valid, float* __restrict__ dtable,
@@ -358,39 +377,62 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
   constexpr int N = S::N;
   constexpr int U = 4;
   __shared__ float share[8][32 * N];
+  __shared__ int long_chunk;
   after_previous();
-  const int p0 = blockIdx.x * per, p1 = p0 + per;
-  if (p1 >= rows) return;
-  const int n = *n_valid;
-  const int tok = stok[p1 - 1], here = stok[p1], before = p0 > 0 ? stok[p0 - 1] : -1;
-  if (p1 >= n || here != tok || before == tok) return;
-  // the chunks behind this one whose first row is of the run: 256 looked at at once
+  const int wp = warp_id(), lane = lane_id();
+  const int chunk = blockIdx.x * 8 + wp;
+  const int p0 = chunk * per, p1 = p0 + per;
+  const S cols(blockIdx.y, H);
+  float acc[N];
+  // the sum of part[k][0] over [k0, k1) added to acc
+  const auto add_parts = [&](int k0, int k1) {
+#pragma unroll 1
+    for (int k = k0; k < k1; k += U) {
+      Pack<float, N> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u < k1) cols.template load<float>(part + 2ll * (k + u) * H, v[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k + u >= k1) break;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += v[u].v[i];
+      }
+    }
+  };
+  if (threadIdx.x == 0) long_chunk = -1;
+  __syncthreads();
+  if (p1 < rows) {
+    // all loads at once; what lies behind the last valid row is not used
+    const int n = *n_valid;
+    const int tok = stok[p1 - 1], before = p0 > 0 ? stok[p0 - 1] : -1;
+    const int q = p1 + lane * per;  // the first rows of the 32 chunks behind
+    const int ahead = q < rows ? stok[q] : -1;
+    const int more = __popc(__ballot_sync(0xffffffffu, q < n && ahead == tok));
+    if (more > 8 && before != tok) {
+      if (lane == 0) long_chunk = chunk;
+    } else if (more > 0 && before != tok) {
+      cols.load(part + (2ll * chunk + 1) * H, acc);
+      add_parts(chunk + 1, chunk + 1 + more);
+      cols.write_run(dtable + tok * ld_t, acc, scale, add);
+    }
+  }
+  __syncthreads();
+  const int from = long_chunk;
+  if (from < 0) return;
+  const int n = *n_valid, tok = stok[(from + 1) * per];
   int chunks = 0;
-  for (int k = blockIdx.x + 1;; k += 256) {
-    const int p = (k + static_cast<int>(threadIdx.x)) * per;
+  for (int k = from + 1;; k += 256) {
+    const long long p = static_cast<long long>(k + threadIdx.x) * per;
     const int more = __syncthreads_count(p < n && stok[p] == tok);
     chunks += more;
     if (more < 256) break;
   }
-  const int each = (chunks + 7) / 8, wp = warp_id(), lane = lane_id();
-  const int k0 = blockIdx.x + 1 + wp * each, k1 = blockIdx.x + 1 + min(chunks, (wp + 1) * each);
-  const S cols(blockIdx.y, H);
-  float acc[N];
+  const int each = (chunks + 7) / 8;
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  if (wp == 0) cols.load(part + (2ll * blockIdx.x + 1) * H, acc);
-  for (int k = k0; k < k1; k += U) {
-    Pack<float, N> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k + u < k1) cols.template load<float>(part + 2ll * (k + u) * H, v[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (k + u >= k1) break;
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += v[u].v[i];
-    }
-  }
+  if (wp == 0) cols.load(part + (2ll * from + 1) * H, acc);
+  add_parts(from + 1 + wp * each, from + 1 + min(chunks, (wp + 1) * each));
 #pragma unroll
   for (int i = 0; i < N; ++i) share[wp][i * 32 + lane] = acc[i];
   __syncthreads();
@@ -499,11 +541,22 @@ int cfb_scaled_embedding_fwd(const void* table, int type, long long ld, long lon
 // the partial sums, each from a 32-byte border on
 static long long words_of_8(long long n) { return (n + 7) / 8 * 8; }
 
+// Blocks of the sort (a power of two) and the places each has for its tokens (whole warps).
+struct SortPlan {
+  int shift, span;
+  long long words() const { return (static_cast<long long>(span) << shift) / 32; }
+};
+static SortPlan sort_plan(long long V) {
+  int shift = 7;  // 128 blocks, or as many as keep the tokens of one under kMaxSpan
+  while (((V - 1) >> shift) + 1 > kMaxSpan) ++shift;
+  return {shift, static_cast<int>((((V - 1) >> shift) + 32) / 32 * 32)};
+}
+
 long long cfb_scaled_embedding_bwd_workspace(long long V, int rows, int H) {
   if (rows <= kFewRows) return 0;
   const int per = chunk_rows(rows);
   const long long chunks = (rows + per - 1) / per;
-  return 4 * (8 + 2 * words_of_8(rows) + words_of_8((V + 31) / 32) + 2 * chunks * H);
+  return 4 * (8 + 2 * words_of_8(rows) + words_of_8(sort_plan(V).words()) + 2 * chunks * H);
 }
 
 int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void* ids, int ids32,
@@ -537,11 +590,9 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
   int* order = n_valid + 8;
   int* stok = order + words_of_8(rows);
   uint32_t* absent = reinterpret_cast<uint32_t*>(stok + words_of_8(rows));
-  float* part = reinterpret_cast<float*>(absent + words_of_8((V + 31) / 32));
-  // one block for each SM where the vocabulary allows, ranges of whole warps
-  long long span = ((V + 147) / 148 + 31) / 32 * 32;
-  if (span > kMaxSpan) span = kMaxSpan;
-  const int smem = static_cast<int>(32 * span * sizeof(int)) +
+  const SortPlan plan = sort_plan(V);
+  float* part = reinterpret_cast<float*>(absent + words_of_8(plan.words()));
+  const int smem = static_cast<int>(32 * plan.span * sizeof(int)) +
                    (rows <= kKeyRows ? (rows + 1) / 2 * 4 : 0);
   static bool allowed[64] = {};
   int dev = 0;
@@ -552,22 +603,24 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
       return -3;
     allowed[dev] = true;
   }
-  sort_tokens_kernel<<<static_cast<unsigned>((V + span - 1) / span), 1024, smem, st>>>(
-      ids, ids32, n_ids, id_rows, rows, V, pad, static_cast<int>(span), order, stok, n_valid,
-      absent, err);
+  sort_tokens_kernel<<<1u << plan.shift, 1024, smem, st>>>(
+      ids, ids32, static_cast<unsigned>(n_ids < INT32_MAX ? n_ids : INT32_MAX), id_rows, rows,
+      static_cast<int>(V), pad <= INT32_MAX ? static_cast<int>(pad) : -1, plan.shift, plan.span,
+      order, stok, n_valid, absent, err);
   if (const int rc = launch_status()) return rc;
   const int per = chunk_rows(rows);
   const int chunks = (rows + per - 1) / per;
   return with_type(type, [&](auto t) {
     using T = typename decltype(t)::type;
     const int sums = static_cast<int>((static_cast<long long>(chunks) * slabs + 3) / 4);
-    const int clears = add ? 0 : static_cast<int>((V + 31) / 32);
+    const int clears = add ? 0 : static_cast<int>((V + kClear - 1) / kClear);
     if (const int rc = launch_behind(wide ? embed_grad_kernel<T, 8> : embed_grad_kernel<T, 1>,
                                      dim3(sums + clears), dim3(128), 0, st,
                                      static_cast<const T*>(dy), ld, order, stok, n_valid, absent,
-                                     dtable, ld_t, part, rows, H, slabs, per, sums, scale, add))
+                                     dtable, ld_t, part, rows, H, slabs, per, sums, plan.shift,
+                                     plan.span, static_cast<int>(V), scale, add))
       return rc;
-    return launch_behind(wide ? embed_join_kernel<8> : embed_join_kernel<1>, dim3(chunks, slabs),
+    return launch_behind(wide ? embed_join_kernel<8> : embed_join_kernel<1>, dim3((chunks + 7) / 8, slabs),
                          dim3(256), 0, st, stok, n_valid, dtable, ld_t, part, rows, H, per, scale,
                          add);
   });
