@@ -285,7 +285,7 @@ struct SlabCols {
 // part[chunk][0]: the sum of the rows of a run that began in an earlier chunk;
 // part[chunk][1]: of a run that begins here and goes on in the next chunk.
 template <typename T, int W>
-__global__ void __launch_bounds__(128, 6) embed_grad_kernel(
+__global__ void __launch_bounds__(128, 8) embed_grad_kernel(
     const T* __restrict__ dy, long long ld, const int* __restrict__ order,
     const int* __restrict__ stok, const int* __restrict__ n_valid,
     const uint32_t* __restrict__ absent, float* __restrict__ dtable, long long ld_t,
@@ -328,9 +328,9 @@ __global__ void __launch_bounds__(128, 6) embed_grad_kernel(
   const int behind = p0 + per < n ? after : -1;
   const bool from_before = before == __shfl_sync(0xffffffffu, my_tok, 0);
   const S cols(item % slabs, H);
-  float acc[N];
+  F2 acc[N / 2];
 #pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int i = 0; i < N / 2; ++i) acc[i] = f2(0.f);
   bool head = from_before;  // acc sums the run that began before the chunk
 #pragma unroll 1
   for (int j = 0; j < m; j += U) {
@@ -343,22 +343,27 @@ __global__ void __launch_bounds__(128, 6) embed_grad_kernel(
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (j + u >= m) break;
-      float f[N];
-      unpack<T, N>(k[u], f);
+      F2 f[N / 2];
+      unpack_f2<T, N>(k[u], f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] += f[i];
+      for (int i = 0; i < N / 2; ++i) acc[i] = acc[i] + f[i];
       const int tok = __shfl_sync(0xffffffffu, my_tok, j + u);
       const bool last = j + u + 1 == m;
       const int next = __shfl_sync(0xffffffffu, my_tok, (j + u + 1) & 31);
       const bool goes_on = (last ? behind : next) == tok;
       if (goes_on && !last) continue;
-      if (head || goes_on) {
-        cols.store(part + (2ll * chunk + (head ? 0 : 1)) * H, acc);
-      } else {
-        cols.write_run(dtable + tok * ld_t, acc, scale, add);
-      }
+      float sum[N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      for (int i = 0; i < N / 2; ++i) {
+        sum[2 * i] = halves(acc[i]).x;
+        sum[2 * i + 1] = halves(acc[i]).y;
+        acc[i] = f2(0.f);
+      }
+      if (head || goes_on) {
+        cols.store(part + (2ll * chunk + (head ? 0 : 1)) * H, sum);
+      } else {
+        cols.write_run(dtable + tok * ld_t, sum, scale, add);
+      }
       head = false;
     }
   }
