@@ -794,106 +794,168 @@ void zero_unless_error(Tensor& buf, const Tensor& err) {
                "zero_unless_error");
 }
 
-// ---- row operators around the blocks (argument checks of shapes and types: ops/fused.py)
+// ---- row operators around the blocks
+// Refusals are ValueErrors, as those of the CPU path (ops/fused.py) of the same functions.
 inline int type_code(const Tensor& t, const char* name) {
   switch (t.scalar_type()) {
     case at::kBFloat16: return kBF16;
     case at::kHalf: return kF16;
     case at::kFloat: return kF32;
-    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32"); return -1;
+    default: TORCH_CHECK_VALUE(false, name, " must be bfloat16, float16 or float32"); return -1;
   }
 }
 // A tensor of the operator's device (absent tensors pass).
 inline void same_device(const Tensor& first, const c10::optional<Tensor>& t, const char* name) {
   if (t.has_value() && t->defined())
-    TORCH_CHECK(t->device() == first.device(), name, " is on ", t->device(), ", not on ",
-                first.device());
+    TORCH_CHECK_VALUE(t->device() == first.device(), name, " is on ", t->device(), ", not on ",
+                      first.device());
+}
+// [rows, H] with columns next to each other and rows that do not overlap (rows < 0: any number).
+inline void check_rows(const Tensor& t, int64_t rows, int64_t H, const char* what,
+                       const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 2 && t.size(1) == H && (t.stride(1) == 1 || H <= 1) &&
+                        (t.stride(0) >= H || t.size(0) <= 1) && (rows < 0 || t.size(0) == rows),
+                    what, ": ", name, " must be row-major [", rows, ", ", H, "], got ", t.sizes());
+}
+inline void check_vector(const Tensor& t, int64_t n, at::ScalarType type, const char* what,
+                         const char* name) {
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous(),
+                    what, ": ", name, " must be contiguous ", type, " [", n, "]");
 }
 inline int row_count(int64_t rows, const char* what) {
-  TORCH_CHECK(rows < (1ll << 30), what, ": ", rows, " rows");
+  TORCH_CHECK_VALUE(rows < (1ll << 30), what, ": ", rows, " rows");
   return static_cast<int>(rows);
+}
+inline bool is_index(const Tensor& t) {
+  return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt;
 }
 
 // out[r] = scale * table[ids[r]]
-void scaled_embedding_fwd(const Tensor& table, const Tensor& ids, Tensor& out, double scale) {
-  check_cuda(table, "table");
-  same_device(table, ids, "ids");
-  same_device(table, out, "out");
+Tensor scaled_embedding_fwd(const Tensor& table, const Tensor& ids_in, double scale,
+                            const c10::optional<Tensor>& out_in) {
+  const char* what = "scaled_embedding_fwd";
+  TORCH_CHECK_VALUE(table.dim() == 2, what, ": table must be [V, H]");
+  const int64_t H = table.size(1);
+  check_rows(table, -1, H, what, "table");
+  TORCH_CHECK_VALUE(is_index(ids_in), what, ": ids must be int64 or int32");
+  same_device(table, ids_in, "ids");
+  same_device(table, out_in, "out");
   const c10::cuda::CUDAGuard guard(table.device());
+  const Tensor ids = ids_in.contiguous();
+  const int rows = row_count(ids.numel(), what);
+  if (out_in.has_value()) check_rows(*out_in, rows, H, what, "out");
+  Tensor out = out_in.has_value() ? *out_in : at::empty({rows, H}, table.options());
   CFB_CHECK_RC(cfb_scaled_embedding_fwd(
                    table.data_ptr(), type_code(table, "table"), table.stride(0), table.size(0),
                    ids.data_ptr(), ids.scalar_type() == at::kInt, out.data_ptr(),
-                   type_code(out, "out"), out.stride(0),
-                   row_count(ids.numel(), "scaled_embedding_fwd"), table.size(1),
+                   type_code(out, "out"), out.stride(0), rows, static_cast<int>(H),
                    static_cast<float>(scale), err_word(table.get_device()).data_ptr<int>(),
                    cur_stream()),
-               "scaled_embedding_fwd");
+               what);
+  return out;
 }
 
 // dtable[v] (+)= scale * sum of the dy rows of token v
-void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids, const c10::optional<Tensor>& id_rows,
-                          Tensor& dtable, double scale, int64_t pad, bool accumulate) {
-  check_cuda(dy, "dy");
-  same_device(dy, ids, "ids");
+void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids_in, Tensor& dtable, double scale,
+                          const c10::optional<Tensor>& id_rows, c10::optional<int64_t> padding_idx,
+                          bool accumulate) {
+  const char* what = "scaled_embedding_bwd";
+  TORCH_CHECK_VALUE(dy.dim() == 2, what, ": dy must be [R, H]");
+  const int64_t H64 = dy.size(1);
+  check_rows(dy, -1, H64, what, "dy");
+  check_rows(dtable, -1, H64, what, "dtable");
+  TORCH_CHECK_VALUE(dtable.scalar_type() == at::kFloat, what, ": dtable must be fp32");
+  TORCH_CHECK_VALUE(is_index(ids_in), what, ": ids must be int64 or int32");
+  TORCH_CHECK_VALUE(!padding_idx.has_value() || *padding_idx >= 0, what,
+                    ": padding_idx is negative");
+  if (id_rows.has_value())
+    check_vector(*id_rows, dy.size(0), at::kInt, what, "id_rows");
+  else
+    TORCH_CHECK_VALUE(ids_in.numel() == dy.size(0), what, ": ", ids_in.numel(), " ids for ",
+                      dy.size(0), " rows");
+  same_device(dy, ids_in, "ids");
   same_device(dy, id_rows, "id_rows");
   same_device(dy, dtable, "dtable");
   const c10::cuda::CUDAGuard guard(dy.device());
-  const int rows = row_count(dy.size(0), "scaled_embedding_bwd"), H = dy.size(1);
+  const Tensor ids = ids_in.contiguous();
+  const int rows = row_count(dy.size(0), what), H = static_cast<int>(H64);
   Tensor work;
   const int64_t bytes = cfb_scaled_embedding_bwd_workspace(dtable.size(0), rows, H);
   if (bytes > 0) work = at::empty({bytes}, dy.options().dtype(at::kByte));
   CFB_CHECK_RC(cfb_scaled_embedding_bwd(
                    dy.data_ptr(), type_code(dy, "dy"), dy.stride(0), ids.data_ptr(),
-                   ids.scalar_type() == at::kInt, ids.numel(), opt_ptr<int>(id_rows), pad,
-                   dtable.data_ptr<float>(), dtable.stride(0), dtable.size(0), rows, H,
-                   static_cast<float>(scale), accumulate, bytes > 0 ? work.data_ptr() : nullptr,
+                   ids.scalar_type() == at::kInt, ids.numel(), opt_ptr<int>(id_rows),
+                   padding_idx.value_or(-1), dtable.data_ptr<float>(), dtable.stride(0),
+                   dtable.size(0), rows, H, static_cast<float>(scale), accumulate,
+                   bytes > 0 ? work.data_ptr() : nullptr,
                    err_word(dy.get_device()).data_ptr<int>(), cur_stream()),
-               "scaled_embedding_bwd");
+               what);
 }
 
-CfbBlockNorms block_norms_args(const Tensor& h, const c10::optional<Tensor>& x, int resid_type,
+// Checks what both directions share; T rows of h.
+CfbBlockNorms block_norms_args(const char* what, const Tensor& h, const c10::optional<Tensor>& x,
                                const Tensor& w_post, const c10::optional<Tensor>& w_pre,
                                const c10::optional<Tensor>& gate, double block_scale,
                                double resid_scale) {
   CfbBlockNorms p = {};
+  TORCH_CHECK_VALUE(h.dim() == 2, what, ": h must be [T, H]");
+  const int64_t T = h.size(0), H = h.size(1);
+  check_rows(h, T, H, what, "h");
+  TORCH_CHECK_VALUE(H <= kBlockNormsMaxH, what, ": hidden size ", H, " is over ",
+                    kBlockNormsMaxH);
   p.type = type_code(h, "h");
-  p.resid_type = resid_type;
-  p.H = h.size(1);
-  TORCH_CHECK(p.H <= kBlockNormsMaxH, "block norms: hidden size ", p.H, " is over ",
-              kBlockNormsMaxH);
+  p.H = static_cast<int>(H);
   p.h = h.data_ptr();
   p.ld_h = h.stride(0);
-  if (x.has_value() && x->defined()) {
+  if (x.has_value()) {
+    check_rows(*x, T, H, what, "x (y)");
     p.x = x->data_ptr();
     p.ld_x = x->stride(0);
   }
+  check_vector(w_post, H, h.scalar_type(), what, "w_post");
+  if (w_pre.has_value()) check_vector(*w_pre, H, h.scalar_type(), what, "w_pre");
   p.w_post = w_post.data_ptr();
   p.w_pre = opt_ptr<void>(w_pre);
-  if (gate.has_value() && gate->defined()) {
+  if (gate.has_value()) {
+    if (gate->dim() == 1) {
+      check_vector(*gate, H, h.scalar_type(), what, "a channel's gate");
+      p.gate_kind = kGateChannel;
+    } else if (gate->dim() == 2 && gate->size(1) == 1 && gate->scalar_type() == at::kFloat) {
+      TORCH_CHECK_VALUE(gate->size(0) == T, what, ": a token's gate must be fp32 [", T, ", 1]");
+      p.gate_kind = kGateToken;
+      p.ld_gate = gate->stride(0);
+    } else {
+      check_rows(*gate, T, H, what, "an element's gate");
+      TORCH_CHECK_VALUE(gate->scalar_type() == h.scalar_type(), what, ": an element's gate must be ",
+                        h.scalar_type());
+      p.gate_kind = kGateElement;
+      p.ld_gate = gate->stride(0);
+    }
     p.gate = gate->data_ptr();
-    p.ld_gate = gate->dim() == 2 ? gate->stride(0) : 0;
-    p.gate_kind = gate->dim() == 1 ? kGateChannel
-                  : gate->scalar_type() == at::kFloat && gate->size(1) == 1 ? kGateToken
-                                                                             : kGateElement;
   }
   p.block_scale = static_cast<float>(block_scale);
   p.resid_scale = static_cast<float>(resid_scale);
-  check_cuda(h, "h");
-  same_device(h, x, "x");
+  same_device(h, x, "x (y)");
   same_device(h, w_post, "w_post");
   same_device(h, w_pre, "w_pre");
   same_device(h, gate, "gate");
   return p;
 }
+inline int resid_code(const char* what, const Tensor& t, const Tensor& h, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == h.scalar_type() || t.scalar_type() == at::kFloat, what, ": ",
+                    name, " must be ", h.scalar_type(), " or fp32");
+  return type_code(t, name);
+}
 
-// (y, n, rstd_post, rstd_pre); n and rstd_pre are undefined without w_pre
+// (y, n, rstd_post, rstd_pre); n and rstd_pre are None without w_pre
 std::tuple<Tensor, c10::optional<Tensor>, Tensor, c10::optional<Tensor>> block_norms_fwd(
     const Tensor& h, const Tensor& x, const Tensor& w_post, const c10::optional<Tensor>& w_pre,
     double eps, const c10::optional<Tensor>& gate, double block_scale, double resid_scale) {
-  const CfbBlockNorms p = block_norms_args(h, x, type_code(x, "x"), w_post, w_pre, gate,
-                                           block_scale, resid_scale);
+  const char* what = "block_norms_fwd";
+  CfbBlockNorms p = block_norms_args(what, h, x, w_post, w_pre, gate, block_scale, resid_scale);
+  p.resid_type = resid_code(what, x, h, "x");
   const c10::cuda::CUDAGuard guard(h.device());
-  const int rows = row_count(h.size(0), "block_norms_fwd");
+  const int rows = row_count(h.size(0), what);
   const auto f32 = h.options().dtype(at::kFloat);
   Tensor y = at::empty({rows, p.H}, x.options()), rstd_post = at::empty({rows}, f32);
   c10::optional<Tensor> n, rstd_pre;
@@ -905,7 +967,7 @@ std::tuple<Tensor, c10::optional<Tensor>, Tensor, c10::optional<Tensor>> block_n
                                    p.w_pre ? n->data_ptr() : nullptr, rstd_post.data_ptr<float>(),
                                    p.w_pre ? rstd_pre->data_ptr<float>() : nullptr, rows,
                                    cur_stream()),
-               "block_norms_fwd");
+               what);
   return {y, n, rstd_post, rstd_pre};
 }
 
@@ -917,10 +979,38 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> block_norms_bwd(
     const c10::optional<Tensor>& dw_pre, const c10::optional<Tensor>& gate,
     const c10::optional<Tensor>& dgate, double block_scale, double resid_scale,
     const c10::optional<Tensor>& rows, bool accumulate) {
-  const Tensor& up = dy.has_value() ? *dy : *dn;
-  const Tensor& resid = y.has_value() ? *y : *dy;
-  const CfbBlockNorms p = block_norms_args(h, y, type_code(resid, "y"), w_post, w_pre, gate,
-                                           block_scale, resid_scale);
+  const char* what = "block_norms_bwd";
+  const bool pre = w_pre.has_value();
+  TORCH_CHECK_VALUE(dn.has_value() == pre && y.has_value() == pre && rstd_pre.has_value() == pre &&
+                        dw_pre.has_value() == pre && (pre || dy.has_value()),
+                    what, ": dn, y, rstd_pre and dw_pre go with w_pre, and one of dy and dn is needed");
+  CfbBlockNorms p = block_norms_args(what, h, y, w_post, w_pre, gate, block_scale, resid_scale);
+  const int64_t T = h.size(0), H = h.size(1);
+  const Tensor& up = pre ? *dn : *dy;
+  const Tensor& resid = pre ? *y : *dy;
+  TORCH_CHECK_VALUE(up.dim() == 2, what, ": dy and dn must be [R, ", H, "]");
+  const int64_t R64 = up.size(0);
+  p.resid_type = resid_code(what, resid, h, "y (dy)");
+  if (dy.has_value()) {
+    check_rows(*dy, R64, H, what, "dy");
+    TORCH_CHECK_VALUE(dy->scalar_type() == resid.scalar_type(), what, ": dy must be ",
+                      resid.scalar_type());
+  }
+  if (pre) {
+    check_rows(*dn, R64, H, what, "dn");
+    TORCH_CHECK_VALUE(dn->scalar_type() == h.scalar_type(), what, ": dn must be ", h.scalar_type());
+    check_vector(*rstd_pre, T, at::kFloat, what, "rstd_pre");
+    check_vector(*dw_pre, H, at::kFloat, what, "dw_pre");
+  }
+  check_vector(rstd_post, T, at::kFloat, what, "rstd_post");
+  check_vector(dw_post, H, at::kFloat, what, "dw_post");
+  if (rows.has_value())
+    check_vector(*rows, R64, at::kInt, what, "rows");
+  else
+    TORCH_CHECK_VALUE(R64 == T, what, ": ", R64, " gradient rows for ", T, " rows");
+  TORCH_CHECK_VALUE(dgate.has_value() == (p.gate_kind == kGateChannel), what, ": dgate is the fp32 [",
+                    H, "] buffer of a learned gate");
+  if (dgate.has_value()) check_vector(*dgate, H, at::kFloat, what, "dgate");
   same_device(h, dy, "dy");
   same_device(h, dn, "dn");
   same_device(h, rstd_post, "rstd_post");
@@ -929,8 +1019,9 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> block_norms_bwd(
   same_device(h, dw_pre, "dw_pre");
   same_device(h, dgate, "dgate");
   same_device(h, rows, "rows");
+  row_count(T, what);
   const c10::cuda::CUDAGuard guard(h.device());
-  const int R = row_count(up.size(0), "block_norms_bwd");
+  const int R = row_count(R64, what);
   Tensor dx = at::empty({R, p.H}, resid.options()), dh = at::empty({R, p.H}, h.options());
   c10::optional<Tensor> dg = dgate;
   if (p.gate_kind == kGateToken) dg = at::empty({R, 1}, gate->options());
@@ -942,40 +1033,47 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> block_norms_bwd(
       cfb_block_norms_bwd(&p, opt_ptr<void>(dy), dy.has_value() ? dy->stride(0) : 0,
                           opt_ptr<void>(dn), dn.has_value() ? dn->stride(0) : 0,
                           rstd_post.data_ptr<float>(), opt_ptr<float>(rstd_pre), opt_ptr<int>(rows),
-                          h.size(0), dx.data_ptr(), dh.data_ptr(),
+                          T, dx.data_ptr(), dh.data_ptr(),
                           p.gate_kind != kGateNone ? dg->data_ptr() : nullptr,
                           dw_post.data_ptr<float>(),
                           dw_pre.has_value() ? dw_pre->data_ptr<float>() : nullptr, accumulate,
                           R > 0 ? work.data_ptr() : nullptr, R,
                           err_word(h.get_device()).data_ptr<int>(), cur_stream()),
-      "block_norms_bwd");
+      what);
   return {dx, dh, dg};
 }
 
 // The non-empty tensors of a gradient list and where their scaled values go.  Checks that no output
 // overlaps another output or another tensor of the list.
-std::vector<CfbTensorRef> tensor_refs(const std::vector<Tensor>& grads,
-                                      const std::vector<Tensor>& outs, bool* in_place) {
+std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor>& grads,
+                                      const std::vector<Tensor>* outs, bool* in_place) {
   struct Span {
     uintptr_t lo, hi;
     size_t index;
     bool written;
   };
+  TORCH_CHECK_VALUE(!grads.empty(), what, ": empty list");
+  TORCH_CHECK_VALUE(!outs || outs->size() == grads.size(), what, ": ", grads.size(),
+                    " gradients, ", outs ? outs->size() : 0, " outputs");
   std::vector<CfbTensorRef> refs;
   std::vector<Span> spans;
   refs.reserve(grads.size());
+  spans.reserve(2 * grads.size());
   bool same = true;
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& g = grads[i];
-    TORCH_CHECK(g.layout() == at::kStrided && g.is_cuda() && g.device() == grads[0].device(),
-                "gradient ", i, " must be a dense tensor on ", grads[0].device());
-    TORCH_CHECK(g.is_non_overlapping_and_dense(), "gradient ", i, " has gaps or overlaps itself");
+    TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.is_cuda() && g.device() == grads[0].device(),
+                      what, ": tensor ", i, " must be a dense tensor on ", grads[0].device());
+    TORCH_CHECK_VALUE(g.is_non_overlapping_and_dense(), what, ": tensor ", i,
+                      " has gaps or overlaps itself");
     CfbTensorRef r = {g.data_ptr(), nullptr, g.numel(), type_code(g, "a gradient"), 0};
-    if (!outs.empty()) {
-      const Tensor& o = outs[i];
-      TORCH_CHECK(o.device() == g.device() && o.sizes() == g.sizes() &&
-                      (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
-                  "output ", i, " must have the device, sizes and strides of gradient ", i);
+    if (outs) {
+      const Tensor& o = (*outs)[i];
+      TORCH_CHECK_VALUE(o.layout() == at::kStrided && o.device() == g.device() &&
+                            o.sizes() == g.sizes() &&
+                            (o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous())),
+                        what, ": output ", i,
+                        " must have the device, sizes and strides of its gradient");
       r.out = o.data_ptr();
       r.out_type = type_code(o, "an output");
       const uintptr_t a = reinterpret_cast<uintptr_t>(r.ptr), b = reinterpret_cast<uintptr_t>(r.out);
@@ -991,8 +1089,8 @@ std::vector<CfbTensorRef> tensor_refs(const std::vector<Tensor>& grads,
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
   uintptr_t end = 0, end_written = 0;  // of all spans so far, and of the written ones
   for (const Span& s : spans) {
-    TORCH_CHECK(s.lo >= (s.written ? end : end_written), "tensor ", s.index,
-                " of the list overlaps another that is written");
+    TORCH_CHECK_VALUE(s.lo >= (s.written ? end : end_written), what, ": tensor ", s.index,
+                      " overlaps another that is written");
     end = std::max(end, s.hi);
     if (s.written) end_written = std::max(end_written, s.hi);
   }
@@ -1000,46 +1098,58 @@ std::vector<CfbTensorRef> tensor_refs(const std::vector<Tensor>& grads,
   return refs;
 }
 
-// Sum of squares of the list in the elements of `partial` (fp32): their sum is the list's.
-void grad_list_sumsq(const std::vector<Tensor>& grads, Tensor& partial) {
-  TORCH_CHECK(!grads.empty(), "grad_list_sumsq: empty list");
-  const std::vector<CfbTensorRef> refs = tensor_refs(grads, {}, nullptr);
-  TORCH_CHECK(partial.scalar_type() == at::kFloat && partial.is_contiguous() &&
-                  partial.device() == grads[0].device(),
-              "grad_list_sumsq: partial must be contiguous fp32 on the gradients' device");
-  const c10::cuda::CUDAGuard guard(partial.device());
+inline void check_f32(const Tensor& t, const Tensor& first, const char* what, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() > 0 &&
+                        t.device() == first.device(),
+                    what, ": ", name, " must be contiguous fp32 on ", first.device());
+}
+
+constexpr int64_t kListBlocks = 148 * 8;  // partial sums of a list, at most, for each launch
+
+// Sum of squares of the tensors in the elements of a new fp32 tensor: their sum is the list's.
+Tensor sumsq_of(const std::vector<CfbTensorRef>& refs, const Tensor& first) {
   const int count = static_cast<int>(refs.size()), groups = cfb_grad_list_groups(count);
-  const int64_t per = partial.numel() / groups;
-  TORCH_CHECK(per > 0, "grad_list_sumsq: partial needs ", groups, " elements");
-  if (count == 0 || per * groups < partial.numel()) partial.zero_();
-  if (count == 0) return;
+  if (count == 0) return at::zeros({1}, first.options().dtype(at::kFloat));
+  int64_t per = 0;  // no more blocks than chunks
+  for (const CfbTensorRef& r : refs) per += r.numel / 32768 + 1;
+  per = std::min(per, kListBlocks);
+  Tensor partial = at::empty({per * groups}, first.options().dtype(at::kFloat));
   CFB_CHECK_RC(cfb_grad_list_sumsq(refs.data(), count, partial.data_ptr<float>(),
                                    static_cast<int>(per), cur_stream()),
                "grad_list_sumsq");
+  return partial;
+}
+Tensor grad_list_sumsq(const std::vector<Tensor>& grads) {
+  const std::vector<CfbTensorRef> refs = tensor_refs("grad_list_sumsq", grads, nullptr, nullptr);
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  return sumsq_of(refs, grads[0]);
 }
 
-// out_i = g_i * extra_scale * min(1, max_norm / (norm + 1e-6)), norm = extra_scale * sqrt(sum of
-// partial)
-void grad_list_scale(const std::vector<Tensor>& grads, const std::vector<Tensor>& outs,
-                     const Tensor& partial, double max_norm, double extra_scale, Tensor& norm) {
-  TORCH_CHECK(!grads.empty() && outs.size() == grads.size(), "grad_list_scale: ", grads.size(),
-              " gradients, ", outs.size(), " outputs");
-  TORCH_CHECK(partial.scalar_type() == at::kFloat && partial.is_contiguous() &&
-                  partial.numel() > 0 && partial.device() == grads[0].device() &&
-                  norm.scalar_type() == at::kFloat && norm.numel() == 1 &&
-                  norm.device() == grads[0].device(),
-              "grad_list_scale: partial and norm must be fp32 on the gradients' device");
+// norm = extra_scale * sqrt(sum of extra_sumsq, or of the tensors' squares);
+// out_i = g_i * extra_scale * min(1, max_norm / (norm + 1e-6)), in place without outs
+Tensor grad_list_clip(const std::vector<Tensor>& grads,
+                      const c10::optional<std::vector<Tensor>>& outs, double max_norm,
+                      double extra_scale, const c10::optional<Tensor>& norm_in,
+                      const c10::optional<Tensor>& extra_sumsq) {
+  const char* what = "grad_list_clip_";
   bool in_place = false;
-  std::vector<CfbTensorRef> refs = tensor_refs(grads, outs, &in_place);
+  std::vector<CfbTensorRef> refs =
+      tensor_refs(what, grads, outs.has_value() ? &*outs : &grads, &in_place);
+  if (norm_in.has_value()) check_f32(*norm_in, grads[0], what, "norm");
+  if (extra_sumsq.has_value()) check_f32(*extra_sumsq, grads[0], what, "extra_sumsq");
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  const Tensor partial = extra_sumsq.has_value() ? *extra_sumsq : sumsq_of(refs, grads[0]);
+  // the norm and, behind it, a word for the kernels' factor
+  Tensor both = at::empty({2}, grads[0].options().dtype(at::kFloat));
+  Tensor norm = norm_in.has_value() ? *norm_in : both.narrow(0, 0, 1);
   if (refs.empty()) refs.push_back({nullptr, nullptr, 0, kF32, kF32});  // the norm is still due
-  const c10::cuda::CUDAGuard guard(partial.device());
-  Tensor factor = at::empty({1}, norm.options());
   CFB_CHECK_RC(cfb_grad_list_scale(refs.data(), static_cast<int>(refs.size()),
                                    partial.data_ptr<float>(), static_cast<int>(partial.numel()),
                                    static_cast<float>(max_norm), static_cast<float>(extra_scale),
-                                   norm.data_ptr<float>(), factor.data_ptr<float>(), in_place,
+                                   norm.data_ptr<float>(), both.data_ptr<float>() + 1, in_place,
                                    cur_stream()),
-               "grad_list_scale");
+               what);
+  return norm;
 }
 
 // Dispatcher-visible attention ops on token-major rows, used by the graph rewriter's filtered
@@ -1122,7 +1232,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block_norms_fwd", &block_norms_fwd);
   m.def("block_norms_bwd", &block_norms_bwd);
   m.def("grad_list_sumsq", &grad_list_sumsq);
-  m.def("grad_list_scale", &grad_list_scale);
+  m.def("grad_list_clip", &grad_list_clip);
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd", &ce_bwd, py::arg("logits"), py::arg("rows"), py::arg("labels"),
         py::arg("lse"), py::arg("dloss"), py::arg("dlogits"), py::arg("vocab_start") = 0);

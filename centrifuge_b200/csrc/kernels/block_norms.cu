@@ -237,6 +237,7 @@ __global__ void __launch_bounds__(NW < 8 ? 256 : NW * 32) block_norms_bwd_kernel
   constexpr int kTeams = NW < 8 ? 8 / NW : 1;
   static_assert(!std::is_same<C, WideCols>::value || kTeams == 1 || NV == 1,
                 "wide columns step by the block");
+  let_next_start();
   __shared__ float red[kTeams][2][R * NW];
   const int H = a.H;
   const int team = kTeams > 1 ? warp_id() / NW : 0;
@@ -467,6 +468,7 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
   __shared__ uint64_t full[kTeams][kMaxStages];
   __shared__ float red[kTeams][3][NW];
   __shared__ int abort_flag;
+  let_next_start();
   const int H = a.H;
   const int team = threadIdx.x / NT, tid = threadIdx.x % NT;
   const bool pre = a.w_pre != nullptr;
@@ -789,6 +791,7 @@ __global__ void __launch_bounds__(1024) block_norms_join_kernel(
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
   const int which = blockIdx.y;
+  after_previous();
   if (which == 0 && dw_pre == nullptr) return;
   float s = 0.f;
   if (c < H) {
@@ -1064,10 +1067,10 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
       return 0;
     }
     const bool channel = a.gate_kind == kGateChannel;
-    block_norms_join_kernel<TH><<<dim3((H + 31) / 32, 2), 1024, 0, st>>>(
-        part, blocks, H, static_cast<const TH*>(a.w_post),
-        channel ? static_cast<const TH*>(a.gate) : nullptr, a.w_pre ? dw_pre : nullptr, dw_post,
-        channel ? static_cast<float*>(dgate) : nullptr, add);
-    return launch_status();
+    return launch_behind(block_norms_join_kernel<TH>, dim3((H + 31) / 32, 2), dim3(1024), 0, st,
+                         part, blocks, H, static_cast<const TH*>(a.w_post),
+                         channel ? static_cast<const TH*>(a.gate) : nullptr,
+                         a.w_pre ? dw_pre : nullptr, dw_post,
+                         channel ? static_cast<float*>(dgate) : nullptr, add);
   });
 }

@@ -21,6 +21,7 @@ constexpr int kListChunk = 32768;  // elements
 
 template <int CAP>
 struct GradList {
+  static constexpr int kCap = CAP;
   const void* ptr[CAP];
   void* out[CAP];
   long long numel[CAP];
@@ -78,6 +79,7 @@ __device__ __forceinline__ float chunk_sumsq(const T* p, int n) {
 template <int CAP>
 __global__ void __launch_bounds__(256) grad_list_sumsq_kernel(const __grid_constant__ GradList<CAP> l,
                                                               float* __restrict__ partial) {
+  let_next_start();
   double sum = 0.0;
   for (int c = blockIdx.x; c < l.chunks; c += gridDim.x) {
     const int t = tensor_of(l, c);
@@ -155,6 +157,7 @@ __device__ __forceinline__ float clip_factor(const float* partial, int n_partial
 __global__ void __launch_bounds__(256) grad_list_factor_kernel(
     const float* __restrict__ partial, int n_partial, float max_norm, float extra_scale,
     float* __restrict__ norm_out, float* __restrict__ factor) {
+  after_previous();
   const float k = clip_factor(partial, n_partial, max_norm, extra_scale, norm_out);
   if (threadIdx.x == 0) *factor = k;
 }
@@ -167,6 +170,7 @@ __global__ void __launch_bounds__(256) grad_list_scale_kernel(
     const __grid_constant__ GradList<CAP> l, const float* __restrict__ partial, int n_partial,
     float max_norm, float extra_scale, float* __restrict__ norm_out,
     const float* __restrict__ factor, int in_place) {
+  after_previous();
   const float k = n_partial > 0 ? clip_factor(partial, n_partial, max_norm, extra_scale,
                                               blockIdx.x == 0 ? norm_out : nullptr)
                                 : *factor;
@@ -244,12 +248,19 @@ int cfb_grad_list_scale(const CfbTensorRef* refs, int count, const float* partia
   for (int i = 0; i < count; ++i) chunks += (refs[i].numel + kListChunk - 1) / kListChunk;
   const bool joined = chunks > 148 * 8;
   if (joined)
-    grad_list_factor_kernel<<<1, 256, 0, st>>>(partial, n_partial, max_norm, extra_scale, norm,
-                                               factor);
+    if (const int rc = launch_behind(grad_list_factor_kernel, dim3(1), dim3(256), 0, st, partial,
+                                     n_partial, max_norm, extra_scale, norm, factor))
+      return rc;
   return each_group(refs, count, [&](const auto& l, int g) {
-    grad_list_scale_kernel<<<l.chunks > 0 ? l.chunks : 1, 256, 0, st>>>(
-        l, partial, joined ? 0 : n_partial, max_norm, extra_scale, g == 0 ? norm : nullptr, factor,
-        in_place);
-    return launch_status();
+    constexpr int kCap = std::remove_reference_t<decltype(l)>::kCap;
+    const dim3 grid(l.chunks > 0 ? l.chunks : 1);
+    const int sums = joined ? 0 : n_partial;
+    if (joined || g > 0) {  // thousands of blocks that wait would be in the way of the ones before
+      grad_list_scale_kernel<kCap><<<grid, 256, 0, st>>>(l, partial, sums, max_norm, extra_scale,
+                                                         g == 0 ? norm : nullptr, factor, in_place);
+      return launch_status();
+    }
+    return launch_behind(grad_list_scale_kernel<kCap>, grid, dim3(256), 0, st, l, partial, sums,
+                         max_norm, extra_scale, norm, factor, in_place);
   });
 }

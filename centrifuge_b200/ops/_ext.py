@@ -15,7 +15,7 @@ _proxy = None
 # Kernels launched by one call of each binding (for the launch counter).
 _LAUNCHES_PER_CALL = {"rmsnorm_bwd": 2, "attn_bwd": 2, "attn_bwd_mma": 3, "gemm_error_word": 0,
                       "status_block": 0, "set_wait_limits": 0, "gemm_plan": 0,
-                      "scaled_embedding_bwd": 3, "block_norms_bwd": 2}
+                      "scaled_embedding_bwd": 3, "block_norms_bwd": 2, "grad_list_clip": 2}
 
 
 class LaunchCounter:

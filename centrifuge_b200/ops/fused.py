@@ -154,6 +154,8 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
     type than the table, e.g. an fp32 residual stream) with unit column stride and any row stride;
     ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
     the status block and gives a zero row."""
+    if table.is_cuda:
+        return kernels().scaled_embedding_fwd(table, ids, scale, out)
     _need(table.dim() == 2 and _rows2d(table, table.shape[1]) and table.dtype in _ROW_TYPES,
           "scaled_embedding_fwd: table must be a row-major bf16, fp16 or fp32 [V, H]")
     _need(ids.dtype in (torch.int64, torch.int32), "scaled_embedding_fwd: ids must be int64 or int32")
@@ -165,11 +167,7 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
         _need(_rows2d(out, H) and out.shape[0] == ids.shape[0] and out.dtype in _ROW_TYPES,
               "scaled_embedding_fwd: out must be a row-major bf16, fp16 or fp32 [{}, {}]",
               ids.shape[0], H)
-    if not table.is_cuda:
-        out.copy_(table[ids.long()].float() * scale)
-        return out
-    kernels().scaled_embedding_fwd(table, ids.contiguous(), out, scale)
-    return out
+    return out.copy_(table[ids.long()].float() * scale)
 
 
 def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tensor,
@@ -184,6 +182,9 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
     Rows of token ``padding_idx`` add nothing.  Without ``accumulate`` the gradient replaces what
     ``dtable`` held: rows of tokens that do not occur become zero.  On the GPU a token outside the
     table or a row id outside ``ids`` records an error in the status block and adds nothing."""
+    if dy.is_cuda:
+        kernels().scaled_embedding_bwd(dy, ids, dtable, scale, id_rows, padding_idx, accumulate)
+        return dtable
     _need(dy.dim() == 2 and _rows2d(dy, dy.shape[1]) and dy.dtype in _ROW_TYPES,
           "scaled_embedding_bwd: dy must be a row-major bf16, fp16 or fp32 [R, H]")
     _need(ids.dtype in (torch.int64, torch.int32), "scaled_embedding_bwd: ids must be int64 or int32")
@@ -198,17 +199,13 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
         _need(id_rows.dtype == torch.int32 and id_rows.dim() == 1 and id_rows.is_contiguous()
               and id_rows.shape[0] == dy.shape[0],
               "scaled_embedding_bwd: id_rows must be contiguous int32 [{}]", dy.shape[0])
-    if not dy.is_cuda:
-        tok = (ids if id_rows is None else ids[id_rows.long()]).long()
-        g = dy.float() * scale
-        if padding_idx is not None:
-            g, tok = g[tok != padding_idx], tok[tok != padding_idx]
-        if not accumulate:
-            dtable.zero_()
-        return dtable.index_add_(0, tok, g)
-    kernels().scaled_embedding_bwd(dy, ids.contiguous(), id_rows, dtable, scale,
-                                   -1 if padding_idx is None else padding_idx, accumulate)
-    return dtable
+    tok = (ids if id_rows is None else ids[id_rows.long()]).long()
+    g = dy.float() * scale
+    if padding_idx is not None:
+        g, tok = g[tok != padding_idx], tok[tok != padding_idx]
+    if not accumulate:
+        dtable.zero_()
+    return dtable.index_add_(0, tok, g)
 
 
 # ---------------------------------------------------------------- norms around a block
@@ -239,6 +236,8 @@ def block_norms_fwd(h: torch.Tensor, x: torch.Tensor, w_post: torch.Tensor,
     stream ``x``, ``y`` has that type or fp32.  ``gate``: ``None``, a learned ``[H]``, a weight for
     each token (fp32 ``[T, 1]``), or ``[T, H]``.  ``h``, ``x`` and ``gate`` may have any row stride.
     ``H`` up to 16384."""
+    if h.is_cuda:
+        return kernels().block_norms_fwd(h, x, w_post, w_pre, eps, gate, block_scale, resid_scale)
     T, H = h.shape if h.dim() == 2 else (-1, -1)
     _need(T >= 0 and _rows2d(h, H) and h.dtype in _ROW_TYPES,
           "block_norms_fwd: h must be a row-major bf16, fp16 or fp32 [T, H]")
@@ -249,10 +248,8 @@ def block_norms_fwd(h: torch.Tensor, x: torch.Tensor, w_post: torch.Tensor,
     _need(H <= 16384, "block_norms_fwd: hidden size {} is over 16384", H)
     if gate is not None:
         _check_gate("block_norms_fwd", gate, T, H, h.dtype)
-    if not h.is_cuda:
-        y, n, rp, rq = ref.block_norms(h, x, w_post, w_pre, eps, gate, block_scale, resid_scale)
-        return y.to(x.dtype), None if n is None else n.to(h.dtype), rp, rq
-    return kernels().block_norms_fwd(h, x, w_post, w_pre, eps, gate, block_scale, resid_scale)
+    y, n, rp, rq = ref.block_norms(h, x, w_post, w_pre, eps, gate, block_scale, resid_scale)
+    return y.to(x.dtype), None if n is None else n.to(h.dtype), rp, rq
 
 
 def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: torch.Tensor,
@@ -272,6 +269,10 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
     added to (written without ``accumulate``); a token's or element's gate returns its gradient
     for the ``R`` rows.  On the GPU a row id outside ``h`` records an error in the status block and
     gives zero rows."""
+    if h.is_cuda:
+        return kernels().block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre, dw_post,
+                                         dw_pre, gate, dgate, block_scale, resid_scale, rows,
+                                         accumulate)
     name = "block_norms_bwd"
     T, H = h.shape if h.dim() == 2 else (-1, -1)
     _need(T >= 0 and _rows2d(h, H) and h.dtype in _ROW_TYPES,
@@ -309,22 +310,18 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
     learned = gate is not None and gate.dim() == 1
     _need((dgate is not None) == learned and (not learned or _vector(dgate, H, torch.float32)),
           "{}: dgate is the fp32 [{}] buffer of a learned gate", name, H)
-    if not h.is_cuda:
-        if rows is not None:
-            at = rows.long()
-            h, rstd_post = h[at], rstd_post[at]
-            y, rstd_pre = (y[at], rstd_pre[at]) if pre else (None, None)
-            gate = gate if gate is None or learned else gate[at]
-        dx, dh, dp, dq, dg = ref.block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre,
-                                                 gate, block_scale, resid_scale)
-        for acc, d in ((dw_post, dp), (dw_pre, dq), (dgate, dg if learned else None)):
-            if acc is not None:
-                acc.copy_(acc + d if accumulate else d)
-        return (dx.to(resid), dh.to(h.dtype),
-                dgate if gate is None or learned else dg.to(gate.dtype))
-    return kernels().block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre, dw_post,
-                                     dw_pre, gate, dgate, block_scale, resid_scale, rows,
-                                     accumulate)
+    if rows is not None:
+        at = rows.long()
+        h, rstd_post = h[at], rstd_post[at]
+        y, rstd_pre = (y[at], rstd_pre[at]) if pre else (None, None)
+        gate = gate if gate is None or learned else gate[at]
+    dx, dh, dp, dq, dg = ref.block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre,
+                                             gate, block_scale, resid_scale)
+    for acc, d in ((dw_post, dp), (dw_pre, dq), (dgate, dg if learned else None)):
+        if acc is not None:
+            acc.copy_(acc + d if accumulate else d)
+    return (dx.to(resid), dh.to(h.dtype),
+            dgate if gate is None or learned else dg.to(gate.dtype))
 
 
 # ---------------------------------------------------------------- cross entropy
@@ -435,26 +432,16 @@ def grad_norm_clip_coef(grad: torch.Tensor, max_norm: float, extra_scale: float,
     return coef
 
 
-def grad_list_sumsq(grads: Sequence[torch.Tensor],
-                    partial: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Sum of squares of all elements of a list of tensors, as fp32 partial sums whose total it is
-    (``partial``, one for each block).  Ranks that hold different parameters add their totals (an
-    all-reduce of ``partial.sum()``) and give the result to :func:`grad_list_clip_` as
-    ``extra_sumsq``."""
+def grad_list_sumsq(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    """Sum of squares of all elements of a list of tensors, as fp32 partial sums whose total it is.
+    Ranks that hold different parameters add their totals (an all-reduce of ``.sum()``) and give the
+    result to :func:`grad_list_clip_` as ``extra_sumsq``."""
     grads = list(grads)
+    if grads and grads[0].is_cuda:
+        return kernels().grad_list_sumsq(grads)
     _need(len(grads) > 0, "grad_list_sumsq: empty list")
     _check_grads("grad_list_sumsq", grads)
-    if not grads[0].is_cuda:
-        total = sum(g.double().pow(2).sum() for g in grads).float().view(1)
-        if partial is None:
-            return total
-        partial.zero_()
-        partial[:1] = total
-        return partial
-    if partial is None:
-        partial = torch.empty(148 * 8, dtype=torch.float32, device=grads[0].device)
-    kernels().grad_list_sumsq(grads, partial)
-    return partial
+    return sum(g.double().pow(2).sum() for g in grads).float().view(1)
 
 
 def _check_grads(name: str, grads: List[torch.Tensor]) -> None:
@@ -508,27 +495,26 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
         raise ValueError(f"grad_list_clip_: extra_scale = {extra_scale} is not positive")
     if not grads:
         return torch.zeros(1) if norm is None else norm.zero_()
+    if grads[0].is_cuda:
+        return kernels().grad_list_clip(grads, None if out is None else list(out), max_norm,
+                                        extra_scale, norm, extra_sumsq)
     _check_grads("grad_list_clip_", grads)
     outs = grads if out is None else list(out)
     if out is not None:
         _need(len(outs) == len(grads), "grad_list_clip_: {} gradients, {} outputs", len(grads),
               len(outs))
         _check_grads("grad_list_clip_", outs)
+    _check_spans(grads, outs)
     if norm is None:
         norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
-    if not grads[0].is_cuda:
-        _check_spans(grads, outs)  # the kernels' binding checks the same
     if extra_sumsq is None:
         extra_sumsq = grad_list_sumsq(grads)
-    if not grads[0].is_cuda:
-        norm.copy_((extra_sumsq.double().sum().sqrt() * extra_scale).view(1))
-        k = extra_scale
-        if max_norm > 0:
-            k = (max_norm / (norm.view(()) + 1e-6)).clamp(max=1.0) * extra_scale
-        for g, o in zip(grads, outs):
-            o.copy_(g.float() * k)
-        return norm
-    kernels().grad_list_scale(grads, outs, extra_sumsq, max_norm, extra_scale, norm)
+    norm.copy_((extra_sumsq.double().sum().sqrt() * extra_scale).view(1))
+    k = extra_scale
+    if max_norm > 0:
+        k = (max_norm / (norm.view(()) + 1e-6)).clamp(max=1.0) * extra_scale
+    for g, o in zip(grads, outs):
+        o.copy_(g.float() * k)
     return norm
 
 
