@@ -565,3 +565,189 @@ def test_refusals(dev):
     no(fused.grad_list_clip_, [g[:50], t(50)], 1.0, out=[t(50), g[25:75]])
     no(fused.grad_list_clip_, [g[::2]], 1.0)
     no(fused.grad_list_clip_, [t(1).expand(10)], 1.0)
+
+
+# ---------------------------------------------------------------- together
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("dtype,tol", [
+    (F32, 2e-5),  # some hundred roundings of 2^-24
+    # about 13 roundings of half a bf16 step on the longest way through three blocks and back,
+    # each of which moves a gradient by at most 2^-8 of its norm
+    (BF, 13 * 2.0 ** -8)])
+def test_step_of_a_model_with_norms_on_both_sides(dev, dtype, tol):
+    """Scaled embedding, three linear blocks with the norms after and before them, the gradient on
+    the kept rows only, and clipping of all gradients, against autograd in 64 bits."""
+    g = gen(dev, 11)
+    V, H, T, R, L = 60, 48, 90, 41, 3
+    scale, a, b = 4.0, 0.75, 0.5
+    table = rand(g, V, H, dtype=dtype, scale=0.25)
+    ids = torch.randint(0, V // 4, (2, T // 2), generator=g, device=dev)
+    rows = torch.randperm(T, generator=g, device=dev)[:R].sort().values.int()
+    W = [rand(g, H, H, dtype=dtype, scale=H ** -0.5) for _ in range(L)]
+    post = [rand(g, H, dtype=dtype, scale=0.1, shift=1.0) for _ in range(L)]
+    pre = [rand(g, H, dtype=dtype, scale=0.1, shift=1.0) for _ in range(L)]
+    gates = [torch.rand(T, 1, generator=g, device=dev), rand(g, H, dtype=dtype, shift=1.0),
+             rand(g, T, H, dtype=dtype, shift=1.0)]
+    c = rand(g, R, H, dtype=dtype)
+
+    def one_step():
+        x = n = fused.scaled_embedding_fwd(table, ids, scale)
+        saved = []
+        for i in range(L):
+            h = n @ W[i]
+            y, n_next, rp, rq = fused.block_norms_fwd(h, x, post[i], pre[i], EPS, gates[i], b, a)
+            saved.append((n, h, y, rp, rq))
+            x, n = y, n_next
+        f32 = dict(dtype=F32, device=dev)
+        dw = torch.zeros(L, 3, H, **f32)
+        dW = torch.zeros(L, H, H, **f32)
+        dE = torch.full((V, H), 7.0, **f32)
+        dgate = [None] * L
+        dy, dn = None, c
+        for i in reversed(range(L)):
+            n, h, y, rp, rq = saved[i]
+            dy, dh, dgate[i] = fused.block_norms_bwd(
+                dy, dn, h, y, rp, rq, post[i], pre[i], dw[i, 0], dw[i, 1], gate=gates[i],
+                dgate=dw[i, 2] if i == 1 else None, block_scale=b, resid_scale=a, rows=rows)
+            dW[i] = n[rows.long()].float().t() @ dh.float()
+            dn = dh @ W[i].t()
+        fused.scaled_embedding_bwd((dy.float() + dn.float()).to(dtype), ids, dE, scale,
+                                   id_rows=rows, accumulate=False)
+        grads = [dE, dW, dw]
+        norm = fused.grad_list_clip_(grads, 0.5)
+        return [*grads, dgate[0], dgate[2], norm]
+
+    got = one_step()
+    again = one_step()
+    assert all(torch.equal(p, q) for p, q in zip(got, again))  # the same bits
+
+    # the same in 64 bits, with the loss on the kept rows
+    leaf = [t.double().requires_grad_() for t in (table, *W, *post, *pre, *gates)]
+    E, w64, post64, pre64, g64 = (leaf[0], leaf[1:1 + L], leaf[1 + L:1 + 2 * L],
+                                  leaf[1 + 2 * L:1 + 3 * L], leaf[1 + 3 * L:])
+    x = n = E[ids.reshape(-1)] * scale
+    for i in range(L):
+        x, n, _, _, _ = norms_formula({"h": n @ w64[i], "x": x, "w_post": post64[i],
+                                       "w_pre": pre64[i], "gate": g64[i]}, a, b)
+    at = rows.long()
+    (n[at] * c.double()).sum().backward()
+    dw = torch.stack([torch.stack([post64[i].grad, pre64[i].grad,
+                                   g64[1].grad if i == 1 else torch.zeros_like(post64[i])])
+                      for i in range(L)])
+    want = [E.grad, torch.stack([w.grad for w in w64]), dw]
+    norm = math.sqrt(sum(float(t.square().sum()) for t in want))
+    assert norm > 1.0
+    want = [t * (0.5 / (norm + 1e-6)) for t in want] + [g64[0].grad[at], g64[2].grad[at],
+                                                        torch.tensor([norm])]
+    for p, q, what in zip(got, want, ("dE", "dW", "dw", "dgate token", "dgate element", "norm")):
+        q = q.to(p.device)
+        err = float((p.double() - q).norm() / q.norm())
+        assert err < tol, (what, err)
+
+
+# ---------------------------------------------------------------- streams, graphs, long offsets
+def _all_operators(g, k=1.0):
+    """Inputs on the GPU, and a call of every operator on them that returns what it writes."""
+    T, R, H, V = 300, 200, 256, 500
+    s = {"table": rand(g, V, H, dtype=BF, scale=k), "ids": torch.randint(0, V, (T,), generator=g, device="cuda"),
+         "rows": torch.randperm(T, generator=g, device="cuda")[:R].sort().values.int(),
+         "h": rand(g, T, H, dtype=BF), "x": rand(g, T, H, dtype=BF, scale=k),
+         "w": rand(g, 2, H, dtype=BF, shift=1.0), "gate": rand(g, H, dtype=BF),
+         "dy": rand(g, R, H, dtype=BF), "dn": rand(g, R, H, dtype=BF, scale=k),
+         "grads": rand(g, 3, 40000, scale=k)}
+
+    def call(s):
+        e = fused.scaled_embedding_fwd(s["table"], s["ids"], 2.0)
+        y, n, rp, rq = fused.block_norms_fwd(s["h"], s["x"], s["w"][0], s["w"][1], EPS, s["gate"])
+        acc = torch.empty(3, H, device="cuda")
+        dx, dh, _ = fused.block_norms_bwd(s["dy"], s["dn"], s["h"], y, rp, rq, s["w"][0], s["w"][1],
+                                          acc[0], acc[1], s["gate"], acc[2], rows=s["rows"],
+                                          accumulate=False)
+        dE = torch.empty(V, H, device="cuda")
+        fused.scaled_embedding_bwd(dx, s["ids"], dE, 2.0, id_rows=s["rows"], accumulate=False)
+        few = torch.ones(V, H, device="cuda")
+        fused.scaled_embedding_bwd(dx[:50], s["ids"], few, 2.0, id_rows=s["rows"][:50])
+        out = torch.empty(3, 40000, dtype=BF, device="cuda")
+        norm = fused.grad_list_clip_(list(s["grads"]), 1.0, out=list(out))
+        return [e, y, n, rp, rq, dx, dh, acc, dE, few, out, norm]
+
+    return s, call
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed_with_other_inputs():
+    """Two graphs of the same calls, replayed in turn and with new inputs in place of the old."""
+    g = gen("cuda", 21)
+    sets = [_all_operators(g, k) for k in (1.0, 3.0)]
+    for s, call in sets:
+        call(s)
+    torch.cuda.synchronize()
+    graphs = []
+    for s, call in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = call(s)
+        graphs.append((graph, res))
+    for turn in range(3):
+        for (graph, res), (s, call) in zip(graphs, sets):
+            graph.replay()
+        for (graph, res), (s, call) in zip(graphs, sets):
+            want = call(s)
+            assert all(torch.equal(p, q) for p, q in zip(res, want))
+        for s, _ in sets:  # new values in the same places
+            for k in ("h", "x", "dy", "dn", "grads", "table"):
+                s[k].copy_(rand(g, *s[k].shape, scale=turn + 0.5))
+            s["ids"].copy_(torch.randint(0, 500, (300,), generator=g, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_on_two_streams_at_once():
+    g = gen("cuda", 22)
+    sets = [_all_operators(g, k) for k in (1.0, 2.0)]
+    want = [call(s) for s, call in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        got = []
+        for st, (s, call) in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(call(s))
+        torch.cuda.synchronize()
+        for p, q in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(p, q))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows that begin behind element 2^31 of their tensors."""
+    g = gen("cuda", 23)
+    H, T = 4096, 530_000
+    h = torch.zeros(T, H, dtype=BF, device="cuda")
+    x = torch.zeros(T, H, dtype=BF, device="cuda")
+    some = torch.tensor([0, 1, T - 3, T - 1], device="cuda")
+    h[some], x[some] = rand(g, 4, H, dtype=BF), rand(g, 4, H, dtype=BF)
+    w = torch.ones(H, dtype=BF, device="cuda")
+    y, n, rp, rq = fused.block_norms_fwd(h, x, w, w, EPS)
+    parts = fused.block_norms_fwd(h[some], x[some], w, w, EPS)
+    for p, q in zip((y, n, rp, rq), parts):
+        assert torch.equal(p[some], q)
+    assert not y[T // 2].any()
+    dn = rand(g, 4, H, dtype=BF)
+    acc = torch.zeros(4, H, device="cuda")
+    one = fused.block_norms_bwd(None, dn, h, y, rp, rq, w, w, acc[0], acc[1], rows=some.int())
+    two = fused.block_norms_bwd(None, dn, h[some], y[some], rp[some], rq[some], w, w, acc[2], acc[3])
+    assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1])
+    assert torch.equal(acc[:2], acc[2:])
+    del y, n, x
+    # gradient rows and table rows past 2^31 elements
+    ids = torch.zeros(T, dtype=torch.long, device="cuda")
+    ids[some] = torch.tensor([5, T - 1, T - 1, 7], device="cuda")
+    dt = torch.empty(T, H, device="cuda")
+    fused.scaled_embedding_bwd(h, ids, dt, padding_idx=0, accumulate=False)
+    assert torch.equal(dt[5], h[0].float()) and torch.equal(dt[7], h[T - 1].float())
+    assert torch.equal(dt[T - 1], h[1].float() + h[T - 3].float())
+    assert int(dt.any(1).sum()) == 3
+    back = fused.scaled_embedding_fwd(dt, torch.tensor([T - 1, 0], device="cuda"))
+    assert torch.equal(back[0], dt[T - 1]) and not back[1].any()
+    norm = fused.grad_list_clip_([dt], 1.0)
+    assert float(norm) == pytest.approx(float(dt[[5, 7, T - 1]].double().norm()) * float(norm), rel=1e-4)
