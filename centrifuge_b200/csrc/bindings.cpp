@@ -876,9 +876,11 @@ void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids_in, Tensor& dtable
   same_device(dy, ids_in, "ids");
   same_device(dy, id_rows, "id_rows");
   same_device(dy, dtable, "dtable");
+  const int rows = row_count(dy.size(0), what), H = static_cast<int>(H64);
+  TORCH_CHECK_VALUE(dtable.size(0) <= (1ll << 30) && (dtable.size(0) > 0 || rows == 0), what,
+                    ": a table of ", dtable.size(0), " rows");
   const c10::cuda::CUDAGuard guard(dy.device());
   const Tensor ids = ids_in.contiguous();
-  const int rows = row_count(dy.size(0), what), H = static_cast<int>(H64);
   Tensor work;
   const int64_t bytes = cfb_scaled_embedding_bwd_workspace(dtable.size(0), rows, H);
   if (bytes > 0) work = at::empty({bytes}, dy.options().dtype(at::kByte));

@@ -331,6 +331,7 @@ __device__ __forceinline__ void after_previous() {
 __device__ __forceinline__ void let_next_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+inline int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : -3; }
 template <typename... P, typename... A>
 int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t st,
                   A&&... args) {
@@ -344,9 +345,12 @@ int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStr
   attr.val.programmaticStreamSerializationAllowed = 1;
   c.attrs = &attr;
   c.numAttrs = 1;
-  return cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) == cudaSuccess ? 0 : -3;
+  if (cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) != cudaSuccess) {
+    launch_status();  // the error is this launch's, not the next one's
+    return -3;
+  }
+  return 0;
 }
 
-inline int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : -3; }
 
 }  // namespace cfb

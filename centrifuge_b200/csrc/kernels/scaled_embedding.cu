@@ -262,7 +262,8 @@ struct SlabCols {
   }
   // Adds a run's sum to its table row, or writes it there.  No other thread has these elements, so
   // the additions of the reduction instructions happen once each and in no order that could vary;
-  // unlike a load and a store they do not make the warp wait for the table.
+  // unlike a load and a store they do not make the warp wait for the table.  (They take subnormal
+  // numbers, below 1.2e-38, as zeros.)
   __device__ __forceinline__ void write_run(float* row, const float* acc, float scale,
                                             int add) const {
     float o[N];
@@ -572,8 +573,8 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
                              long long n_ids, const int* id_rows, long long pad, float* dtable,
                              long long ld_t, long long V, int rows, int H, float scale, int add,
                              void* work, int* err, cudaStream_t st) {
-  if (V <= 0 || V > INT32_MAX) return -11;
-  if (H == 0) return 0;
+  if (V < 0 || V > (1ll << 30) || (V == 0 && rows > 0)) return -11;
+  if (H == 0 || V == 0) return 0;
   const bool wide = H % 8 == 0 && rows_of_8(dy, ld, type) && rows_of_8(dtable, ld_t, kF32);
   if (rows == 0) {
     if (add) return 0;

@@ -190,6 +190,7 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
     _need(ids.dtype in (torch.int64, torch.int32), "scaled_embedding_bwd: ids must be int64 or int32")
     _need(_rows2d(dtable, dy.shape[1]) and dtable.dtype == torch.float32,
           "scaled_embedding_bwd: dtable must be a row-major fp32 [V, {}]", dy.shape[1])
+    _need(dtable.shape[0] > 0 or dy.shape[0] == 0, "scaled_embedding_bwd: a table of 0 rows")
     _need(padding_idx is None or padding_idx >= 0, "scaled_embedding_bwd: padding_idx is negative")
     ids = ids.reshape(-1)
     if id_rows is None:

@@ -526,6 +526,8 @@ def test_refusals(dev):
     no(fused.scaled_embedding_bwd, dy, ids, t(8, 16, dtype=BF))
     no(fused.scaled_embedding_bwd, dy, ids, t(8, 15))
     no(fused.scaled_embedding_bwd, dy, ids, t(1, 16).expand(8, 16))
+    no(fused.scaled_embedding_bwd, dy, ids, t(0, 16))
+    no(fused.scaled_embedding_bwd, dy, ids, dt, padding_idx=-1)
     no(fused.scaled_embedding_bwd, dy, ids, dt, id_rows=ids)
     no(fused.scaled_embedding_bwd, dy, ids, dt, id_rows=ids[:3].int())
 
