@@ -788,7 +788,7 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
 // in block order.  Block: 32 columns x 32 slices of the blocks.
 template <typename TH>
 __global__ void __launch_bounds__(1024) block_norms_join_kernel(
-    const float* __restrict__ part, int blocks, int H, const TH* __restrict__ w_post,
+    const float* part, int blocks, int H, const TH* __restrict__ w_post,
     const TH* __restrict__ gate, float* __restrict__ dw_pre, float* __restrict__ dw_post,
     float* __restrict__ dgate, int add) {
   __shared__ float red[32][33];

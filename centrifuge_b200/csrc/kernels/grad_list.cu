@@ -155,7 +155,7 @@ __device__ __forceinline__ float clip_factor(const float* partial, int n_partial
 }
 
 __global__ void __launch_bounds__(256) grad_list_factor_kernel(
-    const float* __restrict__ partial, int n_partial, float max_norm, float extra_scale,
+    const float* partial, int n_partial, float max_norm, float extra_scale,
     float* __restrict__ norm_out, float* __restrict__ factor) {
   after_previous();
   const float k = clip_factor(partial, n_partial, max_norm, extra_scale, norm_out);
@@ -167,9 +167,9 @@ __global__ void __launch_bounds__(256) grad_list_factor_kernel(
 // from a launch of its own, or, with n_partial, from the partial sums.
 template <int CAP>
 __global__ void __launch_bounds__(256) grad_list_scale_kernel(
-    const __grid_constant__ GradList<CAP> l, const float* __restrict__ partial, int n_partial,
+    const __grid_constant__ GradList<CAP> l, const float* partial, int n_partial,
     float max_norm, float extra_scale, float* __restrict__ norm_out,
-    const float* __restrict__ factor, int in_place) {
+    const float* factor, int in_place) {
   after_previous();
   const float k = n_partial > 0 ? clip_factor(partial, n_partial, max_norm, extra_scale,
                                               blockIdx.x == 0 ? norm_out : nullptr)

@@ -323,7 +323,9 @@ inline bool rows_of(int W, const void* p, long long ld, int code) {
 inline bool rows_of_8(const void* p, long long ld, int code) { return rows_of(8, p, ld, code); }
 
 // A kernel that is launched behind another one of the same operator: it may start while that one
-// ends, and waits for its results itself (after_previous() before it reads them).
+// ends, and waits for its results itself (after_previous() before it reads them).  Those results
+// change during its life, so its pointers to them are not __restrict__: loads of memory that a
+// kernel may take for constant can pass the wait or come from a stale cache line.
 __device__ __forceinline__ void after_previous() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

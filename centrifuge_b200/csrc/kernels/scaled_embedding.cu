@@ -291,9 +291,9 @@ struct SlabCols {
 // part[chunk][1]: of a run that begins here and goes on in the next chunk.
 template <typename T, int W>
 __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
-    const T* __restrict__ dy, long long ld, const int* __restrict__ order,
-    const int* __restrict__ stok, const int* __restrict__ n_valid,
-    const uint32_t* __restrict__ absent, float* __restrict__ dtable, long long ld_t,
+    const T* __restrict__ dy, long long ld, const int* order,
+    const int* stok, const int* n_valid,
+    const uint32_t* absent, float* __restrict__ dtable, long long ld_t,
     float* __restrict__ part, int rows, int H, int slabs, int per, int sum_blocks, int shift,
     int span, int vocab, float scale, int add) {
   using S = SlabCols<W>;
@@ -380,8 +380,8 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
 // each, and the shares are added in their order.
 template <int W>
 __global__ void __launch_bounds__(256) embed_join_kernel(
-    const int* __restrict__ stok, const int* __restrict__ n_valid, float* __restrict__ dtable,
-    long long ld_t, const float* __restrict__ part, int rows, int H, int per, float scale,
+    const int* stok, const int* n_valid, float* __restrict__ dtable,
+    long long ld_t, const float* part, int rows, int H, int per, float scale,
     int add) {
   using S = SlabCols<W>;
   constexpr int N = S::N;
