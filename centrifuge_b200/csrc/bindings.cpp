@@ -4,6 +4,7 @@
 // kernel on the current CUDA stream.  A non-zero launcher status raises a RuntimeError: there is
 // no fallback path on the GPU.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -826,6 +827,11 @@ inline int row_count(int64_t rows, const char* what) {
   TORCH_CHECK_VALUE(rows < (1ll << 30), what, ": ", rows, " rows");
   return static_cast<int>(rows);
 }
+// An uninitialised tensor on the device of `like`, without the dispatcher's detour: the small calls
+// of these operators are bound by the host, and allocations are most of their time.
+inline Tensor new_empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
+}
 inline bool is_index(const Tensor& t) {
   return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt;
 }
@@ -844,7 +850,7 @@ Tensor scaled_embedding_fwd(const Tensor& table, const Tensor& ids_in, double sc
   const Tensor ids = ids_in.contiguous();
   const int rows = row_count(ids.numel(), what);
   if (out_in.has_value()) check_rows(*out_in, rows, H, what, "out");
-  Tensor out = out_in.has_value() ? *out_in : at::empty({rows, H}, table.options());
+  Tensor out = out_in.has_value() ? *out_in : new_empty({rows, H}, table.scalar_type(), table);
   CFB_CHECK_RC(cfb_scaled_embedding_fwd(
                    table.data_ptr(), type_code(table, "table"), table.stride(0), table.size(0),
                    ids.data_ptr(), ids.scalar_type() == at::kInt, out.data_ptr(),
@@ -883,7 +889,7 @@ void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids_in, Tensor& dtable
   const Tensor ids = ids_in.contiguous();
   Tensor work;
   const int64_t bytes = cfb_scaled_embedding_bwd_workspace(dtable.size(0), rows, H);
-  if (bytes > 0) work = at::empty({bytes}, dy.options().dtype(at::kByte));
+  if (bytes > 0) work = new_empty({bytes}, at::kByte, dy);
   CFB_CHECK_RC(cfb_scaled_embedding_bwd(
                    dy.data_ptr(), type_code(dy, "dy"), dy.stride(0), ids.data_ptr(),
                    ids.scalar_type() == at::kInt, ids.numel(), opt_ptr<int>(id_rows),
@@ -958,12 +964,11 @@ std::tuple<Tensor, c10::optional<Tensor>, Tensor, c10::optional<Tensor>> block_n
   p.resid_type = resid_code(what, x, h, "x");
   const c10::cuda::CUDAGuard guard(h.device());
   const int rows = row_count(h.size(0), what);
-  const auto f32 = h.options().dtype(at::kFloat);
-  Tensor y = at::empty({rows, p.H}, x.options()), rstd_post = at::empty({rows}, f32);
+  Tensor y = new_empty({rows, p.H}, x.scalar_type(), h), rstd_post = new_empty({rows}, at::kFloat, h);
   c10::optional<Tensor> n, rstd_pre;
   if (p.w_pre) {
-    n = at::empty({rows, p.H}, h.options());
-    rstd_pre = at::empty({rows}, f32);
+    n = new_empty({rows, p.H}, h.scalar_type(), h);
+    rstd_pre = new_empty({rows}, at::kFloat, h);
   }
   CFB_CHECK_RC(cfb_block_norms_fwd(&p, static_cast<float>(eps), y.data_ptr(),
                                    p.w_pre ? n->data_ptr() : nullptr, rstd_post.data_ptr<float>(),
@@ -1024,13 +1029,13 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> block_norms_bwd(
   row_count(T, what);
   const c10::cuda::CUDAGuard guard(h.device());
   const int R = row_count(R64, what);
-  Tensor dx = at::empty({R, p.H}, resid.options()), dh = at::empty({R, p.H}, h.options());
+  Tensor dx = new_empty({R, p.H}, resid.scalar_type(), h), dh = new_empty({R, p.H}, h.scalar_type(), h);
   c10::optional<Tensor> dg = dgate;
-  if (p.gate_kind == kGateToken) dg = at::empty({R, 1}, gate->options());
-  if (p.gate_kind == kGateElement) dg = at::empty({R, p.H}, h.options());
+  if (p.gate_kind == kGateToken) dg = new_empty({R, 1}, at::kFloat, h);
+  if (p.gate_kind == kGateElement) dg = new_empty({R, p.H}, h.scalar_type(), h);
   Tensor work;
   if (R > 0)
-    work = at::empty({cfb_block_norms_bwd_workspace(R, p.H)}, h.options().dtype(at::kByte));
+    work = new_empty({cfb_block_norms_bwd_workspace(R, p.H)}, at::kByte, h);
   CFB_CHECK_RC(
       cfb_block_norms_bwd(&p, opt_ptr<void>(dy), dy.has_value() ? dy->stride(0) : 0,
                           opt_ptr<void>(dn), dn.has_value() ? dn->stride(0) : 0,
@@ -1115,7 +1120,7 @@ Tensor sumsq_of(const std::vector<CfbTensorRef>& refs, const Tensor& first) {
   int64_t per = 0;  // no more blocks than chunks
   for (const CfbTensorRef& r : refs) per += r.numel / 32768 + 1;
   per = std::min(per, kListBlocks);
-  Tensor partial = at::empty({per * groups}, first.options().dtype(at::kFloat));
+  Tensor partial = new_empty({per * groups}, at::kFloat, first);
   CFB_CHECK_RC(cfb_grad_list_sumsq(refs.data(), count, partial.data_ptr<float>(),
                                    static_cast<int>(per), cur_stream()),
                "grad_list_sumsq");
@@ -1138,17 +1143,24 @@ Tensor grad_list_clip(const std::vector<Tensor>& grads,
   std::vector<CfbTensorRef> refs =
       tensor_refs(what, grads, outs.has_value() ? &*outs : &grads, &in_place);
   if (norm_in.has_value()) check_f32(*norm_in, grads[0], what, "norm");
-  if (extra_sumsq.has_value()) check_f32(*extra_sumsq, grads[0], what, "extra_sumsq");
+  if (extra_sumsq.has_value()) {
+    check_f32(*extra_sumsq, grads[0], what, "extra_sumsq");
+    if (norm_in.has_value()) {  // the norm is written while blocks still read the sums
+      const uintptr_t n = reinterpret_cast<uintptr_t>(norm_in->data_ptr());
+      const uintptr_t e = reinterpret_cast<uintptr_t>(extra_sumsq->data_ptr());
+      TORCH_CHECK_VALUE(n + norm_in->nbytes() <= e || n >= e + extra_sumsq->nbytes(), what,
+                        ": norm overlaps extra_sumsq");
+    }
+  }
   const c10::cuda::CUDAGuard guard(grads[0].device());
-  const Tensor partial = extra_sumsq.has_value() ? *extra_sumsq : sumsq_of(refs, grads[0]);
-  // the norm and, behind it, a word for the kernels' factor
-  Tensor both = at::empty({2}, grads[0].options().dtype(at::kFloat));
-  Tensor norm = norm_in.has_value() ? *norm_in : both.narrow(0, 0, 1);
+  const Tensor own = extra_sumsq.has_value() ? Tensor() : sumsq_of(refs, grads[0]);
+  const Tensor& partial = extra_sumsq.has_value() ? *extra_sumsq : own;
+  Tensor norm = norm_in.has_value() ? *norm_in : new_empty({1}, at::kFloat, grads[0]);
   if (refs.empty()) refs.push_back({nullptr, nullptr, 0, kF32, kF32});  // the norm is still due
   CFB_CHECK_RC(cfb_grad_list_scale(refs.data(), static_cast<int>(refs.size()),
                                    partial.data_ptr<float>(), static_cast<int>(partial.numel()),
                                    static_cast<float>(max_norm), static_cast<float>(extra_scale),
-                                   norm.data_ptr<float>(), both.data_ptr<float>() + 1, in_place,
+                                   norm.data_ptr<float>(), in_place,
                                    cur_stream()),
                what);
   return norm;

@@ -138,42 +138,39 @@ __device__ __forceinline__ void chunk_scale_to(const TI* p, void* o, int type, l
     chunk_scale(p, static_cast<__half*>(o) + at, n, k);
 }
 
-// The factor of the list's elements; every thread of the block gets it.
-__device__ __forceinline__ float clip_factor(const float* partial, int n_partial, float max_norm,
-                                             float extra_scale, float* norm_out) {
+// The norm from the partial sums; every thread of the block gets it.
+__device__ __forceinline__ float joined_norm(const float* partial, int n_partial,
+                                             float extra_scale) {
   double s = 0.0;
   for (int i = threadIdx.x; i < n_partial; i += 256) s += static_cast<double>(partial[i]);
   s = block_sum_f64(s);
-  const float norm = static_cast<float>(sqrt(s) * static_cast<double>(extra_scale));
-  float k = extra_scale;
-  if (max_norm > 0.f) {
-    const float c = max_norm / (norm + 1e-6f);
-    k = (c >= 1.f ? 1.f : c) * extra_scale;  // a norm that is no number leaves none in the output
-  }
-  if (norm_out && threadIdx.x == 0) *norm_out = norm;
-  return k;
+  return static_cast<float>(sqrt(s) * static_cast<double>(extra_scale));
+}
+// What the elements are multiplied by.
+__device__ __forceinline__ float clip_factor(float norm, float max_norm, float extra_scale) {
+  if (!(max_norm > 0.f)) return extra_scale;
+  const float c = max_norm / (norm + 1e-6f);
+  return (c >= 1.f ? 1.f : c) * extra_scale;  // a norm that is no number leaves none in the output
 }
 
-__global__ void __launch_bounds__(256) grad_list_factor_kernel(
-    const float* partial, int n_partial, float max_norm, float extra_scale,
-    float* __restrict__ norm_out, float* __restrict__ factor) {
+__global__ void __launch_bounds__(256) grad_list_norm_kernel(const float* partial, int n_partial,
+                                                             float extra_scale, float* norm) {
   after_previous();
-  const float k = clip_factor(partial, n_partial, max_norm, extra_scale, norm_out);
-  if (threadIdx.x == 0) *factor = k;
+  const float v = joined_norm(partial, n_partial, extra_scale);
+  if (threadIdx.x == 0) *norm = v;
 }
 
 // One chunk a block: the hardware's dealing of short blocks keeps more of the memory busy than 1184
-// blocks that loop (1.1 G elements bf16 -> fp32: 1012 us against 1109 to 1129 us).  The factor comes
-// from a launch of its own, or, with n_partial, from the partial sums.
+// blocks that loop (1.1 G elements bf16 -> fp32: 987 us in all against 1380).  The norm comes from a
+// launch of its own, or, with n_partial, from the partial sums.
 template <int CAP>
 __global__ void __launch_bounds__(256) grad_list_scale_kernel(
-    const __grid_constant__ GradList<CAP> l, const float* partial, int n_partial,
-    float max_norm, float extra_scale, float* __restrict__ norm_out,
-    const float* factor, int in_place) {
+    const __grid_constant__ GradList<CAP> l, const float* partial, int n_partial, float max_norm,
+    float extra_scale, float* norm, int in_place) {
   after_previous();
-  const float k = n_partial > 0 ? clip_factor(partial, n_partial, max_norm, extra_scale,
-                                              blockIdx.x == 0 ? norm_out : nullptr)
-                                : *factor;
+  const float v = n_partial > 0 ? joined_norm(partial, n_partial, extra_scale) : *norm;
+  if (n_partial > 0 && blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
+  const float k = clip_factor(v, max_norm, extra_scale);
   if (in_place && k == 1.f) return;
   const int c = l.chunks - 1 - static_cast<int>(blockIdx.x);
   if (c < 0) return;
@@ -239,8 +236,8 @@ int cfb_grad_list_sumsq(const CfbTensorRef* refs, int count, float* partial, int
 }
 
 int cfb_grad_list_scale(const CfbTensorRef* refs, int count, const float* partial, int n_partial,
-                        float max_norm, float extra_scale, float* norm, float* factor,
-                        int in_place, cudaStream_t st) {
+                        float max_norm, float extra_scale, float* norm, int in_place,
+                        cudaStream_t st) {
   if (count <= 0 || n_partial <= 0) return -11;
   // Where there are few blocks each of them joins the partial sums itself, which saves a launch;
   // with many that costs each of them more than the launch does.
@@ -248,8 +245,8 @@ int cfb_grad_list_scale(const CfbTensorRef* refs, int count, const float* partia
   for (int i = 0; i < count; ++i) chunks += (refs[i].numel + kListChunk - 1) / kListChunk;
   const bool joined = chunks > 148 * 8;
   if (joined)
-    if (const int rc = launch_behind(grad_list_factor_kernel, dim3(1), dim3(256), 0, st, partial,
-                                     n_partial, max_norm, extra_scale, norm, factor))
+    if (const int rc = launch_behind(grad_list_norm_kernel, dim3(1), dim3(256), 0, st, partial,
+                                     n_partial, extra_scale, norm))
       return rc;
   return each_group(refs, count, [&](const auto& l, int g) {
     constexpr int kCap = std::remove_reference_t<decltype(l)>::kCap;
@@ -257,10 +254,10 @@ int cfb_grad_list_scale(const CfbTensorRef* refs, int count, const float* partia
     const int sums = joined ? 0 : n_partial;
     if (joined || g > 0) {  // thousands of blocks that wait would be in the way of the ones before
       grad_list_scale_kernel<kCap><<<grid, 256, 0, st>>>(l, partial, sums, max_norm, extra_scale,
-                                                         g == 0 ? norm : nullptr, factor, in_place);
+                                                         norm, in_place);
       return launch_status();
     }
     return launch_behind(grad_list_scale_kernel<kCap>, grid, dim3(256), 0, st, l, partial, sums,
-                         max_norm, extra_scale, norm, factor, in_place);
+                         max_norm, extra_scale, norm, in_place);
   });
 }

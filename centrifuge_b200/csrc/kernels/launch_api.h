@@ -276,7 +276,7 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
 // each of cfb_grad_list_groups(count) launches; scale joins all n_partial of them and writes
 // out = g * extra_scale * min(1, max_norm / (norm + 1e-6)) (max_norm <= 0: no limit), norm =
 // extra_scale * sqrt(sum); with in_place (out = ptr everywhere) nothing is written when that factor
-// is one.  `factor`: one fp32 of scratch.
+// is one.
 struct CfbTensorRef {
   const void* ptr;
   void* out;
@@ -287,5 +287,5 @@ int cfb_grad_list_groups(int count);
 int cfb_grad_list_sumsq(const CfbTensorRef* refs, int count, float* partial, int per_group,
                         cudaStream_t st);
 int cfb_grad_list_scale(const CfbTensorRef* refs, int count, const float* partial, int n_partial,
-                        float max_norm, float extra_scale, float* norm, float* factor,
-                        int in_place, cudaStream_t st);
+                        float max_norm, float extra_scale, float* norm, int in_place,
+                        cudaStream_t st);

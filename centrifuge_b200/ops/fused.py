@@ -506,6 +506,8 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
               len(outs))
         _check_grads("grad_list_clip_", outs)
     _check_spans(grads, outs)
+    _need(norm is None or extra_sumsq is None or norm.data_ptr() != extra_sumsq.data_ptr(),
+          "grad_list_clip_: norm overlaps extra_sumsq")
     if norm is None:
         norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
     if extra_sumsq is None:

@@ -561,6 +561,8 @@ def test_refusals(dev):
     no(fused.grad_list_clip_, [g], 1.0, out=[])
     no(fused.grad_list_clip_, [g], 1.0, out=[t(99)])
     no(fused.grad_list_sumsq, [])
+    no(fused.grad_list_clip_, [g], 1.0, norm=z[:1], extra_sumsq=z[:1])
+    no(fused.grad_list_clip_, [g], 1.0, norm=t(0))
     no(fused.grad_list_clip_, [g, g], 1.0)  # the same tensor twice
     no(fused.grad_list_clip_, [g[:60], g[50:]], 1.0)
     no(fused.grad_list_clip_, [t(100), t(100)], 1.0, out=[g[:], g[:]])
