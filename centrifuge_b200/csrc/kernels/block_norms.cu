@@ -228,7 +228,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_pairs
 // With p = dn y and q = dY h the row sums and the column sums share their products.  While a block
 // works, the rows of its next turn are on their way to the L2 cache.
 template <typename C, typename TH, typename TX, int NW, int NV, int R>
-__global__ void __launch_bounds__(NW < 8 ? 256 : NW * 32) block_norms_bwd_kernel(
+__global__ void __launch_bounds__(NW < 8 ? 256 : NW * 32, C::P == 1 ? (NW <= 8 ? 3 : NW <= 16 ? 2 : 1) : 1)
+    block_norms_bwd_kernel(
     NormRows a, const TX* __restrict__ dy, long long ld_dy, const TH* __restrict__ dn,
     long long ld_dn, const float* __restrict__ rstd_post, const float* __restrict__ rstd_pre,
     const int* __restrict__ row_ids, long long n_rows, TX* __restrict__ dx, TH* __restrict__ dh,
