@@ -34,7 +34,8 @@ namespace cfb {
 constexpr int kMaxSpan = 1024;  // tokens of one block of the sort
 constexpr int kKeyRows = 32768; // rows whose keys a block of the sort holds in shared memory
 constexpr int kClear = 8;       // table rows that one block clears
-constexpr int kFewRows = 128;   // up to here one launch does it all
+constexpr int kFewRows = 128;   // up to here one launch does it all (a row id fits 8 bits)
+constexpr int kWarpRun = 24;    // rows of a token that one warp sums there by itself
 
 // Sorted positions of one warp of the gradient: few where few rows would leave SMs idle, more where
 // there are enough, since every chunk border costs a partial sum.
@@ -230,6 +231,9 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
 }
 
 // A lane's columns of a slab of rows: eight neighbours (W = 8), or four columns 32 apart (W = 1).
+// Loads are made without a branch, columns behind the row from its first one, and in the place where
+// they stand: behind a branch, or moved to where they are used, one is waited for before the next
+// one is made.
 template <int W>
 struct SlabCols {
   static constexpr int N = W == 8 ? 8 : 4;
@@ -237,19 +241,21 @@ struct SlabCols {
   int c, H;
   __device__ __forceinline__ SlabCols(int slab, int H_) : c(slab * kSlab + lane_id() * W), H(H_) {}
   template <typename T>
-  __device__ __forceinline__ void load(const T* row, Pack<T, N>& k) const {
-    if constexpr (W == 8) {
-      if (c < H) k = load_pack<T, 8>(row + c);
+  __device__ __forceinline__ Pack<T, N> load(const T* row) const {
+    Pack<T, N> k;
+    if constexpr (W == 8 && sizeof(k) == 16) {
+      uint32_t* u = reinterpret_cast<uint32_t*>(&k);
+      asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+                   : "l"(row + (c < H ? c : 0)));
+      return k;
+    } else if constexpr (W == 8) {
+      return load_pack<T, 8>(row + (c < H ? c : 0));
     } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (c + 32 * i < H) k.v[i] = row[c + 32 * i];
+      for (int i = 0; i < N; ++i) k.v[i] = row[c + 32 * i < H ? c + 32 * i : 0];
+      return k;
     }
-  }
-  __device__ __forceinline__ void load(const float* row, float* f) const {
-    Pack<float, N> k;
-    load<float>(row, k);
-    unpack<float, N>(k, f);
   }
   __device__ __forceinline__ void store(float* row, const float* f) const {
     if constexpr (W == 8) {
@@ -322,14 +328,15 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
   const int chunk = item / slabs;
   const int p0 = chunk * per;
   const int lane = lane_id();
-  // all loads at once; what lies behind the last valid row is not used
+  // all loads at once; what lies behind the last valid row was never written, and is not used
   const int n = *n_valid;
-  const int my_row = lane < per && p0 + lane < rows ? order[p0 + lane] : 0;
+  int my_row = lane < per && p0 + lane < rows ? order[p0 + lane] : 0;
   const int my_tok = lane < per && p0 + lane < rows ? stok[p0 + lane] : -1;
   const int before = p0 > 0 && p0 <= rows ? stok[p0 - 1] : -1;
   const int after = p0 + per < rows ? stok[p0 + per] : -1;
   if (p0 >= n) return;
   const int m = min(per, n - p0);
+  if (lane >= m) my_row = 0;  // a row that is there: the loads below ask no further
   const int behind = p0 + per < n ? after : -1;
   const bool from_before = before == __shfl_sync(0xffffffffu, my_tok, 0);
   const S cols(item % slabs, H);
@@ -342,8 +349,8 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
     Pack<T, N> k[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int row = __shfl_sync(0xffffffffu, my_row, (j + u) & 31);
-      if (j + u < m) cols.load(dy + row * ld, k[u]);
+      const int row = __shfl_sync(0xffffffffu, my_row, (j + u) & 31);  // 0 behind the last one
+      k[u] = cols.load(dy + row * ld);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -401,7 +408,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
       Pack<float, N> v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (k + u < k1) cols.template load<float>(part + 2ll * (k + u) * H, v[u]);
+        v[u] = cols.load(part + 2ll * min(k + u, k1 - 1) * H);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (k + u >= k1) break;
@@ -422,7 +429,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
     if (more > 8 && before != tok) {
       if (lane == 0) long_chunk = chunk;
     } else if (more > 0 && before != tok) {
-      cols.load(part + (2ll * chunk + 1) * H, acc);
+      unpack<float, N>(cols.load(part + (2ll * chunk + 1) * H), acc);
       add_parts(chunk + 1, chunk + 1 + more);
       cols.write_run(dtable + tok * ld_t, acc, scale, add);
     }
@@ -441,7 +448,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
   const int each = (chunks + 7) / 8;
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  if (wp == 0) cols.load(part + (2ll * from + 1) * H, acc);
+  if (wp == 0) unpack<float, N>(cols.load(part + (2ll * from + 1) * H), acc);
   add_parts(from + 1 + wp * each, from + 1 + min(chunks, (wp + 1) * each));
 #pragma unroll
   for (int i = 0; i < N; ++i) share[wp][i * 32 + lane] = acc[i];
@@ -455,10 +462,12 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
 }
 
 // Up to kFewRows rows.  Blocks [0, row_blocks): a warp for each row and slab, which does nothing
-// unless the row is the first of its token, and then sums that token's rows in row order.  The
-// blocks behind them clear the table rows of tokens that do not occur, 32 each.
+// unless the row is the first of its token, and then sums that token's rows in row order; runs of
+// over kWarpRun rows are left to all four warps of the block, a quarter each, and the quarters are
+// added in their order (the warps of a block have different rows and so different tokens).  The
+// blocks behind them clear the table rows of tokens that do not occur, kClear each.
 template <typename T, int W>
-__global__ void __launch_bounds__(128) embed_grad_few_kernel(
+__global__ void __launch_bounds__(128, 6) embed_grad_few_kernel(
     const T* __restrict__ dy, long long ld, const void* __restrict__ ids, int ids32,
     long long n_ids, const int* __restrict__ id_rows, long long pad, float* __restrict__ dtable,
     long long ld_t, long long V, int rows, int H, int slabs, int row_blocks, float scale, int add,
@@ -467,55 +476,91 @@ __global__ void __launch_bounds__(128) embed_grad_few_kernel(
   constexpr int N = S::N;
   constexpr int U = sizeof(T) == 4 && W == 8 ? 4 : 8;
   __shared__ int tok[kFewRows];
+  __shared__ uint8_t list[4][kFewRows];  // for each warp the rows of its token, in row order
+  __shared__ int found[4];
+  __shared__ float share[4][32 * N];
   __shared__ uint32_t present;
-  const int tid = threadIdx.x, wp = warp_id();
+  const int tid = threadIdx.x, wp = warp_id(), lane = lane_id();
   if (tid == 0) present = 0;
   for (int r = tid; r < rows; r += 128)
     tok[r] = row_token(r, ids, ids32, n_ids, id_rows, V, pad, blockIdx.x == 0 ? err : nullptr);
   __syncthreads();
   if (static_cast<int>(blockIdx.x) >= row_blocks) {
-    const long long lo = (static_cast<long long>(blockIdx.x) - row_blocks) * 32;
+    const long long lo = (static_cast<long long>(blockIdx.x) - row_blocks) * kClear;
     for (int r = tid; r < rows; r += 128)
-      if (tok[r] >= lo && tok[r] < lo + 32) atomicOr(&present, 1u << (tok[r] - lo));
+      if (tok[r] >= lo && tok[r] < lo + kClear) atomicOr(&present, 1u << (tok[r] - lo));
     __syncthreads();
-    for (int t = wp; t < 32; t += 4)
+    for (int t = wp; t < kClear; t += 4)
       if (lo + t < V && !(present >> t & 1)) clear_row<W>(dtable + (lo + t) * ld_t, H);
     return;
   }
   const int item = blockIdx.x * 4 + wp;
-  const int r = item / slabs;
-  if (r >= rows || tok[r] < 0) return;
-  const int mine = tok[r];
-  bool first = true;
-  for (int q = lane_id(); q < r; q += 32) first = first && tok[q] != mine;
-  if (!__all_sync(0xffffffffu, first)) return;
-  const S cols(item % slabs, H);
-  float acc[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  for (int base = r / 32 * 32; base < rows; base += 32) {
-    const int q = base + lane_id();
-    unsigned todo = __ballot_sync(0xffffffffu, q >= r && q < rows && tok[q] == mine);
-    while (todo) {
-      Pack<T, N> k[U];
-      const int n = min(U, __popc(todo));
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (u < n) {
-          cols.load(dy + (base + __ffs(todo) - 1) * ld, k[u]);
-          todo &= todo - 1;
-        }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u >= n) break;
-        float f[N];
-        unpack<T, N>(k[u], f);
-#pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += f[i];
-      }
+  const int r = item % rows, slab = item / rows;
+  const int mine = slab < slabs ? tok[r] : -1;
+  bool first = mine >= 0;
+  for (int q = lane; q < r; q += 32) first = first && tok[q] != mine;
+  int n = 0;
+  if (__all_sync(0xffffffffu, first)) {
+    for (int base = r / 32 * 32; base < rows; base += 32) {
+      const int q = base + lane;
+      const bool hit = q >= r && q < rows && tok[q] == mine;
+      const unsigned hits = __ballot_sync(0xffffffffu, hit);
+      if (hit) list[wp][n + __popc(hits & ((1u << lane) - 1))] = static_cast<uint8_t>(q);
+      n += __popc(hits);
     }
   }
-  cols.write_run(dtable + mine * ld_t, acc, scale, add);
+  if (lane == 0) found[wp] = n;
+  float acc[N];
+  // acc: the sum of the rows [from, to) of the list of warp w
+  const auto sum_rows = [&](const S& cols, int w, int from, int to) {
+    F2 sum[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) sum[i] = f2(0.f);
+#pragma unroll 1
+    for (int j = from; j < to; j += U) {
+      Pack<T, N> k[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) k[u] = cols.load(dy + list[w][min(j + u, to - 1)] * ld);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j + u >= to) break;
+        F2 f[N / 2];
+        unpack_f2<T, N>(k[u], f);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) sum[i] = sum[i] + f[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      acc[2 * i] = halves(sum[i]).x;
+      acc[2 * i + 1] = halves(sum[i]).y;
+    }
+  };
+  __syncwarp();
+  if (n > 0 && n <= kWarpRun) {
+    const S cols(slab, H);
+    sum_rows(cols, wp, 0, n);
+    cols.write_run(dtable + mine * ld_t, acc, scale, add);
+  }
+  __syncthreads();
+  for (int w = 0; w < 4; ++w) {
+    const int all = found[w];
+    if (all <= kWarpRun) continue;
+    const int quarter = (all + 3) / 4, other = blockIdx.x * 4 + w;
+    const S cols(other / rows, H);
+    sum_rows(cols, w, min(all, wp * quarter), min(all, (wp + 1) * quarter));
+#pragma unroll
+    for (int i = 0; i < N; ++i) share[wp][i * 32 + lane] = acc[i];
+    __syncthreads();
+    if (wp == 0) {
+#pragma unroll
+      for (int k = 1; k < 4; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += share[k][i * 32 + lane];
+      cols.write_run(dtable + tok[other % rows] * ld_t, acc, scale, add);
+    }
+    __syncthreads();
+  }
 }
 
 template <int W>
@@ -586,7 +631,8 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
   const int slabs = (H + slab - 1) / slab;
   if (rows <= kFewRows) {
     const int row_blocks = (rows * slabs + 3) / 4;
-    const unsigned blocks = row_blocks + (add ? 0 : static_cast<unsigned>((V + 31) / 32));
+    const unsigned blocks =
+        row_blocks + (add ? 0 : static_cast<unsigned>((V + kClear - 1) / kClear));
     return with_type(type, [&](auto t) {
       using T = typename decltype(t)::type;
       auto* kernel = wide ? embed_grad_few_kernel<T, 8> : embed_grad_few_kernel<T, 1>;
