@@ -21,9 +21,9 @@
 //   3. embed_join_kernel    the chunk in which a crossing run begins adds the partial sums up in
 //                           chunk order and writes the table row.
 //
-// Measured, 8192 kept of 16384 rows x 2048 bf16, 32000 tokens of text, the table replaced: 63 us a
+// Measured, 8192 kept of 16384 rows x 2048 bf16, 32000 tokens of text, the table replaced: 58 us a
 // pass (8 us sort, 45 us sums and clearing at 296 MB, the join; 45 us is all of it at the copy rate);
-// 8192 rows x 4096 of 128256 tokens: 331 us (2.17 GB, 332 us at the copy rate).
+// 8192 rows x 4096 of 128256 tokens: 315 us (2.17 GB, 332 us at the copy rate).
 //
 // A handful of rows takes one launch instead (embed_grad_few_kernel).  Every element of the table is
 // written by one thread, once: two runs give the same bits.
@@ -33,7 +33,7 @@ namespace cfb {
 
 constexpr int kMaxSpan = 1024;  // tokens of one block of the sort
 constexpr int kKeyRows = 32768; // rows whose keys a block of the sort holds in shared memory
-constexpr int kClear = 8;       // table rows that one block clears
+constexpr int kClear = 4;       // table rows that one block clears (8: 63 us a pass below, 4: 61)
 constexpr int kFewRows = 128;   // up to here one launch does it all (a row id fits 8 bits)
 constexpr int kWarpRun = 24;    // rows of a token that one warp sums there by itself
 
@@ -92,8 +92,7 @@ __device__ __forceinline__ void clear_row(float* t, int H) {
 // Block b of 2^shift places the rows of the tokens t 2^shift + b at their sorted positions, which are
 // by block and t.  Each of the 32 warps takes a contiguous part of the rows; hist[w][t] first counts
 // the rows of the block's token t in part w and then, after the scan, is the next position of such a
-// row.  A thread has eight tokens in
-// flight; up to kKeyRows rows the second pass finds which of them are of the block in shared memory.
+// row.  A thread has eight tokens in flight; up to kKeyRows rows the second pass finds which of them are of the block in shared memory.
 __global__ void __launch_bounds__(1024) sort_tokens_kernel(
     const void* __restrict__ ids, int ids32, unsigned n_ids, const int* __restrict__ id_rows,
     int rows, int V, int pad, int shift, int span, int* __restrict__ order,
@@ -231,9 +230,9 @@ __global__ void __launch_bounds__(1024) sort_tokens_kernel(
 }
 
 // A lane's columns of a slab of rows: eight neighbours (W = 8), or four columns 32 apart (W = 1).
-// Loads are made without a branch, columns behind the row from its first one, and in the place where
-// they stand: behind a branch, or moved to where they are used, one is waited for before the next
-// one is made.
+// Loads are made without a branch, columns behind the row from its first one, and what is not wanted
+// of a batch is set to zero without one: a load behind a branch, or one whose value is used behind
+// one, is waited for before the next is made (115 rows of one token, 256 wide: 31 us, now 8).
 template <int W>
 struct SlabCols {
   static constexpr int N = W == 8 ? 8 : 4;
@@ -256,6 +255,23 @@ struct SlabCols {
       for (int i = 0; i < N; ++i) k.v[i] = row[c + 32 * i < H ? c + 32 * i : 0];
       return k;
     }
+  }
+  // The same into shared memory, on its way until the thread waits for its cp.async groups.
+  template <typename T>
+  __device__ __forceinline__ void fetch(const T* row, Pack<T, N>* to) const {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(*to) / 16); ++i)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to) + i * 16),
+                   "l"(reinterpret_cast<const uint8_t*>(row + (c < H ? c : 0)) + i * 16)
+                   : "memory");
+  }
+  // The same, zeros where it is not wanted.
+  template <typename T>
+  __device__ __forceinline__ Pack<T, N> load_if(bool wanted, const T* row) const {
+    Pack<T, N> k = load(row);
+#pragma unroll
+    for (int i = 0; i < N; ++i) k.v[i] = wanted ? k.v[i] : from_f32<T>(0.f);
+    return k;
   }
   __device__ __forceinline__ void store(float* row, const float* f) const {
     if constexpr (W == 8) {
@@ -304,7 +320,12 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
     int span, int vocab, float scale, int add) {
   using S = SlabCols<W>;
   constexpr int N = S::N;
-  constexpr int U = 4;  // rows in flight
+  // Rows in flight: with whole packs they go to shared memory, each lane's to a place of its own,
+  // since the branches at the ends of runs would have loads into registers wait for each other
+  // (8192 kept of 16384 x 2048: 61 us a pass with four rows in registers, 58 with 16 in shared memory).
+  constexpr bool kStaged = W == 8;
+  constexpr int U = !kStaged ? 4 : sizeof(T) == 2 ? 16 : 8;
+  __shared__ Pack<T, N> stage[kStaged ? 4 : 1][kStaged ? U : 1][32];
   after_previous();
   let_next_start();
   // blocks that sum and blocks that clear in turn, as long as there are both: the ones wait for
@@ -346,17 +367,26 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
   bool head = from_before;  // acc sums the run that began before the chunk
 #pragma unroll 1
   for (int j = 0; j < m; j += U) {
-    Pack<T, N> k[U];
+    Pack<T, N> k[kStaged ? 1 : U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int row = __shfl_sync(0xffffffffu, my_row, (j + u) & 31);  // 0 behind the last one
-      k[u] = cols.load(dy + row * ld);
+      if constexpr (kStaged) {
+        if (j + u < m) cols.fetch(dy + row * ld, &stage[warp_id()][u][lane]);
+      } else {
+        k[u] = cols.load(dy + row * ld);
+      }
     }
-#pragma unroll
+    if constexpr (kStaged)
+      asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+#pragma unroll(kStaged ? 1 : U)
     for (int u = 0; u < U; ++u) {
       if (j + u >= m) break;
       F2 f[N / 2];
-      unpack_f2<T, N>(k[u], f);
+      if constexpr (kStaged)
+        unpack_f2<T, N>(stage[warp_id()][u][lane], f);
+      else
+        unpack_f2<T, N>(k[u], f);
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) acc[i] = acc[i] + f[i];
       const int tok = __shfl_sync(0xffffffffu, my_tok, j + u);
@@ -392,7 +422,7 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
     int add) {
   using S = SlabCols<W>;
   constexpr int N = S::N;
-  constexpr int U = 4;
+  constexpr int U = 8;  // partial sums in flight
   __shared__ float share[8][32 * N];
   __shared__ int long_chunk;
   after_previous();
@@ -408,13 +438,11 @@ __global__ void __launch_bounds__(256) embed_join_kernel(
       Pack<float, N> v[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        v[u] = cols.load(part + 2ll * min(k + u, k1 - 1) * H);
+        v[u] = cols.load_if(k + u < k1, part + 2ll * min(k + u, k1 - 1) * H);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (k + u >= k1) break;
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] += v[u].v[i];
-      }
     }
   };
   if (threadIdx.x == 0) long_chunk = -1;
@@ -521,7 +549,7 @@ __global__ void __launch_bounds__(128, 6) embed_grad_few_kernel(
       Pack<T, N> k[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) k[u] = cols.load(dy + list[w][min(j + u, to - 1)] * ld);
-#pragma unroll
+  #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (j + u >= to) break;
         F2 f[N / 2];

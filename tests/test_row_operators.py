@@ -82,7 +82,8 @@ def grad_of_table(dy, tok, V, scale):
     (2000, 2056, 900, 900, HF, False, "one"), (500, 96, 4000, 3333, BF, False, "half"),
     (32, 33, 64, 64, F32, False, "runs"), (32, 7, 33, 32, BF, True, "runs"),
     (40, 2048, 70, 65, F32, False, "text"), (40, 2500, 70, 65, BF, False, "text"),
-    (64, 16, 100, 0, BF, False, "uniform"), (50, 2048, 512, 511, BF, False, "half"),
+    (64, 16, 100, 0, BF, False, "uniform"), (50, 1030, 200, 192, BF, False, "one"),
+    (50, 1032, 200, 193, BF, False, "half"), (50, 2048, 512, 511, BF, False, "half"),
     (900, 300, 513, 513, HF, True, "text"), (7, 520, 600, 129, F32, False, "one"),
     (300, 1033, 500, 130, BF, False, "text"),
 ])
