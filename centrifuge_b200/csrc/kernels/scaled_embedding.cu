@@ -556,10 +556,10 @@ __global__ void __launch_bounds__(128, 6) embed_grad_few_kernel(
     for (int j = from; j < to; j += U) {
       Pack<T, N> k[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) k[u] = cols.load(dy + list[w][min(j + u, to - 1)] * ld);
-  #pragma unroll
+      for (int u = 0; u < U; ++u)
+        k[u] = cols.load_if(j + u < to, dy + list[w][min(j + u, to - 1)] * ld);
+#pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (j + u >= to) break;
         F2 f[N / 2];
         unpack_f2<T, N>(k[u], f);
 #pragma unroll
@@ -712,8 +712,8 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
                                      dtable, ld_t, part, rows, H, slabs, per, sums, plan.shift,
                                      plan.span, static_cast<int>(V), scale, add))
       return rc;
-    return launch_behind(wide ? embed_join_kernel<8> : embed_join_kernel<1>, dim3((chunks + 7) / 8, slabs),
-                         dim3(256), 0, st, stok, n_valid, dtable, ld_t, part, rows, H, per, scale,
-                         add);
+    return launch_behind(wide ? embed_join_kernel<8> : embed_join_kernel<1>,
+                         dim3((chunks + 7) / 8, slabs), dim3(256), 0, st, stok, n_valid, dtable,
+                         ld_t, part, rows, H, per, scale, add);
   });
 }
