@@ -34,7 +34,9 @@ namespace cfb {
 constexpr int kMaxSpan = 1024;  // tokens of one block of the sort
 constexpr int kKeyRows = 32768; // rows whose keys a block of the sort holds in shared memory
 constexpr int kClear = 4;       // table rows that one block clears (8: 63 us a pass below, 4: 61)
-constexpr int kFewRows = 128;   // up to here one launch does it all (a row id fits 8 bits)
+// Up to here one launch does it all (a row id fits 8 bits).  256 rows x 1024 of 3000 tokens: 8 us for
+// 12 sorted, x 4096 and most of one token 20 for 20.
+constexpr int kFewRows = 256;
 constexpr int kWarpRun = 24;    // rows of a token that one warp sums there by itself
 
 // Sorted positions of one warp of the gradient: few where few rows would leave SMs idle, more where

@@ -83,7 +83,9 @@ def grad_of_table(dy, tok, V, scale):
     (32, 33, 64, 64, F32, False, "runs"), (32, 7, 33, 32, BF, True, "runs"),
     (40, 2048, 70, 65, F32, False, "text"), (40, 2500, 70, 65, BF, False, "text"),
     (64, 16, 100, 0, BF, False, "uniform"), (50, 1030, 200, 192, BF, False, "one"),
-    (50, 1032, 200, 193, BF, False, "half"), (50, 2048, 512, 511, BF, False, "half"),
+    (50, 1032, 200, 193, BF, False, "half"), (50, 1032, 300, 256, F32, False, "one"),
+    (50, 1031, 300, 256, HF, False, "half"), (50, 1032, 300, 257, BF, False, "one"),
+    (50, 1031, 300, 257, F32, False, "half"), (50, 2048, 512, 511, BF, False, "half"),
     (900, 300, 513, 513, HF, True, "text"), (7, 520, 600, 129, F32, False, "one"),
     (300, 1033, 500, 130, BF, False, "text"),
 ])
@@ -722,6 +724,46 @@ def test_on_two_streams_at_once():
         torch.cuda.synchronize()
         for p, q in zip(got, want):
             assert all(torch.equal(x, y) for x, y in zip(p, q))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [200, 257, 3000])
+@pytest.mark.parametrize("H", [256, 515])
+def test_table_gradient_captured_and_on_two_streams(rows, H):
+    """The sorted gradient's launches in graphs that share a pool, and beside each other."""
+    g = gen("cuda", 24)
+    sets = []
+    for k in range(2):
+        ids = torch.randint(0, 700, (rows,), generator=g, device="cuda")
+        ids[::3] = 11 + k
+        sets.append((rand(g, rows, H, dtype=BF), ids, torch.empty(700, H, device="cuda")))
+
+    def call(s):
+        fused.scaled_embedding_bwd(*s, 0.5, accumulate=False)
+        return fused.scaled_embedding_bwd(*s, 2.0)
+
+    want = [call(s).clone() for s in sets]
+    for (dy, ids, _), w in zip(sets, want):
+        close(w, *grad_of_table(dy, ids, 700, 2.5), "dtable")
+    torch.cuda.synchronize()
+    graphs = []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=graphs[0].pool() if len(graphs) > 1 else None):
+            call(s)
+    for _ in range(3):
+        for (_, _, table), graph in zip(sets, graphs):
+            table.fill_(float("nan"))
+            graph.replay()
+        assert all(torch.equal(s[2], w) for s, w in zip(sets, want))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        torch.cuda.synchronize()
+        for st, s in zip(streams, sets):
+            with torch.cuda.stream(st):
+                call(s)
+        torch.cuda.synchronize()
+        assert all(torch.equal(s[2], w) for s, w in zip(sets, want))
 
 
 @pytest.mark.gpu
