@@ -823,6 +823,13 @@ inline void check_vector(const Tensor& t, int64_t n, at::ScalarType type, const 
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous(),
                     what, ": ", name, " must be contiguous ", type, " [", n, "]");
 }
+// The bytes of a tensor of one dimension.
+struct Bytes {
+  uintptr_t lo, hi;
+  explicit Bytes(const Tensor& t)
+      : lo(reinterpret_cast<uintptr_t>(t.data_ptr())), hi(lo + t.nbytes()) {}
+  bool overlaps(const Bytes& o) const { return lo < o.hi && o.lo < hi; }
+};
 inline int row_count(int64_t rows, const char* what) {
   TORCH_CHECK_VALUE(rows < (1ll << 30), what, ": ", rows, " rows");
   return static_cast<int>(rows);
@@ -1026,6 +1033,20 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> block_norms_bwd(
   same_device(h, dw_pre, "dw_pre");
   same_device(h, dgate, "dgate");
   same_device(h, rows, "rows");
+  // the buffers of a parameter that is used twice are one, and get both gradients
+  const Tensor* sums[] = {&dw_post, pre ? &*dw_pre : nullptr, dgate.has_value() ? &*dgate : nullptr};
+  const Tensor* params[] = {&w_post, pre ? &*w_pre : nullptr, dgate.has_value() ? &*gate : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    if (!sums[i]) continue;
+    const Bytes a(*sums[i]);
+    for (int j = 0; j < 3; ++j) {
+      TORCH_CHECK_VALUE(j >= i || !sums[j] || Bytes(*sums[j]).lo == a.lo ||
+                            !a.overlaps(Bytes(*sums[j])),
+                        what, ": dw_post, dw_pre and dgate overlap in part");
+      TORCH_CHECK_VALUE(!params[j] || !a.overlaps(Bytes(*params[j])), what,
+                        ": dw_post, dw_pre or dgate overlaps a weight or the gate");
+    }
+  }
   row_count(T, what);
   const c10::cuda::CUDAGuard guard(h.device());
   const int R = row_count(R64, what);

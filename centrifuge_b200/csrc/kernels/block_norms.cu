@@ -785,17 +785,19 @@ __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 
   }
 }
 
-// dw_pre (blockIdx.y = 0), dw_post and a channel gate's gradient (1) from the blocks' column sums,
-// in block order.  Block: 32 columns x 32 slices of the blocks.
+// dw_pre (which = 0), dw_post and a channel gate's gradient (which = 1) from the blocks' column sums,
+// in block order; which = first + blockIdx.y.  Block: 32 columns x 32 slices of the blocks.  The
+// three buffers may be one another (a parameter that is used in two places), so they are not
+// __restrict__, and dw_pre has a launch of its own where it is one of the others.
 template <typename TH>
 __global__ void __launch_bounds__(1024) block_norms_join_kernel(
     const float* part, int blocks, int H, const TH* __restrict__ w_post,
-    const TH* __restrict__ gate, float* __restrict__ dw_pre, float* __restrict__ dw_post,
-    float* __restrict__ dgate, int add) {
+    const TH* __restrict__ gate, float* dw_pre, float* dw_post, float* dgate, int add_pre,
+    int add_post, int add_gate, int first) {
   __shared__ float red[32][33];
   const int cx = threadIdx.x & 31, ry = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + cx;
-  const int which = blockIdx.y;
+  const int which = first + blockIdx.y;
   after_previous();
   if (which == 0 && dw_pre == nullptr) return;
   float s = 0.f;
@@ -809,11 +811,11 @@ __global__ void __launch_bounds__(1024) block_norms_join_kernel(
   const int col = blockIdx.x * 32 + ry;
   if (cx != 0 || col >= H) return;
   if (which == 0) {
-    dw_pre[col] = (add ? dw_pre[col] : 0.f) + s;
+    dw_pre[col] = (add_pre ? dw_pre[col] : 0.f) + s;
     return;
   }
-  dw_post[col] = (add ? dw_post[col] : 0.f) + (gate ? s * to_f32(gate[col]) : s);
-  if (dgate) dgate[col] = (add ? dgate[col] : 0.f) + s * to_f32(w_post[col]);
+  dw_post[col] = (add_post ? dw_post[col] : 0.f) + (gate ? s * to_f32(gate[col]) : s);
+  if (dgate) dgate[col] = (add_gate ? dgate[col] : 0.f) + s * to_f32(w_post[col]);
 }
 
 // f(TypeTag<TH>, TypeTag<TX>): the residual stream has the block's type or fp32.
@@ -1071,11 +1073,25 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
     } else if (add) {
       return 0;
     }
+    // What two gradients share gets the sum of both: dw_pre first, then dw_post, then dgate.
     const bool channel = a.gate_kind == kGateChannel;
-    return launch_behind(block_norms_join_kernel<TH>, dim3((H + 31) / 32, 2), dim3(1024), 0, st,
-                         part, blocks, H, static_cast<const TH*>(a.w_post),
-                         channel ? static_cast<const TH*>(a.gate) : nullptr,
-                         a.w_pre ? dw_pre : nullptr, dw_post,
-                         channel ? static_cast<float*>(dgate) : nullptr, add);
+    float* pre = a.w_pre ? dw_pre : nullptr;
+    float* gate_sum = channel ? static_cast<float*>(dgate) : nullptr;
+    const bool post_on_pre = pre != nullptr && dw_post == pre;
+    const bool gate_on_pre = pre != nullptr && gate_sum == pre;
+    const bool apart = !post_on_pre && !gate_on_pre;
+    const auto* w_post = static_cast<const TH*>(a.w_post);
+    const auto* gate = channel ? static_cast<const TH*>(a.gate) : nullptr;
+    const unsigned columns = (H + 31) / 32;
+    const int add_post = add || post_on_pre;
+    const int add_gate = add || gate_on_pre || gate_sum == dw_post;
+    const int rc = launch_behind(block_norms_join_kernel<TH>, dim3(columns, apart ? 2 : 1),
+                                 dim3(1024), 0, st, part, blocks, H, w_post, gate, pre, dw_post,
+                                 gate_sum, add, add_post, add_gate, 0);
+    if (rc || apart) return rc;
+    block_norms_join_kernel<TH><<<columns, 1024, 0, st>>>(part, blocks, H, w_post, gate, pre,
+                                                          dw_post, gate_sum, add, add_post,
+                                                          add_gate, 1);
+    return launch_status();
   });
 }

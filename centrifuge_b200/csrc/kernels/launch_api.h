@@ -264,7 +264,8 @@ int cfb_block_norms_fwd(const CfbBlockNorms* p, float eps, void* y, void* n, flo
 // Gradient on the rows row_ids[0, rows) (or 0 .. rows) of h and y; a row id outside [0, n_rows)
 // records kErrBounds and gives zero rows.  dgate: [rows, 1] fp32 or [rows, H] for a token's or
 // element's gate, [H] fp32 for a channel's.  dw_post, dw_pre and a channel's dgate are added to
-// with `add`.
+// with `add`; they may be one another (the sum of the gradients goes there), and must not overlap
+// otherwise, nor overlap a weight or the gate.
 long long cfb_block_norms_bwd_workspace(int rows, int H);
 int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy, const void* dn,
                         long long ld_dn, const float* rstd_post, const float* rstd_pre,

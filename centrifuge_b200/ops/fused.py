@@ -146,6 +146,12 @@ def _vector(t: torch.Tensor, H: int, dtype: torch.dtype) -> bool:
     return t.dim() == 1 and t.shape[0] == H and t.dtype == dtype and t.is_contiguous()
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share bytes."""
+    lo, at = a.data_ptr(), b.data_ptr()
+    return lo < at + b.numel() * b.element_size() and at < lo + a.numel() * a.element_size()
+
+
 def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``out[r] = scale * table[ids[r]]``, rounded once.
@@ -267,8 +273,9 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
     ``dy [R, H]`` is the gradient that reaches ``y`` past the next block (``None``: none does) and
     ``dn [R, H]`` that of ``n``; without ``w_pre``, ``dn``, ``y``, ``rstd_pre`` and ``dw_pre`` are
     ``None``.  ``dw_post``, ``dw_pre`` and, for a learned gate, ``dgate`` are fp32 ``[H]`` buffers,
-    added to (written without ``accumulate``); a token's or element's gate returns its gradient
-    for the ``R`` rows.  On the GPU a row id outside ``h`` records an error in the status block and
+    added to (written without ``accumulate``); a buffer given for two of them (one parameter in both
+    places) gets the sum of both gradients, other overlaps are refused.  A token's or element's gate
+    returns its gradient for the ``R`` rows.  On the GPU a row id outside ``h`` records an error in the status block and
     gives zero rows."""
     if h.is_cuda:
         return kernels().block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre, dw_post,
@@ -311,6 +318,13 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
     learned = gate is not None and gate.dim() == 1
     _need((dgate is not None) == learned and (not learned or _vector(dgate, H, torch.float32)),
           "{}: dgate is the fp32 [{}] buffer of a learned gate", name, H)
+    sums = [t for t in (dw_post, dw_pre, dgate) if t is not None]
+    params = [t for t in (w_post, w_pre, gate if learned else None) if t is not None]
+    for i, s in enumerate(sums):
+        _need(all(s.data_ptr() == t.data_ptr() or not _overlap(s, t) for t in sums[:i]),
+              "{}: dw_post, dw_pre and dgate overlap in part", name)
+        _need(not any(_overlap(s, t) for t in params),
+              "{}: dw_post, dw_pre or dgate overlaps a weight or the gate", name)
     if rows is not None:
         at = rows.long()
         h, rstd_post = h[at], rstd_post[at]
@@ -318,9 +332,11 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
         gate = gate if gate is None or learned else gate[at]
     dx, dh, dp, dq, dg = ref.block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre,
                                              gate, block_scale, resid_scale)
-    for acc, d in ((dw_post, dp), (dw_pre, dq), (dgate, dg if learned else None)):
+    written = set()
+    for acc, d in ((dw_pre, dq), (dw_post, dp), (dgate, dg if learned else None)):
         if acc is not None:
-            acc.copy_(acc + d if accumulate else d)
+            acc.copy_(acc + d if accumulate or acc.data_ptr() in written else d)
+            written.add(acc.data_ptr())
     return (dx.to(resid), dh.to(h.dtype),
             dgate if gate is None or learned else dg.to(gate.dtype))
 

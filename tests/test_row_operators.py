@@ -359,6 +359,43 @@ def test_block_norms_gradient_against_differences(dev, gate):
 
 
 @pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("accumulate", [True, False])
+@pytest.mark.parametrize("which", [(0, 0, 1), (0, 1, 0), (0, 1, 1), (0, 0, 0)])
+@pytest.mark.parametrize("T,H,dtype", [(300, 2048, BF), (40, 2049, F32), (0, 64, HF)])
+def test_block_norms_bwd_of_a_shared_parameter(dev, accumulate, which, T, H, dtype):
+    """One buffer for two or all of dw_post, dw_pre and dgate gets the sum of their gradients."""
+    g, c = norms_case(dev, T, H, dtype, dtype, "channel", True, seed=9)
+    y, _, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS, c["gate"])
+    dy, dn = rand(g, T, H, dtype=dtype), rand(g, T, H, dtype=dtype)
+
+    def grads(a, b, d, accumulate):
+        fused.block_norms_bwd(dy, dn, c["h"], y, rp, rq, c["w_post"], c["w_pre"], a, b,
+                              gate=c["gate"], dgate=d, accumulate=accumulate)
+
+    alone = torch.empty(3, H, device=dev)
+    grads(*alone, False)
+    base = rand(g, 2, H)
+    for _ in range(3):
+        acc = base.clone()
+        grads(*(acc[i] for i in which), accumulate)
+        for i in range(max(which) + 1):
+            parts = [alone[k].double() for k in range(3) if which[k] == i]
+            if accumulate:
+                parts.append(base[i].double())
+            # each gradient is rounded once alone (its product with the gate or the weight, where the
+            # sum may fuse it) and once in the sum, which has at most four terms
+            close(acc[i], sum(parts), 4 * U * sum(p.abs() for p in parts), f"buffer {i}")
+    buf = torch.zeros(2 * H, device=dev)
+    for a, b, d in ((buf[:H], buf[1:H + 1], alone[2]), (alone[0], buf[:H], buf[H - 1:2 * H - 1])):
+        with pytest.raises(ValueError, match="overlap in part"):
+            grads(a, b, d, accumulate)
+    if dtype == F32:
+        for over in ("w_post", "w_pre", "gate"):
+            with pytest.raises(ValueError, match="overlaps a weight or the gate"):
+                grads(alone[0], alone[1], c[over], accumulate)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
 def test_block_norms_odd_values(dev):
     """Rows of zeros stay finite; what is no number in one row stays in its row; no rows at all."""
     _, c = norms_case(dev, 5, 64, BF, BF, "channel", True)
