@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <string>
 #include <tuple>
 #include <vector>
 
@@ -823,7 +824,7 @@ inline void check_vector(const Tensor& t, int64_t n, at::ScalarType type, const 
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous(),
                     what, ": ", name, " must be contiguous ", type, " [", n, "]");
 }
-// The bytes of a tensor of one dimension.
+// The bytes of a contiguous tensor.
 struct Bytes {
   uintptr_t lo, hi;
   explicit Bytes(const Tensor& t)
@@ -1071,13 +1072,16 @@ std::tuple<Tensor, Tensor, c10::optional<Tensor>> block_norms_bwd(
   return {dx, dh, dg};
 }
 
-// The non-empty tensors of a gradient list and where their scaled values go.  Checks that no output
-// overlaps another output or another tensor of the list.
+// The non-empty tensors of a gradient list and where their scaled values go.  Checks that nothing
+// that is written (the outputs and the norm) overlaps anything else of the call: blocks write while
+// others still read the list and the sums.
 std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor>& grads,
-                                      const std::vector<Tensor>* outs, bool* in_place) {
+                                      const std::vector<Tensor>* outs, bool* in_place,
+                                      const c10::optional<Tensor>& norm = c10::nullopt,
+                                      const c10::optional<Tensor>& sums = c10::nullopt) {
   struct Span {
     uintptr_t lo, hi;
-    size_t index;
+    std::ptrdiff_t index;  // -1: norm, -2: extra_sumsq
     bool written;
   };
   TORCH_CHECK_VALUE(!grads.empty(), what, ": empty list");
@@ -1086,8 +1090,10 @@ std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor
   std::vector<CfbTensorRef> refs;
   std::vector<Span> spans;
   refs.reserve(grads.size());
-  spans.reserve(2 * grads.size());
+  spans.reserve(2 * grads.size() + 2);
   bool same = true;
+  if (norm.has_value()) spans.push_back({Bytes(*norm).lo, Bytes(*norm).hi, -1, true});
+  if (sums.has_value()) spans.push_back({Bytes(*sums).lo, Bytes(*sums).hi, -2, false});
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& g = grads[i];
     TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.is_cuda() && g.device() == grads[0].device(),
@@ -1108,8 +1114,9 @@ std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor
       const bool own = r.out == r.ptr && r.out_type == r.type;
       same = same && own;
       if (r.numel > 0) {
-        if (!own) spans.push_back({a, a + g.nbytes(), i, false});
-        spans.push_back({b, b + o.nbytes(), i, true});
+        const auto at = static_cast<std::ptrdiff_t>(i);
+        if (!own) spans.push_back({a, a + g.nbytes(), at, false});
+        spans.push_back({b, b + o.nbytes(), at, true});
       }
     }
     if (r.numel > 0) refs.push_back(r);
@@ -1117,8 +1124,11 @@ std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor
   std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
   uintptr_t end = 0, end_written = 0;  // of all spans so far, and of the written ones
   for (const Span& s : spans) {
-    TORCH_CHECK_VALUE(s.lo >= (s.written ? end : end_written), what, ": tensor ", s.index,
-                      " overlaps another that is written");
+    TORCH_CHECK_VALUE(s.lo >= (s.written ? end : end_written), what, ": ",
+                      s.index == -1   ? "norm"
+                      : s.index == -2 ? "extra_sumsq"
+                                      : "tensor " + std::to_string(s.index),
+                      " and another tensor overlap, and one of them is written");
     end = std::max(end, s.hi);
     if (s.written) end_written = std::max(end_written, s.hi);
   }
@@ -1126,10 +1136,11 @@ std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor
   return refs;
 }
 
-inline void check_f32(const Tensor& t, const Tensor& first, const char* what, const char* name) {
-  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() > 0 &&
-                        t.device() == first.device(),
-                    what, ": ", name, " must be contiguous fp32 on ", first.device());
+inline void check_f32(const Tensor& t, const std::vector<Tensor>& grads, const char* what,
+                      const char* name) {
+  TORCH_CHECK_VALUE(!grads.empty() && t.scalar_type() == at::kFloat && t.is_contiguous() &&
+                        t.numel() > 0 && t.device() == grads[0].device(),
+                    what, ": ", name, " must be contiguous fp32 on the device of the list");
 }
 
 constexpr int64_t kListBlocks = 148 * 8;  // partial sums of a list, at most, for each launch
@@ -1161,18 +1172,10 @@ Tensor grad_list_clip(const std::vector<Tensor>& grads,
                       const c10::optional<Tensor>& extra_sumsq) {
   const char* what = "grad_list_clip_";
   bool in_place = false;
-  std::vector<CfbTensorRef> refs =
-      tensor_refs(what, grads, outs.has_value() ? &*outs : &grads, &in_place);
-  if (norm_in.has_value()) check_f32(*norm_in, grads[0], what, "norm");
-  if (extra_sumsq.has_value()) {
-    check_f32(*extra_sumsq, grads[0], what, "extra_sumsq");
-    if (norm_in.has_value()) {  // the norm is written while blocks still read the sums
-      const uintptr_t n = reinterpret_cast<uintptr_t>(norm_in->data_ptr());
-      const uintptr_t e = reinterpret_cast<uintptr_t>(extra_sumsq->data_ptr());
-      TORCH_CHECK_VALUE(n + norm_in->nbytes() <= e || n >= e + extra_sumsq->nbytes(), what,
-                        ": norm overlaps extra_sumsq");
-    }
-  }
+  if (norm_in.has_value()) check_f32(*norm_in, grads, what, "norm");
+  if (extra_sumsq.has_value()) check_f32(*extra_sumsq, grads, what, "extra_sumsq");
+  std::vector<CfbTensorRef> refs = tensor_refs(what, grads, outs.has_value() ? &*outs : &grads,
+                                               &in_place, norm_in, extra_sumsq);
   const c10::cuda::CUDAGuard guard(grads[0].device());
   const Tensor own = extra_sumsq.has_value() ? Tensor() : sumsq_of(refs, grads[0]);
   const Tensor& partial = extra_sumsq.has_value() ? *extra_sumsq : own;

@@ -468,23 +468,33 @@ def _check_grads(name: str, grads: List[torch.Tensor]) -> None:
             raise ValueError(f"{name}: tensor {i} must be a dense bf16, fp16 or fp32 tensor on {dev}")
 
 
-def _check_spans(grads: List[torch.Tensor], outs: List[torch.Tensor]) -> None:
-    """Outputs shaped like their gradients, dense, and apart from every other tensor."""
+def _check_spans(grads: List[torch.Tensor], outs: List[torch.Tensor],
+                 norm: Optional[torch.Tensor], extra_sumsq: Optional[torch.Tensor]) -> None:
+    """Outputs shaped like their gradients and dense; nothing that is written (the outputs and the
+    norm) overlaps anything else."""
     spans, end, end_written = [], 0, 0
+
+    def add(t: torch.Tensor, name: str, written: bool) -> None:
+        lo = t.data_ptr()
+        if t.numel():
+            spans.append((lo, lo + t.numel() * t.element_size(), name, written))
+
     for i, (g, o) in enumerate(zip(grads, outs)):
         _need(o.shape == g.shape and (o.stride() == g.stride()
                                       or o.is_contiguous() and g.is_contiguous()),
               "grad_list_clip_: output {} must have the sizes and strides of its gradient", i)
         _need(torch.ops.aten.is_non_overlapping_and_dense.default(g),
               "grad_list_clip_: tensor {} has gaps or overlaps itself", i)
-        own = o.data_ptr() == g.data_ptr() and o.dtype == g.dtype
-        for t in (o,) if own else (g, o):
-            lo = t.data_ptr()
-            if t.numel():
-                spans.append((lo, lo + t.numel() * t.element_size(), i, t is o))
-    for lo, hi, i, written in sorted(spans):
+        if not (o.data_ptr() == g.data_ptr() and o.dtype == g.dtype):
+            add(g, f"tensor {i}", False)
+        add(o, f"tensor {i}", True)
+    if norm is not None:
+        add(norm, "norm", True)
+    if extra_sumsq is not None:
+        add(extra_sumsq, "extra_sumsq", False)
+    for lo, hi, name, written in sorted(spans):
         _need(lo >= (end if written else end_written),
-              "grad_list_clip_: tensor {} overlaps another that is written", i)
+              "grad_list_clip_: {} and another tensor overlap, and one of them is written", name)
         end, end_written = max(end, hi), max(end_written, hi) if written else end_written
 
 
@@ -504,8 +514,8 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
     own (see :func:`grad_list_sumsq`).
 
     Tensors are bf16, fp16 or fp32, of any size and alignment, in any dense layout (``out[i]``
-    in that of ``grads[i]``); the list may mix types.  Tensors that overlap another one that is
-    written, and tensors with gaps, are refused.  The squares are fp32 (an element above 1.8e19
+    in that of ``grads[i]``); the list may mix types.  Tensors with gaps are refused, and so are
+    outputs and a ``norm`` that overlap anything else of the call.  The squares are fp32 (an element above 1.8e19
     makes the norm infinite)."""
     grads = list(grads)
     if not extra_scale > 0:
@@ -521,9 +531,7 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
         _need(len(outs) == len(grads), "grad_list_clip_: {} gradients, {} outputs", len(grads),
               len(outs))
         _check_grads("grad_list_clip_", outs)
-    _check_spans(grads, outs)
-    _need(norm is None or extra_sumsq is None or norm.data_ptr() != extra_sumsq.data_ptr(),
-          "grad_list_clip_: norm overlaps extra_sumsq")
+    _check_spans(grads, outs, norm, extra_sumsq)
     if norm is None:
         norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
     if extra_sumsq is None:

@@ -547,6 +547,27 @@ def test_grad_list_over_ranks_and_coef(dev):
     assert float(coef) == pytest.approx(0.25, rel=1e-4)
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_grad_list_clip_refuses_a_norm_or_sums_in_the_list(dev):
+    """What is written while other blocks read it, or read while others write it."""
+    buf = torch.ones(300, device=dev)
+    keep = buf.clone()
+    g, o, sums, norm = buf[:100], buf[100:200], buf[200:208], buf[299:]
+    for kw in (dict(norm=g[3:4]), dict(norm=g[99:]), dict(out=[o], norm=o[:1]),
+               dict(out=[o], norm=g[:1]),  # o only: g is read
+               dict(extra_sumsq=g[4:8]), dict(out=[o], extra_sumsq=buf[196:204]),
+               dict(norm=sums[3:4], extra_sumsq=sums), dict(norm=sums[:1], extra_sumsq=sums)):
+        with pytest.raises(ValueError, match="overlap"):
+            fused.grad_list_clip_([g], 1.0, **kw)
+        assert torch.equal(buf, keep)
+    # sums in a gradient that is only read, and neighbours, are fine
+    n = fused.grad_list_clip_([g], 1.0, out=[o], norm=norm, extra_sumsq=g[:16])
+    assert n.data_ptr() == norm.data_ptr() and float(n) == 4.0
+    assert torch.equal(g, keep[:100]) and torch.equal(sums, keep[200:208])
+    close(o, torch.full((100,), 0.25 / (1 + 2.5e-7), dtype=torch.float64, device=dev),
+          torch.full((100,), 4 * U, dtype=torch.float64, device=dev), "out")
+
+
 # ---------------------------------------------------------------- refusals
 @pytest.mark.parametrize("dev", CPU_GPU)
 def test_refusals(dev):
