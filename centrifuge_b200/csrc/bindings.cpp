@@ -1084,7 +1084,6 @@ std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor
     std::ptrdiff_t index;  // -1: norm, -2: extra_sumsq
     bool written;
   };
-  TORCH_CHECK_VALUE(!grads.empty(), what, ": empty list");
   TORCH_CHECK_VALUE(!outs || outs->size() == grads.size(), what, ": ", grads.size(),
                     " gradients, ", outs ? outs->size() : 0, " outputs");
   std::vector<CfbTensorRef> refs;
@@ -1136,11 +1135,10 @@ std::vector<CfbTensorRef> tensor_refs(const char* what, const std::vector<Tensor
   return refs;
 }
 
-inline void check_f32(const Tensor& t, const std::vector<Tensor>& grads, const char* what,
-                      const char* name) {
-  TORCH_CHECK_VALUE(!grads.empty() && t.scalar_type() == at::kFloat && t.is_contiguous() &&
-                        t.numel() > 0 && t.device() == grads[0].device(),
-                    what, ": ", name, " must be contiguous fp32 on the device of the list");
+inline void check_f32(const Tensor& t, const Tensor& first, const char* what, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() > 0 &&
+                        t.device() == first.device(),
+                    what, ": ", name, " must be contiguous fp32 on ", first.device());
 }
 
 constexpr int64_t kListBlocks = 148 * 8;  // partial sums of a list, at most, for each launch
@@ -1159,6 +1157,7 @@ Tensor sumsq_of(const std::vector<CfbTensorRef>& refs, const Tensor& first) {
   return partial;
 }
 Tensor grad_list_sumsq(const std::vector<Tensor>& grads) {
+  TORCH_CHECK_VALUE(!grads.empty(), "grad_list_sumsq: empty list");
   const std::vector<CfbTensorRef> refs = tensor_refs("grad_list_sumsq", grads, nullptr, nullptr);
   const c10::cuda::CUDAGuard guard(grads[0].device());
   return sumsq_of(refs, grads[0]);
@@ -1172,14 +1171,17 @@ Tensor grad_list_clip(const std::vector<Tensor>& grads,
                       const c10::optional<Tensor>& extra_sumsq) {
   const char* what = "grad_list_clip_";
   bool in_place = false;
-  if (norm_in.has_value()) check_f32(*norm_in, grads, what, "norm");
-  if (extra_sumsq.has_value()) check_f32(*extra_sumsq, grads, what, "extra_sumsq");
+  // a rank without parameters has the others' sums all the same
+  TORCH_CHECK_VALUE(!grads.empty() || extra_sumsq.has_value(), what, ": empty list");
+  const Tensor& first = grads.empty() ? *extra_sumsq : grads[0];
+  if (norm_in.has_value()) check_f32(*norm_in, first, what, "norm");
+  if (extra_sumsq.has_value()) check_f32(*extra_sumsq, first, what, "extra_sumsq");
   std::vector<CfbTensorRef> refs = tensor_refs(what, grads, outs.has_value() ? &*outs : &grads,
                                                &in_place, norm_in, extra_sumsq);
-  const c10::cuda::CUDAGuard guard(grads[0].device());
-  const Tensor own = extra_sumsq.has_value() ? Tensor() : sumsq_of(refs, grads[0]);
+  const c10::cuda::CUDAGuard guard(first.device());
+  const Tensor own = extra_sumsq.has_value() ? Tensor() : sumsq_of(refs, first);
   const Tensor& partial = extra_sumsq.has_value() ? *extra_sumsq : own;
-  Tensor norm = norm_in.has_value() ? *norm_in : new_empty({1}, at::kFloat, grads[0]);
+  Tensor norm = norm_in.has_value() ? *norm_in : new_empty({1}, at::kFloat, first);
   if (refs.empty()) refs.push_back({nullptr, nullptr, 0, kF32, kF32});  // the norm is still due
   CFB_CHECK_RC(cfb_grad_list_scale(refs.data(), static_cast<int>(refs.size()),
                                    partial.data_ptr<float>(), static_cast<int>(partial.numel()),

@@ -461,8 +461,8 @@ def grad_list_sumsq(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     return sum(g.double().pow(2).sum() for g in grads).float().view(1)
 
 
-def _check_grads(name: str, grads: List[torch.Tensor]) -> None:
-    dev = grads[0].device
+def _check_grads(name: str, grads: List[torch.Tensor], dev: Optional[torch.device] = None) -> None:
+    dev = dev or grads[0].device
     for i, g in enumerate(grads):
         if g.dtype not in _ROW_TYPES or g.device != dev or g.layout != torch.strided:
             raise ValueError(f"{name}: tensor {i} must be a dense bf16, fp16 or fp32 tensor on {dev}")
@@ -511,7 +511,7 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
     optimizer's fp32 buffer).  Returns ``norm`` (fp32 ``[1]``).  ``max_norm <= 0`` sets no limit.
     A norm that is infinite or no number is returned as such, and carries over to the gradients as
     the formula says.  ``extra_sumsq``: fp32 partial sums of squares to use instead of the list's
-    own (see :func:`grad_list_sumsq`).
+    own (see :func:`grad_list_sumsq`); the norm is theirs for an empty list too.
 
     Tensors are bf16, fp16 or fp32, of any size and alignment, in any dense layout (``out[i]``
     in that of ``grads[i]``); the list may mix types.  Tensors with gaps are refused, and so are
@@ -520,20 +520,21 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
     grads = list(grads)
     if not extra_scale > 0:
         raise ValueError(f"grad_list_clip_: extra_scale = {extra_scale} is not positive")
-    if not grads:
-        return torch.zeros(1) if norm is None else norm.zero_()
-    if grads[0].is_cuda:
-        return kernels().grad_list_clip(grads, None if out is None else list(out), max_norm,
-                                        extra_scale, norm, extra_sumsq)
-    _check_grads("grad_list_clip_", grads)
     outs = grads if out is None else list(out)
-    if out is not None:
-        _need(len(outs) == len(grads), "grad_list_clip_: {} gradients, {} outputs", len(grads),
-              len(outs))
-        _check_grads("grad_list_clip_", outs)
+    _need(len(outs) == len(grads), "grad_list_clip_: {} gradients, {} outputs", len(grads),
+          len(outs))
+    if not grads and extra_sumsq is None:
+        return torch.zeros(1) if norm is None else norm.zero_()
+    first = grads[0] if grads else extra_sumsq
+    if first.is_cuda:
+        return kernels().grad_list_clip(grads, None if out is None else outs, max_norm, extra_scale,
+                                        norm, extra_sumsq)
+    if grads:
+        _check_grads("grad_list_clip_", grads)
+        _check_grads("grad_list_clip_", outs, first.device)
     _check_spans(grads, outs, norm, extra_sumsq)
     if norm is None:
-        norm = torch.empty(1, dtype=torch.float32, device=grads[0].device)
+        norm = torch.empty(1, dtype=torch.float32, device=first.device)
     if extra_sumsq is None:
         extra_sumsq = grad_list_sumsq(grads)
     norm.copy_((extra_sumsq.double().sum().sqrt() * extra_scale).view(1))

@@ -548,6 +548,21 @@ def test_grad_list_over_ranks_and_coef(dev):
 
 
 @pytest.mark.parametrize("dev", CPU_GPU)
+def test_grad_list_of_a_rank_without_parameters(dev):
+    """The norm comes from the other ranks' sums; an output without a gradient is refused."""
+    sums = torch.tensor([3.0, 6.0], device=dev)
+    n = fused.grad_list_clip_([], 1.0, 0.5, extra_sumsq=sums)
+    assert n.device == sums.device and n.shape == (1,) and float(n) == 1.5
+    norm = torch.empty(1, device=dev)
+    assert fused.grad_list_clip_([], 1.0, norm=norm, extra_sumsq=sums) is norm or dev == "cuda"
+    assert float(norm) == 3.0 and float(fused.grad_list_clip_([], 1.0, norm=norm)) == 0.0
+    with pytest.raises(ValueError):
+        fused.grad_list_clip_([], 1.0, out=[norm])
+    with pytest.raises(ValueError):
+        fused.grad_list_clip_([], 1.0, norm=sums[:1], extra_sumsq=sums)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
 def test_grad_list_clip_refuses_a_norm_or_sums_in_the_list(dev):
     """What is written while other blocks read it, or read while others write it."""
     buf = torch.ones(300, device=dev)
