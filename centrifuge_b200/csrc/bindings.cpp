@@ -1174,7 +1174,10 @@ Tensor grad_list_clip(const std::vector<Tensor>& grads,
   // a rank without parameters has the others' sums all the same
   TORCH_CHECK_VALUE(!grads.empty() || extra_sumsq.has_value(), what, ": empty list");
   const Tensor& first = grads.empty() ? *extra_sumsq : grads[0];
-  if (norm_in.has_value()) check_f32(*norm_in, first, what, "norm");
+  if (norm_in.has_value()) {
+    check_f32(*norm_in, first, what, "norm");
+    TORCH_CHECK_VALUE(norm_in->numel() == 1, what, ": norm has ", norm_in->numel(), " elements");
+  }
   if (extra_sumsq.has_value()) check_f32(*extra_sumsq, first, what, "extra_sumsq");
   std::vector<CfbTensorRef> refs = tensor_refs(what, grads, outs.has_value() ? &*outs : &grads,
                                                &in_place, norm_in, extra_sumsq);

@@ -532,12 +532,17 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
     if grads:
         _check_grads("grad_list_clip_", grads)
         _check_grads("grad_list_clip_", outs, first.device)
+    for name, t in (("norm", norm), ("extra_sumsq", extra_sumsq)):
+        _need(t is None or t.dtype == torch.float32 and t.is_contiguous() and t.numel() > 0
+              and t.device == first.device, "grad_list_clip_: {} must be contiguous fp32 on {}", name,
+              first.device)
+    _need(norm is None or norm.numel() == 1, "grad_list_clip_: norm has more than one element")
     _check_spans(grads, outs, norm, extra_sumsq)
     if norm is None:
         norm = torch.empty(1, dtype=torch.float32, device=first.device)
     if extra_sumsq is None:
         extra_sumsq = grad_list_sumsq(grads)
-    norm.copy_((extra_sumsq.double().sum().sqrt() * extra_scale).view(1))
+    norm.copy_((extra_sumsq.double().sum().sqrt() * extra_scale).view(norm.shape))
     k = extra_scale
     if max_norm > 0:
         k = (max_norm / (norm.view(()) + 1e-6)).clamp(max=1.0) * extra_scale

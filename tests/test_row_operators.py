@@ -583,6 +583,21 @@ def test_grad_list_clip_refuses_a_norm_or_sums_in_the_list(dev):
           torch.full((100,), 4 * U, dtype=torch.float64, device=dev), "out")
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_grad_list_clip_checks_norm_and_sums(dev):
+    """The CPU and the GPU take the same buffers: one fp32 element, and contiguous fp32 sums."""
+    g = torch.full((4,), 2.0, device=dev)
+    two = torch.zeros(2, device=dev)
+    for kw in (dict(norm=two), dict(norm=two[:1].double()), dict(norm=two[:0]),
+               dict(extra_sumsq=two.double()), dict(extra_sumsq=two.new_ones(6)[::2]),
+               dict(extra_sumsq=two[:0])):
+        with pytest.raises(ValueError):
+            fused.grad_list_clip_([g], 1.0, **kw)
+        assert bool((g == 2.0).all()) and not two.any()
+    norm = torch.zeros((), device=dev)
+    assert float(fused.grad_list_clip_([g], 8.0, norm=norm)) == 4.0 and float(norm) == 4.0
+
+
 # ---------------------------------------------------------------- refusals
 @pytest.mark.parametrize("dev", CPU_GPU)
 def test_refusals(dev):
