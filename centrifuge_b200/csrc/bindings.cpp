@@ -824,12 +824,24 @@ inline void check_vector(const Tensor& t, int64_t n, at::ScalarType type, const 
   TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.is_contiguous(),
                     what, ": ", name, " must be contiguous ", type, " [", n, "]");
 }
-// The bytes of a contiguous tensor.
+// The bytes of a row-major tensor [rows, width], or of any contiguous tensor as one row.
 struct Bytes {
   uintptr_t lo, hi;
-  explicit Bytes(const Tensor& t)
-      : lo(reinterpret_cast<uintptr_t>(t.data_ptr())), hi(lo + t.nbytes()) {}
-  bool overlaps(const Bytes& o) const { return lo < o.hi && o.lo < hi; }
+  int64_t step, width;  // bytes; step 0: one row
+  explicit Bytes(const Tensor& t) : lo(reinterpret_cast<uintptr_t>(t.data_ptr())) {
+    const bool rows = t.dim() == 2 && t.size(0) > 1 && !t.is_contiguous();
+    step = rows ? t.stride(0) * t.element_size() : 0;
+    width = rows ? t.size(1) * t.element_size() : t.nbytes();
+    hi = lo + (rows ? (t.size(0) - 1) * step + width : width);
+  }
+  bool overlaps(const Bytes& o) const {
+    if (lo >= hi || o.lo >= o.hi || lo >= o.hi || o.lo >= hi) return false;
+    const int64_t s = std::max(step, o.step);  // both may be columns of one buffer's rows
+    if (s == 0 || (step != 0 && step != s) || (o.step != 0 && o.step != s)) return true;
+    const int64_t at = o.lo >= lo ? static_cast<int64_t>((o.lo - lo) % s)
+                                  : (s - static_cast<int64_t>((lo - o.lo) % s)) % s;
+    return at < width || at + o.width > s;
+  }
 };
 inline int row_count(int64_t rows, const char* what) {
   TORCH_CHECK_VALUE(rows < (1ll << 30), what, ": ", rows, " rows");
@@ -858,6 +870,11 @@ Tensor scaled_embedding_fwd(const Tensor& table, const Tensor& ids_in, double sc
   const Tensor ids = ids_in.contiguous();
   const int rows = row_count(ids.numel(), what);
   if (out_in.has_value()) check_rows(*out_in, rows, H, what, "out");
+  if (out_in.has_value()) {  // rows are written while others are still read
+    const Bytes b(*out_in);
+    TORCH_CHECK_VALUE(!b.overlaps(Bytes(table)) && !b.overlaps(Bytes(ids)), what,
+                      ": out overlaps the table or the ids");
+  }
   Tensor out = out_in.has_value() ? *out_in : new_empty({rows, H}, table.scalar_type(), table);
   CFB_CHECK_RC(cfb_scaled_embedding_fwd(
                    table.data_ptr(), type_code(table, "table"), table.stride(0), table.size(0),
@@ -895,6 +912,10 @@ void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids_in, Tensor& dtable
                     ": a table of ", dtable.size(0), " rows");
   const c10::cuda::CUDAGuard guard(dy.device());
   const Tensor ids = ids_in.contiguous();
+  const Bytes written(dtable);  // while others still read
+  TORCH_CHECK_VALUE(!written.overlaps(Bytes(dy)) && !written.overlaps(Bytes(ids)) &&
+                        (!id_rows.has_value() || !written.overlaps(Bytes(*id_rows))),
+                    what, ": dtable overlaps dy, the ids or id_rows");
   Tensor work;
   const int64_t bytes = cfb_scaled_embedding_bwd_workspace(dtable.size(0), rows, H);
   if (bytes > 0) work = new_empty({bytes}, at::kByte, dy);

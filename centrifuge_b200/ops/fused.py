@@ -147,9 +147,20 @@ def _vector(t: torch.Tensor, H: int, dtype: torch.dtype) -> bool:
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two contiguous tensors share bytes."""
-    lo, at = a.data_ptr(), b.data_ptr()
-    return lo < at + b.numel() * b.element_size() and at < lo + a.numel() * a.element_size()
+    """Whether two tensors, contiguous or row-major ``[rows, width]``, share bytes."""
+    def layout(t):
+        rows = t.dim() == 2 and t.shape[0] > 1 and not t.is_contiguous()
+        step = t.stride(0) * t.element_size() if rows else 0
+        width = (t.shape[1] if rows else t.numel()) * t.element_size()
+        return t.data_ptr(), t.data_ptr() + (t.shape[0] - 1 if rows else 0) * step + width, step, width
+
+    (lo, hi, step, width), (lo2, hi2, step2, width2) = layout(a), layout(b)
+    if lo >= hi or lo2 >= hi2 or lo >= hi2 or lo2 >= hi:
+        return False
+    s = max(step, step2)  # both may be columns of one buffer's rows
+    if s == 0 or step not in (0, s) or step2 not in (0, s):
+        return True
+    return (lo2 - lo) % s < width or (lo2 - lo) % s + width2 > s
 
 
 def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
@@ -157,8 +168,8 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
     """``out[r] = scale * table[ids[r]]``, rounded once.
 
     ``table [V, H]`` and ``out [ids.numel(), H]`` are bf16, fp16 or fp32 (``out`` may have another
-    type than the table, e.g. an fp32 residual stream) with unit column stride and any row stride;
-    ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
+    type than the table, e.g. an fp32 residual stream) with unit column stride and any row stride,
+    apart from each other; ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
     the status block and gives a zero row."""
     if table.is_cuda:
         return kernels().scaled_embedding_fwd(table, ids, scale, out)
@@ -173,6 +184,8 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
         _need(_rows2d(out, H) and out.shape[0] == ids.shape[0] and out.dtype in _ROW_TYPES,
               "scaled_embedding_fwd: out must be a row-major bf16, fp16 or fp32 [{}, {}]",
               ids.shape[0], H)
+        _need(not _overlap(out, table) and not _overlap(out, ids),
+              "scaled_embedding_fwd: out overlaps the table or the ids")
     return out.copy_(table[ids.long()].float() * scale)
 
 
@@ -184,7 +197,8 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
     order (same bits on every run).
 
     Row ``r`` has token ``ids[id_rows[r]]`` (``ids[r]`` without ``id_rows``).  ``dy [R, H]`` is
-    bf16, fp16 or fp32 and ``dtable [V, H]`` fp32, both with unit column stride and any row stride.
+    bf16, fp16 or fp32 and ``dtable [V, H]`` fp32, both with unit column stride and any row stride,
+    apart from each other.
     Rows of token ``padding_idx`` add nothing.  Without ``accumulate`` the gradient replaces what
     ``dtable`` held: rows of tokens that do not occur become zero.  On the GPU a token outside the
     table or a row id outside ``ids`` records an error in the status block and adds nothing."""
@@ -206,6 +220,8 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
         _need(id_rows.dtype == torch.int32 and id_rows.dim() == 1 and id_rows.is_contiguous()
               and id_rows.shape[0] == dy.shape[0],
               "scaled_embedding_bwd: id_rows must be contiguous int32 [{}]", dy.shape[0])
+    _need(not any(_overlap(dtable, t) for t in (dy, ids, id_rows) if t is not None),
+          "scaled_embedding_bwd: dtable overlaps dy, the ids or id_rows")
     tok = (ids if id_rows is None else ids[id_rows.long()]).long()
     g = dy.float() * scale
     if padding_idx is not None:

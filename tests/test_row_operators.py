@@ -175,6 +175,34 @@ def test_scaled_embedding_reports_bad_indices():
         assert not dt.any()
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_scaled_embedding_refuses_what_is_read_and_written(dev):
+    """An output over an input of the same call; columns of one buffer's rows are apart."""
+    buf = torch.zeros(8, 48, device=dev)
+    ids = torch.zeros(8, dtype=torch.long, device=dev)
+    a, b = buf[:, :16], buf[:, 16:32]
+    a.fill_(3.0)
+    for out in (a, buf[:, 8:24], buf.view(-1)[48:176].view(8, 16)):
+        with pytest.raises(ValueError, match="overlap"):
+            fused.scaled_embedding_fwd(a, ids, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            fused.scaled_embedding_bwd(a, ids, out)
+    over_ids = torch.zeros(8 * 16, device=dev).view(8, 16)
+    with pytest.raises(ValueError, match="overlap"):
+        fused.scaled_embedding_fwd(a, over_ids.view(torch.long).view(-1)[8:16], out=over_ids)
+    with pytest.raises(ValueError, match="overlap"):
+        fused.scaled_embedding_bwd(a, over_ids.view(torch.long).view(-1)[8:16], over_ids)
+    with pytest.raises(ValueError, match="overlap"):
+        fused.scaled_embedding_bwd(a, ids, over_ids,
+                                   id_rows=over_ids.view(torch.int32).view(-1)[:8])
+    fused.scaled_embedding_fwd(a, ids, 2.0, out=b)
+    assert bool((b == 6.0).all()) and not buf[:, 32:].any()
+    fused.scaled_embedding_bwd(b, ids, a, 0.5)
+    assert bool((a[0] == 27.0).all()) and bool((a[1:] == 3.0).all())
+    fused.scaled_embedding_bwd(buf[7:, 32:], ids[:1], a, accumulate=False)  # one row in the gaps
+    assert not a.any() and bool((b == 6.0).all())
+
+
 # ---------------------------------------------------------------- norms around a block
 def norms_case(dev, T, H, dtype, resid, gate, pre, pad=0, skew=0, seed=0):
     g = gen(dev, 1000 * T + H + seed)
