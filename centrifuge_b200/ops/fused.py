@@ -146,6 +146,12 @@ def _vector(t: torch.Tensor, H: int, dtype: torch.dtype) -> bool:
     return t.dim() == 1 and t.shape[0] == H and t.dtype == dtype and t.is_contiguous()
 
 
+def _need_index(index: torch.Tensor, n: int, what: str) -> None:
+    """CPU: an index outside ``[0, n)`` is an error (a negative one would count from the end)."""
+    if index.numel() and not 0 <= int(index.min()) <= int(index.max()) < n:
+        raise IndexError(f"{what} outside [0, {n})")
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors, contiguous or row-major ``[rows, width]``, share bytes."""
     def layout(t):
@@ -170,7 +176,7 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
     ``table [V, H]`` and ``out [ids.numel(), H]`` are bf16, fp16 or fp32 (``out`` may have another
     type than the table, e.g. an fp32 residual stream) with unit column stride and any row stride,
     apart from each other; ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
-    the status block and gives a zero row."""
+    the status block and gives a zero row; on the CPU it raises ``IndexError``."""
     if table.is_cuda:
         return kernels().scaled_embedding_fwd(table, ids, scale, out)
     _need(table.dim() == 2 and _rows2d(table, table.shape[1]) and table.dtype in _ROW_TYPES,
@@ -186,6 +192,7 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
               ids.shape[0], H)
         _need(not _overlap(out, table) and not _overlap(out, ids),
               "scaled_embedding_fwd: out overlaps the table or the ids")
+    _need_index(ids, table.shape[0], "scaled_embedding_fwd: an id is")
     return out.copy_(table[ids.long()].float() * scale)
 
 
@@ -201,7 +208,8 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
     apart from each other.
     Rows of token ``padding_idx`` add nothing.  Without ``accumulate`` the gradient replaces what
     ``dtable`` held: rows of tokens that do not occur become zero.  On the GPU a token outside the
-    table or a row id outside ``ids`` records an error in the status block and adds nothing."""
+    table or a row id outside ``ids`` records an error in the status block and adds nothing; on the
+    CPU it raises ``IndexError`` and ``dtable`` stays as it was."""
     if dy.is_cuda:
         kernels().scaled_embedding_bwd(dy, ids, dtable, scale, id_rows, padding_idx, accumulate)
         return dtable
@@ -222,10 +230,13 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
               "scaled_embedding_bwd: id_rows must be contiguous int32 [{}]", dy.shape[0])
     _need(not any(_overlap(dtable, t) for t in (dy, ids, id_rows) if t is not None),
           "scaled_embedding_bwd: dtable overlaps dy, the ids or id_rows")
+    if id_rows is not None:
+        _need_index(id_rows, ids.shape[0], "scaled_embedding_bwd: a row id is")
     tok = (ids if id_rows is None else ids[id_rows.long()]).long()
     g = dy.float() * scale
     if padding_idx is not None:
         g, tok = g[tok != padding_idx], tok[tok != padding_idx]
+    _need_index(tok, dtable.shape[0], "scaled_embedding_bwd: a token is")
     if not accumulate:
         dtable.zero_()
     return dtable.index_add_(0, tok, g)
@@ -291,8 +302,8 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
     ``None``.  ``dw_post``, ``dw_pre`` and, for a learned gate, ``dgate`` are fp32 ``[H]`` buffers,
     added to (written without ``accumulate``); a buffer given for two of them (one parameter in both
     places) gets the sum of both gradients, other overlaps are refused.  A token's or element's gate
-    returns its gradient for the ``R`` rows.  On the GPU a row id outside ``h`` records an error in the status block and
-    gives zero rows."""
+    returns its gradient for the ``R`` rows.  On the GPU a row id outside ``h`` records an error in
+    the status block and gives zero rows; on the CPU it raises ``IndexError``."""
     if h.is_cuda:
         return kernels().block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre, dw_post,
                                          dw_pre, gate, dgate, block_scale, resid_scale, rows,
@@ -342,6 +353,7 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
         _need(not any(_overlap(s, t) for t in params),
               "{}: dw_post, dw_pre or dgate overlaps a weight or the gate", name)
     if rows is not None:
+        _need_index(rows, T, f"{name}: a row id is")
         at = rows.long()
         h, rstd_post = h[at], rstd_post[at]
         y, rstd_pre = (y[at], rstd_pre[at]) if pre else (None, None)

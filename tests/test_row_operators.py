@@ -175,6 +175,29 @@ def test_scaled_embedding_reports_bad_indices():
         assert not dt.any()
 
 
+@pytest.mark.parametrize("bad", [-1, 8, 1 << 40])
+def test_bad_indices_raise_on_the_cpu(bad):
+    """The CPU path refuses ids and row ids outside their range; nothing counts from the end."""
+    table, dy, dt = torch.ones(8, 16), torch.ones(3, 16), torch.zeros(8, 16)
+    ids = torch.tensor([1, bad, 2])
+    with pytest.raises(IndexError):
+        fused.scaled_embedding_fwd(table, ids)
+    with pytest.raises(IndexError):
+        fused.scaled_embedding_bwd(dy, ids, dt, accumulate=False, padding_idx=1)
+    h = torch.ones(8, 16)
+    r, w = torch.ones(8), torch.ones(16)
+    if bad < 1 << 31:
+        rows = ids.int()
+        with pytest.raises(IndexError):
+            fused.scaled_embedding_bwd(dy, torch.arange(8), dt, id_rows=rows)
+        with pytest.raises(IndexError):
+            fused.block_norms_bwd(dy, dy, h, h, r, r, w, w, dt[0], dt[1], rows=rows)
+    assert not dt.any()
+    # a padding token adds nothing, wherever it lies
+    fused.scaled_embedding_bwd(dy, torch.tensor([1, 9, 2]), dt, padding_idx=9)
+    assert bool((dt[1:3] == 1.0).all()) and not dt[3:].any()
+
+
 @pytest.mark.parametrize("dev", CPU_GPU)
 def test_scaled_embedding_refuses_what_is_read_and_written(dev):
     """An output over an input of the same call; columns of one buffer's rows are apart."""
