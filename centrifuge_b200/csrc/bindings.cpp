@@ -852,6 +852,10 @@ inline int row_count(int64_t rows, const char* what) {
 inline Tensor new_empty(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
   return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
+inline int embed_width(int64_t H, const char* what) {
+  TORCH_CHECK_VALUE(H <= kEmbedMaxH, what, ": hidden size ", H, " is over ", kEmbedMaxH);
+  return static_cast<int>(H);
+}
 inline bool is_index(const Tensor& t) {
   return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt;
 }
@@ -861,7 +865,7 @@ Tensor scaled_embedding_fwd(const Tensor& table, const Tensor& ids_in, double sc
                             const c10::optional<Tensor>& out_in) {
   const char* what = "scaled_embedding_fwd";
   TORCH_CHECK_VALUE(table.dim() == 2, what, ": table must be [V, H]");
-  const int64_t H = table.size(1);
+  const int H = embed_width(table.size(1), what);
   check_rows(table, -1, H, what, "table");
   TORCH_CHECK_VALUE(is_index(ids_in), what, ": ids must be int64 or int32");
   same_device(table, ids_in, "ids");
@@ -879,7 +883,7 @@ Tensor scaled_embedding_fwd(const Tensor& table, const Tensor& ids_in, double sc
   CFB_CHECK_RC(cfb_scaled_embedding_fwd(
                    table.data_ptr(), type_code(table, "table"), table.stride(0), table.size(0),
                    ids.data_ptr(), ids.scalar_type() == at::kInt, out.data_ptr(),
-                   type_code(out, "out"), out.stride(0), rows, static_cast<int>(H),
+                   type_code(out, "out"), out.stride(0), rows, H,
                    static_cast<float>(scale), err_word(table.get_device()).data_ptr<int>(),
                    cur_stream()),
                what);
@@ -892,13 +896,13 @@ void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids_in, Tensor& dtable
                           bool accumulate) {
   const char* what = "scaled_embedding_bwd";
   TORCH_CHECK_VALUE(dy.dim() == 2, what, ": dy must be [R, H]");
-  const int64_t H64 = dy.size(1);
-  check_rows(dy, -1, H64, what, "dy");
-  check_rows(dtable, -1, H64, what, "dtable");
+  const int H = embed_width(dy.size(1), what);
+  check_rows(dy, -1, H, what, "dy");
+  check_rows(dtable, -1, H, what, "dtable");
   TORCH_CHECK_VALUE(dtable.scalar_type() == at::kFloat, what, ": dtable must be fp32");
   TORCH_CHECK_VALUE(is_index(ids_in), what, ": ids must be int64 or int32");
-  TORCH_CHECK_VALUE(!padding_idx.has_value() || *padding_idx >= 0, what,
-                    ": padding_idx is negative");
+  TORCH_CHECK_VALUE(!padding_idx.has_value() || (*padding_idx >= 0 && *padding_idx < (1ll << 31)),
+                    what, ": padding_idx is negative or over 31 bits");
   if (id_rows.has_value())
     check_vector(*id_rows, dy.size(0), at::kInt, what, "id_rows");
   else
@@ -907,7 +911,7 @@ void scaled_embedding_bwd(const Tensor& dy, const Tensor& ids_in, Tensor& dtable
   same_device(dy, ids_in, "ids");
   same_device(dy, id_rows, "id_rows");
   same_device(dy, dtable, "dtable");
-  const int rows = row_count(dy.size(0), what), H = static_cast<int>(H64);
+  const int rows = row_count(dy.size(0), what);
   TORCH_CHECK_VALUE(dtable.size(0) <= (1ll << 30) && (dtable.size(0) > 0 || rows == 0), what,
                     ": a table of ", dtable.size(0), " rows");
   const c10::cuda::CUDAGuard guard(dy.device());

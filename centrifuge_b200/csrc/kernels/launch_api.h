@@ -227,14 +227,15 @@ int cfb_symm_pull_reduce(const float* mc_base, const float* const* peer_base_dev
 int cfb_zero_unless_error(float* buf, long long n, const int* err, cudaStream_t st);
 
 // ---- row operators around the blocks (row counts below 2^30; ld: elements between rows)
-// out[r] = scale * table[ids[r]]; ids int64, or int32 with ids32.  An id outside [0, V) records
+constexpr int kEmbedMaxH = 65535 * 128;  // slabs of columns are a grid's second dimension
+// H up to kEmbedMaxH.  out[r] = scale * table[ids[r]]; ids int64, or int32 with ids32.  An id outside [0, V) records
 // kErrBounds and gives a zero row.
 int cfb_scaled_embedding_fwd(const void* table, int type, long long ld, long long V,
                              const void* ids, int ids32, void* out, int out_type,
                              long long ld_out, int rows, int H, float scale, int* err,
                              cudaStream_t st);
 // dtable[v] = (add ? dtable[v] : 0) + scale * sum of dy[r] over the rows r with ids[id_rows[r]] = v
-// (ids[r] without id_rows), v != pad (pad < 0: none).  `work`: scratch of
+// (ids[r] without id_rows), v != pad (pad < 0: none, pad < 2^31).  `work`: scratch of
 // cfb_scaled_embedding_bwd_workspace bytes, 32-byte aligned.
 long long cfb_scaled_embedding_bwd_workspace(long long V, int rows, int H);
 int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void* ids, int ids32,

@@ -627,6 +627,7 @@ int cfb_scaled_embedding_fwd(const void* table, int type, long long ld, long lon
                              const void* ids, int ids32, void* out, int out_type,
                              long long ld_out, int rows, int H, float scale, int* err,
                              cudaStream_t st) {
+  if (H > kEmbedMaxH) return -11;
   if (rows == 0 || H == 0) return 0;
   const bool wide = H % 8 == 0 && rows_of_8(table, ld, type) && rows_of_8(out, ld_out, out_type);
   return with_type(type, [&](auto ti) {
@@ -667,7 +668,8 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
                              long long n_ids, const int* id_rows, long long pad, float* dtable,
                              long long ld_t, long long V, int rows, int H, float scale, int add,
                              void* work, int* err, cudaStream_t st) {
-  if (V < 0 || V > (1ll << 30) || (V == 0 && rows > 0)) return -11;
+  if (V < 0 || V > (1ll << 30) || (V == 0 && rows > 0) || H > kEmbedMaxH || pad > INT32_MAX)
+    return -11;
   if (H == 0 || V == 0) return 0;
   const bool wide = H % 8 == 0 && rows_of_8(dy, ld, type) && rows_of_8(dtable, ld_t, kF32);
   if (rows == 0) {
@@ -710,7 +712,7 @@ int cfb_scaled_embedding_bwd(const void* dy, int type, long long ld, const void*
   }
   sort_tokens_kernel<<<1u << plan.shift, 1024, smem, st>>>(
       ids, ids32, static_cast<unsigned>(n_ids < INT32_MAX ? n_ids : INT32_MAX), id_rows, rows,
-      static_cast<int>(V), pad <= INT32_MAX ? static_cast<int>(pad) : -1, plan.shift, plan.span,
+      static_cast<int>(V), static_cast<int>(pad), plan.shift, plan.span,
       order, stok, n_valid, absent, err);
   if (const int rc = launch_status()) return rc;
   const int per = chunk_rows(rows);

@@ -128,6 +128,7 @@ def embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tensor,
     return dtable
 
 
+_EMBED_MAX_H = 65535 * 128
 _ROW_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
@@ -175,12 +176,14 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
 
     ``table [V, H]`` and ``out [ids.numel(), H]`` are bf16, fp16 or fp32 (``out`` may have another
     type than the table, e.g. an fp32 residual stream) with unit column stride and any row stride,
-    apart from each other; ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
+    apart from each other, ``H`` up to 8388480; ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
     the status block and gives a zero row; on the CPU it raises ``IndexError``."""
     if table.is_cuda:
         return kernels().scaled_embedding_fwd(table, ids, scale, out)
     _need(table.dim() == 2 and _rows2d(table, table.shape[1]) and table.dtype in _ROW_TYPES,
           "scaled_embedding_fwd: table must be a row-major bf16, fp16 or fp32 [V, H]")
+    _need(table.shape[1] <= _EMBED_MAX_H, "scaled_embedding_fwd: hidden size {} is over {}",
+          table.shape[1], _EMBED_MAX_H)
     _need(ids.dtype in (torch.int64, torch.int32), "scaled_embedding_fwd: ids must be int64 or int32")
     ids = ids.reshape(-1)
     H = table.shape[1]
@@ -206,7 +209,7 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
     Row ``r`` has token ``ids[id_rows[r]]`` (``ids[r]`` without ``id_rows``).  ``dy [R, H]`` is
     bf16, fp16 or fp32 and ``dtable [V, H]`` fp32, both with unit column stride and any row stride,
     apart from each other.
-    Rows of token ``padding_idx`` add nothing.  Without ``accumulate`` the gradient replaces what
+    Rows of token ``padding_idx`` (below 2^31) add nothing.  Without ``accumulate`` the gradient replaces what
     ``dtable`` held: rows of tokens that do not occur become zero.  On the GPU a token outside the
     table or a row id outside ``ids`` records an error in the status block and adds nothing; on the
     CPU it raises ``IndexError`` and ``dtable`` stays as it was."""
@@ -219,7 +222,10 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
     _need(_rows2d(dtable, dy.shape[1]) and dtable.dtype == torch.float32,
           "scaled_embedding_bwd: dtable must be a row-major fp32 [V, {}]", dy.shape[1])
     _need(dtable.shape[0] > 0 or dy.shape[0] == 0, "scaled_embedding_bwd: a table of 0 rows")
-    _need(padding_idx is None or padding_idx >= 0, "scaled_embedding_bwd: padding_idx is negative")
+    _need(dy.shape[1] <= _EMBED_MAX_H, "scaled_embedding_bwd: hidden size {} is over {}",
+          dy.shape[1], _EMBED_MAX_H)
+    _need(padding_idx is None or 0 <= padding_idx < 1 << 31,
+          "scaled_embedding_bwd: padding_idx is negative or over 31 bits")
     ids = ids.reshape(-1)
     if id_rows is None:
         _need(ids.shape[0] == dy.shape[0], "scaled_embedding_bwd: {} ids for {} rows",

@@ -175,6 +175,33 @@ def test_scaled_embedding_reports_bad_indices():
         assert not dt.any()
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_scaled_embedding_refuses_the_too_large(dev):
+    """Widths whose slabs no grid has, before anything of the table is written, and padding tokens
+    that the sort cannot compare."""
+    ids = torch.zeros(300, dtype=torch.long, device=dev)
+    dt = torch.ones(1, 65535 * 128 + 1, device=dev)
+    dy = torch.ones(1, dt.shape[1], dtype=BF, device=dev)
+    for call in (lambda: fused.scaled_embedding_bwd(dy, ids[:1], dt),
+                 lambda: fused.scaled_embedding_fwd(dy, ids)):
+        with pytest.raises(ValueError, match="over 8388480"):
+            call()
+    assert bool((dt == 1.0).all())
+    if dev == "cuda":
+        from centrifuge_b200.ops._ext import kernels
+        kernels().status_block(0).zero_()
+    for rows in (3, 300):  # the largest padding token is no error, whatever the number of rows
+        small = torch.zeros(4, 8, device=dev)
+        pads = torch.full((rows,), (1 << 31) - 1, device=dev)
+        one = torch.ones(rows, 8, device=dev)
+        fused.scaled_embedding_bwd(one, pads, small, padding_idx=(1 << 31) - 1)
+        assert not small.any()
+        with pytest.raises(ValueError, match="over 31 bits"):
+            fused.scaled_embedding_bwd(one, pads, small, padding_idx=1 << 31)
+    if dev == "cuda":
+        assert int(kernels().status_block(0)[0]) == 0
+
+
 @pytest.mark.parametrize("bad", [-1, 8, 1 << 40])
 def test_bad_indices_raise_on_the_cpu(bad):
     """The CPU path refuses ids and row ids outside their range; nothing counts from the end."""
