@@ -1295,6 +1295,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ex2_poly", &ex2_poly);
   m.def("embedding_bwd", &embedding_bwd, py::arg("dy"), py::arg("ids"), py::arg("id_rows"),
         py::arg("dtable"), py::arg("deterministic") = true);
+  m.def("row_launches", [] { return cfb_row_launches().load(); });
   m.def("scaled_embedding_fwd", &scaled_embedding_fwd);
   m.def("scaled_embedding_bwd", &scaled_embedding_bwd);
   m.def("block_norms_fwd", &block_norms_fwd);

@@ -3,6 +3,8 @@
 // stream.  Every launcher returns 0 on success and a negative code on a bad argument or a
 // launch failure.
 #pragma once
+#include <atomic>
+
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -225,6 +227,12 @@ int cfb_symm_pull_reduce(const float* mc_base, const float* const* peer_base_dev
                          cudaStream_t st);
 // buf[0, n) = 0 unless err[0] != 0 (buf 16-byte aligned)
 int cfb_zero_unless_error(float* buf, long long n, const int* err, cudaStream_t st);
+
+// Launches of the row operators by this process: how many a call makes depends on its sizes.
+inline std::atomic<long long>& cfb_row_launches() {
+  static std::atomic<long long> launches{0};
+  return launches;
+}
 
 // ---- row operators around the blocks (row counts below 2^30; ld: elements between rows)
 constexpr int kEmbedMaxH = 65535 * 128;  // slabs of columns are a grid's second dimension

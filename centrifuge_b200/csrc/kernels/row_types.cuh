@@ -333,7 +333,11 @@ __device__ __forceinline__ void after_previous() {
 __device__ __forceinline__ void let_next_start() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
-inline int launch_status() { return cudaGetLastError() == cudaSuccess ? 0 : -3; }
+inline int launch_status() {
+  if (cudaGetLastError() != cudaSuccess) return -3;
+  ++cfb_row_launches();
+  return 0;
+}
 template <typename... P, typename... A>
 int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t st,
                   A&&... args) {
@@ -348,9 +352,10 @@ int launch_behind(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStr
   c.attrs = &attr;
   c.numAttrs = 1;
   if (cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) != cudaSuccess) {
-    launch_status();  // the error is this launch's, not the next one's
+    cudaGetLastError();  // the error is this launch's, not the next one's
     return -3;
   }
+  ++cfb_row_launches();
   return 0;
 }
 

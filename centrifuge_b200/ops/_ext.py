@@ -12,20 +12,29 @@ _mod = None
 _err = None
 _proxy = None
 
-# Kernels launched by one call of each binding (for the launch counter).
+# Kernels launched by one call of each binding (for the launch counter).  The row operators' launches
+# depend on their sizes and are counted by the module itself.
 _LAUNCHES_PER_CALL = {"rmsnorm_bwd": 2, "attn_bwd": 2, "attn_bwd_mma": 3, "gemm_error_word": 0,
                       "status_block": 0, "set_wait_limits": 0, "gemm_plan": 0,
-                      "scaled_embedding_bwd": 3, "block_norms_bwd": 2, "grad_list_clip": 2}
+                      "row_launches": 0, "scaled_embedding_fwd": 0, "scaled_embedding_bwd": 0,
+                      "block_norms_fwd": 0, "block_norms_bwd": 0, "grad_list_sumsq": 0,
+                      "grad_list_clip": 0}
 
 
 class LaunchCounter:
     """Counts sm_100a kernel launches issued through the bindings."""
 
     def __init__(self):
-        self.count = 0
+        self.calls = 0  # launches told by _LAUNCHES_PER_CALL
+        self._counted = 0  # launches the module had counted at the last reset
+
+    @property
+    def count(self) -> int:
+        return self.calls + (_mod.row_launches() if _mod is not None else 0) - self._counted
 
     def reset(self) -> int:
-        n, self.count = self.count, 0
+        n = self.count
+        self.calls, self._counted = 0, self._counted + n - self.calls
         return n
 
 
@@ -43,7 +52,7 @@ class _Counted:
         n = _LAUNCHES_PER_CALL.get(name, 1)
 
         def call(*args, **kwargs):
-            counter.count += n
+            counter.calls += n
             return fn(*args, **kwargs)
 
         setattr(self, name, call)

@@ -176,8 +176,9 @@ def scaled_embedding_fwd(table: torch.Tensor, ids: torch.Tensor, scale: float = 
 
     ``table [V, H]`` and ``out [ids.numel(), H]`` are bf16, fp16 or fp32 (``out`` may have another
     type than the table, e.g. an fp32 residual stream) with unit column stride and any row stride,
-    apart from each other, ``H`` up to 8388480; ``ids`` int64 or int32, any shape.  On the GPU an id outside the vocabulary records an error in
-    the status block and gives a zero row; on the CPU it raises ``IndexError``."""
+    apart from each other, ``H`` up to 8388480; ``ids`` int64 or int32, any shape.  On the GPU an id
+    outside the vocabulary records an error in the status block and gives a zero row; on the CPU it
+    raises ``IndexError``."""
     if table.is_cuda:
         return kernels().scaled_embedding_fwd(table, ids, scale, out)
     _need(table.dim() == 2 and _rows2d(table, table.shape[1]) and table.dtype in _ROW_TYPES,
@@ -208,11 +209,12 @@ def scaled_embedding_bwd(dy: torch.Tensor, ids: torch.Tensor, dtable: torch.Tens
 
     Row ``r`` has token ``ids[id_rows[r]]`` (``ids[r]`` without ``id_rows``).  ``dy [R, H]`` is
     bf16, fp16 or fp32 and ``dtable [V, H]`` fp32, both with unit column stride and any row stride,
-    apart from each other.
-    Rows of token ``padding_idx`` (below 2^31) add nothing.  Without ``accumulate`` the gradient replaces what
-    ``dtable`` held: rows of tokens that do not occur become zero.  On the GPU a token outside the
-    table or a row id outside ``ids`` records an error in the status block and adds nothing; on the
-    CPU it raises ``IndexError`` and ``dtable`` stays as it was."""
+    apart from each other, ``H`` up to 8388480.  Rows of token ``padding_idx`` (below 2^31) add
+    nothing.  Without ``accumulate`` the gradient replaces what ``dtable`` held: rows of tokens that
+    do not occur become zero.  Where it is added, the GPU takes subnormal numbers (below 1.2e-38) as
+    zeros.  On the GPU a token outside the table or a row id outside ``ids`` records an error in the
+    status block and adds nothing; on the CPU it raises ``IndexError`` and ``dtable`` stays as it
+    was."""
     if dy.is_cuda:
         kernels().scaled_embedding_bwd(dy, ids, dtable, scale, id_rows, padding_idx, accumulate)
         return dtable

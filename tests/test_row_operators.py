@@ -676,6 +676,56 @@ def test_grad_list_clip_checks_norm_and_sums(dev):
     assert float(fused.grad_list_clip_([g], 8.0, norm=norm)) == 4.0 and float(norm) == 4.0
 
 
+# ---------------------------------------------------------------- launch counter
+def test_launch_counter_adds_what_the_module_counts(monkeypatch):
+    from centrifuge_b200.ops import _ext
+
+    class Module:
+        made = 5
+
+        def row_launches(self):
+            return self.made
+
+    mod = Module()
+    monkeypatch.setattr(_ext, "_mod", mod)
+    counter = _ext.LaunchCounter()
+    assert counter.reset() == 5 and counter.count == 0
+    mod.made, counter.calls = 8, 2
+    assert counter.count == 5 and counter.reset() == 5 and counter.reset() == 0
+
+
+@pytest.mark.gpu
+def test_launch_counter_of_the_row_operators():
+    """As many as a call makes: they depend on rows, tensors and chunks."""
+    from centrifuge_b200.ops._ext import counter
+    g = gen("cuda", 3)
+
+    def made(f):
+        counter.reset()
+        f()
+        return counter.reset()
+
+    ids = torch.randint(0, 40, (300,), generator=g, device="cuda")
+    dy, dt = rand(g, 300, 64), torch.zeros(40, 64, device="cuda")
+    assert made(lambda: fused.scaled_embedding_fwd(dt, ids)) == 1
+    for rows, accumulate, n in ((0, True, 0), (0, False, 1), (1, True, 1), (256, False, 1),
+                                (257, True, 3), (300, False, 3)):
+        assert made(lambda: fused.scaled_embedding_bwd(dy[:rows], ids[:rows], dt,
+                                                       accumulate=accumulate)) == n, rows
+    h, w, acc = rand(g, 30, 64), torch.ones(64, device="cuda"), torch.zeros(2, 64, device="cuda")
+    res = []
+    assert made(lambda: res.extend(fused.block_norms_fwd(h, h, w, w, EPS))) == 1
+    y, _, rp, rq = res
+    for a, b, n in ((0, 1, 2), (1, 1, 3)):
+        assert made(lambda: fused.block_norms_bwd(h, h, h, y, rp, rq, w, w, acc[a], acc[b])) == n
+    part = rand(g, 40_000_000, scale=1e-3)
+    sums = torch.ones(3, device="cuda")
+    for grads, kw, n in (([h], {}, 2), ([h], dict(extra_sumsq=sums), 1), ([], dict(extra_sumsq=sums), 1),
+                         ([part], {}, 3), (list(part[:1500].split(1)), {}, 5)):
+        assert made(lambda: fused.grad_list_clip_(grads, 1.0, **kw)) == n, len(grads)
+    assert made(lambda: fused.grad_list_sumsq([h, part])) == 1
+
+
 # ---------------------------------------------------------------- refusals
 @pytest.mark.parametrize("dev", CPU_GPU)
 def test_refusals(dev):
