@@ -175,6 +175,114 @@ def test_scaled_embedding_reports_bad_indices():
         assert not dt.any()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("ids32", [False, True])
+@pytest.mark.parametrize("V,T,R", [(500, 300, 257), (500, 3000, 2900), (200000, 3000, 2900),
+                                   (500, 50000, 40000)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_table_gradient_of_many_rows_reports_bad_indices(ids32, V, T, R, accumulate):
+    """Tokens and row ids out of range among rows that are sorted: recorded, and nothing else moves."""
+    from centrifuge_b200.ops._ext import kernels
+    status = kernels().status_block(0)
+    g = gen("cuda", V + R)
+    good_ids = torch.randint(0, V, (T,), generator=g, device="cuda")
+    good_rows = torch.randperm(T, generator=g, device="cuda")[:R]
+    bad_tokens = [-1, V, -V, (1 << 31) - 1, -(1 << 31)] + ([] if ids32 else [1 << 31, 1 << 32, 1 << 40])
+    bad_rows = [-1, T, (1 << 31) - 1, -(1 << 31)]
+    dy = rand(g, R, 24, dtype=BF)
+    before = rand(g, V, 24)
+
+    def check(ids, rows, keep, code):
+        status.zero_()
+        got = before.clone()
+        fused.scaled_embedding_bwd(dy, ids.int() if ids32 else ids, got, 0.5, id_rows=rows.int(),
+                                   accumulate=accumulate)
+        assert int(status[0]) == code
+        status.zero_()
+        want, tol = grad_of_table(dy[keep], good_ids[good_rows[keep]], V, 0.5)
+        if accumulate:
+            want = want + before.double()
+            tol = tol + 2 * U * want.abs()
+        close(got, want, tol, "dtable")
+
+    check(good_ids, good_rows, torch.ones(R, dtype=torch.bool, device="cuda"), 0)
+    some = torch.arange(0, R, 7, device="cuda")  # the rows that are made bad
+    some = some[: len(some) // len(bad_tokens) * len(bad_tokens)]
+    ids = good_ids.clone()
+    ids[good_rows[some]] = torch.tensor(bad_tokens, device="cuda").repeat(len(some) // len(bad_tokens))
+    keep = torch.ones(R, dtype=torch.bool, device="cuda")
+    keep[some] = False
+    check(ids, good_rows, keep, 128)
+    rows = good_rows.clone()
+    rows[some] = torch.tensor(bad_rows, device="cuda").repeat(len(some))[:len(some)]
+    check(good_ids, rows, keep, 128)
+    one = good_ids.clone()  # a single one, in the last row
+    one[good_rows[-1]] = V
+    keep[:] = True
+    keep[-1] = False
+    check(one, good_rows, keep, 128)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,H,R,share", [(32000, 64, 40000, 0.3), (300, 65, 40000, 0.5),
+                                         (140000, 32, 66000, 0.9), (32000, 40, 20000, 0.95)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_table_gradient_of_a_large_batch(V, H, R, share, accumulate):
+    """Text and one frequent token, over and under the rows whose keys the sort holds."""
+    g = gen("cuda", R + H)
+    u = torch.rand(R, generator=g, device="cuda", dtype=torch.float64)
+    ids = (torch.exp(u * math.log(V)) - 1).long().clamp(0, V - 1)
+    ids[torch.rand(R, generator=g, device="cuda") < share] = V // 2
+    dy = rand(g, R, H, dtype=BF)
+    before = rand(g, V, H)
+    got = before.clone()
+    fused.scaled_embedding_bwd(dy, ids, got, 1.5, accumulate=accumulate)
+    want, tol = grad_of_table(dy, ids, V, 1.5)
+    if accumulate:
+        want = want + before.double()
+        tol = tol + 2 * U * want.abs()
+    close(got, want, tol, "dtable")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("run", [16, 17, 143, 144, 145, 160, 4095, 4096, 4097, 4112, 4113, 4128, 8192,
+                                 8208, 8209, 9000])
+@pytest.mark.parametrize("H", [16, 9])
+def test_table_gradient_of_one_run(run, H):
+    """The first token in `run` of 9000 rows: chunks of 16 rows, the join's share of one warp (eight
+    more chunks) and its steps of 256 chunks begin and end there."""
+    g = gen("cuda", run)
+    ids = torch.arange(9000, device="cuda") % 77 + 1
+    ids[:run] = 0
+    ids = ids[torch.randperm(9000, generator=g, device="cuda")]
+    dy = rand(g, 9000, H, dtype=HF)
+    got = torch.full((100, H), 5.0, device="cuda")
+    fused.scaled_embedding_bwd(dy, ids, got, accumulate=False)
+    close(got, *grad_of_table(dy, ids, 100, 1.0), "dtable")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,H", [(6000, 513), (6000, 512), (200, 513), (200, 512), (6000, 3)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_table_gradient_off_the_vector_borders(R, H, dtype, accumulate):
+    """Rows that begin anywhere, by value; nothing beside the table's columns is written."""
+    g = gen("cuda", R + H)
+    ids = torch.randint(0, 290, (R,), generator=g, device="cuda")
+    ids[::5] = 7
+    dy = rand(g, R, H, dtype=dtype, skew=3)
+    base = rand(g, 300, H + 4)
+    keep = base.clone()
+    got = base[:, 1:H + 1]
+    fused.scaled_embedding_bwd(dy, ids, got, 0.5, accumulate=accumulate)
+    want, tol = grad_of_table(dy, ids, 300, 0.5)
+    if accumulate:
+        want = want + keep[:, 1:H + 1].double()
+        tol = tol + 2 * U * want.abs()
+    close(got, want, tol, "dtable")
+    assert torch.equal(base[:, 0], keep[:, 0]) and torch.equal(base[:, H + 1:], keep[:, H + 1:])
+
+
 @pytest.mark.parametrize("dev", CPU_GPU)
 def test_scaled_embedding_refuses_the_too_large(dev):
     """Widths whose slabs no grid has, before anything of the table is written, and padding tokens
@@ -404,6 +512,17 @@ def test_block_norms_bwd(dev, T, H, dtype, resid, gate, pre, kept, accumulate, w
 
 @pytest.mark.parametrize("dev", CPU_GPU)
 @pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
+@pytest.mark.parametrize("T,H,dtype,resid,pre", [
+    (61, 2400, BF, BF, True), (43, 3400, HF, HF, True), (29, 4800, BF, F32, True),
+    (75, 1536, BF, F32, False), (31, 2401, BF, BF, False), (90, 96, HF, HF, False)])
+def test_block_norms_at_widths_of_other_teams(dev, T, H, dtype, resid, gate, pre):
+    """Every gate at the widths between the powers of two, and without the norm before a block."""
+    test_block_norms_fwd(dev, T, H, dtype, resid, gate, pre, 0, 0)
+    test_block_norms_bwd(dev, T, H, dtype, resid, gate, pre, True, True, True, 0, 0)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
 def test_block_norms_gradient_against_differences(dev, gate):
     """Central differences of the 64-bit formula along random directions."""
     g, c = norms_case(dev, 6, 40, F32, F32, gate, True, seed=3)
@@ -524,6 +643,40 @@ def test_block_norms_bwd_reports_bad_rows(gate, pre):
         status.zero_()
     for p, q in zip(*res):
         assert torch.equal(p, q)  # the bad rows add nothing and come back as zeros
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,H,dtype,resid", [(1000, 513, BF, BF), (1000, 250, HF, F32),
+                                             (700, 2048, F32, F32), (400, 8200, BF, BF),
+                                             (400, 8192, BF, F32), (300, 2050, BF, BF),
+                                             (900, 256, BF, BF), (300, 4096, BF, F32)])
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "element"])
+@pytest.mark.parametrize("pre", [True, False])
+def test_block_norms_bwd_reports_bad_rows_at_other_widths(T, H, dtype, resid, gate, pre):
+    """The kernels beside the ring, and its other teams: a row id out of range is recorded, gives zero
+    rows and adds nothing."""
+    from centrifuge_b200.ops._ext import kernels
+    status = kernels().status_block(0)
+    status.zero_()
+    g, c = norms_case("cuda", T, H, dtype, resid, gate, pre)
+    y, _, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS, c["gate"])
+    rows = torch.arange(T, dtype=torch.int32, device="cuda")
+    good = rows % 3 != 0
+    out = torch.where(rows % 2 == 0, -1 - rows, T + rows)
+    bad = torch.where(good, rows, torch.where(rows % 9 == 0, (1 << 31) - 1 - rows, out))
+    dy, dn = rand(g, T, H, dtype=resid), rand(g, T, H, dtype=dtype)
+    res = []
+    for ids, w in ((bad, good.new_ones(T, 1)), (rows, good.unsqueeze(1))):
+        acc = torch.zeros(3, H, device="cuda")
+        dx, dh, dg = fused.block_norms_bwd(
+            dy * w, dn * w if pre else None, c["h"], y if pre else None, rp, rq, c["w_post"],
+            c["w_pre"], acc[0], acc[1] if pre else None, gate=c["gate"],
+            dgate=acc[2] if gate == "channel" else None, rows=ids)
+        res.append((dx, dh, acc, *([] if dg is None else [dg])))
+        assert int(status[0]) == (128 if ids is bad else 0)
+        status.zero_()
+    for p, q in zip(*res):
+        assert bool(p.any()) and torch.equal(p, q)
 
 
 # ---------------------------------------------------------------- gradient lists
