@@ -1034,7 +1034,12 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
 #define CFB_BWD(NW, NV) return launch_bwd<WideCols, TH, TX, NW, NV>(b, st)
 #define CFB_RING(NW, NV) blocks = launch_ring<TH, TX, NW, NV>(b, st)
       if (W == 8) {
-        // A ring of two rows always fits up to 1024 columns, and up to 4096 of two bytes.
+        // A ring of two rows always fits up to 1024 columns, and up to 4096 of two bytes.  Sixteen
+        // columns a thread, as few warps as that takes: 8192 x 2048 46.5 us, 51.3 with eight columns
+        // in eight warps, 108 with 32 in two; x 2304 59.6 with five warps, 70.4 with eight; x 512 and
+        // x 1024, eight columns, 51.2 and 49.0 (of 32768 and 16384 rows), 60.6 and 60.4 with sixteen.
+        // With an fp32 stream a ring for two blocks an SM ends at 3400 columns, and over 2560 a row
+        // takes 16 warps: x 4096 113 us, 149 with eight (but x 3400 109 for 93, x 2600 101 for 84).
         int blocks = 0;
         if (H <= 256) CFB_RING(1, 1);
         else if (H <= 512) CFB_RING(2, 1);
@@ -1045,7 +1050,6 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
             else if (H <= 2560) CFB_RING(5, 2);
             else if (H <= 4096) {
               if constexpr (sizeof(TX) == 4) CFB_RING(16, 1);
-              else if (H <= 3584) CFB_RING(7, 2);
               else CFB_RING(8, 2);
             } else if (H <= 8192) CFB_RING(16, 2);
           }
