@@ -828,11 +828,18 @@ inline void check_vector(const Tensor& t, int64_t n, at::ScalarType type, const 
 struct Bytes {
   uintptr_t lo, hi;
   int64_t step, width;  // bytes; step 0: one row
-  explicit Bytes(const Tensor& t) : lo(reinterpret_cast<uintptr_t>(t.data_ptr())) {
-    const bool rows = t.dim() == 2 && t.size(0) > 1 && !t.is_contiguous();
-    step = rows ? t.stride(0) * t.element_size() : 0;
-    width = rows ? t.size(1) * t.element_size() : t.nbytes();
-    hi = lo + (rows ? (t.size(0) - 1) * step + width : width);
+  explicit Bytes(const Tensor& t) : lo(reinterpret_cast<uintptr_t>(t.const_data_ptr())) {
+    const int64_t size = static_cast<int64_t>(t.itemsize());
+    const at::IntArrayRef n = t.sizes();
+    if (n.size() == 2 && n[0] > 1 && !t.is_contiguous()) {
+      step = t.strides()[0] * size;
+      width = n[1] * size;
+      hi = lo + (n[0] - 1) * step + width;
+    } else {
+      step = 0;
+      width = t.numel() * size;
+      hi = lo + width;
+    }
   }
   bool overlaps(const Bytes& o) const {
     if (lo >= hi || o.lo >= o.hi || lo >= o.hi || o.lo >= hi) return false;

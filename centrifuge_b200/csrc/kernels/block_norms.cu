@@ -42,8 +42,8 @@ struct NormRows {
 //
 // Short blocks, dealt by the hardware, with rows in registers; each first asks the L2 cache for the
 // rows of the block that will follow it on its SM, so that the loads of a block that waits for its
-// sums are already under way.  Measured for 16384 x 2048 bf16 with a channel's gate (floor 41.1 us):
-// 44.1 us (46.4 without the request ahead, 86 with one row in registers for two warps, 54 with
+// sums are already under way.  The kernel alone, 16384 x 2048 bf16 with a channel's gate (floor 41.1
+// us): 44.1 us (46.4 without the request ahead, 86 with one row in registers for two warps, 54 with
 // R = 4 rows and eight columns a thread); 8192 x 4096: 46.1 us (51.5); 4096 x 8192: 50.9 us (61.1).
 template <typename TH, typename TX, int NW, int NV, int R>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) block_norms_fwd_kernel(
@@ -455,9 +455,9 @@ __global__ void __launch_bounds__(NW < 8 ? 256 : NW * 32, C::P == 1 ? (NW <= 8 ?
 // memory in fp32, in two planes of the four low and the four high columns of each group of eight,
 // so that a thread's two 16-byte reads have no bank conflicts.
 //
-// Bound by memory over many rows: 8192 kept x 2048 bf16 with a channel's gate take 41 us (66 with
-// loads into registers), 8192 more 31 us more, which is the copy rate; the rest is the first rows'
-// latency and the column sums' write.
+// Bound by memory over many rows: 8192 kept x 2048 bf16 with a channel's gate take 41 us in the kernel
+// alone (66 with loads into registers), 8192 more 31 us more, which is the copy rate; the rest is the
+// first rows' latency and the column sums' write.
 template <typename TH, typename TX, int NW, int NV>
 __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 ? 16 / NW : 1)
     block_norms_bwd_ring_kernel(NormRows a, const TX* __restrict__ dy, long long ld_dy,
@@ -1038,8 +1038,9 @@ int cfb_block_norms_bwd(const CfbBlockNorms* p, const void* dy, long long ld_dy,
         // columns a thread, as few warps as that takes: 8192 x 2048 46.5 us, 51.3 with eight columns
         // in eight warps, 108 with 32 in two; x 2304 59.6 with five warps, 70.4 with eight; x 512 and
         // x 1024, eight columns, 51.2 and 49.0 (of 32768 and 16384 rows), 60.6 and 60.4 with sixteen.
-        // With an fp32 stream a ring for two blocks an SM ends at 3400 columns, and over 2560 a row
-        // takes 16 warps: x 4096 113 us, 149 with eight (but x 3400 109 for 93, x 2600 101 for 84).
+        // With an fp32 stream the ring of two blocks of eight warps ends at 3520 columns, and over
+        // 2560 a row takes 16 warps: x 4096 113 us, 149 with eight (x 3400 109 for 93, x 2600 101
+        // for 84).
         int blocks = 0;
         if (H <= 256) CFB_RING(1, 1);
         else if (H <= 512) CFB_RING(2, 1);

@@ -7,12 +7,14 @@
 // mixed types.  The whole list travels in the kernel's parameters (no table in device memory to
 // fill, so a captured graph holds all it needs), every tensor is cut into chunks of kListChunk
 // elements, and the chunks of all tensors are dealt to the blocks: two or three launches for up to
-// 1024 tensors, whatever their sizes.  Bound by memory: one read for the norm, and, where something is written, one
-// read and one write; the second pass takes the chunks in reverse, so that what the first read last
-// still lies in the L2 cache.
+// 1024 tensors, whatever their sizes.  Bound by memory: one read for the norm, and, where something
+// is written, one read and one write; the second pass takes the chunks in reverse, so that what the
+// first read last still lies in the L2 cache.
 //
-// Squares are summed in fp32 within a chunk's share of a thread (128 values) and in fp64 beyond it;
-// each block writes one partial sum, and partial sums are joined in a fixed order.
+// Squares are summed in fp32 within a chunk's share of a thread (128 values), and a block's shares in
+// fp64.  Each block writes its sum rounded to fp32, which is what ranks exchange (the rounding, 2^-25
+// of the norm at most, is below that of the norm itself); these are joined in fp64, in a fixed order.
+// So a sum of squares above 3.4e38 may be infinite, and one below 1.2e-38 loses bits.
 #include "row_types.cuh"
 
 namespace cfb {

@@ -33,17 +33,26 @@ namespace cfb {
 
 constexpr int kMaxSpan = 1024;  // tokens of one block of the sort
 constexpr int kKeyRows = 32768; // rows whose keys a block of the sort holds in shared memory
-constexpr int kClear = 4;       // table rows that one block clears (8: 63 us a pass below, 4: 61)
+// Table rows that one block clears: the gradient measured above took 63.5 us with 8 and 61 with 4,
+// before the steps that made it 55.
+constexpr int kClear = 4;
 // Up to here one launch does it all (a row id fits 8 bits).  256 rows x 1024 of 3000 tokens: 8 us for
 // 12 sorted, x 4096 and most of one token 20 for 20.
 constexpr int kFewRows = 256;
-constexpr int kWarpRun = 24;    // rows of a token that one warp sums there by itself
+// Rows of a token that one warp sums there by itself; of more the block's four warps have a quarter
+// each.  128 rows of 3000 tokens, us for none / 24 / 64 / any by itself: x 256 text 5.4 / 3.3 / 3.3 /
+// 3.3, nine tenths one token 4.7 / 4.5 / 4.5 / 8.3; 256 rows x 1024, a fifth one token 8.3 (none), 6.2,
+// 6.9, 6.9; x 4096, nine tenths 15.7, 14.2, 14.1, 22.3 (128 rows).
+constexpr int kWarpRun = 24;
 
 constexpr int kAhead = 128;     // blocks of the gradient that request rows during the sort
 constexpr int kAheadBytes = 32 << 20;  // and what they request: the rate of the memory times the sort
 
 // Sorted positions of one warp of the gradient: few where few rows would leave SMs idle, more where
-// there are enough, since every chunk border costs a partial sum.
+// there are enough, since every chunk border costs a partial sum.  us a pass with 8 / 16 / 32: 1000
+// rows x 4096 added to 32000 tokens 16.7 / 22.8, 2000 x 1024 15.8 / 21.8; replacing, x 2048 of 32000
+// tokens of text, 4000 rows 49.4 / 48.3 / 49.4, 8192 rows 55.9 / 52.0 / 52.3 (x 512: 21.8 / 21.2 /
+// 22.7), 16384 rows 73.5 / 65.5 / 63.8, 32768 rows 109.5 / 92.3 / 87.5.
 inline int chunk_rows(int rows) { return rows >= 32768 ? 32 : rows >= 2048 ? 16 : 8; }
 
 template <typename TI, typename TO, int W>
@@ -105,7 +114,8 @@ __device__ __forceinline__ void clear_row(float* t, int H) {
 // Block b of 2^shift places the rows of the tokens t 2^shift + b at their sorted positions, which are
 // by block and t.  Each of the 32 warps takes a contiguous part of the rows; hist[w][t] first counts
 // the rows of the block's token t in part w and then, after the scan, is the next position of such a
-// row.  A thread has eight tokens in flight; up to kKeyRows rows the second pass finds which of them are of the block in shared memory.
+// row.  A thread has eight tokens in flight; up to kKeyRows rows the second pass finds which of them
+// are of the block in shared memory.
 __global__ void __launch_bounds__(1024) sort_tokens_kernel(
     const void* __restrict__ ids, int ids32, unsigned n_ids, const int* __restrict__ id_rows,
     int rows, int V, int pad, int shift, int span, int* __restrict__ order,
@@ -347,7 +357,7 @@ __global__ void __launch_bounds__(128, 8) embed_grad_kernel(
   const bool sums = b < both ? b % 2 == 0 : sum_blocks > clear_blocks;
   const int block = b < both ? b / 2 : b - both / 2;
   // The sort leaves the memory idle: the first blocks ask the L2 cache for what it can bring in
-  // meanwhile.  (8192 kept of 16384 x 2048: 58 -> 55 us a pass, added to the table 35 -> 31.)
+  // meanwhile.  (8192 kept of 16384 x 2048: 58 -> 55 us a pass, added to the table 35 -> 30.)
   const long long bytes = static_cast<long long>(H) * sizeof(T);
   if (b < kAhead && bytes <= 65536) {
     const int some = min(rows, kAheadBytes / static_cast<int>(bytes));

@@ -551,8 +551,9 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
 
     Tensors are bf16, fp16 or fp32, of any size and alignment, in any dense layout (``out[i]``
     in that of ``grads[i]``); the list may mix types.  Tensors with gaps are refused, and so are
-    outputs and a ``norm`` that overlap anything else of the call.  The squares are fp32 (an element above 1.8e19
-    makes the norm infinite)."""
+    outputs and a ``norm`` that overlap anything else of the call.  The
+    squares and their partial sums are fp32: a norm (before ``extra_scale``) above 1.8e19 may come
+    out infinite, and elements below 1e-19 count with fewer bits, below 2.6e-23 not at all."""
     grads = list(grads)
     if not extra_scale > 0:
         raise ValueError(f"grad_list_clip_: extra_scale = {extra_scale} is not positive")

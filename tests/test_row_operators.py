@@ -758,6 +758,17 @@ def test_grad_list_norm_of_odd_values(dev):
 
 
 @pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("value,n", [(1.7e18, 100), (1.5e19, 1), (1.1e-19, 70000), (3e-18, 5)])
+def test_grad_list_norm_of_large_and_small_values(dev, value, n):
+    """Sums of squares up to 3.4e38, and squares down to 1.2e-38, keep the bound of the norm."""
+    g = torch.full((n,), value, device=dev)
+    norm = fused.grad_list_clip_([g], 0.0)
+    want = float(g[0].double()) * math.sqrt(n)
+    assert abs(float(norm) - want) <= (70 + 4) * U * want
+    assert float(fused.grad_list_sumsq([g]).double().sum()) == pytest.approx(want * want, rel=1e-5)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
 def test_grad_list_over_ranks_and_coef(dev):
     """Two lists whose sums of squares are added, as ranks with different parameters do it."""
     a, b = grad_list(dev, [1000, 77], (F32,), 1), grad_list(dev, [500], (BF,), 2)
