@@ -591,9 +591,14 @@ def grad_list_clip_(grads: Sequence[torch.Tensor], max_norm: float, extra_scale:
 def grad_list_clip_coef(grads: Sequence[torch.Tensor], max_norm: float, extra_scale: float,
                         coef: torch.Tensor, norm: torch.Tensor) -> torch.Tensor:
     """:func:`grad_norm_clip_coef` of a list of tensors: ``coef`` and ``norm`` for an optimizer that
-    takes the factor itself (:func:`adamw_`'s ``grad_scale``); the gradients are only read."""
-    return grad_norm_clip_coef(grads[0], max_norm, extra_scale, coef, norm,
-                               extra_sumsq=grad_list_sumsq(grads))
+    takes the factor itself (:func:`adamw_`'s ``grad_scale``); the gradients are only read.  ``coef``
+    and ``norm`` are one fp32 element each, on the device of the list."""
+    grads = list(grads)
+    sums = grad_list_sumsq(grads)
+    for name, t in (("coef", coef), ("norm", norm)):
+        _need(t.dtype == torch.float32 and t.numel() == 1 and t.device == sums.device,
+              "grad_list_clip_coef: {} must be one fp32 element on {}", name, sums.device)
+    return grad_norm_clip_coef(sums, max_norm, extra_scale, coef, norm, extra_sumsq=sums)
 
 
 # ---------------------------------------------------------------- attention

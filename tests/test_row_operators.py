@@ -840,6 +840,25 @@ def test_grad_list_clip_checks_norm_and_sums(dev):
     assert float(fused.grad_list_clip_([g], 8.0, norm=norm)) == 4.0 and float(norm) == 4.0
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_grad_list_clip_coef_checks_its_buffers(dev):
+    """What the kernel writes is on its device; a list of bf16 tensors, its first one empty."""
+    g = [torch.empty(0, dtype=BF, device=dev), torch.full((2, 8), 0.5, dtype=BF, device=dev)]
+    one = torch.zeros(1, device=dev)
+    bad = [one.double(), torch.zeros(2, device=dev), one[:0], one.int()]
+    if dev == "cuda":
+        bad.append(torch.zeros(1))
+    for t in bad:
+        for kw in (dict(coef=t, norm=one), dict(coef=one, norm=t)):
+            with pytest.raises(ValueError):
+                fused.grad_list_clip_coef(g, 1.0, 1.0, **kw)
+    with pytest.raises(ValueError, match="empty list"):
+        fused.grad_list_clip_coef([], 1.0, 1.0, one, one.clone())
+    norm = one.clone()
+    fused.grad_list_clip_coef(iter(g), 1.0, 1.0, one, norm)
+    assert float(norm) == 2.0 and float(one) == pytest.approx(0.5, rel=1e-6)
+
+
 # ---------------------------------------------------------------- launch counter
 def test_launch_counter_adds_what_the_module_counts(monkeypatch):
     from centrifuge_b200.ops import _ext
