@@ -1109,6 +1109,35 @@ def test_captured_and_replayed_with_other_inputs():
 
 
 @pytest.mark.gpu
+def test_shared_buffers_and_other_ranks_sums_captured():
+    """A shared parameter's gradient and a rank without parameters, in a graph that is replayed."""
+    g, c = norms_case("cuda", 200, 264, BF, BF, "channel", True)
+    y, _, rp, rq = fused.block_norms_fwd(c["h"], c["x"], c["w_post"], c["w_pre"], EPS, c["gate"])
+    dy, dn = rand(g, 200, 264, dtype=BF), rand(g, 200, 264, dtype=BF)
+    acc, sums = torch.zeros(2, 264, device="cuda"), torch.tensor([9.0, 16.0], device="cuda")
+
+    def call():
+        for which, accumulate in (((0, 0, 0), False), ((0, 1, 0), True), ((1, 1, 0), True)):
+            fused.block_norms_bwd(dy, dn, c["h"], y, rp, rq, c["w_post"], c["w_pre"], acc[which[0]],
+                                  acc[which[1]], c["gate"], acc[which[2]], accumulate=accumulate)
+        return fused.grad_list_clip_([], 1.0, extra_sumsq=sums)
+
+    call()
+    acc.zero_()
+    call()
+    want = acc.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = call()
+    for k in (1.0, 2.0):
+        acc.zero_()
+        sums.mul_(k * k)
+        graph.replay()
+        assert torch.equal(acc, want) and float(norm) == 5.0 * k
+
+
+@pytest.mark.gpu
 def test_on_two_streams_at_once():
     g = gen("cuda", 22)
     sets = [_all_operators(g, k) for k in (1.0, 2.0)]
