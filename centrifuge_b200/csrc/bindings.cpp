@@ -9,6 +9,8 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
+#include <initializer_list>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -1227,6 +1229,396 @@ Tensor grad_list_clip(const std::vector<Tensor>& grads,
   return norm;
 }
 
+// ---- linear layers with bias, activation and residual
+inline int half_code(const Tensor& t, const char* what, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, what, ": ",
+                    name, " must be bfloat16 or float16");
+  return t.scalar_type() == at::kHalf ? kF16 : kBF16;
+}
+inline void same_type(const Tensor& first, const Tensor& t, const char* what, const char* name) {
+  TORCH_CHECK_VALUE(t.scalar_type() == first.scalar_type(), what, ": ", name, " must be ",
+                    first.scalar_type());
+}
+inline int act_code(int64_t act, const char* what) {
+  TORCH_CHECK_VALUE(act >= kActNone && act <= kActGeluTanh, what, ": unknown activation ", act);
+  return static_cast<int>(act);
+}
+// Nothing that is written (`out`) shares bytes with what the call reads, unless it is the same
+// elements, each of which is read and written by one thread (`in_place`).
+inline void check_apart(const char* what, const char* name, const Tensor& out,
+                        std::initializer_list<const Tensor*> inputs,
+                        const Tensor* in_place = nullptr) {
+  const Bytes b(out);
+  for (const Tensor* t : inputs) {
+    if (!t || !t->defined()) continue;
+    if (t == in_place && t->const_data_ptr() == out.const_data_ptr() &&
+        t->strides() == out.strides() && t->scalar_type() == out.scalar_type())
+      continue;
+    TORCH_CHECK_VALUE(!b.overlaps(Bytes(*t)), what, ": ", name, " overlaps another tensor of the call");
+  }
+}
+inline const Tensor* opt(const c10::optional<Tensor>& t) {
+  return t.has_value() && t->defined() ? &*t : nullptr;
+}
+void run_linear(CfbLinear& p, const Tensor& like, const char* what) {
+  p.err = err_word(like.get_device()).data_ptr<int>();
+  Tensor work;
+  const int64_t bytes = cfb_linear_workspace(&p);
+  if (bytes > 0) {
+    work = new_empty({bytes}, at::kByte, like);
+    p.work = work.data_ptr();
+  }
+  CFB_CHECK_RC(cfb_linear(&p, cur_stream()), what);
+}
+
+// y = act(x w^T + bias) + resid; z, when given, receives the activation's argument
+Tensor linear_act_fwd(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& bias,
+                      int64_t act, const c10::optional<Tensor>& resid,
+                      const c10::optional<Tensor>& out_in, const c10::optional<Tensor>& z) {
+  const char* what = "linear_act_fwd";
+  CfbLinear p = {};
+  p.kind = kLinearFwd;
+  p.type = half_code(x, what, "x");
+  TORCH_CHECK_VALUE(x.dim() == 2 && w.dim() == 2, what, ": x must be [T, K] and w [N, K]");
+  const int64_t T = x.size(0), K = x.size(1), N = w.size(0);
+  check_rows(x, T, K, what, "x");
+  check_rows(w, N, K, what, "w");
+  same_type(x, w, what, "w");
+  TORCH_CHECK_VALUE(K > 0, what, ": x has no columns");
+  same_device(x, w, "w");
+  same_device(x, bias, "bias");
+  same_device(x, resid, "resid");
+  same_device(x, out_in, "out");
+  same_device(x, z, "z");
+  if (bias.has_value()) check_vector(*bias, N, x.scalar_type(), what, "bias");
+  p.M = row_count(T, what);
+  p.N = row_count(N, what);
+  p.K = row_count(K, what);
+  const Tensor* const r = opt(resid);
+  if (r) {
+    check_rows(*r, T, N, what, "resid");
+    same_type(x, *r, what, "resid");
+    p.R = r->data_ptr();
+    p.ldr = r->stride(0);
+  }
+  if (z.has_value()) {
+    check_rows(*z, T, N, what, "z");
+    same_type(x, *z, what, "z");
+    check_apart(what, "z", *z, {&x, &w, opt(bias), r, opt(out_in)});
+    p.Z = z->data_ptr();
+    p.ldz = z->stride(0);
+  }
+  if (out_in.has_value()) {
+    check_rows(*out_in, T, N, what, "out");
+    same_type(x, *out_in, what, "out");
+    check_apart(what, "out", *out_in, {&x, &w, opt(bias), r}, r);
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor out = out_in.has_value() ? *out_in : new_empty({T, N}, x.scalar_type(), x);
+  p.A = x.data_ptr();
+  p.lda = x.stride(0);
+  p.B = w.data_ptr();
+  p.ldb = w.stride(0);
+  p.D = out.data_ptr();
+  p.ldd = out.stride(0);
+  p.bias = opt_ptr<void>(bias);
+  p.act = act_code(act, what);
+  run_linear(p, x, what);
+  return out;
+}
+
+// dz = (dy w) act'(z[z_rows])
+Tensor linear_act_dgrad(const Tensor& dy, const Tensor& w, const Tensor& z, int64_t act,
+                        const c10::optional<Tensor>& z_rows, const c10::optional<Tensor>& out_in) {
+  const char* what = "linear_act_dgrad";
+  CfbLinear p = {};
+  p.kind = kLinearDgrad;
+  p.type = half_code(dy, what, "dy");
+  TORCH_CHECK_VALUE(dy.dim() == 2 && w.dim() == 2 && z.dim() == 2, what,
+                    ": dy must be [R, K], w [K, N] and z [T, N]");
+  const int64_t R = dy.size(0), K = dy.size(1), N = w.size(1), T = z.size(0);
+  check_rows(dy, R, K, what, "dy");
+  check_rows(w, K, N, what, "w");
+  check_rows(z, T, N, what, "z");
+  same_type(dy, w, what, "w");
+  same_type(dy, z, what, "z");
+  TORCH_CHECK_VALUE(K > 0, what, ": dy has no columns");
+  same_device(dy, w, "w");
+  same_device(dy, z, "z");
+  same_device(dy, z_rows, "z_rows");
+  same_device(dy, out_in, "out");
+  if (z_rows.has_value())
+    check_vector(*z_rows, R, at::kInt, what, "z_rows");
+  else
+    TORCH_CHECK_VALUE(R == T, what, ": ", R, " gradient rows for ", T, " rows of z");
+  if (out_in.has_value()) {
+    check_rows(*out_in, R, N, what, "out");
+    same_type(dy, *out_in, what, "out");
+    check_apart(what, "out", *out_in, {&dy, &w, &z, opt(z_rows)},
+                z_rows.has_value() ? nullptr : &z);
+  }
+  p.M = row_count(R, what);
+  p.N = row_count(N, what);
+  p.K = row_count(K, what);
+  row_count(T, what);
+  const c10::cuda::CUDAGuard guard(dy.device());
+  Tensor out = out_in.has_value() ? *out_in : new_empty({R, N}, dy.scalar_type(), dy);
+  p.A = dy.data_ptr();
+  p.lda = dy.stride(0);
+  p.B = w.data_ptr();
+  p.ldb = w.stride(0);
+  p.D = out.data_ptr();
+  p.ldd = out.stride(0);
+  p.Z = z.data_ptr();
+  p.ldz = z.stride(0);
+  p.z_rows = opt_ptr<int>(z_rows);
+  p.n_z = T;
+  p.act = act_code(act, what);
+  run_linear(p, dy, what);
+  return out;
+}
+
+// dw (+)= dy^T x, dbias (+)= the sum of dy's rows
+void linear_bias_wgrad(const Tensor& dy, const Tensor& x, Tensor& dw,
+                       const c10::optional<Tensor>& dbias, bool accumulate) {
+  const char* what = "linear_bias_wgrad";
+  CfbLinear p = {};
+  p.kind = kLinearWgrad;
+  p.type = half_code(dy, what, "dy");
+  TORCH_CHECK_VALUE(dy.dim() == 2 && x.dim() == 2, what, ": dy must be [R, N] and x [R, K]");
+  const int64_t R = dy.size(0), N = dy.size(1), K = x.size(1);
+  check_rows(dy, R, N, what, "dy");
+  check_rows(x, R, K, what, "x");
+  check_rows(dw, N, K, what, "dw");
+  same_type(dy, x, what, "x");
+  TORCH_CHECK_VALUE(dw.scalar_type() == at::kFloat, what, ": dw must be fp32");
+  same_device(dy, x, "x");
+  same_device(dy, dw, "dw");
+  same_device(dy, dbias, "dbias");
+  check_apart(what, "dw", dw, {&dy, &x, opt(dbias)});
+  if (dbias.has_value()) {
+    check_vector(*dbias, N, at::kFloat, what, "dbias");
+    check_apart(what, "dbias", *dbias, {&dy, &x});
+  }
+  p.M = row_count(N, what);
+  p.N = row_count(K, what);
+  p.K = row_count(R, what);
+  const c10::cuda::CUDAGuard guard(dy.device());
+  p.A = dy.data_ptr();
+  p.lda = dy.stride(0);
+  p.B = x.data_ptr();
+  p.ldb = x.stride(0);
+  p.D = dw.data_ptr();
+  p.ldd = dw.stride(0);
+  p.add = accumulate;
+  p.dbias = const_cast<float*>(opt_ptr<float>(dbias));
+  run_linear(p, dy, what);
+}
+
+// ---- layer norm
+// (y, mean, rstd)
+std::tuple<Tensor, Tensor, Tensor> layernorm_fwd(const Tensor& x, const c10::optional<Tensor>& w,
+                                                 const c10::optional<Tensor>& b, double eps,
+                                                 const c10::optional<Tensor>& out_in) {
+  const char* what = "layernorm_fwd";
+  TORCH_CHECK_VALUE(x.dim() == 2, what, ": x must be [T, H]");
+  const int64_t T = x.size(0), H = x.size(1);
+  check_rows(x, T, H, what, "x");
+  TORCH_CHECK_VALUE(H <= kLayerNormMaxH, what, ": hidden size ", H, " is over ", kLayerNormMaxH);
+  const Tensor& typed = w.has_value() ? *w : b.has_value() ? *b : out_in.has_value() ? *out_in : x;
+  const int type = type_code(typed, "w");
+  const int x_type = resid_code(what, x, typed, "x");
+  if (w.has_value()) check_vector(*w, H, typed.scalar_type(), what, "w");
+  if (b.has_value()) check_vector(*b, H, typed.scalar_type(), what, "b");
+  same_device(x, w, "w");
+  same_device(x, b, "b");
+  same_device(x, out_in, "out");
+  if (out_in.has_value()) {
+    check_rows(*out_in, T, H, what, "out");
+    same_type(typed, *out_in, what, "out");
+    check_apart(what, "out", *out_in, {&x, opt(w), opt(b)});
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int rows = row_count(T, what);
+  Tensor y = out_in.has_value() ? *out_in : new_empty({T, H}, typed.scalar_type(), x);
+  Tensor mean = new_empty({T}, at::kFloat, x), rstd = new_empty({T}, at::kFloat, x);
+  CFB_CHECK_RC(cfb_layernorm_fwd(x.data_ptr(), x_type, x.stride(0), opt_ptr<void>(w),
+                                 opt_ptr<void>(b), type, static_cast<float>(eps), y.data_ptr(),
+                                 y.stride(0), mean.data_ptr<float>(), rstd.data_ptr<float>(), rows,
+                                 static_cast<int>(H), cur_stream()),
+               what);
+  return {y, mean, rstd};
+}
+
+Tensor layernorm_bwd(const Tensor& dy, const Tensor& x, const Tensor& mean, const Tensor& rstd,
+                     const c10::optional<Tensor>& w, const c10::optional<Tensor>& dw,
+                     const c10::optional<Tensor>& db, const c10::optional<Tensor>& rows,
+                     const c10::optional<Tensor>& dres, bool accumulate) {
+  const char* what = "layernorm_bwd";
+  TORCH_CHECK_VALUE(dy.dim() == 2 && x.dim() == 2, what, ": dy must be [R, H] and x [T, H]");
+  const int64_t R = dy.size(0), T = x.size(0), H = x.size(1);
+  check_rows(dy, R, H, what, "dy");
+  check_rows(x, T, H, what, "x");
+  TORCH_CHECK_VALUE(H <= kLayerNormMaxH, what, ": hidden size ", H, " is over ", kLayerNormMaxH);
+  const int type = type_code(dy, "dy");
+  const int x_type = resid_code(what, x, dy, "x");
+  check_vector(mean, T, at::kFloat, what, "mean");
+  check_vector(rstd, T, at::kFloat, what, "rstd");
+  if (w.has_value()) check_vector(*w, H, dy.scalar_type(), what, "w");
+  if (dres.has_value()) {
+    check_rows(*dres, R, H, what, "dres");
+    same_type(x, *dres, what, "dres");
+  }
+  if (rows.has_value())
+    check_vector(*rows, R, at::kInt, what, "rows");
+  else
+    TORCH_CHECK_VALUE(R == T, what, ": ", R, " gradient rows for ", T, " rows");
+  same_device(dy, x, "x");
+  same_device(dy, mean, "mean");
+  same_device(dy, rstd, "rstd");
+  same_device(dy, w, "w");
+  same_device(dy, dw, "dw");
+  same_device(dy, db, "db");
+  same_device(dy, rows, "rows");
+  same_device(dy, dres, "dres");
+  const Tensor* const sums[] = {opt(dw), opt(db)};
+  for (int i = 0; i < 2; ++i) {
+    if (!sums[i]) continue;
+    const char* name = i ? "db" : "dw";
+    check_vector(*sums[i], H, at::kFloat, what, name);
+    check_apart(what, name, *sums[i], {&dy, &x, &mean, &rstd, opt(w), opt(rows), opt(dres),
+                                       i ? opt(dw) : nullptr});
+  }
+  row_count(T, what);
+  const int n = row_count(R, what);
+  const c10::cuda::CUDAGuard guard(dy.device());
+  Tensor dx = new_empty({R, H}, x.scalar_type(), dy), work;
+  if (n > 0 && H > 0)
+    work = new_empty({cfb_layernorm_bwd_workspace(n, static_cast<int>(H))}, at::kByte, dy);
+  CFB_CHECK_RC(
+      cfb_layernorm_bwd(dy.data_ptr(), type, dy.stride(0), x.data_ptr(), x_type, x.stride(0),
+                        mean.data_ptr<float>(), rstd.data_ptr<float>(), opt_ptr<void>(w),
+                        opt_ptr<void>(dres), dres.has_value() ? dres->stride(0) : 0,
+                        opt_ptr<int>(rows), T, dx.data_ptr(), const_cast<float*>(opt_ptr<float>(dw)),
+                        const_cast<float*>(opt_ptr<float>(db)), accumulate,
+                        work.defined() ? work.data_ptr() : nullptr, n, static_cast<int>(H),
+                        err_word(dy.get_device()).data_ptr<int>(), cur_stream()),
+      what);
+  return dx;
+}
+
+// ---- distillation
+CfbDistill distill_args(const char* what, const Tensor& logits, const Tensor& ids, const Tensor& top,
+                        double temperature, const c10::optional<Tensor>& labels) {
+  CfbDistill p = {};
+  TORCH_CHECK_VALUE(logits.dim() == 2, what, ": logits must be [T, V]");
+  const int64_t T = logits.size(0), V = logits.size(1);
+  check_rows(logits, T, V, what, "logits");
+  TORCH_CHECK_VALUE(V > 0 && V <= kDistillMaxVocab, what, ": ", V, " logits a row, not 1 to ",
+                    kDistillMaxVocab);
+  TORCH_CHECK_VALUE(ids.dim() == 2 && is_index(ids), what, ": top_ids must be int64 or int32 [T, K]");
+  const int64_t K = ids.size(1);
+  TORCH_CHECK_VALUE(K > 0 && K <= kDistillMaxTop, what, ": ", K, " listed logits a row, not 1 to ",
+                    kDistillMaxTop);
+  check_rows(ids, T, K, what, "top_ids");
+  check_rows(top, T, K, what, "top_logits");
+  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(temperature), what, ": temperature = ",
+                    temperature, " is not positive");
+  same_device(logits, ids, "top_ids");
+  same_device(logits, top, "top_logits");
+  same_device(logits, labels, "labels");
+  if (labels.has_value()) check_vector(*labels, T, at::kLong, what, "labels");
+  row_count(T, what);
+  p.type = type_code(logits, "logits");
+  p.V = static_cast<int>(V);
+  p.K = static_cast<int>(K);
+  p.z = logits.data_ptr();
+  p.ld = logits.stride(0);
+  p.ids = ids.data_ptr();
+  p.ids64 = ids.scalar_type() == at::kLong;
+  p.ld_ids = ids.stride(0);
+  p.top = top.data_ptr();
+  p.top_type = type_code(top, "top_logits");
+  p.ld_top = top.stride(0);
+  p.labels = reinterpret_cast<const long long*>(opt_ptr<int64_t>(labels));
+  p.temperature = temperature;
+  p.err = err_word(logits.get_device()).data_ptr<int>();
+  return p;
+}
+
+// (kd, ce, lse, stats); ce and lse are None without labels
+std::tuple<Tensor, c10::optional<Tensor>, c10::optional<Tensor>, Tensor> distill_fwd(
+    const Tensor& logits, const Tensor& top_ids, const Tensor& top_logits, double temperature,
+    const c10::optional<Tensor>& top_lse, const c10::optional<Tensor>& labels) {
+  const char* what = "distill_fwd";
+  const c10::cuda::CUDAGuard guard(logits.device());
+  CfbDistill p = distill_args(what, logits, top_ids, top_logits, temperature, labels);
+  const int64_t T = logits.size(0);
+  same_device(logits, top_lse, "top_lse");
+  if (top_lse.has_value()) check_vector(*top_lse, T, at::kFloat, what, "top_lse");
+  p.top_lse = opt_ptr<float>(top_lse);
+  Tensor kd = new_empty({T}, at::kFloat, logits), stats = new_empty({T, 4}, at::kFloat, logits);
+  c10::optional<Tensor> ce, lse;
+  if (labels.has_value()) {
+    ce = new_empty({T}, at::kFloat, logits);
+    lse = new_empty({T}, at::kFloat, logits);
+  }
+  CFB_CHECK_RC(cfb_distill_fwd(&p, kd.data_ptr<float>(), ce ? ce->data_ptr<float>() : nullptr,
+                               lse ? lse->data_ptr<float>() : nullptr, stats.data_ptr<float>(),
+                               static_cast<int>(T), cur_stream()),
+               what);
+  return {kd, ce, lse, stats};
+}
+
+Tensor distill_bwd(const Tensor& logits, const Tensor& top_ids, const Tensor& top_logits,
+                   const Tensor& stats, const Tensor& dkd, double temperature,
+                   const c10::optional<Tensor>& labels, const c10::optional<Tensor>& lse,
+                   const c10::optional<Tensor>& dce, const c10::optional<Tensor>& rows,
+                   const c10::optional<Tensor>& out_in) {
+  const char* what = "distill_bwd";
+  const c10::cuda::CUDAGuard guard(logits.device());
+  CfbDistill p = distill_args(what, logits, top_ids, top_logits, temperature, labels);
+  const int64_t T = logits.size(0), V = logits.size(1);
+  TORCH_CHECK_VALUE(dkd.dim() == 1, what, ": dkd must be [R]");
+  const int64_t R = dkd.size(0);
+  check_vector(dkd, R, at::kFloat, what, "dkd");
+  TORCH_CHECK_VALUE(stats.dim() == 2 && stats.size(0) == T && stats.size(1) == 4 &&
+                        stats.scalar_type() == at::kFloat && stats.is_contiguous() &&
+                        reinterpret_cast<uintptr_t>(stats.const_data_ptr()) % 16 == 0,
+                    what, ": stats must be contiguous fp32 [", T, ", 4] on a boundary of 16 bytes");
+  TORCH_CHECK_VALUE(lse.has_value() == labels.has_value() && dce.has_value() == labels.has_value(),
+                    what, ": labels, lse and dce go together");
+  if (labels.has_value()) {
+    check_vector(*lse, T, at::kFloat, what, "lse");
+    check_vector(*dce, R, at::kFloat, what, "dce");
+  }
+  if (rows.has_value())
+    check_vector(*rows, R, at::kInt, what, "rows");
+  else
+    TORCH_CHECK_VALUE(R == T, what, ": ", R, " gradient rows for ", T, " rows");
+  same_device(logits, stats, "stats");
+  same_device(logits, dkd, "dkd");
+  same_device(logits, lse, "lse");
+  same_device(logits, dce, "dce");
+  same_device(logits, rows, "rows");
+  same_device(logits, out_in, "out");
+  if (out_in.has_value()) {
+    check_rows(*out_in, R, V, what, "out");
+    same_type(logits, *out_in, what, "out");
+    check_apart(what, "out", *out_in,
+                {&logits, &top_ids, &top_logits, &stats, &dkd, opt(labels), opt(lse), opt(dce),
+                 opt(rows)},
+                rows.has_value() ? nullptr : &logits);
+  }
+  const int n = row_count(R, what);
+  Tensor out = out_in.has_value() ? *out_in : new_empty({R, V}, logits.scalar_type(), logits);
+  CFB_CHECK_RC(cfb_distill_bwd(&p, stats.data_ptr<float>(), opt_ptr<float>(lse),
+                               dkd.data_ptr<float>(), opt_ptr<float>(dce), opt_ptr<int>(rows), T,
+                               out.data_ptr(), out.stride(0), n, cur_stream()),
+               what);
+  return out;
+}
+
 // Dispatcher-visible attention ops on token-major rows, used by the graph rewriter's filtered
 // attention node (centrifuge_b200._filter_C) for SDPA graphs of arbitrary models.
 std::tuple<Tensor, Tensor> attn_fwd_rows(const Tensor& qkv, int64_t B, int64_t S, int64_t nh,
@@ -1309,6 +1701,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("block_norms_bwd", &block_norms_bwd);
   m.def("grad_list_sumsq", &grad_list_sumsq);
   m.def("grad_list_clip", &grad_list_clip);
+  m.def("linear_act_fwd", &linear_act_fwd);
+  m.def("linear_act_dgrad", &linear_act_dgrad);
+  m.def("linear_bias_wgrad", &linear_bias_wgrad);
+  m.def("layernorm_fwd", &layernorm_fwd);
+  m.def("layernorm_bwd", &layernorm_bwd);
+  m.def("distill_fwd", &distill_fwd);
+  m.def("distill_bwd", &distill_bwd);
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd", &ce_bwd, py::arg("logits"), py::arg("rows"), py::arg("labels"),
         py::arg("lse"), py::arg("dloss"), py::arg("dlogits"), py::arg("vocab_start") = 0);

@@ -299,3 +299,75 @@ int cfb_grad_list_sumsq(const CfbTensorRef* refs, int count, float* partial, int
 int cfb_grad_list_scale(const CfbTensorRef* refs, int count, const float* partial, int n_partial,
                         float max_norm, float extra_scale, float* norm, int in_place,
                         cudaStream_t st);
+
+// ---- linear layers with bias, activation and residual (formulas in linear_act.cu).  Operands and
+// outputs bf16 or fp16 with any row stride and alignment of an element; dw and dbias fp32.
+enum { kLinearFwd = 0, kLinearDgrad = 1, kLinearWgrad = 2 };
+enum { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
+struct CfbLinear {
+  int kind, type;
+  int M, N, K;  // the output is [M, N]; K > 0 but for wgrad
+  const void* A;  // fwd x [M, K], dgrad dy [M, K], wgrad dy [K, M]
+  long long lda;
+  const void* B;  // fwd w [N, K], dgrad w [K, N], wgrad x [K, N]
+  long long ldb;
+  void* D;  // y, dz or dw
+  long long ldd;
+  const void* bias;  // fwd: [N] or null
+  const void* R;     // fwd: residual [M, N] or null
+  long long ldr;
+  void* Z;  // fwd: receives z, or null; dgrad: z, read at the rows z_rows (all when null)
+  long long ldz;
+  const int* z_rows;  // an id outside [0, n_z) records kErrBounds and gives a zero row
+  long long n_z;
+  int act;
+  int add;       // wgrad: add to dw and dbias
+  float* dbias;  // wgrad: [M] or null
+  void* work;    // cfb_linear_workspace bytes, 16-byte aligned
+  int* err;
+};
+long long cfb_linear_workspace(const CfbLinear* p);
+int cfb_linear(const CfbLinear* p, cudaStream_t st);
+
+// Layer norm (formulas in layernorm.cu): x has type x_type (type or fp32), y, dy, w and b `type`; w
+// and b may be null.  H up to kLayerNormMaxH.
+constexpr int kLayerNormMaxH = 16384;
+int cfb_layernorm_fwd(const void* x, int x_type, long long ld_x, const void* w, const void* b,
+                      int type, float eps, void* y, long long ld_y, float* mean, float* rstd,
+                      int rows, int H, cudaStream_t st);
+// On the rows row_ids[0, rows) (or 0 .. rows) of x, mean and rstd; a row id outside [0, n_rows)
+// records kErrBounds and gives a zero row.  dres (x_type, or null) is added to dx [rows, H].  dw and
+// db (fp32 [H], or null) are added to with `add`.
+long long cfb_layernorm_bwd_workspace(int rows, int H);
+int cfb_layernorm_bwd(const void* dy, int type, long long ld_dy, const void* x, int x_type,
+                      long long ld_x, const float* mean, const float* rstd, const void* w,
+                      const void* dres, long long ld_res, const int* row_ids, long long n_rows,
+                      void* dx, float* dw, float* db, int add, void* work, int rows, int H,
+                      int* err, cudaStream_t st);
+
+// Distillation from a teacher's top logits beside the labels' cross entropy (formulas in distill.cu).
+constexpr int kDistillMaxTop = 1024, kDistillMaxVocab = 1 << 20;
+struct CfbDistill {
+  int type, V, K;
+  const void* z;  // logits
+  long long ld;
+  const void* ids;  // [*, K] int32, or int64 with ids64
+  int ids64;
+  long long ld_ids;
+  const void* top;  // [*, K]
+  int top_type;
+  long long ld_top;
+  const float* top_lse;     // null: the teacher's shares sum to one over the list
+  const long long* labels;  // null: no cross entropy
+  double temperature;
+  int* err;
+};
+// kd, ce (with labels), lse (with labels) [rows], stats [rows, 4]
+int cfb_distill_fwd(const CfbDistill* p, float* kd, float* ce, float* lse, float* stats, int rows,
+                    cudaStream_t st);
+// out [rows, V]: the gradient of sum dkd kd + dce ce at the rows row_ids (or 0 .. rows) of all inputs
+// but dkd and dce; a row id outside [0, n_rows) records kErrBounds and gives a zero row.  out may be
+// the logits themselves without row_ids.
+int cfb_distill_bwd(const CfbDistill* p, const float* stats, const float* lse, const float* dkd,
+                    const float* dce, const int* row_ids, long long n_rows, void* out,
+                    long long ld_out, int rows, cudaStream_t st);

@@ -18,7 +18,9 @@ _LAUNCHES_PER_CALL = {"rmsnorm_bwd": 2, "attn_bwd": 2, "attn_bwd_mma": 3, "gemm_
                       "status_block": 0, "set_wait_limits": 0, "gemm_plan": 0,
                       "row_launches": 0, "scaled_embedding_fwd": 0, "scaled_embedding_bwd": 0,
                       "block_norms_fwd": 0, "block_norms_bwd": 0, "grad_list_sumsq": 0,
-                      "grad_list_clip": 0}
+                      "grad_list_clip": 0, "linear_act_fwd": 0, "linear_act_dgrad": 0,
+                      "linear_bias_wgrad": 0, "layernorm_fwd": 0, "layernorm_bwd": 0,
+                      "distill_fwd": 0, "distill_bwd": 0}
 
 
 class LaunchCounter:

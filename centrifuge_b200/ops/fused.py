@@ -377,6 +377,196 @@ def block_norms_bwd(dy: Optional[torch.Tensor], dn: Optional[torch.Tensor], h: t
             dgate if gate is None or learned else dg.to(gate.dtype))
 
 
+# ---------------------------------------------------------------- layer norm
+def _check_apart(name: str, what: str, out: torch.Tensor, inputs,
+                 in_place: Optional[torch.Tensor] = None) -> None:
+    for t in inputs:
+        same = t is not None and t is in_place and t.data_ptr() == out.data_ptr() and (
+            t.stride() == out.stride())
+        _need(t is None or same or not _overlap(out, t), "{}: {} overlaps another tensor of the call",
+              name, what)
+
+
+def layernorm_fwd(x: torch.Tensor, w: Optional[torch.Tensor], b: Optional[torch.Tensor], eps: float,
+                  out: Optional[torch.Tensor] = None):
+    """``y = (x - mean) rstd w + b`` with ``rstd = (mean of (x - mean)^2 + eps)^-1/2`` of each row:
+    ``(y, mean, rstd)``, the last two fp32 ``[T]``.
+
+    ``w`` and ``b`` (contiguous ``[H]``; without one it is one, or zero) and ``y`` are bf16, fp16 or
+    fp32, and ``x [T, H]`` has their type or is an fp32 residual stream (without both, ``y`` has the
+    type of ``out``, or of ``x``).  ``x`` and ``out`` may have any row stride and alignment, and do
+    not overlap.  ``H`` up to 16384."""
+    if x.is_cuda:
+        return kernels().layernorm_fwd(x, w, b, eps, out)
+    name = "layernorm_fwd"
+    T, H = x.shape if x.dim() == 2 else (-1, -1)
+    _need(T >= 0 and _rows2d(x, H), "{}: x must be row-major [T, H]", name)
+    _need(H <= 16384, "{}: hidden size {} is over 16384", name, H)
+    dtype = next(t for t in (w, b, out, x) if t is not None).dtype
+    _need(dtype in _ROW_TYPES and x.dtype in (dtype, torch.float32), "{}: x must be {} or fp32", name,
+          dtype)
+    _need(all(t is None or _vector(t, H, dtype) for t in (w, b)),
+          "{}: w and b must be contiguous {} [{}]", name, dtype, H)
+    if out is not None:
+        _need(_rows2d(out, H) and out.shape[0] == T and out.dtype == dtype,
+              "{}: out must be row-major {} [{}, {}]", name, dtype, T, H)
+        _check_apart(name, "out", out, (x, w, b))
+    y, mean, rstd = ref.layernorm(x, w, b, eps)
+    return y.to(dtype) if out is None else out.copy_(y), mean, rstd
+
+
+def layernorm_bwd(dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                  w: Optional[torch.Tensor], dw: Optional[torch.Tensor],
+                  db: Optional[torch.Tensor], rows: Optional[torch.Tensor] = None,
+                  dres: Optional[torch.Tensor] = None, accumulate: bool = True) -> torch.Tensor:
+    """``dx = dres + d(layernorm)/dx`` on the rows ``rows`` of ``x`` and the saved statistics (int32
+    ``[R]``; all when ``None``).
+
+    ``dy [R, H]`` and ``w`` are bf16, fp16 or fp32; ``x``, ``dres [R, H]`` (the gradient that reaches
+    ``x`` past the norm, or ``None``) and ``dx`` have that type or fp32.  ``dw`` and ``db`` are fp32
+    ``[H]`` buffers (``None``: not wanted), added to (written without ``accumulate``) in a fixed
+    order; what is written overlaps nothing else.  On the GPU a row id outside ``x`` records an error
+    in the status block, gives a zero row and adds nothing; on the CPU it raises ``IndexError``."""
+    if dy.is_cuda:
+        return kernels().layernorm_bwd(dy, x, mean, rstd, w, dw, db, rows, dres, accumulate)
+    name = "layernorm_bwd"
+    T, H = x.shape if x.dim() == 2 else (-1, -1)
+    _need(T >= 0 and _rows2d(x, H) and _rows2d(dy, H),
+          "{}: dy must be row-major [R, H] and x [T, H]", name)
+    R = dy.shape[0]
+    _need(H <= 16384, "{}: hidden size {} is over 16384", name, H)
+    _need(dy.dtype in _ROW_TYPES and x.dtype in (dy.dtype, torch.float32),
+          "{}: x must be {} or fp32", name, dy.dtype)
+    _need(_vector(mean, T, torch.float32) and _vector(rstd, T, torch.float32),
+          "{}: mean and rstd must be contiguous fp32 [{}]", name, T)
+    _need(w is None or _vector(w, H, dy.dtype), "{}: w must be contiguous {} [{}]", name, dy.dtype, H)
+    _need(dres is None or _rows2d(dres, H) and dres.shape[0] == R and dres.dtype == x.dtype,
+          "{}: dres must be row-major {} [{}, {}]", name, x.dtype, R, H)
+    if rows is None:
+        _need(R == T, "{}: {} gradient rows for {} rows", name, R, T)
+    else:
+        _need(rows.dtype == torch.int32 and rows.dim() == 1 and rows.shape[0] == R
+              and rows.is_contiguous(), "{}: rows must be contiguous int32 [{}]", name, R)
+    for what, t, other in (("dw", dw, None), ("db", db, dw)):
+        if t is not None:
+            _need(_vector(t, H, torch.float32), "{}: {} must be contiguous fp32 [{}]", name, what, H)
+            _check_apart(name, what, t, (dy, x, mean, rstd, w, rows, dres, other))
+    if rows is not None:
+        _need_index(rows, T, f"{name}: a row id is")
+        x, mean, rstd = x[rows.long()], mean[rows.long()], rstd[rows.long()]
+    dx, gw, gb = ref.layernorm_bwd(dy, x, mean, rstd, w, dres)
+    for t, g in ((dw, gw), (db, gb)):
+        if t is not None:
+            t.copy_(t + g if accumulate else g)
+    return dx.to(x.dtype)
+
+
+# ---------------------------------------------------------------- distillation
+def _check_distill(name: str, logits, top_ids, top_logits, temperature: float, labels) -> None:
+    T, V = logits.shape if logits.dim() == 2 else (-1, -1)
+    _need(T >= 0 and _rows2d(logits, V) and logits.dtype in _ROW_TYPES,
+          "{}: logits must be row-major bf16, fp16 or fp32 [T, V]", name)
+    _need(0 < V <= 1 << 20, "{}: {} logits a row, not 1 to {}", name, V, 1 << 20)
+    K = top_ids.shape[1] if top_ids.dim() == 2 else -1
+    _need(0 < K <= 1024, "{}: {} listed logits a row, not 1 to 1024", name, K)
+    _need(top_ids.dtype in (torch.int64, torch.int32) and _rows2d(top_ids, K)
+          and top_ids.shape[0] == T, "{}: top_ids must be int64 or int32 [{}, K]", name, T)
+    _need(top_logits.dtype in _ROW_TYPES and _rows2d(top_logits, K) and top_logits.shape[0] == T,
+          "{}: top_logits must be bf16, fp16 or fp32 [{}, {}]", name, T, K)
+    _need(temperature > 0 and math.isfinite(temperature), "{}: temperature = {} is not positive", name,
+          temperature)
+    _need(labels is None or _vector(labels, T, torch.int64), "{}: labels must be int64 [{}]", name, T)
+
+
+def distill_fwd(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: torch.Tensor,
+                temperature: float = 1.0, top_lse: Optional[torch.Tensor] = None,
+                labels: Optional[torch.Tensor] = None):
+    """Per-token divergence of a student from a teacher of whom the top logits are known, and the
+    labels' cross entropy, in one pass over the student's logits: ``(kd, ce, lse, stats)``.
+
+    ``logits [T, V]`` are the student's; the teacher's ``top_logits [T, K]`` belong to the tokens
+    ``top_ids [T, K]`` (int64 or int32; a negative id leaves an entry out, so lists may be of any
+    length, and a token named twice has the sum of its shares).  With ``q = softmax(logits / tau)``,
+    ``tau = temperature``:
+
+    * without ``top_lse`` the teacher's shares are ``p = softmax(top_logits / tau)`` over the list and
+      ``kd = sum p (log p - log q)``; an empty list, or one of ``-inf`` alone, gives 0.
+    * ``top_lse [T]`` (fp32) is ``log sum exp`` of *all* the teacher's logits ``/ tau``; then
+      ``p = exp(top_logits / tau - top_lse)``, and what is left of 1 is compared with the student's
+      share of all tokens outside the list (where the student gives them any).
+
+    ``kd`` is not scaled by ``tau^2``.  With ``labels`` (int64 ``[T]``; negative: ignored, 0), ``ce``
+    and ``lse`` are those of :func:`ce_fwd`, without them ``None``.  ``stats`` (fp32 ``[T, 4]``:
+    ``log sum exp(logits / tau)``, the same of the tokens outside the list, their share less the
+    teacher's, and the teacher's normaliser) is what :func:`distill_bwd` needs.
+
+    Logits and ``top_logits`` are bf16, fp16 or fp32 with any row stride and alignment, ``V`` up to
+    1048576, ``K`` up to 1024.  On the GPU an id or label outside the vocabulary records an error in
+    the status block and is left out; on the CPU it raises ``IndexError``."""
+    if logits.is_cuda:
+        return kernels().distill_fwd(logits, top_ids, top_logits, temperature, top_lse, labels)
+    name = "distill_fwd"
+    _check_distill(name, logits, top_ids, top_logits, temperature, labels)
+    T, V = logits.shape
+    _need(top_lse is None or _vector(top_lse, T, torch.float32), "{}: top_lse must be fp32 [{}]", name,
+          T)
+    _need_index(top_ids.clamp(min=0), V, f"{name}: an id is")
+    if labels is not None:
+        _need_index(labels.clamp(min=0), V, f"{name}: a label is")
+    return tuple(None if t is None else t.float()
+                 for t in ref.distill(logits, top_ids, top_logits, temperature, top_lse, labels))
+
+
+def distill_bwd(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: torch.Tensor,
+                stats: torch.Tensor, dkd: torch.Tensor, temperature: float = 1.0,
+                labels: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                dce: Optional[torch.Tensor] = None, rows: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """dlogits of ``sum dkd kd + dce ce`` (:func:`distill_fwd`) for the rows ``rows`` (int32 ``[R]``;
+    all when ``None``), rounded once: what both losses give, in one pass.
+
+    ``dkd [R]`` and ``dce [R]`` are fp32; ``labels``, ``lse`` (of the forward) and ``dce`` go
+    together.  A weight of zero adds nothing, whatever the row holds.  ``out [R, V]`` has the type of
+    the logits and any row stride, and may be the logits themselves without ``rows``; other overlaps
+    are refused.  On the GPU a row id outside the logits records an error in the status block and
+    gives a zero row; on the CPU it raises ``IndexError``."""
+    if logits.is_cuda:
+        return kernels().distill_bwd(logits, top_ids, top_logits, stats, dkd, temperature, labels, lse,
+                                     dce, rows, out)
+    name = "distill_bwd"
+    _check_distill(name, logits, top_ids, top_logits, temperature, labels)
+    T, V = logits.shape
+    _need(dkd.dim() == 1 and _vector(dkd, dkd.shape[0], torch.float32), "{}: dkd must be fp32 [R]",
+          name)
+    R = dkd.shape[0]
+    _need(stats.shape == (T, 4) and stats.dtype == torch.float32 and stats.is_contiguous(),
+          "{}: stats must be contiguous fp32 [{}, 4]", name, T)
+    _need((lse is None) == (labels is None) and (dce is None) == (labels is None),
+          "{}: labels, lse and dce go together", name)
+    _need(labels is None or _vector(lse, T, torch.float32) and _vector(dce, R, torch.float32),
+          "{}: lse must be fp32 [{}] and dce fp32 [{}]", name, T, R)
+    if rows is None:
+        _need(R == T, "{}: {} gradient rows for {} rows", name, R, T)
+    else:
+        _need(_vector(rows, R, torch.int32), "{}: rows must be contiguous int32 [{}]", name, R)
+    if out is not None:
+        _need(_rows2d(out, V) and out.shape[0] == R and out.dtype == logits.dtype,
+              "{}: out must be row-major {} [{}, {}]", name, logits.dtype, R, V)
+        _check_apart(name, "out", out,
+                     (logits, top_ids, top_logits, stats, dkd, labels, lse, dce, rows),
+                     logits if rows is None else None)
+    if rows is not None:
+        _need_index(rows, T, f"{name}: a row id is")
+        at = rows.long()
+        logits, top_ids, top_logits, stats = logits[at], top_ids[at], top_logits[at], stats[at]
+        labels, lse = (None, None) if labels is None else (labels[at], lse[at])
+    _need_index(top_ids.clamp(min=0), V, f"{name}: an id is")
+    if labels is not None:
+        _need_index(labels.clamp(min=0), V, f"{name}: a label is")
+    g = ref.distill_bwd(logits, top_ids, top_logits, stats, dkd, temperature, labels, lse, dce)
+    return g.to(logits.dtype) if out is None else out.copy_(g)
+
+
 # ---------------------------------------------------------------- cross entropy
 def ce_fwd(logits: torch.Tensor, labels: torch.Tensor, loss: Optional[torch.Tensor] = None,
            lse: Optional[torch.Tensor] = None):

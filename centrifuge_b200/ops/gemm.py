@@ -6,6 +6,12 @@ Shapes follow the PyTorch ``F.linear`` convention: ``x [T, K]``, ``w [N, K]``, `
 * ``linear_dgrad``   dx = dy w             (w read MN-major: no transpose copy)
 * ``linear_wgrad``   dW (+)= dy^T x        (both read MN-major; fp32 accumulate epilogue)
 
+Layers with a bias and an activation (csrc/kernels/linear_act.cu), bf16 or fp16, of any size:
+
+* ``linear_act_fwd``     z = x w^T + bias,  y = act(z) + resid
+* ``linear_act_dgrad``   dz = (dy w) act'(z)   (through a layer into the activation below it)
+* ``linear_bias_wgrad``  dW (+)= dy^T x,  dbias (+)= sum of the rows of dy
+
 CPU tensors run the fp32 reference (``torch.matmul``); CUDA tensors always run the kernel.
 """
 from __future__ import annotations
@@ -163,3 +169,130 @@ def linear_wgrad(dy: torch.Tensor, x: torch.Tensor, dw: torch.Tensor,
                  accumulate: bool = True, alpha: float = 1.0) -> torch.Tensor:
     """``dw (+)= alpha * dy^T x``; ``dw`` is fp32 ``[N, K]`` (the flat gradient bucket)."""
     return gemm(dy, x, dw, True, True, EPI_F32_ACC if accumulate else EPI_F32, None, alpha)
+
+
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh")
+_HALF_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _act_code(name: str, act: str) -> int:
+    if act not in ACTIVATIONS:
+        raise ValueError(f"{name}: act = {act!r} is none of {', '.join(ACTIVATIONS)}")
+    return ACTIVATIONS.index(act)
+
+
+def _check_out(name: str, what: str, out: torch.Tensor, shape, dtype: torch.dtype, inputs,
+               in_place: Optional[torch.Tensor] = None):
+    from .fused import _need, _overlap, _rows2d
+    _need(_rows2d(out, shape[1]) and out.shape[0] == shape[0] and out.dtype == dtype,
+          "{}: {} must be row-major {} {}", name, what, dtype, list(shape))
+    for t in inputs:
+        same = t is in_place and t is not None and t.data_ptr() == out.data_ptr() and (
+            t.stride() == out.stride() and t.dtype == out.dtype)
+        _need(t is None or same or not _overlap(out, t), "{}: {} overlaps another tensor of the call",
+              name, what)
+
+
+def linear_act_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   act: str = "none", resid: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None,
+                   z: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``y = act(x w^T + bias) + resid``, rounded once.
+
+    ``x [T, K]``, ``w [N, K]`` and ``resid [T, N]`` are bf16 or fp16 of one type, row-major with any
+    row stride and alignment (rows that do not start on 16 bytes are laid out anew for the call);
+    ``bias [N]`` is contiguous; any ``T``, ``N`` and ``K > 0``.  ``act``: one of :data:`ACTIVATIONS`
+    (``gelu`` by the normal distribution, ``gelu_tanh`` by its approximation).  ``z [T, N]``, when
+    given, receives the rounded ``x w^T + bias``, which :func:`linear_act_dgrad` needs.  ``out`` may
+    be ``resid`` itself; other overlaps are refused."""
+    code = _act_code("linear_act_fwd", act)
+    if x.is_cuda:
+        return kernels().linear_act_fwd(x, w, bias, code, resid, out, z)
+    from . import reference as ref
+    from .fused import _need, _rows2d, _vector
+    name = "linear_act_fwd"
+    _need(x.dtype in _HALF_TYPES + (torch.float32,), "{}: x must be bfloat16 or float16", name)
+    _need(x.dim() == 2 and w.dim() == 2 and _rows2d(x, x.shape[1]) and _rows2d(w, x.shape[1])
+          and w.dtype == x.dtype, "{}: x must be row-major [T, K] and w {} [N, K]", name, x.dtype)
+    _need(x.shape[1] > 0, "{}: x has no columns", name)
+    shape = (x.shape[0], w.shape[0])
+    _need(bias is None or _vector(bias, shape[1], x.dtype), "{}: bias must be contiguous {} [{}]",
+          name, x.dtype, shape[1])
+    _need(resid is None or _rows2d(resid, shape[1]) and resid.shape[0] == shape[0]
+          and resid.dtype == x.dtype, "{}: resid must be row-major {} {}", name, x.dtype, shape)
+    if z is not None:
+        _check_out(name, "z", z, shape, x.dtype, (x, w, bias, resid, out))
+    if out is not None:
+        _check_out(name, "out", out, shape, x.dtype, (x, w, bias, resid), resid)
+    y, zf = ref.linear_act(x, w, bias, act, resid)
+    if z is not None:
+        z.copy_(zf)
+    return y.to(x.dtype) if out is None else out.copy_(y)
+
+
+def linear_act_dgrad(dy: torch.Tensor, w: torch.Tensor, z: torch.Tensor, act: str,
+                     z_rows: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dz = (dy w) act'(z[z_rows])``: the gradient ``dy [R, K]`` of a layer's output through its
+    weight ``w [K, N]`` and the activation that made its input, whose argument ``z [T, N]`` the
+    forward kept; on the rows ``z_rows`` (int32 ``[R]``; all when ``None``).  The product is not
+    stored or rounded.  Types and layouts as in :func:`linear_act_fwd`; ``out`` may be ``z`` itself
+    without ``z_rows``.  On the GPU a row id outside ``z`` records an error in the status block and
+    gives a zero row; on the CPU it raises ``IndexError``."""
+    code = _act_code("linear_act_dgrad", act)
+    if dy.is_cuda:
+        return kernels().linear_act_dgrad(dy, w, z, code, z_rows, out)
+    from . import reference as ref
+    from .fused import _need, _need_index, _rows2d
+    name = "linear_act_dgrad"
+    _need(dy.dtype in _HALF_TYPES + (torch.float32,), "{}: dy must be bfloat16 or float16", name)
+    _need(dy.dim() == 2 and w.dim() == 2 and _rows2d(dy, dy.shape[1]) and _rows2d(w, w.shape[1])
+          and w.shape[0] == dy.shape[1] and w.dtype == dy.dtype,
+          "{}: dy must be row-major [R, K] and w {} [K, N]", name, dy.dtype)
+    _need(dy.shape[1] > 0, "{}: dy has no columns", name)
+    shape = (dy.shape[0], w.shape[1])
+    _need(_rows2d(z, shape[1]) and z.dtype == dy.dtype, "{}: z must be row-major {} [T, {}]", name,
+          dy.dtype, shape[1])
+    if z_rows is None:
+        _need(z.shape[0] == shape[0], "{}: {} gradient rows for {} rows of z", name, shape[0],
+              z.shape[0])
+    else:
+        _need(z_rows.dtype == torch.int32 and z_rows.dim() == 1 and z_rows.is_contiguous()
+              and z_rows.shape[0] == shape[0], "{}: z_rows must be contiguous int32 [{}]", name,
+              shape[0])
+    if out is not None:
+        _check_out(name, "out", out, shape, dy.dtype, (dy, w, z, z_rows),
+                   z if z_rows is None else None)
+    if z_rows is not None:
+        _need_index(z_rows, z.shape[0], f"{name}: a row id is")
+    dz = ref.linear_act_dgrad(dy, w, z if z_rows is None else z[z_rows.long()], act)
+    return dz.to(dy.dtype) if out is None else out.copy_(dz)
+
+
+def linear_bias_wgrad(dy: torch.Tensor, x: torch.Tensor, dw: torch.Tensor,
+                      dbias: Optional[torch.Tensor] = None,
+                      accumulate: bool = True) -> torch.Tensor:
+    """``dw (+)= dy^T x`` and ``dbias (+)= sum of the rows of dy`` (written without ``accumulate``),
+    each summed in fp32 in a fixed order.  ``dy [R, N]`` and ``x [R, K]`` as in
+    :func:`linear_act_fwd` (without rows nothing is added), ``dw [N, K]`` fp32 with any row stride,
+    ``dbias [N]`` contiguous fp32; what is written overlaps nothing else."""
+    if dy.is_cuda:
+        kernels().linear_bias_wgrad(dy, x, dw, dbias, accumulate)
+        return dw
+    from .fused import _need, _overlap, _rows2d, _vector
+    name = "linear_bias_wgrad"
+    _need(dy.dtype in _HALF_TYPES + (torch.float32,), "{}: dy must be bfloat16 or float16", name)
+    _need(dy.dim() == 2 and x.dim() == 2 and _rows2d(dy, dy.shape[1]) and _rows2d(x, x.shape[1])
+          and x.shape[0] == dy.shape[0] and x.dtype == dy.dtype,
+          "{}: dy must be row-major [R, N] and x {} [R, K]", name, dy.dtype)
+    _check_out(name, "dw", dw, (dy.shape[1], x.shape[1]), torch.float32, (dy, x, dbias))
+    if dbias is not None:
+        _need(_vector(dbias, dy.shape[1], torch.float32), "{}: dbias must be contiguous fp32 [{}]",
+              name, dy.shape[1])
+        _need(not _overlap(dbias, dy) and not _overlap(dbias, x),
+              "{}: dbias overlaps another tensor of the call", name)
+    g = dy.float()
+    dw.copy_(g.t() @ x.float() + (dw if accumulate else 0.0))
+    if dbias is not None:
+        dbias.copy_(g.sum(0) + (dbias if accumulate else 0.0))
+    return dw

@@ -61,6 +61,120 @@ def block_norms_bwd(dy, dn, h, y, rstd_post, rstd_pre, w_post, w_pre, gate=None,
     return resid_scale * dY, dh, dw_post, dw_pre, dgate
 
 
+def layernorm(x, w, b, eps):
+    """``(y, mean, rstd)`` (fp32)."""
+    xf = x.float()
+    mean = xf.mean(-1)
+    d = xf - mean.unsqueeze(-1)
+    rstd = torch.rsqrt(d.pow(2).mean(-1) + eps)
+    y = d * rstd.unsqueeze(-1)
+    if w is not None:
+        y = y * w.float()
+    return y if b is None else y + b.float(), mean, rstd
+
+
+def layernorm_bwd(dy, x, mean, rstd, w, dres=None):
+    """``(dx, dw, db)`` (fp32)."""
+    r = rstd.unsqueeze(-1)
+    n = (x.float() - mean.unsqueeze(-1)) * r
+    g = dy.float() if w is None else dy.float() * w.float()
+    dx = r * (g - g.mean(-1, keepdim=True) - n * (g * n).mean(-1, keepdim=True))
+    if dres is not None:
+        dx = dx + dres.float()
+    return dx, (dy.float() * n).sum(0), dy.float().sum(0)
+
+
+def activation(z: torch.Tensor, act: str) -> torch.Tensor:
+    if act == "relu":
+        return torch.relu(z)
+    if act == "silu":
+        return torch.nn.functional.silu(z)
+    if act == "gelu":  # (1 + erf would lose the small values)
+        return 0.5 * z * torch.erfc(z * -math.sqrt(0.5))
+    if act == "gelu_tanh":
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z * z * z))
+    return z
+
+
+def activation_grad(z: torch.Tensor, act: str) -> torch.Tensor:
+    if act == "none":
+        return torch.ones_like(z)
+    with torch.enable_grad():
+        z = z.detach().requires_grad_()
+        return torch.autograd.grad(activation(z, act).sum(), z)[0]
+
+
+def linear_act(x, w, bias, act, resid):
+    """``(act(z) + resid, z)`` with ``z = x w^T + bias`` (fp32)."""
+    z = x.float() @ w.float().t()
+    if bias is not None:
+        z = z + bias.float()
+    y = activation(z, act)
+    return y if resid is None else y + resid.float(), z
+
+
+def linear_act_dgrad(dy, w, z, act):
+    return (dy.float() @ w.float()) * activation_grad(z.float(), act)
+
+
+def distill(logits, top_ids, top_logits, temperature, top_lse=None, labels=None):
+    """Divergence of the student from a teacher's top logits and the labels' cross entropy (fp64):
+    ``(kd, ce, lse, stats)``; entries with a negative id are left out."""
+    z, ids = logits.double(), top_ids.long()
+    ok, inf = ids >= 0, float("inf")
+    x = z / temperature
+    lse = torch.logsumexp(x, -1)
+    t = (top_logits.double() / temperature).masked_fill(~ok, -inf)
+    norm = torch.logsumexp(t, -1) if top_lse is None else top_lse.double()
+    none = norm == -inf if top_lse is None else torch.zeros_like(norm, dtype=torch.bool)
+    log_p = (t - norm.unsqueeze(-1)).masked_fill(none.unsqueeze(-1), -inf)
+    p = log_p.exp()
+    log_q = x.gather(-1, ids.clamp(min=0)) - lse.unsqueeze(-1)
+    kd = (p * (log_p - log_q)).masked_fill(p == 0, 0.0).sum(-1)
+    base, coef = lse, (~none).double()
+    if top_lse is not None:
+        others = torch.cat([x, x[:, :1]], -1).scatter(-1, ids.masked_fill(~ok, x.shape[-1]), -inf)
+        base = torch.logsumexp(others[:, :-1], -1)
+        share = p.sum(-1)
+        left = (1.0 - share).clamp(min=0.0)
+        rest = (base - lse).masked_fill(base == -inf, -inf)
+        kd = kd + (left * (left.log() - rest)).masked_fill((left == 0) | (base == -inf), 0.0)
+        coef = (share.clamp(min=1.0) * rest.exp() - left).masked_fill(base == -inf, 0.0)
+    stats = torch.stack([lse, base, coef, norm], -1)
+    if labels is None:
+        return kd, None, None, stats
+    full = torch.logsumexp(z, -1)
+    ce = full - z.gather(-1, labels.clamp(min=0).unsqueeze(-1)).squeeze(-1)
+    return kd, ce.masked_fill(labels < 0, 0.0), full, stats
+
+
+def distill_bwd(logits, top_ids, top_logits, stats, dkd, temperature, labels=None, lse=None,
+                dce=None):
+    """Gradient of ``sum dkd kd + dce ce`` (fp64).  A weight of zero adds nothing."""
+    z, ids, st = logits.double(), top_ids.long(), stats.double()
+    V, inf = z.shape[-1], float("inf")
+    ok = ids >= 0
+    k = (dkd.double() / temperature).unsqueeze(-1)
+    x = z / temperature
+    spread = k * st[:, 2:3]
+    g = (torch.exp(x - st[:, 1:2]) * spread).masked_fill(spread == 0, 0.0)
+    t = (top_logits.double() / temperature).masked_fill(~ok, -inf)
+    p = torch.exp(t - st[:, 3:4]).masked_fill(~ok, 0.0)
+    g = torch.cat([g, g[:, :1]], -1)
+    at = ids.masked_fill(~ok, V)
+    q = torch.exp(x.gather(-1, ids.clamp(min=0)) - st[:, 0:1])
+    whole = p.sum(-1, keepdim=True)  # what the teacher's terms add up to: one, but for a list of all
+    whole = torch.where(st[:, 1:2] == -inf, whole, whole.clamp(min=1.0))
+    g.scatter_(-1, at, k * q * whole).scatter_add_(-1, at, -k * p)
+    g = g[:, :V].masked_fill((k == 0), 0.0)
+    if labels is not None:
+        w = dce.double().masked_fill(labels < 0, 0.0).unsqueeze(-1)
+        soft = torch.exp(z - lse.double().unsqueeze(-1))
+        soft.scatter_add_(-1, labels.clamp(min=0).unsqueeze(-1), -torch.ones_like(w))
+        g = g + (w * soft).masked_fill(w == 0, 0.0)
+    return g
+
+
 def rope_table(max_pos: int, head_dim: int, theta: float, device=None) -> torch.Tensor:
     """``[max_pos, head_dim/2, 2]`` fp32 (cos, sin) of ``pos * theta^(-2i/d)`` (HF convention)."""
     inv_freq = 1.0 / (theta ** (torch.arange(0, head_dim, 2, dtype=torch.int64).float() / head_dim))

@@ -1,0 +1,882 @@
+"""Linear layers with bias, activation and residual, layer norm, and distillation from a teacher's top
+logits, against their formulas in 64 bits.
+
+Tolerances are bounds on the rounding errors of the arithmetic, element by element: u = 2^-24 for an
+fp32 operation, k u sum|x| for a sum whose longest chain has k additions (2 k u where the tensor cores
+add, which need not round to nearest), and half a step of the output's type for its one rounding.
+"""
+import math
+
+import pytest
+import torch
+
+from centrifuge_b200.ops import fused, gemm
+from centrifuge_b200.ops import reference as ref
+
+U = 2.0 ** -24
+EPS = 1e-5
+CPU_GPU = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+BF, HF, F32, F64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
+ACTS = gemm.ACTIVATIONS
+
+
+def close(got, want, tol, what):
+    """|got - want| <= tol everywhere, after the rounding to got's type."""
+    info = torch.finfo(got.dtype)
+    tiny = info.smallest_normal * info.eps / 2
+    bound = tol + info.eps / 2 * (want.abs() + tol) + tiny
+    off = (got.double() - want).abs()
+    bad = ~((off <= bound) | ((got.double() == want) & want.isinf()))
+    if bad.any():
+        i = tuple(bad.nonzero()[0].tolist())
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} off, at {i}: got "
+                             f"{float(got[i])}, want {float(want[i])}, bound {float(bound[i])}")
+
+
+def gen(dev, seed):
+    return torch.Generator(device=dev).manual_seed(seed)
+
+
+def rand(g, *shape, dtype=F32, scale=1.0, shift=0.0, pad=0, skew=0):
+    """Normal values; the rows `pad` elements longer than asked for and begun at element `skew`."""
+    if len(shape) == 2 and (pad or skew):
+        t = torch.randn(shape[0], shape[1] + pad + skew, generator=g, device=g.device)
+        return (t * scale + shift).to(dtype)[:, skew:skew + shape[1]]
+    return (torch.randn(*shape, generator=g, device=g.device) * scale + shift).to(dtype)
+
+
+def empty(dev, rows, cols, dtype, pad=0, skew=0):
+    """A buffer of 9s around the [rows, cols] that a call writes, and that view of it."""
+    t = torch.full((rows, cols + pad + skew), 9.0, dtype=dtype, device=dev)
+    return t, t[:, skew:skew + cols]
+
+
+def untouched(buf, cols, skew):
+    return bool((buf[:, :skew] == 9.0).all()) and bool((buf[:, skew + cols:] == 9.0).all())
+
+
+def kept(g, T, R):
+    return torch.randperm(T, generator=g, device=g.device)[:R].sort().values.int()
+
+
+# ---------------------------------------------------------------- linear layers
+def act64(z, act):
+    if act == "relu":
+        return z.clamp(min=0)
+    if act == "silu":
+        return z * torch.sigmoid(z)
+    if act == "gelu":
+        return z * torch.erfc(-z * math.sqrt(0.5)) / 2
+    if act == "gelu_tanh":
+        return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
+    return z
+
+
+def slope64(z, act):
+    z = z.clone().requires_grad_()
+    if act == "relu":
+        return (z > 0).double()
+    return torch.autograd.grad(act64(z, act).sum(), z)[0]
+
+
+# The activations: exponentials of arguments up to 60 that are rounded once or twice (2 * 60 ln 2 u),
+# the hardware's exponential and reciprocal (2^-22 each), a fit with 1.2e-6 (gelu): below 2^-16 in all.
+ACT_REL = 2.0 ** -16
+
+
+def act_tol(z, act):
+    return 0.0 if act in ("none", "relu") else ACT_REL * act64(z, act).abs()
+
+
+def slope_tol(z, act):
+    """Both terms of the slope with the same relative error, and 1 - p of p near one."""
+    if act in ("none", "relu"):
+        return torch.zeros_like(z)
+    if act == "gelu":
+        return ACT_REL * (torch.erfc(-z * math.sqrt(0.5)) / 2 + z.abs() * torch.exp(-z * z / 2) * 0.4)
+    u = z if act == "silu" else 2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+    du = torch.ones_like(z) if act == "silu" else 2 * math.sqrt(2 / math.pi) * (1 + 0.134145 * z * z)
+    p = torch.sigmoid(u)
+    return ACT_REL * p * (1 + z.abs() * (1 - p) * du) + 4 * U * p * z.abs() * du
+
+
+LINEAR = [
+    (256, 256, 512), (1, 64, 32), (1, 8, 1), (3, 1, 5), (130, 72, 200), (257, 100, 130), (64, 33, 40),
+    (300, 130, 257), (128, 64, 64), (129, 65, 65), (5, 2048, 96), (700, 40, 1000), (17, 1000, 2730),
+    (2, 7, 300), (513, 264, 520),
+]
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,K,N", LINEAR)
+@pytest.mark.parametrize("act,bias,resid,save", [
+    ("none", True, False, False), ("gelu", True, True, True), ("gelu_tanh", False, True, True),
+    ("silu", True, False, True), ("relu", True, True, False), ("none", False, True, True)])
+@pytest.mark.parametrize("dtype,pad,skew", [(BF, 0, 0), (HF, 0, 0), (BF, 8, 0), (HF, 5, 1)])
+def test_linear_act_fwd(dev, T, K, N, act, bias, resid, save, dtype, pad, skew):
+    g = gen(dev, T + K + N)
+    x = rand(g, T, K, dtype=dtype, pad=pad, skew=skew)
+    w = rand(g, N, K, dtype=dtype, scale=2.0 / math.sqrt(K), pad=pad, skew=skew)
+    b = rand(g, N, dtype=dtype) if bias else None
+    r = rand(g, T, N, dtype=dtype, pad=pad, skew=skew) if resid else None
+    z_buf, z = empty(dev, T, N, dtype, pad, skew)
+    o_buf, o = empty(dev, T, N, dtype, pad, skew)
+    got = gemm.linear_act_fwd(x, w, b, act=act, resid=r, out=o if pad else None,
+                              z=z if save else None)
+    assert got.dtype == dtype and got.shape == (T, N) and (not pad or got is o)
+    want_z = x.double() @ w.double().t()
+    tol = 2 * (K + 2) * U * (x.double().abs() @ w.double().abs().t())
+    if bias:
+        want_z = want_z + b.double()
+        tol = tol + U * want_z.abs()
+    want = act64(want_z, act)
+    tol_y = 1.13 * tol + act_tol(want_z, act)
+    if resid:
+        want = want + r.double()
+        tol_y = tol_y + 2 * U * (want.abs() + r.double().abs())
+    close(got, want, tol_y, "y")
+    if save:
+        close(z, want_z, tol, "z")
+        assert untouched(z_buf, N, skew)
+    if pad:
+        assert untouched(o_buf, N, skew)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("R,K,N", LINEAR)
+@pytest.mark.parametrize("act,dtype,pad,skew,some", [
+    ("gelu", BF, 0, 0, True), ("gelu_tanh", HF, 0, 0, False), ("silu", BF, 8, 0, True),
+    ("relu", HF, 5, 1, True), ("none", BF, 5, 1, False), ("silu", HF, 0, 0, False)])
+def test_linear_act_dgrad(dev, R, K, N, act, dtype, pad, skew, some):
+    g = gen(dev, R + 2 * K + N)
+    T = 2 * R + 1 if some else R
+    dy = rand(g, R, K, dtype=dtype, pad=pad, skew=skew)
+    w = rand(g, K, N, dtype=dtype, scale=1.0 / math.sqrt(K), pad=pad, skew=skew)
+    z = rand(g, T, N, dtype=dtype, scale=2.0, pad=pad, skew=skew)
+    rows = kept(g, T, R) if some else None
+    buf, o = empty(dev, R, N, dtype, pad, skew)
+    got = gemm.linear_act_dgrad(dy, w, z, act, z_rows=rows, out=o if pad else None)
+    assert got.dtype == dtype and got.shape == (R, N) and (not pad or got is o)
+    zk = (z if rows is None else z[rows.long()]).double()
+    dh, s = dy.double() @ w.double(), slope64(zk, act)
+    tol = 2 * (K + 2) * U * (dy.double().abs() @ w.double().abs())
+    close(got, dh * s, 1.13 * tol + (dh.abs() + tol) * slope_tol(zk, act) + 2 * U * (dh * s).abs(), "dz")
+    assert not pad or untouched(buf, N, skew)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("N,K,R", [(b, a, c) for a, b, c in LINEAR] + [(64, 96, 0), (40, 300, 1500)])
+@pytest.mark.parametrize("dtype,bias,accumulate,pad,skew", [
+    (BF, True, True, 0, 0), (HF, True, False, 0, 0), (BF, False, False, 8, 0), (HF, True, True, 5, 1)])
+def test_linear_bias_wgrad(dev, N, K, R, dtype, bias, accumulate, pad, skew):
+    g = gen(dev, R + K + 3 * N)
+    dy = rand(g, R, N, dtype=dtype, pad=pad, skew=skew)
+    x = rand(g, R, K, dtype=dtype, pad=pad, skew=skew)
+    buf, dw = empty(dev, N, K, F32, pad, skew)
+    dw.copy_(rand(g, N, K))
+    db = rand(g, N) if bias else None
+    before, before_b = dw.clone(), None if db is None else db.clone()
+    assert gemm.linear_bias_wgrad(dy, x, dw, db, accumulate=accumulate) is dw
+    want = dy.double().t() @ x.double()
+    tol = 2 * (R + 2) * U * (dy.double().abs().t() @ x.double().abs())
+    if accumulate:
+        want = want + before.double()
+        tol = tol + U * want.abs()
+    close(dw, want, tol, "dw")
+    assert untouched(buf, K, skew)
+    if bias:
+        want = dy.double().sum(0)
+        tol = (R + 2) * U * dy.double().abs().sum(0)
+        if accumulate:
+            want = want + before_b.double()
+            tol = tol + U * want.abs()
+        close(db, want, tol, "dbias")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,kind", [
+    (4096, 5632, 512, "fwd"), (2100, 2049, 264, "fwd"), (2048, 5632, 512, "dgrad"),
+    (1500, 5000, 136, "dgrad"), (5632, 2048, 1000, "wgrad"), (3000, 2500, 70, "wgrad"),
+    (20000, 300, 64, "fwd")])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_linear_over_many_tiles(M, N, K, kind, dtype):
+    """More tiles than SMs: each block takes several, with both accumulators in turn."""
+    g = gen("cuda", M + N + K)
+    if kind == "fwd":
+        x, w = rand(g, M, K, dtype=dtype), rand(g, N, K, dtype=dtype, scale=K ** -0.5)
+        got = gemm.linear_act_fwd(x, w)
+        want, mass = x.double() @ w.double().t(), x.double().abs() @ w.double().abs().t()
+    elif kind == "dgrad":
+        dy, w = rand(g, M, K, dtype=dtype), rand(g, K, N, dtype=dtype, scale=K ** -0.5)
+        z = rand(g, M, N, dtype=dtype)
+        got = gemm.linear_act_dgrad(dy, w, z, "relu")
+        live = (z > 0).double()
+        want, mass = dy.double() @ w.double() * live, dy.double().abs() @ w.double().abs()
+    else:
+        dy, x = rand(g, K, M, dtype=dtype), rand(g, K, N, dtype=dtype)
+        got = torch.empty(M, N, device="cuda")
+        runs = []
+        for _ in range(2):
+            gemm.linear_bias_wgrad(dy, x, got, accumulate=False)
+            runs.append(got.clone())
+        assert torch.equal(*runs)  # a fixed order
+        want, mass = dy.double().t() @ x.double(), dy.double().abs().t() @ x.double().abs()
+    close(got, want, 2 * (K + 2) * U * mass, kind)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_activations_over_their_range(dev, act, dtype):
+    """Large and small arguments through an identity weight, in both directions."""
+    v = torch.cat([torch.linspace(-12, 12, 1531), torch.tensor([0.0, -0.0, 1e-4, -1e-4, 30.0, -30.0]),
+                   torch.tensor([88.0, -88.0, 200.0, -200.0, 6e4, -6e4])])
+    v = torch.cat([v, v.new_zeros(-v.numel() % 32)]).to(dtype).to(dev).view(-1, 32)
+    eye = torch.eye(32, dtype=dtype, device=dev)
+    z = torch.empty_like(v)
+    y = gemm.linear_act_fwd(v, eye, act=act, z=z)
+    assert torch.equal(z, v)
+    # an exponential below the smallest normal fp32 number may come out as zero; |z| du at most
+    # multiplies it (du: the slope of what gelu_tanh takes the exponential of, for the others smaller)
+    du = 1.6 * (1 + 0.135 * v.double() ** 2)
+    flush = 2.0 ** -126 * (1 + v.double().abs() * (1 + du))
+    close(y, act64(v.double(), act), act_tol(v.double(), act) + flush, "y")
+    one = torch.ones(v.shape[0], 1, dtype=dtype, device=dev)
+    dz = gemm.linear_act_dgrad(one, torch.ones(1, 32, dtype=dtype, device=dev), v, act)
+    d = v.double()
+    close(dz, slope64(d, act), slope_tol(d, act) + flush, "slope")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_linear_odd_values(dev):
+    """A NaN or infinity stays in its row (forward, dgrad) or column (wgrad)."""
+    g = gen(dev, 3)
+    x, w = rand(g, 70, 48, dtype=BF), rand(g, 40, 48, dtype=BF)
+    x[5, 3], x[9, 0] = float("nan"), float("inf")
+    for act in ACTS:
+        y = gemm.linear_act_fwd(x, w, act=act)
+        assert bool(y[5].isnan().all()) and not bool(y[9].isfinite().logical_and(y[9] != 0).any())
+        y[5], y[9] = 0.0, 0.0
+        assert bool(y.isfinite().all())
+    z = rand(g, 70, 48, dtype=BF)
+    z[2, 7] = float("nan")
+    dz = gemm.linear_act_dgrad(torch.ones(70, 40, dtype=BF, device=dev), w, z, "gelu")
+    assert bool(dz[2, 7].isnan()) and int(dz.isfinite().logical_not().sum()) == 1
+    dw, db = torch.empty(48, 40, device=dev), torch.empty(48, device=dev)
+    gemm.linear_bias_wgrad(x, rand(g, 70, 40, dtype=BF), dw, db, accumulate=False)
+    assert bool(dw[3].isnan().all()) and bool(db[3].isnan()) and bool(db[0].isinf())
+    assert bool(dw[4:].isfinite().all()) and bool(db[4:].isfinite().all())
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_linear_in_place(dev):
+    g = gen(dev, 4)
+    x, w = rand(g, 200, 64, dtype=BF), rand(g, 96, 64, dtype=BF)
+    r = rand(g, 200, 96, dtype=BF)
+    want = gemm.linear_act_fwd(x, w, act="gelu", resid=r)
+    assert torch.equal(gemm.linear_act_fwd(x, w, act="gelu", resid=r, out=r), want)
+    z, dy = rand(g, 200, 64, dtype=BF), rand(g, 200, 96, dtype=BF)
+    want = gemm.linear_act_dgrad(dy, w, z, "silu")
+    assert torch.equal(gemm.linear_act_dgrad(dy, w, z, "silu", out=z), want)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_linear_without_rows(dev):
+    x, w = torch.empty(0, 64, dtype=BF, device=dev), torch.ones(32, 64, dtype=BF, device=dev)
+    assert gemm.linear_act_fwd(x, w, act="gelu").shape == (0, 32)
+    assert gemm.linear_act_dgrad(torch.empty(0, 32, dtype=BF, device=dev), w,
+                                 torch.ones(5, 64, dtype=BF, device=dev), "gelu",
+                                 z_rows=torch.empty(0, dtype=torch.int32, device=dev)).shape == (0, 64)
+    buf, dw = empty(dev, 32, 64, F32, 3, 2)
+    db = torch.ones(32, device=dev)
+    dy = torch.empty(0, 32, dtype=BF, device=dev)
+    gemm.linear_bias_wgrad(dy, x, dw, db)
+    assert bool((buf == 9.0).all()) and bool((db == 1.0).all())
+    gemm.linear_bias_wgrad(dy, x, dw, db, accumulate=False)
+    assert not dw.any() and not db.any() and untouched(buf, 64, 2)
+    # a layer without outputs or inputs
+    assert gemm.linear_act_fwd(w, w[:0]).shape == (32, 0)
+    db = torch.zeros(64, device=dev)
+    gemm.linear_bias_wgrad(w, torch.empty(32, 0, dtype=BF, device=dev),
+                           torch.empty(64, 0, device=dev), db)
+    assert bool((db == 32.0).all())
+
+
+# ---------------------------------------------------------------- layer norm
+def ln64(x, w, b):
+    mean = x.mean(-1, keepdim=True)
+    r = ((x - mean).square().mean(-1, keepdim=True) + EPS).rsqrt()
+    n = (x - mean) * r
+    y = n if w is None else n * w
+    return (y if b is None else y + b), mean, r, n
+
+
+LN_CASES = [
+    (256, 256, BF, BF, True, True), (1, 8, BF, BF, True, True), (3, 1, F32, F32, True, True),
+    (17, 33, HF, HF, True, False), (300, 250, BF, F32, True, True), (200, 1000, HF, HF, False, False),
+    (65, 512, BF, F32, True, True), (129, 768, F32, F32, False, True), (77, 2048, BF, BF, True, True),
+    (300, 2048, HF, F32, True, True), (40, 2049, BF, BF, True, True), (33, 4096, BF, F32, True, True),
+    (19, 5632, HF, F32, True, True), (12, 8192, F32, F32, True, True), (9, 8200, BF, BF, True, True),
+    (5, 16384, F32, F32, True, True), (4, 16383, BF, BF, True, True), (2500, 64, BF, BF, True, True),
+    (1300, 512, BF, BF, True, True), (1300, 1024, HF, HF, True, True), (1300, 2048, BF, BF, True, True),
+    (1200, 3000, BF, BF, True, True), (2, 24, BF, BF, True, True), (1300, 250, BF, BF, True, True),
+]
+CHAIN = 160  # the longest chain of additions over a row: 128 of one thread, and the exchanges
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,H,dtype,stream,scale,bias", LN_CASES)
+@pytest.mark.parametrize("pad,skew,shift", [(0, 0, 0.0), (8, 0, 3.0), (5, 1, -20.0)])
+def test_layernorm_fwd(dev, T, H, dtype, stream, scale, bias, pad, skew, shift):
+    g = gen(dev, T + H)
+    x = rand(g, T, H, dtype=stream, scale=2.0, shift=shift, pad=pad, skew=skew)
+    w = rand(g, H, dtype=dtype, scale=0.2, shift=1.0) if scale else None
+    b = rand(g, H, dtype=dtype) if bias else None
+    buf, o = empty(dev, T, H, dtype, pad, skew)
+    given = pad or (w is None and b is None)
+    y, mean, rstd = fused.layernorm_fwd(x, w, b, EPS, out=o if given else None)
+    assert y.dtype == dtype and mean.dtype == rstd.dtype == F32 and (not given or y is o)
+    xd = x.double()
+    want, m, r, n = ln64(xd, None if w is None else w.double(), None if b is None else b.double())
+    d = xd - m
+    tol_m = CHAIN * U * xd.abs().mean(-1, keepdim=True)
+    # the mean's error moves the squares' mean by its square alone, the rounding of x - mean by 2 u
+    var = d.square().mean(-1, keepdim=True)
+    tol_r = r * (((CHAIN + 6) * U * var + tol_m ** 2) / (2 * (var + EPS)) + 4 * U)
+    tol = d.abs() * tol_r + r * (tol_m + 4 * U * d.abs())
+    if w is not None:
+        tol = tol * w.double().abs() + U * want.abs()
+    if b is not None:
+        tol = tol + U * (want.abs() + b.double().abs())
+    close(mean, m[:, 0], tol_m[:, 0], "mean")
+    close(rstd, r[:, 0], tol_r[:, 0], "rstd")
+    close(y, want, tol, "y")
+    assert not given or untouched(buf, H, skew)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,H,dtype,stream,scale,bias", LN_CASES)
+@pytest.mark.parametrize("some,accumulate,res,pad,skew", [
+    (True, False, True, 0, 0), (False, True, False, 8, 0), (True, True, True, 5, 1)])
+def test_layernorm_bwd(dev, T, H, dtype, stream, scale, bias, some, accumulate, res, pad, skew):
+    g = gen(dev, T + 2 * H)
+    R = (T + 1) // 2 if some else T
+    x = rand(g, T, H, dtype=stream, scale=2.0, shift=0.5, pad=pad, skew=skew)
+    w = rand(g, H, dtype=dtype, scale=0.2, shift=1.0) if scale else None
+    dy = rand(g, R, H, dtype=dtype, pad=pad, skew=skew)
+    dres = rand(g, R, H, dtype=stream, pad=pad, skew=skew) if res else None
+    rows = kept(g, T, R) if some else None
+    _, m, r, _ = ln64(x.double(), None, None)
+    mean, rstd = m[:, 0].float(), r[:, 0].float()
+    dw, db = rand(g, H), rand(g, H) if bias else None
+    before, before_b = dw.clone(), None if db is None else db.clone()
+    dx = fused.layernorm_bwd(dy, x, mean, rstd, w, dw, db, rows=rows, dres=dres,
+                             accumulate=accumulate)
+    assert dx.dtype == stream and dx.shape == (R, H)
+    at = slice(None) if rows is None else rows.long()
+    xd, md, rd = x[at].double(), mean[at].double()[:, None], rstd[at].double()[:, None]
+    n, dyd = (xd - md) * rd, dy.double()
+    gr = dyd if w is None else dyd * w.double()
+    m1, m2 = gr.mean(-1, keepdim=True), (gr * n).mean(-1, keepdim=True)
+    want = rd * (gr - m1 - n * m2)
+    k = (CHAIN + 6) * U
+    tol = rd * (k * gr.abs().mean(-1, keepdim=True) + n.abs() * k * (gr * n).abs().mean(-1, keepdim=True)
+                + 6 * U * (gr.abs() + m1.abs() + (n * m2).abs()))
+    if res:
+        want = want + dres.double()
+        tol = tol + U * (want.abs() + dres.double().abs())
+    close(dx, want, tol, "dx")
+    for name, got, old, s in (("dw", dw, before, dyd * n), ("db", db, before_b, dyd)):
+        if got is None:
+            continue
+        want, tol = s.sum(0), (R + 6) * U * s.abs().sum(0)
+        if accumulate:
+            want = want + old.double()
+            tol = tol + U * want.abs()
+        close(got, want, tol, name)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_layernorm_gradient_against_differences(dev):
+    g = gen(dev, 8)
+    T, H, h = 6, 40, 2.0 ** -10
+    x, dy = rand(g, T, H), rand(g, T, H)
+    w, b = rand(g, H), rand(g, H)
+    _, mean, rstd = fused.layernorm_fwd(x, w, b, EPS)
+    dw, db = torch.empty(H, device=dev), torch.empty(H, device=dev)
+    dx = fused.layernorm_bwd(dy, x, mean, rstd, w, dw, db, accumulate=False)
+
+    def total(xx, ww, bb):
+        return float((ln64(xx, ww, bb)[0] * dy.double()).sum())
+
+    leaves = [x.double(), w.double(), b.double()]
+    for i, grad in enumerate((dx, dw, db)):
+        d = rand(g, *leaves[i].shape).double()
+        up, down = list(leaves), list(leaves)
+        up[i], down[i] = leaves[i] + h * d, leaves[i] - h * d
+        slope = (total(*up) - total(*down)) / (2 * h)
+        # the difference's own error is h^2 / 6 of a third derivative that stays below 1e3 here
+        assert abs(float((grad.double() * d).sum()) - slope) < 1e3 * h * h + 1e-4
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_layernorm_odd_rows(dev):
+    """Constant rows, values far from zero, infinities and NaN; without rows and without columns."""
+    g = gen(dev, 5)
+    x = rand(g, 40, 96)
+    x[1], x[2], x[3, 4], x[4, 5] = 7.0, 0.0, float("nan"), float("inf")
+    x[6] = x[6] * 1e-3 + 1e4
+    w, b = torch.ones(96, device=dev), torch.zeros(96, device=dev)
+    y, mean, rstd = fused.layernorm_fwd(x, w, b, EPS)
+    assert not y[1:3].any() and bool(y[3].isnan().all()) and not bool(y[4].isfinite().all())
+    # steps of the values at 1e4 are 2^-10: the mean's error of CHAIN u 1e4 is what is left
+    want = ln64(x[6].double(), None, None)[0]
+    close(y[6], want, 1e4 * CHAIN * U * rstd[6].double() * (1 + want.abs()) + 1e-3, "far from zero")
+    dx = fused.layernorm_bwd(torch.ones_like(x), x, mean, rstd, w, None, None)
+    assert bool(dx[1:3].abs().max() < 1e-2) and bool(dx[3].isnan().all())
+    assert bool(dx[7:].isfinite().all())
+    y, mean, _ = fused.layernorm_fwd(x[:0], w, b, EPS)
+    assert y.shape == (0, 96) and mean.shape == (0,)
+    dw = torch.ones(96, device=dev)
+    args = (x[:0], x[:0], mean, mean, w)
+    assert fused.layernorm_bwd(*args, dw, None).shape == (0, 96) and bool((dw == 1.0).all())
+    fused.layernorm_bwd(*args, dw, None, accumulate=False)
+    assert not dw.any()
+    assert fused.layernorm_fwd(x[:, :0], w[:0], b[:0], EPS)[0].shape == (40, 0)
+
+
+# ---------------------------------------------------------------- distillation
+def distill_case(dev, T, V, K, dtype, top_dtype=F32, tail=True, labels=True, tau=1.0, pad=0, skew=0,
+                 ids64=False, seed=0):
+    g = gen(dev, T + V + K + seed)
+    c = {"logits": rand(g, T, V, dtype=dtype, scale=2.5, pad=pad, skew=skew), "temperature": tau}
+    teacher = c["logits"].float() + rand(g, T, V, scale=0.7)
+    top, ids = teacher.topk(K, dim=1)
+    c["top_lse"] = (teacher.double() / tau).logsumexp(1).float() if tail else None
+    # rows of other lists: short ones, an empty one, a token twice, a share of nothing
+    if T > 2 and K > 2:
+        ids[1, 1:], ids[2] = -1, -5
+    if T > 5 and K > 3:
+        ids[3, 2], top[4, 1], top[5, -1] = ids[3, 0], -math.inf, -80.0
+    c["top_ids"] = ids if ids64 else ids.int()
+    c["top_logits"] = top.to(top_dtype)
+    c["labels"] = None
+    if labels:
+        lab = torch.randint(0, V, (T,), generator=g, device=dev)
+        lab[::3] = c["top_ids"][::3, 0].long()  # (negative where the list is empty)
+        lab[T // 2] = -100
+        c["labels"] = lab
+    return g, c
+
+
+def distill64(c, z=None):
+    """kd and ce from a dense distribution of the teacher, in 64 bits and differentiable in z."""
+    z = c["logits"].double() if z is None else z
+    T, V = z.shape
+    ids, ok = c["top_ids"].long(), c["top_ids"] >= 0
+    logq = torch.log_softmax(z / c["temperature"], 1)
+    t = (c["top_logits"].double() / c["temperature"]).masked_fill(~ok, -math.inf)
+    norm = t.logsumexp(1) if c["top_lse"] is None else c["top_lse"].double()
+    p = torch.exp(t - norm.masked_fill(norm == -math.inf, 0.0)[:, None])
+    named = (t - norm[:, None]).masked_fill(p == 0, 0.0)
+    kd = (p * (named - torch.where(p > 0, logq.gather(1, ids.clamp(min=0)), named))).sum(1)
+    if c["top_lse"] is not None:
+        inside = torch.zeros(T, V + 1, dtype=torch.bool, device=z.device)
+        inside = inside.scatter(1, ids.masked_fill(~ok, V), True)[:, :V]
+        rest = logq.masked_fill(inside, -math.inf).logsumexp(1)
+        left = (1 - p.sum(1)).clamp(min=0)
+        kd = kd + torch.where((left > 0) & ~inside.all(1),
+                              left * (left.clamp(min=1e-300).log() - rest), 0.0)
+    if c["labels"] is None:
+        return kd, None
+    ce = -torch.log_softmax(z, 1).gather(1, c["labels"].clamp(min=0)[:, None])[:, 0]
+    return kd, ce.masked_fill(c["labels"] < 0, 0.0)
+
+
+def log_error(z, tau):
+    """The error of a log of a sum of exponentials (fp32, the hardware's exponential): its argument is
+    rounded (|x| up to the range of the row, where it counts up to 64 binary orders), 2^-22 of the
+    exponential, a chain of 200 additions."""
+    return 2.0 ** -22 + (64 + 200) * U + 3 * U * (z.double() / tau).abs().amax(1)
+
+
+DISTILL = [
+    (40, 64, 4, BF, F32, 1.0, 0, 0), (1, 33, 1, F32, F32, 1.0, 0, 0), (9, 1024, 8, BF, BF, 2.0, 0, 0),
+    (30, 1000, 16, HF, F32, 0.7, 8, 0), (17, 5003, 33, BF, F32, 2.0, 0, 0),
+    (12, 8193, 64, F32, F32, 1.5, 3, 2), (6, 40000, 100, BF, HF, 1.0, 5, 1),
+    (3, 128256, 64, F32, F32, 2.0, 0, 0), (700, 300, 5, BF, F32, 1.0, 1, 1), (8, 7, 7, F32, F32, 1.0, 0, 0),
+    (7, 1200, 1024, BF, F32, 0.7, 0, 0), (650, 9000, 40, HF, F32, 1.0, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,V,K,dtype,top_dtype,tau,pad,skew", DISTILL)
+@pytest.mark.parametrize("tail,labels,ids64", [(False, False, True), (True, True, False),
+                                               (False, True, False), (True, False, True)])
+def test_distill_fwd(dev, T, V, K, dtype, top_dtype, tau, pad, skew, tail, labels, ids64):
+    _, c = distill_case(dev, T, V, K, dtype, top_dtype, tail, labels, tau, pad, skew, ids64)
+    kd, ce, lse, stats = fused.distill_fwd(**c)
+    want_kd, want_ce = distill64(c)
+    z = c["logits"].double()
+    err = log_error(z, tau)
+    # the teacher's side is in 64 bits; the two logarithms and the list's logits times the temperature
+    # carry their errors into sums whose weights add up to at most one
+    close(kd, want_kd, 3 * err, "kd")
+    want = torch.logsumexp(z / tau, 1)
+    close(stats[:, 0], want, err, "lse at the temperature")
+    if not tail:
+        some = (c["top_ids"] >= 0).any(1)
+        assert torch.equal(stats[:, 1], stats[:, 0]) and torch.equal(stats[:, 2] == 1.0, some)
+    assert (ce is None) == (lse is None) == (not labels)
+    if labels:
+        close(lse, torch.logsumexp(z, 1), log_error(z, 1.0), "lse")
+        close(ce, want_ce, 2 * log_error(z, 1.0), "ce")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,V,K,dtype,top_dtype,tau,pad,skew", DISTILL)
+@pytest.mark.parametrize("tail,labels,some,ids64", [
+    (False, False, True, True), (True, True, False, False), (False, True, True, False),
+    (True, False, False, True)])
+def test_distill_bwd(dev, T, V, K, dtype, top_dtype, tau, pad, skew, tail, labels, some, ids64):
+    g, c = distill_case(dev, T, V, K, dtype, top_dtype, tail, labels, tau, pad, skew, ids64)
+    _, _, lse, stats = fused.distill_fwd(**c)
+    R = (2 * T + 2) // 3 if some else T
+    rows = kept(g, T, R) if some else None
+    at = slice(None) if rows is None else rows.long()
+    dkd = rand(g, R)
+    dce = rand(g, R) if labels else None
+    dkd[R // 2] = 0.0
+    buf, o = empty(dev, R, V, dtype, pad, skew)
+    args = {k: c[k] for k in ("logits", "top_ids", "top_logits", "temperature", "labels")}
+    got = fused.distill_bwd(**args, stats=stats, lse=lse, dkd=dkd, dce=dce, rows=rows,
+                            out=o if pad else None)
+    assert got.dtype == dtype and got.shape == (R, V) and (not pad or got is o)
+    z = c["logits"].double().requires_grad_()
+    kd, ce = distill64(c, z)
+    total = (kd[at] * dkd.double()).sum()
+    soft = torch.zeros((), dtype=F64, device=dev)
+    if labels:
+        total = total + (ce[at] * dce.double()).sum()
+        w = dce.double().masked_fill(c["labels"][at] < 0, 0.0).abs()[:, None]
+        soft = torch.softmax(z.detach(), 1)[at] * w
+    want = torch.autograd.grad(total, z)[0][at]
+    # each term is a product with an exponential whose argument is off by the error of a logarithm
+    # and its own rounding; `mass` is the sum of the terms' sizes
+    zd = z.detach()[at]
+    k = dkd.double().abs()[:, None] / tau
+    q = torch.softmax(zd / tau, 1)
+    named = torch.zeros(R, V + 1, dtype=F64, device=dev)
+    ids = c["top_ids"].long()[at]
+    t = c["top_logits"].double()[at] / tau
+    p = torch.exp(t - stats[at, 3:4].double()).masked_fill(ids < 0, 0.0)
+    p = p.masked_fill(p.isnan(), 0.0)
+    named.scatter_add_(1, ids.masked_fill(ids < 0, V), p)
+    inside = torch.zeros_like(named).scatter_(1, ids.masked_fill(ids < 0, V), 1.0)[:, :V].bool()
+    rest = q.masked_fill(inside, 0.0).sum(1, keepdim=True)
+    left = (1 - p.sum(1, keepdim=True)).clamp(min=0) if tail else torch.zeros_like(rest)
+    share = (q / rest.clamp(min=1e-300)).masked_fill(inside, 0.0)
+    mass = k * (q + named[:, :V] + share * (rest + left)) + 2 * soft
+    err = (4 * log_error(zd, min(tau, 1.0)) + 2.0 ** -21)[:, None]
+    norm = 2 * U * stats[at, 3:4].double().abs().masked_fill(stats[at, 3:4].isinf(), 0.0)
+    close(got, want, (err + norm) * mass + 2 * U * (dce.double().abs()[:, None] if labels else 0.0),
+          "dlogits")
+    assert not pad or untouched(buf, V, skew)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("tail", [False, True])
+def test_distill_gradient_against_differences(dev, tail):
+    g, c = distill_case(dev, 7, 50, 6, F32, tail=tail, tau=1.5, seed=3)
+    kd, ce, lse, stats = fused.distill_fwd(**c)
+    dkd, dce = rand(g, 7), rand(g, 7)
+    args = {k: c[k] for k in ("logits", "top_ids", "top_logits", "temperature", "labels")}
+    grad = fused.distill_bwd(**args, stats=stats, lse=lse, dkd=dkd, dce=dce)
+    d, h = rand(g, 7, 50).double(), 2.0 ** -10
+    z = c["logits"].double()
+
+    def total(at):
+        a, b = distill64(c, at)
+        return float((a * dkd.double()).sum() + (b * dce.double()).sum())
+
+    slope = (total(z + h * d) - total(z - h * d)) / (2 * h)
+    assert abs(float((grad.double() * d).sum()) - slope) < 100 * h * h + 1e-4
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_distill_odd_rows(dev):
+    """Masked logits, rows of which nothing is left, weights of zero, lists over the whole vocabulary."""
+    g, c = distill_case(dev, 8, 96, 5, F32, tail=False, labels=True)
+    z = c["logits"]
+    c["top_ids"][6] = torch.arange(5, device=dev)
+    z[6, 50:] = -math.inf  # masked, and nothing of the list
+    c["labels"][:] = torch.arange(8, device=dev)
+    z[7, c["top_ids"][7, 0].long()] = -math.inf  # a named token that the student rules out
+    c["labels"][7] = int(c["top_ids"][7, 1])
+    z[5] = -math.inf  # nothing is left
+    z[4, 3] = float("nan")
+    kd, ce, lse, stats = fused.distill_fwd(**c)
+    assert bool(kd[6].isfinite()) and bool(kd[7] == math.inf) and bool(ce[:4].isfinite().all())
+    assert not bool(kd[5].isfinite()) and bool(kd[4].isnan()) and bool(ce[4].isnan())
+    dkd, dce = torch.ones(8, device=dev), torch.ones(8, device=dev)
+    dkd[4:6] = dce[4:6] = 0.0  # weights of zero, whatever the rows hold
+    args = {k: c[k] for k in ("logits", "top_ids", "top_logits", "temperature", "labels")}
+    got = fused.distill_bwd(**args, stats=stats, lse=lse, dkd=dkd, dce=dce)
+    assert bool(got.isfinite().all()) and not got[4:6].any() and not got[6, 50:].any()
+    # the gradient of a softmax adds up to nothing, the infinite divergence's too
+    assert float(got.double().sum(1).abs().max()) < 1e-5
+    # a list over the whole vocabulary leaves nothing for the rest
+    ids = torch.arange(96, device=dev, dtype=torch.int32).repeat(8, 1)
+    z = rand(g, 8, 96)
+    t = rand(g, 8, 96)
+    kd, _, _, stats = fused.distill_fwd(z, ids, t, top_lse=t.double().logsumexp(1).float())
+    p = torch.softmax(t.double(), 1)
+    want = (p * (p.log() - torch.log_softmax(z.double(), 1))).sum(1)
+    close(kd, want, 4 * log_error(z, 1.0) + 8 * U * t.double().abs().amax(1), "whole vocabulary")
+    assert bool((stats[:, 1] == -math.inf).all()) and not stats[:, 2].any()
+    got = fused.distill_bwd(z, ids, t, stats, torch.ones(8, device=dev))
+    want = torch.softmax(z.double(), 1) - p
+    close(got, want, 1e-5 * (want.abs() + 2 * p), "whole vocabulary's gradient")
+    # without rows
+    kd, ce, lse, stats = fused.distill_fwd(z[:0], ids[:0], t[:0], labels=c["labels"][:0])
+    assert kd.shape == ce.shape == lse.shape == (0,) and stats.shape == (0, 4)
+    rows = torch.empty(0, dtype=torch.int32, device=dev)
+    full = fused.distill_fwd(z, ids, t)[3]
+    assert fused.distill_bwd(z, ids, t, full, torch.empty(0, device=dev), rows=rows).shape == (0, 96)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("V,dtype", [(512, BF), (515, F32), (40000, BF)])
+def test_distill_bwd_in_place(dev, V, dtype):
+    g, c = distill_case(dev, 6, V, 9, dtype, tau=2.0)
+    _, _, lse, stats = fused.distill_fwd(**c)
+    args = {k: c[k] for k in ("logits", "top_ids", "top_logits", "temperature", "labels")}
+    args.update(stats=stats, lse=lse, dkd=rand(g, 6), dce=rand(g, 6))
+    want = fused.distill_bwd(**args)
+    assert torch.equal(fused.distill_bwd(**args, out=c["logits"]), want)
+
+
+def test_distill_definition_against_torch():
+    """Without the teacher's tail the gradient is that of torch's divergence to a dense teacher."""
+    g, c = distill_case("cpu", 5, 40, 40, F32, tail=False, labels=False, tau=2.0, seed=1)
+    c["top_ids"] = torch.stack([torch.randperm(40, generator=g) for _ in range(5)]).int()
+    dense = torch.zeros(5, 40).scatter_(1, c["top_ids"].long(), c["top_logits"].float())
+    z = c["logits"].double().requires_grad_()
+    want = torch.nn.functional.kl_div(torch.log_softmax(z / 2, 1),
+                                      torch.log_softmax(dense.double() / 2, 1), log_target=True,
+                                      reduction="none").nan_to_num(0.0).sum(1)
+    kd, _, _, stats = ref.distill(c["logits"], c["top_ids"], c["top_logits"], 2.0)
+    assert torch.allclose(kd, want, rtol=1e-12, atol=1e-12)
+    got = ref.distill_bwd(c["logits"], c["top_ids"], c["top_logits"], stats, torch.ones(5), 2.0)
+    assert torch.allclose(got, torch.autograd.grad(want.sum(), z)[0], rtol=1e-10, atol=1e-12)
+
+
+# ---------------------------------------------------------------- refusals and bad indices
+def status():
+    from centrifuge_b200.ops._ext import status_block
+    s = status_block(0)
+    s[0] = 0
+    return s
+
+
+def test_bad_indices_raise_on_the_cpu():
+    x, w = torch.ones(4, 8, dtype=BF), torch.ones(8, 16, dtype=BF)
+    z = torch.ones(3, 16, dtype=BF)
+    for bad in (-1, 3):
+        rows = torch.tensor([0, 1, bad, 2], dtype=torch.int32)
+        with pytest.raises(IndexError):
+            gemm.linear_act_dgrad(x, w, z, "gelu", z_rows=rows)
+        dw = torch.ones(8)
+        with pytest.raises(IndexError):
+            fused.layernorm_bwd(x, z[:, :8], torch.zeros(3), torch.ones(3), None, dw, None, rows=rows)
+        assert bool((dw == 1.0).all())
+    logits, ids, top = torch.zeros(3, 10), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2)
+    stats = fused.distill_fwd(logits, ids, top)[3]
+    for bad in (-1, 3):
+        with pytest.raises(IndexError):
+            fused.distill_bwd(logits, ids, top, stats, torch.ones(1),
+                              rows=torch.tensor([bad], dtype=torch.int32))
+    ids[1, 1] = 10
+    with pytest.raises(IndexError):
+        fused.distill_fwd(logits, ids, top)
+    ids[1, 1] = 0
+    with pytest.raises(IndexError):
+        fused.distill_fwd(logits, ids, top, labels=torch.tensor([0, 10, -1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [16, 300, 33])
+def test_linear_dgrad_reports_bad_rows(N):
+    g = gen("cuda", N)
+    dy, w, z = rand(g, 6, 64, dtype=BF), rand(g, 64, N, dtype=BF), rand(g, 5, N, dtype=BF)
+    rows = torch.tensor([0, 4, 5, 2, -1, 1], dtype=torch.int32, device="cuda")
+    s = status()
+    got = gemm.linear_act_dgrad(dy, w, z, "gelu", z_rows=rows)
+    assert int(s[0]) == 128
+    s[0] = 0
+    good = torch.tensor([0, 1, 3, 5], device="cuda")
+    want = gemm.linear_act_dgrad(dy[good], w, z, "gelu", z_rows=rows[good])
+    assert torch.equal(got[good], want) and not got[2].any() and not got[4].any()
+    assert int(s[0]) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,dtype", [(64, BF), (512, BF), (1000, HF), (250, BF), (33, F32), (2048, BF),
+                                     (4096, F32), (16384, BF)])
+def test_layernorm_bwd_reports_bad_rows(H, dtype):
+    g = gen("cuda", H)
+    x, dy, w = rand(g, 9, H, dtype=dtype), rand(g, 5, H, dtype=dtype), rand(g, H, dtype=dtype)
+    _, mean, rstd = fused.layernorm_fwd(x, w, None, EPS)
+    dres = rand(g, 5, H, dtype=dtype)
+    rows = torch.tensor([8, 9, 0, -7, 3], dtype=torch.int32, device="cuda")
+    dw, db = torch.empty(H, device="cuda"), torch.empty(H, device="cuda")
+    s = status()
+    dx = fused.layernorm_bwd(dy, x, mean, rstd, w, dw, db, rows=rows, dres=dres, accumulate=False)
+    assert int(s[0]) == 128
+    s[0] = 0
+    good = torch.tensor([0, 2, 4], device="cuda")
+    gw, gb = torch.empty(H, device="cuda"), torch.empty(H, device="cuda")
+    want = fused.layernorm_bwd(dy[good], x, mean, rstd, w, gw, gb, rows=rows[good], dres=dres[good],
+                               accumulate=False)
+    assert int(s[0]) == 0 and torch.equal(dx[good], want) and not dx[1].any() and not dx[3].any()
+    # the rows may be summed in another order: three of them, and the additions of zeros
+    assert torch.allclose(dw, gw, rtol=0, atol=float(8 * U * gw.abs().max() + 8 * U * dy.abs().sum()))
+    assert torch.allclose(db, gb, rtol=0, atol=float(8 * U * dy.float().abs().sum(0).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [64, 9001])
+def test_distill_reports_bad_indices(V):
+    g, c = distill_case("cuda", 6, V, 4, BF, tail=True, labels=True)
+    c["labels"] = torch.arange(6, device="cuda")
+    fine = {**c, "top_ids": c["top_ids"].clone(), "labels": c["labels"].clone()}
+    c["top_ids"][0, 2], c["labels"][3] = V, V + 7
+    fine["top_ids"][0, 2], fine["labels"][3] = -1, -1
+    s = status()
+    got = fused.distill_fwd(**c)
+    assert int(s[0]) == 128
+    s[0] = 0
+    want = fused.distill_fwd(**fine)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    dkd, dce = rand(g, 3), rand(g, 3)
+    rows = torch.tensor([0, 6, 3], dtype=torch.int32, device="cuda")
+    args = [{k: t[k] for k in ("logits", "top_ids", "top_logits", "temperature", "labels")}
+            for t in (c, fine)]
+    kw = dict(stats=want[3], lse=want[2])
+    a = fused.distill_bwd(**args[0], **kw, dkd=dkd, dce=dce, rows=rows)
+    assert int(s[0]) == 128
+    s[0] = 0
+    at = torch.tensor([0, 2], device="cuda")
+    b = fused.distill_bwd(**args[1], **kw, dkd=dkd[at], dce=dce[at], rows=rows[at])
+    assert int(s[0]) == 0 and torch.equal(a[at], b) and not a[1].any()
+
+
+def linear_refusals(dev):
+    def t(*shape, dtype=BF):
+        return torch.zeros(*shape, dtype=dtype, device=dev)
+
+    x, w, z = t(8, 16), t(24, 16), t(8, 24)
+    buf = t(8, 64)
+    i32 = torch.zeros(8, dtype=torch.int32, device=dev)
+    fwd, dgrad, wgrad = gemm.linear_act_fwd, gemm.linear_act_dgrad, gemm.linear_bias_wgrad
+    return [
+        lambda: fwd(x, w, act="tanh"), lambda: fwd(x.long(), w), lambda: fwd(x, w.half()),
+        lambda: fwd(x, t(24, 15)), lambda: fwd(x.view(-1), w), lambda: fwd(x, w, bias=t(23)),
+        lambda: fwd(x, w, bias=t(24, dtype=F32)), lambda: fwd(x, w, bias=t(48)[::2]),
+        lambda: fwd(x, w, resid=t(8, 23)), lambda: fwd(x, w, out=t(7, 24)),
+        lambda: fwd(x, w, out=t(8, 24, dtype=F32)), lambda: fwd(x, w, z=t(8, 24, dtype=HF)),
+        lambda: fwd(x[:, :0], w[:, :0]), lambda: fwd(x.t(), t(24, 8)),
+        lambda: fwd(x, w, out=z, z=z), lambda: fwd(buf[:, :16], w, out=buf[:, 8:32]),
+        lambda: fwd(x, w, resid=buf[:, :24], out=buf[:, 8:32]),
+        lambda: fwd(x, w, resid=z, z=z),
+        lambda: dgrad(z, w, x, "swish"), lambda: dgrad(z, w, t(7, 16), "gelu"),
+        lambda: dgrad(z, w, x, "gelu", z_rows=i32[:7]), lambda: dgrad(z, w, x, "gelu", z_rows=i32.long()),
+        lambda: dgrad(z, w, x.half(), "gelu"), lambda: dgrad(z, w, x, "gelu", z_rows=i32, out=x),
+        lambda: dgrad(z, w, x, "gelu", out=t(8, 24)), lambda: dgrad(z, t(23, 16), x, "gelu"),
+        lambda: dgrad(z, w, t(8, 17), "gelu"),
+        lambda: dgrad(buf[:, :24], w, x, "gelu", out=buf[:, 8:24]),
+        lambda: wgrad(z, x, t(24, 16)), lambda: wgrad(z, x, t(16, 24, dtype=F32)),
+        lambda: wgrad(z, t(7, 16), t(24, 16, dtype=F32)),
+        lambda: wgrad(z, x, t(24, 16, dtype=F32), t(16, dtype=F32)),
+        lambda: wgrad(z, x, t(24, 16, dtype=F32), t(24)),
+        lambda: (lambda d: wgrad(z, x, d, d.view(-1)[:24]))(t(24, 16, dtype=F32)),
+        lambda: (lambda d: wgrad(d.view(BF)[:8, :24], x, d))(t(24, 16, dtype=F32)),
+    ]
+
+
+def layernorm_refusals(dev):
+    def t(*shape, dtype=F32):
+        return torch.zeros(*shape, dtype=dtype, device=dev)
+
+    x, w, s = t(6, 32, dtype=BF), t(32, dtype=BF), t(6)
+    dw = t(32)
+    i32 = torch.zeros(6, dtype=torch.int32, device=dev)
+    fwd, bwd = fused.layernorm_fwd, fused.layernorm_bwd
+    return [
+        lambda: fwd(x.view(-1), w, None, EPS), lambda: fwd(x, t(31, dtype=BF), None, EPS),
+        lambda: fwd(x, w, t(32), EPS), lambda: fwd(x, t(32), None, EPS), lambda: fwd(x.long(), None, None, EPS),
+        lambda: fwd(x, w, None, EPS, out=x), lambda: fwd(x, w, None, EPS, out=t(6, 32)),
+        lambda: fwd(x.t(), t(6, dtype=BF), None, EPS), lambda: fwd(t(2, 16385), None, None, EPS),
+        lambda: fwd(x, w, None, EPS, out=t(5, 32, dtype=BF)), lambda: fwd(x, t(64, dtype=BF)[::2], None, EPS),
+        lambda: bwd(x[:5], x, s, s, w, dw, None), lambda: bwd(x, x.half(), s, s, w, dw, None),
+        lambda: bwd(x, x, s[:5], s, w, dw, None), lambda: bwd(x, x, s, s.double(), w, dw, None),
+        lambda: bwd(x, x, s, s, t(32), dw, None), lambda: bwd(x, x, s, s, w, t(33), None),
+        lambda: bwd(x, x, s, s, w, w, None), lambda: bwd(x, x, s, s, w, dw, dw),
+        lambda: bwd(x, x, s, s, w, dw, None, dres=t(6, 32)),
+        lambda: bwd(x, x, s, s, w, dw, None, rows=i32[:5]),
+        lambda: bwd(x, x, s, s, w, dw, None, rows=i32.long()),
+        lambda: (lambda d: bwd(x, x, d[:6], s, w, d, None))(t(32)),
+        lambda: (lambda d: bwd(x, d, s, s, w, d[0], None))(t(6, 32)),
+    ]
+
+
+def distill_refusals(dev):
+    def t(*shape, dtype=F32):
+        return torch.zeros(*shape, dtype=dtype, device=dev)
+
+    z, ids, top, lab = t(6, 40), t(6, 4, dtype=torch.int32), t(6, 4), t(6, dtype=torch.long)
+    st, one = t(6, 4), t(6)
+    i32 = t(6, dtype=torch.int32)
+    fwd, bwd = fused.distill_fwd, fused.distill_bwd
+    return [
+        lambda: fwd(z.view(-1), ids, top), lambda: fwd(z.double(), ids, top), lambda: fwd(z, top, top),
+        lambda: fwd(z, ids[:5], top), lambda: fwd(z, ids, top[:, :3]), lambda: fwd(z, ids, top, 0.0),
+        lambda: fwd(z, ids, top, -1.0), lambda: fwd(z, ids, top, math.inf), lambda: fwd(z, ids, top, math.nan),
+        lambda: fwd(z, ids, top, top_lse=one[:5]), lambda: fwd(z, ids, top, top_lse=one.double()),
+        lambda: fwd(z, ids, top, labels=i32), lambda: fwd(z, ids, top, labels=lab[:5]),
+        lambda: fwd(z, ids[:, :0], top[:, :0]), lambda: fwd(z[:, :0], ids, top),
+        lambda: fwd(z, t(6, 1025, dtype=torch.int32), t(6, 1025)), lambda: fwd(z, ids, lab.view(6, 1)),
+        lambda: fwd(t(1, (1 << 20) + 1, dtype=BF), ids[:1], top[:1]),
+        lambda: fwd(z, ids.t().contiguous().t(), top),
+        lambda: bwd(z, ids, top, st[:5], one), lambda: bwd(z, ids, top, st, one[:5]),
+        lambda: bwd(z, ids, top, st, one.half()), lambda: bwd(z, ids, top, st, one, labels=lab),
+        lambda: bwd(z, ids, top, st, one, labels=lab, lse=one), lambda: bwd(z, ids, top, st, one, dce=one),
+        lambda: bwd(z, ids, top, st, one, labels=lab, lse=one, dce=one[:5]),
+        lambda: bwd(z, ids, top, st, one, rows=i32[:5]), lambda: bwd(z, ids, top, st, one, rows=lab),
+        lambda: bwd(z, ids, top, st, one, rows=i32, out=z), lambda: bwd(z, ids, top, st, one, out=t(6, 39)),
+        lambda: bwd(z, ids, top, st, one, out=t(6, 40, dtype=BF)),
+        lambda: (lambda b: bwd(b[:, :40], ids, top, st, one, out=b[:, 8:48]))(t(6, 64)),
+    ]
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("calls", [linear_refusals, layernorm_refusals, distill_refusals])
+def test_refusals(dev, calls):
+    for i, call in enumerate(calls(dev)):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.gpu
+def test_another_device_is_refused():
+    x, w = torch.zeros(4, 16, dtype=BF, device="cuda"), torch.zeros(8, 16, dtype=BF)
+    with pytest.raises(ValueError):
+        gemm.linear_act_fwd(x, w)
+    with pytest.raises(ValueError):
+        gemm.linear_bias_wgrad(x, x, torch.zeros(16, 16))
+    with pytest.raises(ValueError):
+        fused.layernorm_fwd(x, w[0], None, EPS)
+    with pytest.raises(ValueError):
+        fused.distill_fwd(x, torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2, device="cuda"))
