@@ -1129,6 +1129,22 @@ int make_tmap_2d_bf16(CUtensorMap* map, const void* ptr, long long rows, long lo
   return r == CUDA_SUCCESS ? 0 : -2;
 }
 
+// The same matrix (cols a multiple of 64) as {64 columns, rows, groups of 64 columns}: a box is
+// `box_chunks` groups of 64 columns x `box_rows` rows, one group after the other.
+int make_tmap_3d_bf16(CUtensorMap* map, const void* ptr, long long rows, long long cols,
+                      long long ld, int box_rows, int box_chunks) {
+  auto fn = get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[3] = {64, static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(cols / 64)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * 2), 128};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_rows), static_cast<cuuint32_t>(box_chunks)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -2;
+}
+
 static int num_sms() {
   static int n = 0;
   if (n == 0) {

@@ -18,37 +18,51 @@ namespace cfb {
 
 int make_tmap_2d_bf16(CUtensorMap* map, const void* ptr, long long rows, long long cols,
                       long long ld, int box_cols, int box_rows);
+int make_tmap_3d_bf16(CUtensorMap* map, const void* ptr, long long rows, long long cols,
+                      long long ld, int box_rows, int box_chunks);
 
 // ---------------------------------------------------------------- activations
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// On pairs of fp32: an epilogue of 128 x 256 elements has to end while the next tile's products run,
+// and its arithmetic is most of it.
+__device__ __forceinline__ F2 ex2_2(F2 x) {
+  const float2 v = halves(x);
+  float lo, hi;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(v.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(v.y));
+  return f2(lo, hi);
+}
+__device__ __forceinline__ F2 inv_2(F2 x) {
+  const float2 v = halves(x);
+  float lo, hi;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(lo) : "f"(v.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(hi) : "f"(v.y));
+  return f2(lo, hi);
+}
+template <typename F>
+__device__ __forceinline__ F2 each(F2 x, F&& f) {
+  const float2 v = halves(x);
+  return f2(f(v.x), f(v.y));
 }
 // 1 / (1 + 2^x), 0 for large x
-__device__ __forceinline__ float inv_1p_exp2(float x) {
-  return __fdividef(1.f, 1.f + exp2_fast(x));
-}
+__device__ __forceinline__ F2 inv_1p_exp2(F2 x) { return inv_2(ex2_2(x) + f2(1.f)); }
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The normal distribution's mass below z, and its density times sqrt(2 pi).  With a = |z| the mass
-// beyond a is exp(-a^2 / 2) t P(t), t = 1 / (1 + 0.27 a): P is a minimax fit of
-// erfcx(a / sqrt 2) / (2 t) of degree six with a relative error of 1.2e-6, so the small values of
-// the tail are as exact as the others (1 + erf(z / sqrt 2) loses them).
-__device__ __forceinline__ float normal_mass(float z, float& bell) {
-  const float a = fabsf(z);
-  const float t = __fdividef(1.f, fmaf(0.27f, a, 1.f));
-  float p = -0.060966506600379944f;
-  p = fmaf(p, t, 0.1590183675289154f);
-  p = fmaf(p, t, -0.025057457387447357f);
-  p = fmaf(p, t, 0.11830243468284607f);
-  p = fmaf(p, t, 0.09249885380268097f);
-  p = fmaf(p, t, 0.10852396488189697f);
-  p = fmaf(p, t, 0.10767974704504013f);
-  bell = exp2_fast(z * z * (-0.5f * kLog2e));
-  const float tail = bell * t * p;
-  return z < 0.f ? tail : 1.f - tail;
+// The normal distribution's mass beyond a = |z|, and its density times sqrt(2 pi): exp(-a^2 / 2) t P(t)
+// with t = 1 / (1 + 0.27 a), where P is a minimax fit of erfcx(a / sqrt 2) / (2 t) of degree six with a
+// relative error of 1.2e-6, so that small values are as exact as the others (1 + erf(z / sqrt 2) loses
+// them).  a is cut off at 30, far behind the last one whose mass is not zero.
+__device__ __forceinline__ F2 normal_tail(F2 z, F2& a, F2& bell) {
+  a = each(z, [](float v) { return fminf(fabsf(v), 30.f); });
+  const F2 t = inv_2(fma2(f2(0.27f), a, f2(1.f)));
+  F2 p = fma2(f2(-0.060966506600379944f), t, f2(0.1590183675289154f));
+  p = fma2(p, t, f2(-0.025057457387447357f));
+  p = fma2(p, t, f2(0.11830243468284607f));
+  p = fma2(p, t, f2(0.09249885380268097f));
+  p = fma2(p, t, f2(0.10852396488189697f));
+  p = fma2(p, t, f2(0.10767974704504013f));
+  bell = ex2_2(z * z * f2(-0.5f * kLog2e));
+  return bell * t * p;
 }
 
 // gelu by tanh is z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
@@ -56,36 +70,43 @@ constexpr float kGelu1 = -2.f * 0.7978845608028654f * kLog2e;
 constexpr float kGelu3 = kGelu1 * 0.044715f;
 
 template <int ACT>
-__device__ __forceinline__ float act_of(float z) {
-  if constexpr (ACT == kActRelu) return z < 0.f ? 0.f : z;
-  if constexpr (ACT == kActSilu) return z * inv_1p_exp2(-kLog2e * z);
-  if constexpr (ACT == kActGelu) {
-    float bell;
-    return z * normal_mass(z, bell);
+__device__ __forceinline__ F2 act_of(F2 z) {
+  if constexpr (ACT == kActRelu) return each(z, [](float v) { return v < 0.f ? 0.f : v; });
+  if constexpr (ACT == kActSilu) return z * inv_1p_exp2(z * f2(-kLog2e));
+  if constexpr (ACT == kActGelu) {  // z minus the mass above it, or z times the mass below it
+    F2 a, bell;
+    const F2 tail = normal_tail(z, a, bell);
+    return fma2(a * f2(-1.f), tail, each(z, [](float v) { return fmaxf(v, 0.f); }));
   }
-  if constexpr (ACT == kActGeluTanh) return z * inv_1p_exp2(z * fmaf(kGelu3, z * z, kGelu1));
+  if constexpr (ACT == kActGeluTanh)
+    return z * inv_1p_exp2(z * fma2(f2(kGelu3), z * z, f2(kGelu1)));
   return z;
 }
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  if constexpr (ACT == kActRelu) return z > 0.f ? 1.f : z != z ? z : 0.f;
+__device__ __forceinline__ F2 act_slope(F2 z) {
+  if constexpr (ACT == kActRelu)
+    return each(z, [](float v) { return v > 0.f ? 1.f : v != v ? v : 0.f; });
   if constexpr (ACT == kActSilu) {
-    const float p = inv_1p_exp2(-kLog2e * z);
-    return p * fmaf(z, 1.f - p, 1.f);
+    const F2 p = inv_1p_exp2(z * f2(-kLog2e));
+    return p * fma2(z, fma2(p, f2(-1.f), f2(1.f)), f2(1.f));
   }
   if constexpr (ACT == kActGelu) {
-    float bell;
-    const float mass = normal_mass(z, bell);
-    return fmaf(z * 0.3989422804014327f, bell, mass);
+    F2 a, bell;
+    const F2 tail = normal_tail(z, a, bell);
+    const float2 v = halves(z), lo = halves(tail), hi = halves(fma2(tail, f2(-1.f), f2(1.f)));
+    return fma2(z * f2(0.3989422804014327f), bell,
+                f2(v.x < 0.f ? lo.x : hi.x, v.y < 0.f ? lo.y : hi.y));
   }
   if constexpr (ACT == kActGeluTanh) {
     // the second term is zero long before |z| = 30, beyond which z^3 may be infinite
-    const float c = z != z ? z : fminf(fmaxf(z, -30.f), 30.f);
-    const float p = inv_1p_exp2(c * fmaf(kGelu3, c * c, kGelu1));
-    const float du = 2.f * 0.7978845608028654f * fmaf(3.f * 0.044715f, c * c, 1.f);
-    return p + c * p * (1.f - p) * du;
+    const F2 c = each(z, [](float v) { return v != v ? v : fminf(fmaxf(v, -30.f), 30.f); });
+    const F2 sq = c * c;
+    const F2 p = inv_1p_exp2(c * fma2(f2(kGelu3), sq, f2(kGelu1)));
+    constexpr float k = 2.f * 0.7978845608028654f;
+    const F2 du = fma2(f2(3.f * 0.044715f * k), sq, f2(k));
+    return fma2(c * p * fma2(p, f2(-1.f), f2(1.f)), du, p);
   }
-  return 1.f;
+  return f2(1.f);
 }
 // f(ActTag<ACT>): one uniform branch for a whole chunk of columns
 template <int ACT>
@@ -107,7 +128,10 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 struct LinearArgs {
   int M, N, K;
   int a_mn, b_mn;   // operands [K, M], [K, N] in memory instead of [M, K], [N, K]
+  int a_3d, b_3d;   // ... whose tiles one copy brings: {64 columns, k, groups of 64 columns}
   uint32_t idesc;   // instruction descriptor: shape, types and layouts
+  int full;         // units below this are whole tiles, the others pieces of the tiles behind them
+  int pieces;       // pieces a tile
   void* D;
   long long ldd;
   const void* bias;  // [N]
@@ -119,9 +143,11 @@ struct LinearArgs {
   long long n_z;
   int act;
   int add;           // wgrad: add to D
-  int vec;           // the outputs, R and Z allow 16-byte accesses
+  int vec;           // what the outputs, R and Z allow: kRows32, kRows16 or kRowsAny
   int* err;
 };
+// Rows on 32 bytes (every lane reads and writes whole sectors of its row), on 16, or anywhere.
+enum { kRowsAny = 0, kRows16 = 1, kRows32 = 2 };
 
 // CG CTAs on neighbouring SMs share a tile of CG * 128 rows and BN columns.
 template <int CG, int BN>
@@ -131,10 +157,19 @@ struct TileShape {
   static constexpr int A_BYTES = BM * BK * 2, B_BYTES = B_ROWS * BK * 2;
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
   static constexpr int STAGES = 196608 / STAGE_BYTES;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int OUT_BYTES = 4096;  // of each epilogue warp: 32 rows on their way out or in
+  static constexpr int SMEM_BYTES =
+      STAGES * STAGE_BYTES + 8 * OUT_BYTES + 1024 /*align*/ + 256 /*barriers*/;
   static constexpr int TMEM_COLS = 2 * BN;
 };
-constexpr int kLinearThreads = 320;  // producer, issuer, eight epilogue warps
+// Three groups of four warps: producer, issuer and two idle; eight epilogue warps.  Of the registers
+// that the block is launched with (384 x 168 = 64512) the first group gives up what the other two take:
+// 128 x 56 + 256 x 224 = 64512.
+constexpr int kLinearThreads = 384, kEpilogueWarp = 4;
+constexpr int kFewRegisters = 56, kManyRegisters = 224;
+// wgrad: the tensor cores' additions lose 1.1e-9 of the result for each further row (8192 rows:
+// 9.1e-6), so that their sum ends after 1024 rows and is added to fp32 sums in registers.
+constexpr int kSegment = 16;  // blocks of 64 rows
 
 // The m-blocks of a group of 16 take turns, so that their rows and the columns at hand stay in L2.
 __device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int& tm, int& tn) {
@@ -146,175 +181,336 @@ __device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int& tm,
   tm = first + r % size;
   tn = r / size;
 }
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  return pack_bf16x2(lo, hi);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack2(uint32_t u);
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
-  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t u) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&u));
+// The tile and the columns of a unit of work.
+template <int BN>
+__device__ __forceinline__ void unit_at(const LinearArgs& p, int unit, int num_m, int num_n, int& tm,
+                                        int& n0, int& width) {
+  int tn, piece = 0;
+  width = BN;
+  if (unit >= p.full) {
+    const int i = unit - p.full;
+    piece = i % p.pieces;
+    unit = p.full + i / p.pieces;
+    width = BN / p.pieces;
+  }
+  tile_at(unit, num_m, num_n, tm, tn);
+  n0 = tn * BN + piece * width;
 }
 
-// 32 neighbouring elements of a row as 16 words, n of them inside (zeros behind).
+// 16 pairs as words of two elements of T, and back.
 template <typename T>
-__device__ __forceinline__ void load32(const T* p, int n, bool vec, uint32_t* u) {
-  if (vec && n >= 32) {
+__device__ __forceinline__ void pack16(const F2* v, uint32_t* u) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      reinterpret_cast<uint4*>(u)[j] = reinterpret_cast<const uint4*>(p)[j];
-  } else {
-    const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      uint32_t lo = 0, hi = 0;
-      if (2 * j < n) lo = s[2 * j];
-      if (2 * j + 1 < n) hi = s[2 * j + 1];
-      u[j] = lo | (hi << 16);
+  for (int j = 0; j < 16; ++j) {
+    const float2 h = halves(v[j]);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      u[j] = pack_bf16x2(h.x, h.y);
+    } else {
+      const __half2 w = __floats2half2_rn(h.x, h.y);
+      u[j] = *reinterpret_cast<const uint32_t*>(&w);
     }
   }
 }
 template <typename T>
-__device__ __forceinline__ void store32(T* p, int n, bool vec, const float* v) {
-  uint32_t u[16];
+__device__ __forceinline__ F2 unpack2(uint32_t u) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  return f2(h.x, h.y);
+}
+
+// ---------------------------------------------------------------- 32 rows x 32 columns of a warp
+// In the epilogue a lane has a row, which is how TMEM is read, and 64 bytes of it at a time.  Where
+// rows start on 32 bytes, it reads and writes them as whole sectors by 256-bit accesses (stores of 16
+// bytes fill half sectors: the forward of 16384 x 2048 x 5632 with z took 323 us with them).
+// Elsewhere, and at the last columns, chunks pass through shared memory, where they are written by
+// rows and read four lanes (or, element by element, all lanes) to a row, or the other way round; not
+// everywhere, since the products need the shared memory's bandwidth themselves.  The 16-byte quarters
+// of a row are permuted so that neither way has bank conflicts.
+using u16 = unsigned short;
+__device__ __forceinline__ uint4* quarter(uint8_t* buf, int row, int j) {
+  return reinterpret_cast<uint4*>(buf + row * 64 + ((j ^ ((row >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ u16* element(uint8_t* buf, int row, int c) {
+  return reinterpret_cast<u16*>(quarter(buf, row, c >> 3)) + (c & 7);
+}
+__device__ __forceinline__ void put_row(uint8_t* buf, const uint32_t* u) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) u[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
-  if (vec && n >= 32) {
+  for (int j = 0; j < 4; ++j)
+    *quarter(buf, lane_id(), j) = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+}
+__device__ __forceinline__ void get_row(uint8_t* buf, uint32_t* u) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      reinterpret_cast<uint4*>(p)[j] = make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+  for (int j = 0; j < 4; ++j) {
+    const uint4 q = *quarter(buf, lane_id(), j);
+    u[4 * j] = q.x;
+    u[4 * j + 1] = q.y;
+    u[4 * j + 2] = q.z;
+    u[4 * j + 3] = q.w;
+  }
+}
+__device__ __forceinline__ void store_sector(void* p, const uint32_t* u) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(u[0]),
+               "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
+}
+__device__ __forceinline__ void load_sector(const void* p, uint32_t* u) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
+                 "=r"(u[6]), "=r"(u[7])
+               : "l"(p));
+}
+// The lanes' rows of a chunk (16 words each) to rows [0, rows) and columns [0, cols) of dst.
+template <typename T>
+__device__ __forceinline__ void chunk_out(uint8_t* buf, const uint32_t* u, T* dst, long long ld,
+                                          int rows, int cols, int vec) {
+  const int lane = lane_id();
+  if (vec == kRows32 && cols >= 32) {
+    if (lane < rows) {
+      store_sector(dst + lane * ld, u);
+      store_sector(dst + lane * ld + 16, u + 8);
+    }
+    return;
+  }
+  __syncwarp();  // the chunk before has left the buffer
+  put_row(buf, u);
+  __syncwarp();
+  if (vec != kRowsAny && cols >= 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      const uint4 v = *quarter(buf, r, lane & 3);
+      if (r < rows) reinterpret_cast<uint4*>(dst + r * ld)[lane & 3] = v;
+    }
+  } else if (lane < cols) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows) reinterpret_cast<u16*>(dst + r * ld)[lane] = *element(buf, r, lane);
+  }
+}
+// A chunk on its way in: `at` is where a lane's own row begins (-1: there is none, zeros come).
+template <typename T>
+__device__ __forceinline__ void chunk_load(const T* src, long long at, int col, int cols, int vec,
+                                           uint32_t* pre) {
+  const int lane = lane_id();
+  if (vec == kRows32 && cols >= 32) {
+    if (at >= 0) {
+      load_sector(src + at + col, pre);
+      load_sector(src + at + col + 16, pre + 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pre[i] = 0;
+    }
+  } else if (vec != kRowsAny && cols >= 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long row = __shfl_sync(0xffffffffu, at, i * 8 + (lane >> 2));
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (row >= 0) v = reinterpret_cast<const uint4*>(src + row + col)[lane & 3];
+      reinterpret_cast<uint4*>(pre)[i] = v;
+    }
   } else {
-    unsigned short* s = reinterpret_cast<unsigned short*>(p);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if (2 * j < n) s[2 * j] = static_cast<unsigned short>(u[j]);
-      if (2 * j + 1 < n) s[2 * j + 1] = static_cast<unsigned short>(u[j] >> 16);
+    for (int i = 0; i < 16; ++i) {
+      uint32_t w = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const long long row = __shfl_sync(0xffffffffu, at, 2 * i + h);
+        if (row >= 0 && lane < cols)
+          w |= static_cast<uint32_t>(reinterpret_cast<const u16*>(src + row + col)[lane]) << (16 * h);
+      }
+      pre[i] = w;
+    }
+  }
+}
+// ... and what chunk_load brought, as the words of the lane's own row.
+__device__ __forceinline__ void chunk_in(uint8_t* buf, int cols, int vec, const uint32_t* pre,
+                                         uint32_t* own) {
+  const int lane = lane_id();
+  if (vec == kRows32 && cols >= 32) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) own[i] = pre[i];
+    return;
+  }
+  __syncwarp();  // the chunk before has left buf
+  if (vec != kRowsAny && cols >= 32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *quarter(buf, i * 8 + (lane >> 2), lane & 3) = reinterpret_cast<const uint4*>(pre)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      *element(buf, 2 * i, lane) = static_cast<u16>(pre[i]);
+      *element(buf, 2 * i + 1, lane) = static_cast<u16>(pre[i] >> 16);
+    }
+  }
+  __syncwarp();
+  get_row(buf, own);
+}
+// 32 fp32 values of each lane's row to dst (added, with `add`); not on 32 bytes through all of a
+// warp's buffer.
+__device__ __forceinline__ void chunk_out_f32(uint8_t* buf, const float* v, float* dst, long long ld,
+                                              int rows, int cols, int vec, bool add) {
+  const int lane = lane_id();
+  if (vec == kRows32 && cols >= 32) {
+    float* d = dst + lane * ld;
+    if (lane >= rows) return;
+    if (add) {  // each element once: the same bits as a load, an addition and a store
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(d + 4 * j),
+                     "f"(v[4 * j]), "f"(v[4 * j + 1]), "f"(v[4 * j + 2]), "f"(v[4 * j + 3])
+                     : "memory");
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) store_sector(d + 8 * j, reinterpret_cast<const uint32_t*>(v) + 8 * j);
+    }
+    return;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    *reinterpret_cast<float4*>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+        make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  __syncwarp();
+  if (lane < cols) {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r) {
+      if (r >= rows) continue;
+      const float o =
+          reinterpret_cast<const float*>(buf + r * 128 + (((lane >> 2) ^ (r & 7)) << 4))[lane & 3];
+      float* d = dst + r * ld + lane;
+      *d = add ? *d + o : o;
     }
   }
 }
 
-// One row (TMEM lane) of a tile: columns [n0 + first, n0 + last) in chunks of 32, in steps of `step`.
-template <typename T, int KIND>
-__device__ __forceinline__ void epilogue_rows(const LinearArgs& p, uint32_t taddr, int row, int n0,
-                                              int first, int last, int step) {
-  const bool live = row < p.M;
-  const bool vec = p.vec != 0;
-  const T* zrow = nullptr;
-  bool z_ok = false;
-  if (KIND == kLinearDgrad && live) {
-    const long long src = p.z_rows ? p.z_rows[row] : row;
-    z_ok = index_in(src, p.n_z, p.err);
-    zrow = static_cast<const T*>(p.Z) + (z_ok ? src : 0) * p.ldz;
+// The rows of a warp (32 from row0, one a lane) of a unit's columns [n0, n0 + width): every second
+// chunk of 32 from `first`.  wait() is for the product; before it the first chunk that is read from
+// memory is already asked for.
+template <typename T, int KIND, typename F>
+__device__ __forceinline__ bool epilogue_rows(const LinearArgs& p, uint32_t taddr, int row0, int n0,
+                                              int first, int width, uint8_t* buf, F&& wait) {
+  const int vec = p.vec;
+  const int row = row0 + lane_id();
+  const int rows = p.M - row0;  // may be none
+  long long at = -1;            // where the lane's row of `other` begins
+  const T* other = static_cast<const T*>(KIND == kLinearFwd ? p.R : p.Z);
+  if (row < p.M) {
+    if constexpr (KIND == kLinearFwd) {
+      at = static_cast<long long>(row) * p.ldr;
+    } else {
+      const long long src = p.z_rows ? p.z_rows[row] : row;
+      if (index_in(src, p.n_z, p.err)) at = src * p.ldz;
+    }
   }
+  const bool reads = other != nullptr;
+  uint32_t pre[16];
+  if (reads && n0 + first < p.N && first < width)
+    chunk_load(other, at, n0 + first, p.N - n0 - first, vec, pre);
+  if (!wait()) return false;
 #pragma unroll 1
-  for (int c = first; c < last; c += step) {
+  for (int c = first; c < width; c += 64) {
     const int col = n0 + c;
     if (col >= p.N) break;  // the same for the whole warp
-    const int n = p.N - col;
-    uint32_t other[16];  // the residual's or the activation argument's 32 values
-    bool have = false;
-    if (KIND == kLinearFwd && p.R && live) {
-      load32(static_cast<const T*>(p.R) + row * p.ldr + col, n, vec, other);
-      have = true;
-    }
-    if (KIND == kLinearDgrad && z_ok) load32(zrow + col, n, vec, other);
-    uint32_t r[32];
+    const int cols = p.N - col;
+    uint32_t own[16], r[32];
     CFB_TMEM_LD32(taddr + c, r);
+    if (reads) {
+      chunk_in(buf, cols, vec, pre, own);
+      if (c + 64 < width && col + 64 < p.N) chunk_load(other, at, col + 64, cols - 64, vec, pre);
+    }
     tmem_ld_wait();
-    if (!live) continue;
-    float v[32];
+    F2 v[16];
+    uint32_t u[16];
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int j = 0; j < 16; ++j) v[j] = f2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
     if constexpr (KIND == kLinearFwd) {
       if (p.bias) {
-        uint32_t b[16];
-        load32(static_cast<const T*>(p.bias) + col, n,
-               (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, b);
+        const T* b = static_cast<const T*>(p.bias) + col;
+        if (cols >= 32 && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float2 f = unpack2<T>(b[j]);
-          v[2 * j] += f.x;
-          v[2 * j + 1] += f.y;
+          for (int j = 0; j < 4; ++j) {
+            F2 f[4];
+            load_f2<T, 8>(b + 8 * j, f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[4 * j + i] = v[4 * j + i] + f[i];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            v[j] = v[j] + f2(2 * j < cols ? to_f32(b[2 * j]) : 0.f,
+                             2 * j + 1 < cols ? to_f32(b[2 * j + 1]) : 0.f);
         }
       }
-      if (p.Z) store32(static_cast<T*>(p.Z) + row * p.ldz + col, n, vec, v);
+      if (p.Z) {
+        pack16<T>(v, u);
+        chunk_out(buf + 2048, u, static_cast<T*>(p.Z) + row0 * p.ldz + col, p.ldz, rows, cols, vec);
+      }
       with_act(p.act, [&](auto tag) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = act_of<decltype(tag)::act>(v[i]);
+        for (int j = 0; j < 16; ++j) v[j] = act_of<decltype(tag)::act>(v[j]);
       });
-      if (have) {
+      if (reads) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float2 f = unpack2<T>(other[j]);
-          v[2 * j] += f.x;
-          v[2 * j + 1] += f.y;
-        }
+        for (int j = 0; j < 16; ++j) v[j] = v[j] + unpack2<T>(own[j]);
       }
-      store32(static_cast<T*>(p.D) + row * p.ldd + col, n, vec, v);
-    } else if constexpr (KIND == kLinearDgrad) {
-      if (z_ok) {
-        with_act(p.act, [&](auto tag) {
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 f = unpack2<T>(other[j]);
-            v[2 * j] *= act_slope<decltype(tag)::act>(f.x);
-            v[2 * j + 1] *= act_slope<decltype(tag)::act>(f.y);
-          }
-        });
-      } else {  // a row id outside z: recorded, and a zero row
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.f;
-      }
-      store32(static_cast<T*>(p.D) + row * p.ldd + col, n, vec, v);
+      pack16<T>(v, u);
     } else {
-      float* d = static_cast<float*>(p.D) + row * p.ldd + col;
-      if (vec && n >= 32) {
+      with_act(p.act, [&](auto tag) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float4 o = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          if (p.add) {  // each element once: the same bits as a load, an addition and a store
-            asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(d + 4 * j),
-                         "f"(o.x), "f"(o.y), "f"(o.z), "f"(o.w)
-                         : "memory");
-          } else {
-            reinterpret_cast<float4*>(d)[j] = o;
-          }
-        }
-      } else {
+        for (int j = 0; j < 16; ++j) v[j] = v[j] * act_slope<decltype(tag)::act>(unpack2<T>(own[j]));
+      });
+      pack16<T>(v, u);
+      if (at < 0) {  // a row id outside z is recorded, and gives a zero row
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < n) d[i] = p.add ? d[i] + v[i] : v[i];
+        for (int j = 0; j < 16; ++j) u[j] = 0;
       }
+    }
+    chunk_out(buf, u, static_cast<T*>(p.D) + row0 * p.ldd + col, p.ldd, rows, cols, vec);
+  }
+  return true;
+}
+
+// mbar_wait for warps that have nothing else to do for microseconds: polls that the hardware holds for
+// up to 20 us take no issue slots from the producer and the issuer.
+__device__ __forceinline__ bool mbar_wait_idle(uint32_t bar, uint32_t parity, volatile int* abort,
+                                               int* err, int code) {
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(20000)
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (globaltimer_ns() - t0 > local_wait_limit_ns(err)) {
+      *abort = 1;
+      if (err) atomicCAS(err, 0, code);
+      return false;
     }
   }
 }
 
 // Persistent: producer warp 0 (TMA into a ring of stages), issuer warp 1 (tcgen05.mma into one of
 // two accumulators), eight epilogue warps (two to a quadrant of the TMEM lanes, each with half of a
-// tile's columns).  With CG = 2 both CTAs' copies count on the leader's barriers, and the leader
-// issues the products of the pair.  Every wait is bounded.
+// tile's chunks of columns).  With CG = 2 both CTAs' copies count on the leader's barriers, and the
+// leader issues the products of the pair.  The tiles of the last, partly filled wave are cut into
+// pieces of fewer columns.  Every wait is bounded.
 template <int CG, int BN, typename T, int KIND>
 __global__ void __launch_bounds__(kLinearThreads, 1)
     linear_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                  const LinearArgs p) {
+                  const __grid_constant__ CUtensorMap tmPiece, const LinearArgs p) {
   using S = TileShape<CG, BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE_BYTES);
+  uint8_t* out_area = smem + S::STAGES * S::STAGE_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_area + 8 * S::OUT_BYTES);
   uint64_t* empty = full + S::STAGES;
   uint64_t* tfull = empty + S::STAGES;
   uint64_t* tempty = tfull + 2;
@@ -328,8 +524,10 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
   const int group = blockIdx.x / CG, groups = gridDim.x / CG;
   const int num_m = (p.M + CG * S::BM - 1) / (CG * S::BM);
   const int num_n = (p.N + BN - 1) / BN;
-  const int num_tiles = num_m * num_n;
+  const int num_units = p.full + (num_m * num_n - p.full) * p.pieces;
   const int num_kb = (p.K + S::BK - 1) / S::BK;
+  // blocks of k that one accumulator takes
+  const int segment = KIND == kLinearWgrad ? kSegment : num_kb;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
@@ -362,17 +560,22 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t smem_base = smem_u32(smem);
-
-  if (warp == 0) {
-    if (lane == 0) {
+  after_previous();  // (an operand that was laid out anew)
+  if (warp < kEpilogueWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegisters));
+    if (warp == 0 && lane == 0) {
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = group; tile < num_tiles && ok; tile += groups) {
-        int tm, tn;
-        tile_at(tile, num_m, num_n, tm, tn);
+      for (int unit = group; unit < num_units && ok; unit += groups) {
+        int tm, n0, width;
+        unit_at<BN>(p, unit, num_m, num_n, tm, n0, width);
         const int m0 = (tm * CG + static_cast<int>(crank)) * S::BM;
-        const int n0 = tn * BN + static_cast<int>(crank) * S::B_ROWS;
+        const int b_rows = width / CG;
+        n0 += static_cast<int>(crank) * b_rows;
+        const int b_boxes = (b_rows + 63) / 64;  // MN-major
+        const int b_bytes = p.b_mn ? b_boxes * 8192 : b_rows * 128;
+        const CUtensorMap* map_b = width == BN ? &tmB : &tmPiece;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(smem_u32(&empty[stage]), phase ^ 1u, abort_flag, p.err,
                          kErrWaitProducer)) {
@@ -380,7 +583,7 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
             break;
           }
           uint32_t bar = smem_u32(&full[stage]);
-          if (leader) mbar_arrive_expect_tx(bar, CG * S::STAGE_BYTES);
+          if (leader) mbar_arrive_expect_tx(bar, CG * (S::A_BYTES + b_bytes));
           if (CG == 2) bar = mapa_shared(bar, 0);
           const auto load = [&](uint32_t dst, const CUtensorMap* m, int x, int y) {
             if constexpr (CG == 2) tma_load_2d_pair(dst, m, bar, x, y);
@@ -389,17 +592,25 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
           const uint32_t sa = smem_base + stage * S::STAGE_BYTES;
           const uint32_t sb = sa + S::A_BYTES;
           const int k0 = kb * S::BK;
+          const auto load_3d = [&](uint32_t dst, const CUtensorMap* m, int chunk, int y) {
+            if constexpr (CG == 2) tma_load_3d_pair(dst, m, bar, 0, y, chunk);
+            else tma_load_3d(dst, m, bar, 0, y, chunk);
+          };
           if (!p.a_mn) {
             load(sa, &tmA, k0, m0);
+          } else if (p.a_3d) {
+            load_3d(sa, &tmA, m0 / 64, k0);
           } else {
             load(sa, &tmA, m0, k0);
             load(sa + 8192, &tmA, m0 + 64, k0);
           }
           if (!p.b_mn) {
-            load(sb, &tmB, k0, n0);
+            load(sb, map_b, k0, n0);
+          } else if (p.b_3d && width == BN) {
+            load_3d(sb, &tmB, n0 / 64, k0);
           } else {
-#pragma unroll
-            for (int c = 0; c < S::B_ROWS / 64; ++c) load(sb + c * 8192, &tmB, n0 + c * 64, k0);
+            load(sb, map_b, n0, k0);
+            if (b_boxes == 2) load(sb + 8192, map_b, n0 + 64, k0);
           }
           ++issued;
           if (++stage == S::STAGES) {
@@ -412,49 +623,54 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
       // CTAs' copies)
       if (!ok && leader) tma_drain_ring(full, S::STAGES, issued);
     }
-  } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (warp == 1 && lane == 0 && leader) {
       // K-major: 16 columns of k are 32 bytes on; MN-major: 16 rows of k are 2048 bytes on
       const uint32_t a_step = p.a_mn ? 2048 : 32, a_lbo = p.a_mn ? 8192 : 16;
       const uint32_t b_step = p.b_mn ? 2048 : 32, b_lbo = p.b_mn ? 8192 : 16;
       int stage = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = group; tile < num_tiles && ok; tile += groups, ++it) {
-        const int acc = it & 1;
-        if (!mbar_wait(smem_u32(&tempty[acc]), ((it >> 1) & 1) ^ 1u, abort_flag, p.err,
-                       kErrWaitMma)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d = tmem_base + acc * BN;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(smem_u32(&full[stage]), phase, abort_flag, p.err, kErrWaitMma)) {
+      for (int unit = group; unit < num_units && ok; unit += groups) {
+        int tm, n0, width;
+        unit_at<BN>(p, unit, num_m, num_n, tm, n0, width);
+        const uint32_t idesc = (p.idesc & ~(0x3fu << 17)) | (static_cast<uint32_t>(width >> 3) << 17);
+        for (int k_seg = 0; k_seg < num_kb && ok; k_seg += segment, ++it) {
+          const int k_end = min(num_kb, k_seg + segment);
+          const int acc = it & 1;
+          if (!mbar_wait(smem_u32(&tempty[acc]), ((it >> 1) & 1) ^ 1u, abort_flag, p.err,
+                         kErrWaitMma)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_base + stage * S::STAGE_BYTES;
-          const uint32_t sb = sa + S::A_BYTES;
+          const uint32_t d = tmem_base + acc * BN;
+          for (int kb = k_seg; kb < k_end; ++kb) {
+            if (!mbar_wait(smem_u32(&full[stage]), phase, abort_flag, p.err, kErrWaitMma)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sa = smem_base + stage * S::STAGE_BYTES;
+            const uint32_t sb = sa + S::A_BYTES;
 #pragma unroll
-          for (int k = 0; k < S::BK / 16; ++k) {
-            const uint64_t ad = sdesc_sw128(sa + k * a_step, a_lbo, 1024);
-            const uint64_t bd = sdesc_sw128(sb + k * b_step, b_lbo, 1024);
-            const uint32_t accumulate = kb != 0 || k != 0;
-            if constexpr (CG == 2) umma_bf16_ss_pair(d, ad, bd, p.idesc, accumulate);
-            else umma_bf16_ss(d, ad, bd, p.idesc, accumulate);
+            for (int k = 0; k < S::BK / 16; ++k) {
+              const uint64_t ad = sdesc_sw128(sa + k * a_step, a_lbo, 1024);
+              const uint64_t bd = sdesc_sw128(sb + k * b_step, b_lbo, 1024);
+              const uint32_t accumulate = kb != k_seg || k != 0;
+              if constexpr (CG == 2) umma_bf16_ss_pair(d, ad, bd, idesc, accumulate);
+              else umma_bf16_ss(d, ad, bd, idesc, accumulate);
+            }
+            if constexpr (CG == 2) umma_commit_pair_mc(smem_u32(&empty[stage]), 0x3);
+            else umma_commit(smem_u32(&empty[stage]));
+            if (++stage == S::STAGES) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          if constexpr (CG == 2) umma_commit_pair_mc(smem_u32(&empty[stage]), 0x3);
-          else umma_commit(smem_u32(&empty[stage]));
-          if (++stage == S::STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          if (!ok) break;
+          if constexpr (CG == 2) umma_commit_pair_mc(smem_u32(&tfull[acc]), 0x3);
+          else umma_commit(smem_u32(&tfull[acc]));
         }
-        if (!ok) break;
-        if constexpr (CG == 2) umma_commit_pair_mc(smem_u32(&tfull[acc]), 0x3);
-        else umma_commit(smem_u32(&tfull[acc]));
       }
       // all products are done before shared memory or TMEM is given up
       if constexpr (CG == 2) umma_commit_pair(smem_u32(drain));
@@ -463,24 +679,69 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
       mbar_wait(smem_u32(drain), 0, &never, nullptr, 0);
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegisters));
     const int q = warp & 3;  // the quadrant of TMEM lanes that this warp may read
-    const int half = (warp - 2) >> 2;
+    const int half = (warp - kEpilogueWarp) >> 2;
+    uint8_t* buf = out_area + (warp - kEpilogueWarp) * S::OUT_BYTES;
     int it = 0;
-    for (int tile = group; tile < num_tiles; tile += groups, ++it) {
-      int tm, tn;
-      tile_at(tile, num_m, num_n, tm, tn);
-      const int acc = it & 1;
-      if (!mbar_wait(smem_u32(&tfull[acc]), (it >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue))
-        break;
+    bool ok = true;
+    const auto wait = [&] {
+      ok = mbar_wait_idle(smem_u32(&tfull[it & 1]), (it >> 1) & 1, abort_flag, p.err, kErrWaitEpilogue);
       tc_fence_after();
-      const int row = (tm * CG + static_cast<int>(crank)) * S::BM + q * 32 + lane;
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
-      epilogue_rows<T, KIND>(p, taddr, row, tn * BN, half * 32, BN, 64);
+      return ok;
+    };
+    const auto release = [&] {  // the accumulator may be written again
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CG == 2) mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
-        else mbar_arrive(smem_u32(&tempty[acc]));
+        const uint32_t bar = smem_u32(&tempty[it & 1]);
+        if constexpr (CG == 2) mbar_arrive_cluster(mapa_shared(bar, 0));
+        else mbar_arrive(bar);
+      }
+      ++it;
+    };
+    for (int unit = group; unit < num_units && ok; unit += groups) {
+      int tm, n0, width;
+      unit_at<BN>(p, unit, num_m, num_n, tm, n0, width);
+      const int m0 = (tm * CG + static_cast<int>(crank)) * S::BM;
+      const int row0 = m0 + q * 32;
+      const auto taddr = [&] {
+        return tmem_base + (static_cast<uint32_t>(q * 32) << 16) + (it & 1) * BN;
+      };
+      if constexpr (KIND != kLinearWgrad) {
+        if (!epilogue_rows<T, KIND>(p, taddr(), row0, n0, half * 32, width, buf, wait)) break;
+        release();
+      } else {
+        constexpr int NCH = BN / 64;
+        float v[NCH][32];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[i][j] = 0.f;
+        for (int k_seg = 0; k_seg < num_kb; k_seg += kSegment) {
+          if (!wait()) break;
+#pragma unroll
+          for (int i = 0; i < NCH; ++i) {
+            if (half * 32 + 64 * i >= width) continue;
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              uint32_t r[16];
+              CFB_TMEM_LD16(taddr() + half * 32 + 64 * i + h, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[i][h + j] += __uint_as_float(r[j]);
+            }
+          }
+          release();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+          const int col = n0 + half * 32 + 64 * i;
+          if (half * 32 + 64 * i >= width || col >= p.N) continue;
+          chunk_out_f32(buf, v[i], static_cast<float*>(p.D) + row0 * p.ldd + col, p.ldd, p.M - row0,
+                        p.N - col, p.vec, p.add != 0);
+        }
       }
     }
   }
@@ -501,6 +762,7 @@ __global__ void __launch_bounds__(256) relayout_kernel(const unsigned short* __r
                                                        long long ld, int cols,
                                                        unsigned short* __restrict__ dst,
                                                        long long ld_dst, int rows) {
+  let_next_start();
   for (int r = blockIdx.y; r < rows; r += gridDim.y) {
     const unsigned short* s = src + r * ld;
     unsigned short* d = dst + r * ld_dst;
@@ -520,6 +782,7 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ d
   constexpr int SLAB = LANES * W;
   __shared__ float part[GROUPS][SLAB + 1];
   __shared__ float total[SLAB];
+  let_next_start();
   const uint32_t rank = cluster_ctarank();
   const int lane = threadIdx.x % LANES, rg = threadIdx.x / LANES;
   const int slab = blockIdx.x / 8 * SLAB;
@@ -572,8 +835,8 @@ int current_device() {
 }
 
 template <int CG, int BN, typename T, int KIND>
-int launch_linear(const CUtensorMap& ta, const CUtensorMap& tb, const LinearArgs& a,
-                  cudaStream_t st) {
+int launch_linear(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tp,
+                  const LinearArgs& a, bool behind, cudaStream_t st) {
   using S = TileShape<CG, BN>;
   auto* kernel = linear_kernel<CG, BN, T, KIND>;
   static bool allowed[kMaxDevices] = {};
@@ -588,19 +851,27 @@ int launch_linear(const CUtensorMap& ta, const CUtensorMap& tb, const LinearArgs
     allowed[dev] = true;
   }
   const long long tiles = ((a.M + CG * 128LL - 1) / (CG * 128)) * ((a.N + BN - 1LL) / BN);
-  const int groups = static_cast<int>(tiles < 148 / CG ? tiles : 148 / CG);
+  const long long units = a.full + (tiles - a.full) * a.pieces;
+  const int groups = static_cast<int>(units < 148 / CG ? units : 148 / CG);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(groups * CG);
   cfg.blockDim = dim3(kLinearThreads);
   cfg.dynamicSmemBytes = S::SMEM_BYTES;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = CG;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = CG > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kernel, ta, tb, a) != cudaSuccess) {
+  cudaLaunchAttribute attr[2];
+  if (CG > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CG;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (behind) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = attr;
+  if (cudaLaunchKernelEx(&cfg, kernel, ta, tb, tp, a) != cudaSuccess) {
     cudaGetLastError();
     return -3;
   }
@@ -608,26 +879,51 @@ int launch_linear(const CUtensorMap& ta, const CUtensorMap& tb, const LinearArgs
   return 0;
 }
 
-// The tile whose estimated time is least: waves of tiles over the SMs times the time of a tile, in
-// units of a 128 x 256 share at full rate.
+// How the output is cut: the tile (a 256 x 256 pair tile, or 128 x bn of one CTA), and the pieces that
+// the tiles of the pair's last wave are cut into.
 struct LinearPlan {
   int cg, bn;
+  long long full;
+  int pieces;
 };
+// The least estimated time, in units of a pair tile: waves over the SMs times the time of a tile.  A
+// piece of half or a quarter of the columns takes 0.56 or 0.4 of a tile's time (the products of fewer
+// columns are bound by shared memory), the tiles of one CTA 0.73 (128 columns, half of the elements of
+// a CTA's share of a pair tile) and 0.5 (64 columns).
 LinearPlan plan_linear(long long M, long long N) {
-  const auto waves = [](long long tiles, int slots) { return (tiles + slots - 1) / slots; };
-  const double pair = 0.9 * waves(((M + 255) / 256) * ((N + 255) / 256), 74);
-  const double s128 = 0.66 * waves(((M + 127) / 128) * ((N + 127) / 128), 148);
-  const double s64 = 0.45 * waves(((M + 127) / 128) * ((N + 63) / 64), 148);
-  if (pair <= s128 && pair <= s64) return {2, 256};
-  return s128 <= s64 ? LinearPlan{1, 128} : LinearPlan{1, 64};
+  const auto waves = [](long long units, int slots) { return (units + slots - 1) / slots; };
+  const long long pairs = ((M + 255) / 256) * ((N + 255) / 256);
+  const long long full = pairs / 74 * 74, rest = pairs - full;
+  double best = full / 74 + (rest > 0 ? 1.0 : 0.0);
+  LinearPlan plan = {2, 256, pairs, 1};
+  const double times[] = {0.56, 0.4};
+  for (int i = 0; i < 2 && rest > 0; ++i) {
+    const int pieces = 2 << i;
+    const double t = full / 74 + times[i] * waves(rest * pieces, 74);
+    if (t < best) {
+      best = t;
+      plan = {2, 256, full, pieces};
+    }
+  }
+  const double singles[] = {0.73, 0.5};
+  for (int i = 0; i < 2; ++i) {
+    const int bn = 128 >> i;
+    const long long tiles = ((M + 127) / 128) * ((N + bn - 1) / bn);
+    const double t = singles[i] * waves(tiles, 148);
+    if (t < best) {
+      best = t;
+      plan = {1, bn, tiles, 1};
+    }
+  }
+  return plan;
 }
 
 template <typename T, int KIND>
 int launch_plan(const LinearPlan& pl, const CUtensorMap& ta, const CUtensorMap& tb,
-                const LinearArgs& a, cudaStream_t st) {
-  if (pl.cg == 2) return launch_linear<2, 256, T, KIND>(ta, tb, a, st);
-  if (pl.bn == 128) return launch_linear<1, 128, T, KIND>(ta, tb, a, st);
-  return launch_linear<1, 64, T, KIND>(ta, tb, a, st);
+                const CUtensorMap& tp, const LinearArgs& a, bool behind, cudaStream_t st) {
+  if (pl.cg == 2) return launch_linear<2, 256, T, KIND>(ta, tb, tp, a, behind, st);
+  if (pl.bn == 128) return launch_linear<1, 128, T, KIND>(ta, tb, tp, a, behind, st);
+  return launch_linear<1, 64, T, KIND>(ta, tb, tp, a, behind, st);
 }
 
 // An operand in memory: rows and columns, and whether TMA can read it as it is.
@@ -709,13 +1005,16 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
       return -3;
     return 0;
   }
+  bool behind = false;  // the product follows a kernel of the same call
   if (p->kind == kLinearWgrad && p->dbias) {
     const int rc = p->type == kBF16 ? launch_column_sum<__nv_bfloat16>(*p, st)
                                     : launch_column_sum<__half>(*p, st);
     if (rc || p->N == 0) return rc;
+    behind = true;
   }
   if (((p->M + 127LL) / 128) * ((p->N + 63LL) / 64) >= (1LL << 31)) return -11;
   Operand oa = operand_a(*p), ob = operand_b(*p);
+  behind = behind || !oa.direct() || !ob.direct();
   uint8_t* work = static_cast<uint8_t*>(p->work);
   int rc = lay_out(oa, work, st);
   if (rc) return rc;
@@ -730,13 +1029,25 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
   a.b_mn = p->kind != kLinearFwd;
   a.idesc = idesc_bf16_f32(128 * pl.cg, pl.bn, a.a_mn, a.b_mn);
   if (p->type == kF16) a.idesc &= ~((1u << 7) | (1u << 10));  // f16 operands
-  CUtensorMap ta, tb;
-  rc = a.a_mn ? make_tmap_2d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 64)
-              : make_tmap_2d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 128);
+  const int b_rows = pl.bn / pl.cg;
+  a.a_3d = a.a_mn && oa.cols % 64 == 0;  // (128 columns of a tile)
+  a.b_3d = a.b_mn && ob.cols % 64 == 0 && b_rows == 128;
+  CUtensorMap ta, tb, tp;
+  rc = a.a_3d   ? make_tmap_3d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 2)
+       : a.a_mn ? make_tmap_2d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 64)
+                : make_tmap_2d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 128);
   if (rc) return rc * 100 - 1;
-  rc = a.b_mn ? make_tmap_2d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, 64)
-              : make_tmap_2d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, pl.bn / pl.cg);
+  rc = a.b_3d   ? make_tmap_3d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, 2)
+       : a.b_mn ? make_tmap_2d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, 64)
+                : make_tmap_2d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, b_rows);
   if (rc) return rc * 100 - 2;
+  tp = tb;
+  if (pl.pieces > 1 && (!a.b_mn || a.b_3d))
+    rc = make_tmap_2d_bf16(&tp, ob.p, ob.rows, ob.cols, ob.ld, 64,
+                           a.b_mn ? 64 : b_rows / pl.pieces);
+  if (rc) return rc * 100 - 3;
+  a.full = static_cast<int>(pl.full);
+  a.pieces = pl.pieces;
   a.D = p->D;
   a.ldd = p->ldd;
   a.bias = p->bias;
@@ -750,13 +1061,15 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
   a.add = p->add;
   a.err = p->err;
   const int out_type = p->kind == kLinearWgrad ? kF32 : p->type;
-  const int out_width = p->kind == kLinearWgrad ? 4 : 8;
-  a.vec = rows_of(out_width, p->D, p->ldd, out_type) && rows_of_8(p->R, p->ldr, p->type) &&
-          rows_of_8(p->Z, p->ldz, p->type);
+  const auto rows_on = [&](int bytes) {
+    return rows_of(bytes / type_bytes(out_type), p->D, p->ldd, out_type) &&
+           rows_of(bytes / 2, p->R, p->ldr, p->type) && rows_of(bytes / 2, p->Z, p->ldz, p->type);
+  };
+  a.vec = rows_on(32) ? kRows32 : rows_on(16) ? kRows16 : kRowsAny;
 #define CFB_LINEAR(T)                                                                       \
-  (p->kind == kLinearFwd     ? launch_plan<T, kLinearFwd>(pl, ta, tb, a, st)               \
-   : p->kind == kLinearDgrad ? launch_plan<T, kLinearDgrad>(pl, ta, tb, a, st)             \
-                             : launch_plan<T, kLinearWgrad>(pl, ta, tb, a, st))
+  (p->kind == kLinearFwd     ? launch_plan<T, kLinearFwd>(pl, ta, tb, tp, a, behind, st)               \
+   : p->kind == kLinearDgrad ? launch_plan<T, kLinearDgrad>(pl, ta, tb, tp, a, behind, st)             \
+                             : launch_plan<T, kLinearWgrad>(pl, ta, tb, tp, a, behind, st))
   return p->type == kBF16 ? CFB_LINEAR(__nv_bfloat16) : CFB_LINEAR(__half);
 #undef CFB_LINEAR
 }
