@@ -28,7 +28,8 @@ namespace cfb {
 
 constexpr float kL2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;             // the streaming warps'
+constexpr int kBlock = kThreads + 32;    // ... and the lister's
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -88,34 +89,97 @@ struct Sums {
   }
 };
 
+// Eight logits as they lie in memory: -inf in all places, or in those whose bits are set; the largest.
+__device__ __forceinline__ uint32_t ninf2(__nv_bfloat16) { return 0xff80ff80u; }
+__device__ __forceinline__ uint32_t ninf2(__half) { return 0xfc00fc00u; }
+template <typename T>
+__device__ __forceinline__ void set_ninf(Pack<T, 8>& k) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(&k);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(k) / 4); ++i)
+    if constexpr (sizeof(T) == 4) u[i] = 0xff800000u;
+    else u[i] = ninf2(T());
+}
+template <typename T>
+__device__ __forceinline__ void mask_out(Pack<T, 8>& k, uint32_t bits) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(&k);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = bits >> i & 1u ? 0xff800000u : u[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t m = (bits >> (2 * i) & 1u ? 0xffffu : 0u) |
+                         (bits >> (2 * i + 1) & 1u ? 0xffff0000u : 0u);
+      u[i] = (u[i] & ~m) | (ninf2(T()) & m);
+    }
+  }
+}
+template <typename T, int U>
+__device__ __forceinline__ float packs_max(const Pack<T, 8>* k) {
+  if constexpr (std::is_same<T, float>::value) {
+    float m = k[0].v[0];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, k[u].v[i]);
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 m = reinterpret_cast<const T2*>(&k[0])[0];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m = __hmax2(m, reinterpret_cast<const T2*>(&k[u])[i]);
+    return fmaxf(to_f32(m.x), to_f32(m.y));
+  }
+}
+
+// The part of a row that a block has, in columns from v0: single columns up to the first boundary of a
+// pack (`head`), packs of eight, and the columns behind them.
+template <typename T>
+struct Span {
+  const T* z;
+  int n, head, packs;
+  __device__ __forceinline__ Span(const T* at, int n) : z(at), n(n) {
+    constexpr int kAlign = 8 * sizeof(T);
+    const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(at) % kAlign);
+    head = min(n, odd ? (kAlign - odd) / static_cast<int>(sizeof(T)) : 0);
+    packs = (n - head) / 8;
+  }
+  __device__ __forceinline__ int tail() const { return head + packs * 8; }
+  __device__ __forceinline__ Pack<T, 8> pack(int i) const { return load_pack<T, 8>(z + head + i * 8); }
+};
+
 // How exp(z) comes beside exp(z / tau): not wanted or the same; an exponential of its own; the square
 // of the other (tau = 2), which halves the exponentials of a kernel that they would bind.
 enum { kOneNone = 0, kOneOwn = 1, kOneSquare = 2 };
 
+// A row to a block (or, split over its columns, to a cluster of up to eight): eight warps stream the
+// logits, a ninth reads the list, marks its tokens in a bit mask in shared memory for the others, and
+// forms the teacher's terms in 64 bits while they work.
 template <typename T, bool REST, int ONE>
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const DistillArgs p, int splits,
-                                                               int chunk, float* __restrict__ kd,
-                                                               float* __restrict__ ce,
-                                                               float* __restrict__ lse,
-                                                               float* __restrict__ stats) {
+__global__ void __launch_bounds__(kBlock, 4) distill_fwd_kernel(
+    const DistillArgs p, int splits, int chunk, float* __restrict__ kd, float* __restrict__ ce,
+    float* __restrict__ lse, float* __restrict__ stats) {
   constexpr int U = sizeof(T) == 2 ? 4 : 2;  // packs of eight in flight, and as many at work
-  constexpr int kAlign = 8 * sizeof(T);
+  constexpr int kWarps = kThreads / 32 + 1;
   extern __shared__ uint32_t dyn[];
-  __shared__ float red[kThreads / 32][4];
+  __shared__ float red[kWarps][4];
   __shared__ float joined[4];  // this block's max, rest, listed, one
-  const int K = p.list.K, tid = threadIdx.x;
+  const int K = p.list.K, tid = threadIdx.x, lane = lane_id();
+  const bool lister = tid >= kThreads;
   float* sm_t = reinterpret_cast<float*>(dyn);
   float* sm_z = sm_t + K;
-  uint32_t* flags = reinterpret_cast<uint32_t*>(sm_z + K);  // 1: an entry, 2: the first of its token here
+  uint32_t* flags = reinterpret_cast<uint32_t*>(sm_z + K);  // 1: an entry, 2: its token's first; id * 4
   uint32_t* bits = flags + K;
   const long long row = blockIdx.x / splits;
   const int rank = blockIdx.x % splits;
   const int v0 = rank * chunk, n = max(0, min(p.V - v0, chunk));
   const T* z = static_cast<const T*>(p.z) + row * p.ld;
   const T* mine = z + v0;
-  const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(mine) % kAlign);
-  const int head = min(n, odd ? (kAlign - odd) / static_cast<int>(sizeof(T)) : 0);
-  const int packs = (n - head) / 8;
+  const Span<T> span(mine, n);
+  const int head = span.head, packs = span.packs;
   const int shift = 8 - head;  // bit of column i (from v0): i + shift, so a pack's bits are a byte
   const float c = p.inv_temp * kL2e;
 
@@ -123,109 +187,157 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const DistillArgs
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int at = first + u * kThreads + tid;
-      if (at < packs) k[u] = load_pack<T, 8>(mine + head + at * 8);
+      if (at < packs) k[u] = span.pack(at);
+      else set_ninf<T>(k[u]);
     }
   };
   Pack<T, 8> now[U];
-  load(0, now);
+  long long id0 = -1;  // the list's first ids are on their way with the first logits
+  if (!lister) load(0, now);
+  else if (lane < K) id0 = p.list.id(row, lane);
   if (REST) {
-    for (int i = tid; i < (n + 16 + 31) / 32; i += kThreads) bits[i] = 0;
+    for (int i = tid; i < (n + 16 + 31) / 32; i += kBlock) bits[i] = 0;
     __syncthreads();
   }
-  for (int j = tid; j < K; j += kThreads) {
-    const long long id = p.list.id(row, j);
-    uint32_t f = 0;
-    if (id >= 0) {
-      if (id < p.V) {
+  if (lister) {
+    for (int j = lane; j < K; j += 32) {
+      const long long id = j < 32 ? id0 : p.list.id(row, j);
+      uint32_t f = 0;
+      if (id >= 0 && index_in(id, p.V, p.err)) {
         f = 1;
-        sm_t[j] = p.list.logit(row, j);
-        sm_z[j] = to_f32(z[id]);
         const long long i = id - v0;
         if (REST && i >= 0 && i < n) {
           const int b = static_cast<int>(i) + shift;
           const uint32_t bit = 1u << (b & 31);
           if (!(atomicOr(&bits[b >> 5], bit) & bit)) f = 3;
         }
-      } else if (p.err) {
-        atomicCAS(p.err, 0, kErrBounds);
       }
+      flags[j] = f | static_cast<uint32_t>(id) << 2;  // (V is below 2^30)
     }
-    flags[j] = f;
   }
   if (REST) __syncthreads();
 
   Sums s;
-  const uint8_t* byte = reinterpret_cast<const uint8_t*>(bits);
-  // columns that are no whole pack: before the first and behind the last
-  const auto single = [&](int i) {
-    const float v = to_f32(mine[i]);
-    if (REST && (bits[(i + shift) >> 5] >> ((i + shift) & 31) & 1u)) return;
-    s.raise(v, c);
-    const float e = ex2(fmaf(v, c, -s.ref));
-    s.rest += e;
-    if (ONE == kOneOwn) s.one += ex2(fmaf(v, kL2e, -s.ref1));
-    if (ONE == kOneSquare) s.one = fmaf(e, e, s.one);
-  };
-  if (tid < head) single(tid);
-  if (tid < n - head - packs * 8) single(head + packs * 8 + tid);
-  for (int first = 0; first < packs; first += U * kThreads) {
-    Pack<T, 8> next[U];
-    load(first + U * kThreads, next);
-    F2 v[U][4];
-    float m = -INFINITY;
+  // the teacher's part of the divergence, its shares' sum and normaliser (rank 0's ninth warp)
+  double own = 0.0, share = 0.0, norm = 0.0, left = 0.0, log_left = 0.0;
+  bool any = false, label_in = false;
+  float z_label = 0.f;
+  if (!lister) {
+    const uint8_t* byte = reinterpret_cast<const uint8_t*>(bits);
+    // columns that are no whole pack: before the first and behind the last
+    const auto single = [&](int i) {
+      const float v = to_f32(mine[i]);
+      if (REST && (bits[(i + shift) >> 5] >> ((i + shift) & 31) & 1u)) return;
+      s.raise(v, c);
+      const float e = ex2(fmaf(v, c, -s.ref));
+      s.rest += e;
+      if (ONE == kOneOwn) s.one += ex2(fmaf(v, kL2e, -s.ref1));
+      if (ONE == kOneSquare) s.one = fmaf(e, e, s.one);
+    };
+    if (tid < head) single(tid);
+    if (tid < n - head - packs * 8) single(head + packs * 8 + tid);
+    for (int first = 0; first < packs; first += U * kThreads) {
+      Pack<T, 8> next[U];
+      load(first + U * kThreads, next);
+      if (REST) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = first + u * kThreads + tid;
-      if (at < packs) {
-        unpack_f2<T, 8>(now[u], v[u]);
-        if (REST) {
-          const uint32_t b = byte[at + 1];
-          if (b) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 h = halves(v[u][i]);
-              v[u][i] = f2((b >> (2 * i)) & 1u ? -INFINITY : h.x,
-                           (b >> (2 * i + 1)) & 1u ? -INFINITY : h.y);
-            }
-          }
+        for (int u = 0; u < U; ++u) {
+          const int at = first + u * kThreads + tid;
+          const uint32_t b = at < packs ? byte[at + 1] : 0u;
+          if (b) mask_out<T>(now[u], b);
         }
+      }
+      s.raise(packs_max<T, U>(now), c);
+      F2 a = f2(0.f), b1 = f2(0.f);
+      const F2 cc = f2(c), nr = f2(-s.ref), cl = f2(kL2e), nr1 = f2(-s.ref1);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        F2 v[4];
+        unpack_f2<T, 8>(now[u], v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 x = halves(fma2(v[i], cc, nr));
+          const F2 e = f2(ex2(x.x), ex2(x.y));
+          a = a + e;
+          if (ONE == kOneOwn) {
+            const float2 y = halves(fma2(v[i], cl, nr1));
+            b1 = b1 + f2(ex2(y.x), ex2(y.y));
+          }
+          if (ONE == kOneSquare) b1 = fma2(e, e, b1);
+        }
+        now[u] = next[u];
+      }
+      s.rest += sum2(a);
+      if (ONE != kOneNone) s.one += sum2(b1);
+    }
+  } else {
+    for (int j = lane; j < K; j += 32) {
+      const uint32_t f = flags[j];
+      if (f & 1) {
+        sm_t[j] = p.list.logit(row, j);
+        sm_z[j] = to_f32(z[f >> 2]);
+      }
+    }
+    if (REST) {  // the listed tokens, once each
+      for (int j = lane; j < K; j += 32) {
+        if (!(flags[j] & 2)) continue;
+        const float v = sm_z[j];
+        s.raise(v, c);
+        s.listed += ex2(fmaf(v, c, -s.ref));
+        if (ONE != kOneNone) s.one += ex2(fmaf(v, kL2e, -s.ref1));
+      }
+    }
+    if (rank == 0) {
+      const double inv_temp = p.inv_temp64;
+      float hi = -INFINITY;
+      for (int j = lane; j < K; j += 32) {
+        if (!(flags[j] & 1)) continue;
+        any = true;
+        hi = fmaxf(hi, sm_t[j]);
+      }
+      any = __any_sync(0xffffffffu, any);
+      if (REST) {
+        norm = p.top_lse[row];
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[u][i] = f2(-INFINITY);
-      }
+        for (int o = 16; o > 0; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        if (hi > -INFINITY) {
+          double sum = 0.0;
+          for (int j = lane; j < K; j += 32)
+            if (flags[j] & 1) sum += exp((static_cast<double>(sm_t[j]) - hi) * inv_temp);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 h = halves(v[u][i]);
-        m = fmaxf(m, fmaxf(h.x, h.y));
-      }
-      now[u] = next[u];
-    }
-    s.raise(m, c);
-    F2 a = f2(0.f), b1 = f2(0.f);
-    const F2 cc = f2(c), nr = f2(-s.ref), cl = f2(kL2e), nr1 = f2(-s.ref1);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 x = halves(fma2(v[u][i], cc, nr));
-        const F2 e = f2(ex2(x.x), ex2(x.y));
-        a = a + e;
-        if (ONE == kOneOwn) {
-          const float2 y = halves(fma2(v[u][i], cl, nr1));
-          b1 = b1 + f2(ex2(y.x), ex2(y.y));
+          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          norm = hi * inv_temp + log(sum);
+        } else {
+          // no entry, or none with a share; a NaN among them stays one
+          float bad = 0.f;
+          for (int j = lane; j < K; j += 32)
+            if ((flags[j] & 1) && sm_t[j] != sm_t[j]) bad = sm_t[j];
+          any = __any_sync(0xffffffffu, bad != bad);
+          norm = any ? static_cast<double>(NAN) : static_cast<double>(-INFINITY);
         }
-        if (ONE == kOneSquare) b1 = fma2(e, e, b1);
       }
-    s.rest += sum2(a);
-    if (ONE != kOneNone) s.one += sum2(b1);
-  }
-  if (REST) {  // the listed tokens, once each
-    for (int j = tid; j < K; j += kThreads) {
-      if (!(flags[j] & 2)) continue;
-      const float v = sm_z[j];
-      s.raise(v, c);
-      s.listed += ex2(fmaf(v, c, -s.ref));
-      if (ONE != kOneNone) s.one += ex2(fmaf(v, kL2e, -s.ref1));
+      if (any) {
+        for (int j = lane; j < K; j += 32) {
+          if (!(flags[j] & 1)) continue;
+          const double log_p = sm_t[j] * inv_temp - norm;
+          const double pj = exp(log_p);
+          share += pj;
+          if (!(pj == 0.0)) own += pj * (log_p - static_cast<double>(sm_z[j]) * c * kLn2);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          own += __shfl_xor_sync(0xffffffffu, own, o);
+          share += __shfl_xor_sync(0xffffffffu, share, o);
+        }
+      }
+      left = share < 1.0 ? 1.0 - share : share >= 1.0 ? 0.0 : share;
+      if (REST) log_left = log(left);
+      if (p.labels) {
+        const long long label = p.labels[row];
+        label_in = label >= 0 && index_in(label, p.V, p.err);
+        if (label_in) z_label = to_f32(z[label]);
+      }
     }
   }
 
@@ -233,37 +345,47 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const DistillArgs
   float m = s.max;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane_id() == 0) red[warp_id()][0] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, red[w][0]);
   s.raise(m, c);
   const float rest = warp_add(s.rest), listed = REST ? warp_add(s.listed) : 0.f;
   const float one = ONE != kOneNone ? warp_add(s.one) : 0.f;
-  if (lane_id() == 0) {
+  if (lane == 0) {
+    red[warp_id()][0] = m;
     red[warp_id()][1] = rest;
     red[warp_id()][2] = listed;
     red[warp_id()][3] = one;
   }
   __syncthreads();
-  if (tid == 0) {
-    float t[3] = {0.f, 0.f, 0.f};
+  if (!lister && splits == 1) return;
+  // Lane b: warp b's sums, or block b's, relative to the largest maximum of all `n` of them.
+  float top, ref, ref1, rest_sum, list_sum, one_sum;
+  const auto join = [&](float bm, float br, float bl, float bo) {
+    top = bm;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w)
-#pragma unroll
-      for (int i = 0; i < 3; ++i) t[i] += red[w][1 + i];
-    joined[0] = m;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) joined[1 + i] = t[i];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    ref = top == -INFINITY ? 0.f : __fmul_rn(top, c);
+    ref1 = top == -INFINITY ? 0.f : __fmul_rn(top, kL2e);
+    const float f = bm == -INFINITY ? 1.f : ex2(__fmul_rn(bm, c) - ref);  // (sums of nothing are zero)
+    const float f1 = bm == -INFINITY ? 1.f : ex2(__fmul_rn(bm, kL2e) - ref1);
+    rest_sum = warp_add(br * f);
+    list_sum = warp_add(bl * f);
+    one_sum = warp_add(bo * f1);
+  };
+  if (lister) {
+    const bool in = lane < kWarps;
+    join(in ? red[lane][0] : -INFINITY, in ? red[lane][1] : 0.f, in ? red[lane][2] : 0.f,
+         in ? red[lane][3] : 0.f);
   }
-  if (splits > 1) cluster_sync(); else __syncthreads();
-  if (rank == 0 && warp_id() == 0) {
-    const int lane = lane_id();
-    // lane b: block b's sums
-    float bm = -INFINITY, br = 0.f, bl = 0.f, bo = 0.f;
-    if (lane < splits) {
-      const auto peer = [&](int i) {
-        if (splits == 1) return joined[i];
+  if (splits > 1) {
+    if (lister && lane == 0) {
+      joined[0] = top;
+      joined[1] = rest_sum;
+      joined[2] = list_sum;
+      joined[3] = one_sum;
+    }
+    cluster_sync();
+    if (lister && rank == 0) {
+      const auto peer = [&](int i, float none) {
+        if (lane >= splits) return none;
         float v;
         asm volatile("ld.shared::cluster.f32 %0, [%1];"
                      : "=f"(v)
@@ -271,105 +393,64 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(const DistillArgs
                      : "memory");
         return v;
       };
-      bm = peer(0);
-      br = peer(1);
-      bl = peer(2);
-      bo = peer(3);
+      join(peer(0, -INFINITY), peer(1, 0.f), peer(2, 0.f), peer(3, 0.f));
     }
-    float top = bm;
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    top = __shfl_sync(0xffffffffu, top, 0);
-    const float ref = top == -INFINITY ? 0.f : __fmul_rn(top, c);
-    const float ref1 = top == -INFINITY ? 0.f : __fmul_rn(top, kL2e);
-    const float f = bm == -INFINITY ? 1.f : ex2(__fmul_rn(bm, c) - ref);  // (sums of nothing are zero)
-    const float f1 = bm == -INFINITY ? 1.f : ex2(__fmul_rn(bm, kL2e) - ref1);
-    const double rest_sum = warp_add(br * f), list_sum = warp_add(bl * f);
-    const double one_sum = warp_add(bo * f1);
-    const double log_all = ref + log2(rest_sum + list_sum);  // base 2
-    const double log_rest = REST ? ref + log2(rest_sum) : log_all;
-
-    // the teacher's shares
-    double norm;
-    bool any = false;
-    for (int j = lane; j < K; j += 32) any = any || (flags[j] & 1);
-    any = __any_sync(0xffffffffu, any);
-    const double inv_temp = p.inv_temp64;
-    if (REST) {
-      norm = p.top_lse[row];
-    } else {
-      float hi = -INFINITY;
-      for (int j = lane; j < K; j += 32)
-        if (flags[j] & 1) hi = fmaxf(hi, sm_t[j]);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      double sum = 0.0;
-      if (hi > -INFINITY) {
-        for (int j = lane; j < K; j += 32)
-          if (flags[j] & 1) sum += exp((static_cast<double>(sm_t[j]) - hi) * inv_temp);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        norm = hi * inv_temp + log(sum);
-      } else {
-        // no entry, or none with a share; a NaN among them stays one
-        float bad = 0.f;
-        for (int j = lane; j < K; j += 32)
-          if ((flags[j] & 1) && sm_t[j] != sm_t[j]) bad = sm_t[j];
-        any = __any_sync(0xffffffffu, bad != bad);
-        norm = any ? static_cast<double>(NAN) : static_cast<double>(-INFINITY);
-      }
-    }
-    double loss = 0.0, share = 0.0;
-    if (any) {
-      for (int j = lane; j < K; j += 32) {
-        if (!(flags[j] & 1)) continue;
-        const double log_p = sm_t[j] * inv_temp - norm;
-        const double pj = exp(log_p);
-        share += pj;
-        if (!(pj == 0.0))
-          loss += pj * (log_p - (static_cast<double>(sm_z[j]) * c - log_all) * kLn2);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        loss += __shfl_xor_sync(0xffffffffu, loss, o);
-        share += __shfl_xor_sync(0xffffffffu, share, o);
-      }
-    }
+  }
+  if (lister && rank == 0) {
+    // the logarithms of the whole, of the rest's part of it, and of the labels' sum, a lane each
+    const double whole = static_cast<double>(rest_sum) + list_sum;
+    const double part = REST ? rest_sum / whole : 1.0;
+    const double logs = log(lane == 0 ? whole : lane == 1 ? part : static_cast<double>(one_sum));
+    const double log_all = ref * kLn2 + __shfl_sync(0xffffffffu, logs, 0);
+    const double log_q = REST ? __shfl_sync(0xffffffffu, logs, 1) : 0.0;
+    const double log_one = ref1 * kLn2 + __shfl_sync(0xffffffffu, logs, 2);
     if (lane == 0) {
+      double loss = any ? own + share * log_all : 0.0;
       double coef = REST || any ? 1.0 : 0.0;
       if (REST) {
-        const double left = share < 1.0 ? 1.0 - share : share >= 1.0 ? 0.0 : share;
-        const double log_q = (log_rest - log_all) * kLn2;
-        const bool some = rest_sum != 0.0;  // tokens outside the list, not all of them at -inf
-        if (some && !(left == 0.0)) loss += left * (log(left) - log_q);
-        coef = some ? (share > 1.0 ? share : 1.0) * exp(log_q) - left : 0.0;
+        const bool some = rest_sum != 0.f;  // tokens outside the list, not all of them at -inf
+        if (some && !(left == 0.0)) loss += left * (log_left - log_q);
+        coef = some ? (share > 1.0 ? share : 1.0) * part - left : 0.0;
       }
       kd[row] = static_cast<float>(loss);
       float4 o;
-      o.x = static_cast<float>(log_all * kLn2);
-      o.y = static_cast<float>(log_rest * kLn2);
+      o.x = static_cast<float>(log_all);
+      o.y = static_cast<float>(log_all + log_q);
       o.z = static_cast<float>(coef);
       o.w = static_cast<float>(norm);
       reinterpret_cast<float4*>(stats)[row] = o;
       if (p.labels) {
-        const double full = ONE == kOneNone ? log_all : ref1 + log2(one_sum);
-        lse[row] = static_cast<float>(full * kLn2);
-        const long long label = p.labels[row];
-        float l = 0.f;
-        if (label >= 0 && index_in(label, p.V, p.err))
-          l = static_cast<float>((full - static_cast<double>(to_f32(z[label])) * kL2e) * kLn2);
-        ce[row] = l;
+        const double full = ONE == kOneNone ? log_all : log_one;
+        lse[row] = static_cast<float>(full);
+        ce[row] = label_in ? static_cast<float>(full - static_cast<double>(z_label) * kL2e * kLn2) : 0.f;
       }
     }
   }
   if (splits > 1) cluster_sync();  // no block leaves while its sums are read
 }
 
-// out = dkd dkd/dz + dce dce/dz of a row, its columns dealt to `splits` blocks.  The whole range is
-// written as for tokens outside the list; then the listed tokens and the label get their own values,
-// from logits that were read before (out may be the logits).
-template <typename T, bool CE>
-__global__ void __launch_bounds__(kThreads) distill_bwd_kernel(
+__device__ __forceinline__ F2 exp_of(F2 v, float scale, float off) {
+  const float2 x = halves(fma2(v, f2(scale), f2(-off)));
+  return f2(ex2(x.x), ex2(x.y));
+}
+// Slots of the table in which the lister finds a token that is named twice.
+__host__ __device__ inline int table_slots(int K) {
+  int n = 64;
+  while (n < 2 * K) n *= 2;
+  return n;
+}
+
+enum { kCeNone = 0, kCeOwn = 1, kCeSame = 2 };
+
+// out = dkd dkd/dz + dce dce/dz of a row, its columns dealt to `splits` blocks.  Eight warps write the
+// whole range as for tokens outside the list; the lister forms the gradients of the listed tokens and
+// of the label meanwhile, and writes them over it, from logits that it reads before anything is written
+// (out may be the logits).
+//
+// At a temperature of one (kCeSame) one exponential serves both losses: softmax(z) is exp(z - base)
+// times the tokens' share of the whole.
+template <typename T, int CE>
+__global__ void __launch_bounds__(kBlock, 4) distill_bwd_kernel(
     const DistillArgs p, const float* __restrict__ stats, const float* __restrict__ lse,
     const float* __restrict__ dkd, const float* __restrict__ dce, const int* __restrict__ row_ids,
     long long n_rows, T* out_all, long long ld_out, int splits, int chunk) {
@@ -377,149 +458,165 @@ __global__ void __launch_bounds__(kThreads) distill_bwd_kernel(
   constexpr int kAlign = 8 * sizeof(T);
   extern __shared__ uint32_t dyn[];
   const int K = p.list.K, tid = threadIdx.x;
-  float* sm_z = reinterpret_cast<float*>(dyn);
-  float* sm_p = sm_z + K;
-  int* sm_id = reinterpret_cast<int*>(sm_p + K);  // -1: not an entry
+  const bool lister = tid >= kThreads;
   const long long r = blockIdx.x / splits;
   const int v0 = (blockIdx.x % splits) * chunk, n = max(0, min(p.V - v0, chunk));
   long long src = row_ids ? row_ids[r] : r;
-  const bool ok = index_in(src, n_rows, p.err);
+  const bool ok = src >= 0 && src < n_rows;
   if (!ok) src = 0;
-  const T* z_row = static_cast<const T*>(p.z) + src * p.ld;
-  const T* z = z_row + v0;
+  const T* z = static_cast<const T*>(p.z) + src * p.ld;
+  const Span<T> span(z + v0, n);
   T* out = out_all + r * ld_out + v0;
+  const bool wide = reinterpret_cast<uintptr_t>(out + span.head) % kAlign == 0;
+  const auto load = [&](int first, Pack<T, 8>* k) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = first + u * kThreads + tid;
+      if (at < span.packs) k[u] = span.pack(at);
+    }
+  };
+  Pack<T, 8> now[U];
+  if (!lister && wide) load(0, now);
+
+  // the row's weights and what they multiply
   const float k = ok ? dkd[r] * p.inv_temp : 0.f;
   long long label = -1;
   float g1 = 0.f;
   if (CE && ok) {
     label = p.labels[src];
-    if (label >= p.V) {
-      index_in(label, p.V, p.err);
-      label = -1;
-    }
-    if (label >= 0) g1 = dce[r];
-    if (g1 == 0.f) label = -1;
+    if (label >= 0 && label < p.V) g1 = dce[r];
   }
-  const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(z) % kAlign);
-  int head = min(n, odd ? (kAlign - odd) / static_cast<int>(sizeof(T)) : 0);
-  const bool wide = reinterpret_cast<uintptr_t>(out + head) % kAlign == 0;
-  if (k == 0.f && g1 == 0.f) {  // nothing comes from this row
-    for (int i = tid; i < n; i += kThreads) out[i] = from_f32<T>(0.f);
-    return;
-  }
-  const float c = p.inv_temp * kL2e;
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
   if (k != 0.f) st = reinterpret_cast<const float4*>(stats)[src];
   const float gk = k * st.z;
   const bool spread = gk != 0.f;  // also a NaN
+  const float c = p.inv_temp * kL2e;
   const float ref = spread ? st.y * kL2e : 0.f;
-  const float ref1 = g1 != 0.f ? lse[src] * kL2e : 0.f;
-  const float all = st.x * kL2e;
-  // the list, and the logits at it
-  const int entries = k != 0.f ? K : 0;
-  for (int j = tid; j < entries; j += kThreads) {
-    const long long id = p.list.id(src, j);
-    int at = -1;
-    sm_p[j] = 0.f;
-    if (id >= 0 && id < p.V) {
-      at = static_cast<int>(id);
-      sm_z[j] = to_f32(z_row[id]);
-      const double pj = exp(p.list.logit(src, j) * p.inv_temp64 - st.w);
-      sm_p[j] = static_cast<float>(pj);
-    } else if (id >= p.V && p.err) {
-      atomicCAS(p.err, 0, kErrBounds);
-    }
-    sm_id[j] = at;
-  }
-  float z_label = 0.f;
-  if (CE && label >= 0) z_label = to_f32(z_row[label]);
+  const float ref1 = CE && g1 != 0.f ? lse[src] * kL2e : 0.f;
 
-  const auto value = [&](float v) {
-    float g = spread ? gk * ex2(fmaf(v, c, -ref)) : 0.f;
-    if (CE && g1 != 0.f) g = fmaf(g1, ex2(fmaf(v, kL2e, -ref1)), g);
-    return g;
-  };
-  if (wide) {
-    const int packs = (n - head) / 8;
-    const int tail = head + packs * 8;
-    float edge = 0.f;
-    if (tid < head) edge = to_f32(z[tid]);
-    if (tid >= 32 && tid - 32 < n - tail) edge = to_f32(z[tail + tid - 32]);
-    Pack<T, 8> now[U];
-    const auto load = [&](int first, Pack<T, 8>* d) {
+  if (!lister) {
+    const auto stream = [&](auto&& value) {
+      const auto one = [&](float v) { return from_f32<T>(halves(value(f2(v))).x); };
+      if (wide) {
+        if (tid < span.head) out[tid] = one(to_f32(span.z[tid]));
+        const int at = span.tail() + tid;
+        if (at < n) out[at] = one(to_f32(span.z[at]));
+        for (int first = 0; first < span.packs; first += U * kThreads) {
+          Pack<T, 8> next[U];
+          load(first + U * kThreads, next);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = first + u * kThreads + tid;
-        if (at < packs) d[u] = load_pack<T, 8>(z + head + at * 8);
+          for (int u = 0; u < U; ++u) {
+            const int i = first + u * kThreads + tid;
+            if (i < span.packs) {
+              F2 v[4];
+              unpack_f2<T, 8>(now[u], v);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) v[j] = value(v[j]);
+              store_f2<T, 8>(out + span.head + i * 8, v);
+            }
+            now[u] = next[u];
+          }
+        }
+      } else {  // packs of the logits and of out have their boundaries at different columns
+        for (int i0 = tid; i0 < n; i0 += 8 * kThreads) {
+          float v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            v[u] = i0 + u * kThreads < n ? to_f32(span.z[i0 + u * kThreads]) : 0.f;
+#pragma unroll
+          for (int u = 0; u < 8; u += 2) {
+            const float2 g = halves(value(f2(v[u], v[u + 1])));
+            if (i0 + u * kThreads < n) out[i0 + u * kThreads] = from_f32<T>(g.x);
+            if (i0 + (u + 1) * kThreads < n) out[i0 + (u + 1) * kThreads] = from_f32<T>(g.y);
+          }
+        }
       }
     };
-    load(0, now);
-    __syncthreads();  // the listed logits are read before anything is written
-    for (int first = 0; first < packs; first += U * kThreads) {
-      Pack<T, 8> next[U];
-      load(first + U * kThreads, next);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = first + u * kThreads + tid;
-        if (at < packs) {
-          F2 v[4];
-          unpack_f2<T, 8>(now[u], v);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            F2 g = f2(0.f);
-            if (spread) {
-              const float2 x = halves(fma2(v[i], f2(c), f2(-ref)));
-              g = f2(gk) * f2(ex2(x.x), ex2(x.y));
-            }
-            if (CE) {
-              const float2 y = halves(fma2(v[i], f2(kL2e), f2(-ref1)));
-              if (g1 != 0.f) g = fma2(f2(g1), f2(ex2(y.x), ex2(y.y)), g);
-            }
-            v[i] = g;
-          }
-          store_f2<T, 8>(out + head + at * 8, v);
-        }
-        now[u] = next[u];
+    // Without a divergence the one exponential is that of the labels' loss.
+    const float ec = spread ? c : kL2e, er = spread ? ref : ref1;
+    float ge = spread ? gk : g1;
+    if (CE == kCeSame && spread && g1 != 0.f) ge = fmaf(g1, ex2(ref - ref1), gk);
+    __syncthreads();  // the lister has read its logits
+    if (!spread && g1 == 0.f) {
+      stream([](F2) { return f2(0.f); });
+    } else if (CE == kCeOwn && spread && g1 != 0.f) {
+      stream([&](F2 v) {
+        return fma2(f2(g1), exp_of(v, kL2e, ref1), f2(ge) * exp_of(v, ec, er));
+      });
+    } else {
+      stream([&](F2 v) { return f2(ge) * exp_of(v, ec, er); });
+    }
+    __syncthreads();  // what was written above is replaced by the lister
+    return;
+  }
+
+  // -------------------------------------------------------------- the lister
+  const int lane = lane_id();
+  if (lane == 0) {  // (recorded once a row)
+    index_in(ok ? 0 : -1, 1, p.err);
+    if (CE && label >= p.V) index_in(label, p.V, p.err);
+  }
+  int* sm_id = reinterpret_cast<int*>(dyn);  // -1: no entry
+  float* sm_p = reinterpret_cast<float*>(sm_id + K);
+  float* sm_g = sm_p + K;
+  int* table = reinterpret_cast<int*>(sm_g + K);
+  const int slots = table_slots(K);
+  const int entries = k != 0.f ? K : 0;
+  for (int i = lane; entries && i < slots; i += 32) table[i] = -1;
+  __syncwarp();
+  const auto in_range = [&](long long v) { return v >= v0 && v < v0 + n; };
+  const bool labelled = g1 != 0.f;
+  float whole = 0.f;
+  bool twice = false, named = false;
+  for (int j = lane; j < entries; j += 32) {
+    const long long id = p.list.id(src, j);
+    int at = -1;
+    float pj = 0.f;
+    if (id >= 0 && index_in(id, p.V, p.err)) {
+      at = static_cast<int>(id);
+      pj = static_cast<float>(exp(p.list.logit(src, j) * p.inv_temp64 - st.w));
+      unsigned slot = static_cast<unsigned>(at) * 2654435761u;
+      for (;; ++slot) {  // (more slots than entries: it ends)
+        const int old = atomicCAS(&table[slot & (slots - 1)], -1, at);
+        twice = twice || old == at;
+        if (old == -1 || old == at) break;
       }
     }
-    if (tid < head) out[tid] = from_f32<T>(value(edge));
-    if (tid >= 32 && tid - 32 < n - tail) out[tail + tid - 32] = from_f32<T>(value(edge));
-  } else {
-    __syncthreads();
-    for (int i0 = tid; i0 < n; i0 += 8 * kThreads) {
-      float v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = i0 + u * kThreads < n ? to_f32(z[i0 + u * kThreads]) : 0.f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (i0 + u * kThreads < n) out[i0 + u * kThreads] = from_f32<T>(value(v[u]));
-    }
+    named = named || (at >= 0 && at == label);
+    whole += pj;
+    sm_id[j] = at;
+    sm_p[j] = pj;
   }
-  __syncthreads();  // what was written above is replaced below
-  const auto in_range = [&](long long v) { return v >= v0 && v < v0 + n; };
-  const float soft_label = CE && label >= 0 ? ex2(fmaf(z_label, kL2e, -ref1)) : 0.f;
-  for (int j = tid; j < entries; j += kThreads) {
-    const int id = sm_id[j];
-    if (id < 0 || !in_range(id)) continue;
-    float share = 0.f, whole = 0.f;  // a token named twice: both threads form the same sum
-    for (int i = 0; i < K; ++i) {
-      whole += sm_p[i];
-      share += sm_id[i] == id ? sm_p[i] : 0.f;
+  whole = warp_add(whole);
+  // what the teacher's terms add up to: one, but for a list of the whole vocabulary
+  if (st.y > -INFINITY) whole = fmaxf(whole, 1.f);
+  named = __any_sync(0xffffffffu, named);
+  twice = __any_sync(0xffffffffu, twice);
+  __syncwarp();
+  for (int j = lane; j < entries; j += 32) {
+    const int at = sm_id[j];
+    if (at < 0 || !in_range(at)) continue;
+    const float v = to_f32(z[at]);
+    float share = sm_p[j];
+    if (twice) {  // the same token's shares, summed in the list's order by each of its entries
+      share = 0.f;
+      for (int i = 0; i < K; ++i) share += sm_id[i] == at ? sm_p[i] : 0.f;
     }
-    // what the teacher's terms add up to: one, but for a list of the whole vocabulary
-    if (st.y > -INFINITY) whole = fmaxf(whole, 1.f);
-    float g = k * fmaf(whole, ex2(fmaf(sm_z[j], c, -all)), -share);
-    if (CE && g1 != 0.f) g += g1 * (ex2(fmaf(sm_z[j], kL2e, -ref1)) - (id == label ? 1.f : 0.f));
-    out[id - v0] = from_f32<T>(g);
+    float g = k * fmaf(whole, ex2(fmaf(v, c, -st.x * kL2e)), -share);
+    if (CE && labelled) g += g1 * (ex2(fmaf(v, kL2e, -ref1)) - (at == label ? 1.f : 0.f));
+    sm_g[j] = g;
   }
-  if (CE && label >= 0 && tid == kThreads - 1 && in_range(label)) {
-    bool listed = false;
-    for (int i = 0; i < entries; ++i) listed = listed || sm_id[i] == label;
-    if (!listed) {
-      const float g = spread ? gk * ex2(fmaf(z_label, c, -ref)) : 0.f;
-      out[label - v0] = from_f32<T>(g + g1 * (soft_label - 1.f));
-    }
+  float label_grad = 0.f;
+  const bool label_alone = CE && labelled && !named && in_range(label);
+  if (label_alone) {
+    const float v = to_f32(z[label]);
+    label_grad = (spread ? gk * ex2(fmaf(v, c, -ref)) : 0.f) + g1 * (ex2(fmaf(v, kL2e, -ref1)) - 1.f);
   }
+  __syncthreads();
+  __syncthreads();
+  for (int j = lane; j < entries; j += 32)
+    if (sm_id[j] >= 0 && in_range(sm_id[j])) out[sm_id[j] - v0] = from_f32<T>(sm_g[j]);
+  if (label_alone && lane == 0) out[label - v0] = from_f32<T>(label_grad);
 }
 
 }  // namespace cfb
@@ -554,7 +651,7 @@ int launch_fwd(const DistillArgs& a, float* kd, float* ce, float* lse, float* st
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows) * splits);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kBlock);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -611,16 +708,17 @@ int cfb_distill_bwd(const CfbDistill* p, const float* stats, const float* lse, c
   const DistillArgs a = args_of(p);
   const int splits = splits_of(rows, p->V, 4096, 16);
   const int chunk = chunk_of(p->V, splits);
-  const int smem = 12 * p->K;
+  const int smem = 12 * p->K + 4 * table_slots(p->K);
   return with_type(p->type, [&](auto tag) {
     using T = typename decltype(tag)::type;
     const unsigned grid = static_cast<unsigned>(rows) * splits;
-    if (p->labels)
-      distill_bwd_kernel<T, true><<<grid, kThreads, smem, st>>>(
-          a, stats, lse, dkd, dce, row_ids, n_rows, static_cast<T*>(out), ld_out, splits, chunk);
-    else
-      distill_bwd_kernel<T, false><<<grid, kThreads, smem, st>>>(
-          a, stats, lse, dkd, dce, row_ids, n_rows, static_cast<T*>(out), ld_out, splits, chunk);
+    const auto launch = [&](auto* kernel) {
+      kernel<<<grid, kBlock, smem, st>>>(a, stats, lse, dkd, dce, row_ids, n_rows,
+                                         static_cast<T*>(out), ld_out, splits, chunk);
+    };
+    if (!p->labels) launch(distill_bwd_kernel<T, kCeNone>);
+    else if (p->temperature == 1.0) launch(distill_bwd_kernel<T, kCeSame>);
+    else launch(distill_bwd_kernel<T, kCeOwn>);
     return launch_status();
   });
 }

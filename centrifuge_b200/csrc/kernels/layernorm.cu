@@ -9,6 +9,7 @@
 // Bound by memory: each row is read once and stays in registers for the second sum (the squares are
 // of x - mu, so a mean far from zero costs no digits); sums are fp32, each output is rounded once.
 #include "row_types.cuh"
+#include <cstdlib>
 
 namespace cfb {
 
@@ -658,6 +659,27 @@ int cfb_layernorm_fwd(const void* x, int x_type, long long ld_x, const void* w, 
     using TX = typename decltype(tx)::type;
 #define CFB_FWD(NW, NV, R) return launch_fwd<TY, TX, NW, NV, R>(a, st)
     if (W == 8) {
+      static const int var = getenv("CFB_LN") ? atoi(getenv("CFB_LN")) : 0;
+      if (var == 1) {
+        if (H <= 1024) CFB_FWD(1, 4, 1);
+        if (H <= 2048) CFB_FWD(1, 8, 1);
+        if (H <= 4096) CFB_FWD(2, 8, 1);
+      }
+      if (var == 2) {
+        if (H <= 1024) CFB_FWD(1, 4, 2);
+        if (H <= 2048) CFB_FWD(2, 4, 1);
+        if (H <= 4096) CFB_FWD(4, 4, 1);
+      }
+      if (var == 3) {
+        if (H <= 1024) CFB_FWD(1, 4, 1);
+        if (H <= 2048) CFB_FWD(2, 4, 2);
+        if (H <= 4096) CFB_FWD(4, 4, 2);
+      }
+      if (var == 4) {
+        if (H <= 1024) CFB_FWD(2, 2, 2);
+        if (H <= 2048) CFB_FWD(4, 2, 1);
+        if (H <= 4096) CFB_FWD(8, 2, 1);
+      }
       if (rows >= 148 * 8 && sizeof(TX) == 2) {  // several rows a team pay with blocks enough
         if (H <= 256) CFB_FWD(1, 1, 4);
         if (H <= 512) CFB_FWD(1, 2, 2);
