@@ -28,8 +28,12 @@ namespace cfb {
 
 constexpr float kL2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
-constexpr int kThreads = 256;             // the streaming warps'
-constexpr int kBlock = kThreads + 32;    // ... and the lister's
+// A row is streamed by four warps, seven such blocks to an SM: while some wait for their list or sums,
+// others stream (16384 x 32000 bf16 with tail and labels, tau = 2: 213 us; with eight warps and four
+// blocks 237, with two and twelve 212; the gradient of 8192 of its rows 181, 193 and 192 us).
+constexpr int kThreads = 128;          // the streaming warps'
+constexpr int kBlock = kThreads + 32;  // ... and the lister's
+constexpr int kBlocksPerSm = 7;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -155,11 +159,11 @@ struct Span {
 // of the other (tau = 2), which halves the exponentials of a kernel that they would bind.
 enum { kOneNone = 0, kOneOwn = 1, kOneSquare = 2 };
 
-// A row to a block (or, split over its columns, to a cluster of up to eight): eight warps stream the
-// logits, a ninth reads the list, marks its tokens in a bit mask in shared memory for the others, and
+// A row to a block (or, split over its columns, to a cluster of up to eight): four warps stream the
+// logits, a fifth reads the list, marks its tokens in a bit mask in shared memory for the others, and
 // forms the teacher's terms in 64 bits while they work.
 template <typename T, bool REST, int ONE>
-__global__ void __launch_bounds__(kBlock, 4) distill_fwd_kernel(
+__global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
     const DistillArgs p, int splits, int chunk, float* __restrict__ kd, float* __restrict__ ce,
     float* __restrict__ lse, float* __restrict__ stats) {
   constexpr int U = sizeof(T) == 2 ? 4 : 2;  // packs of eight in flight, and as many at work
@@ -218,7 +222,7 @@ __global__ void __launch_bounds__(kBlock, 4) distill_fwd_kernel(
   if (REST) __syncthreads();
 
   Sums s;
-  // the teacher's part of the divergence, its shares' sum and normaliser (rank 0's ninth warp)
+  // the teacher's part of the divergence, its shares' sum and normaliser (rank 0's lister)
   double own = 0.0, share = 0.0, norm = 0.0, left = 0.0, log_left = 0.0;
   bool any = false, label_in = false;
   float z_label = 0.f;
@@ -442,7 +446,7 @@ __host__ __device__ inline int table_slots(int K) {
 
 enum { kCeNone = 0, kCeOwn = 1, kCeSame = 2 };
 
-// out = dkd dkd/dz + dce dce/dz of a row, its columns dealt to `splits` blocks.  Eight warps write the
+// out = dkd dkd/dz + dce dce/dz of a row, its columns dealt to `splits` blocks.  Four warps write the
 // whole range as for tokens outside the list; the lister forms the gradients of the listed tokens and
 // of the label meanwhile, and writes them over it, from logits that it reads before anything is written
 // (out may be the logits).
@@ -450,7 +454,7 @@ enum { kCeNone = 0, kCeOwn = 1, kCeSame = 2 };
 // At a temperature of one (kCeSame) one exponential serves both losses: softmax(z) is exp(z - base)
 // times the tokens' share of the whole.
 template <typename T, int CE>
-__global__ void __launch_bounds__(kBlock, 4) distill_bwd_kernel(
+__global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
     const DistillArgs p, const float* __restrict__ stats, const float* __restrict__ lse,
     const float* __restrict__ dkd, const float* __restrict__ dce, const int* __restrict__ row_ids,
     long long n_rows, T* out_all, long long ld_out, int splits, int chunk) {
@@ -668,11 +672,11 @@ int launch_fwd(const DistillArgs& a, float* kd, float* ce, float* lse, float* st
   return 0;
 }
 
-// Blocks to a row: one where there are rows enough for the SMs, else up to `most` with at least
-// `least` columns each.
-int splits_of(int rows, int V, int least, int most) {
+// Blocks to a row: one where the rows fill `waves` waves of blocks, else up to `most` with at least
+// 4096 columns each.
+int splits_of(int rows, int V, int waves, int most) {
   int s = 1;
-  while (s < most && rows * s < 148 * 4 && V / (2 * s) >= least) s *= 2;
+  while (s < most && rows * s < 148 * kBlocksPerSm * waves && V / (2 * s) >= 4096) s *= 2;
   return s;
 }
 int chunk_of(int V, int splits) { return splits == 1 ? V : (V + splits * 16 - 1) / (splits * 16) * 16; }
@@ -683,7 +687,7 @@ int cfb_distill_fwd(const CfbDistill* p, float* kd, float* ce, float* lse, float
                     cudaStream_t st) {
   if (rows == 0) return 0;
   const DistillArgs a = args_of(p);
-  const int splits = splits_of(rows, p->V, 4096, 8);
+  const int splits = splits_of(rows, p->V, 1, 8);
   const int chunk = chunk_of(p->V, splits);
   const int one = !p->labels || p->temperature == 1.0 ? kOneNone
                   : p->temperature == 2.0             ? kOneSquare
@@ -706,7 +710,7 @@ int cfb_distill_bwd(const CfbDistill* p, const float* stats, const float* lse, c
                     long long ld_out, int rows, cudaStream_t st) {
   if (rows == 0) return 0;
   const DistillArgs a = args_of(p);
-  const int splits = splits_of(rows, p->V, 4096, 16);
+  const int splits = splits_of(rows, p->V, 2, 16);
   const int chunk = chunk_of(p->V, splits);
   const int smem = 12 * p->K + 4 * table_slots(p->K);
   return with_type(p->type, [&](auto tag) {

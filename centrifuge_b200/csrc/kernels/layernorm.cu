@@ -9,7 +9,6 @@
 // Bound by memory: each row is read once and stays in registers for the second sum (the squares are
 // of x - mu, so a mean far from zero costs no digits); sums are fp32, each output is rounded once.
 #include "row_types.cuh"
-#include <cstdlib>
 
 namespace cfb {
 
@@ -42,17 +41,24 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_kernel(
       xp[k][r] = c < H && row0 + r < rows ? load_pack<TX, W>(x + (row0 + r) * ld_x + c)
                                           : zero_pack<TX, W>();
   }
+  Pack<TY, W> wp[NV], bp[NV];  // on their way while the rows' sums are formed
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (tid + k * nt) * W;
+    if (w && c < H) wp[k] = load_pack<TY, W>(w + c);
+    if (b && c < H) bp[k] = load_pack<TY, W>(b + c);
+  }
   const float inv_h = 1.f / static_cast<float>(H);
   float mu[R], sq[R];
+  F2 xv[NV][R][P];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     F2 s = f2(0.f);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      F2 v[P];
-      unpack_f2<TX, W>(xp[k][r], v);
+      unpack_f2<TX, W>(xp[k][r], xv[k][r]);
 #pragma unroll
-      for (int i = 0; i < P; ++i) s = s + v[i];
+      for (int i = 0; i < P; ++i) s = s + xv[k][r][i];
     }
     mu[r] = sum2(s);
   }
@@ -64,12 +70,10 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_kernel(
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       if ((tid + k * nt) * W >= H) continue;
-      F2 v[P];
-      unpack_f2<TX, W>(xp[k][r], v);
 #pragma unroll
       for (int i = 0; i < P; ++i) {
-        v[i] = v[i] + f2(-mu[r]);
-        s = fma2(v[i], v[i], s);
+        xv[k][r][i] = xv[k][r][i] + f2(-mu[r]);
+        s = fma2(xv[k][r][i], xv[k][r][i], s);
       }
     }
     sq[r] = sum2(s);
@@ -88,8 +92,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_kernel(
     const int c = (tid + k * nt) * W;
     if (c >= H) continue;
     F2 wv[P], bv[P];
-    if (w) load_f2<TY, W>(w + c, wv);
-    if (b) load_f2<TY, W>(b + c, bv);
+    if (w) unpack_f2<TY, W>(wp[k], wv);
+    if (b) unpack_f2<TY, W>(bp[k], bv);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       if (!w) wv[i] = f2(1.f);
@@ -97,12 +101,10 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_kernel(
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      F2 v[P];
-      unpack_f2<TX, W>(xp[k][r], v);
+      F2 o[P];
 #pragma unroll
-      for (int i = 0; i < P; ++i)
-        v[i] = fma2((v[i] + f2(-mu[r])) * f2(sq[r]), wv[i], bv[i]);
-      if (row0 + r < rows) store_f2<TY, W>(y + (row0 + r) * ld_y + c, v);
+      for (int i = 0; i < P; ++i) o[i] = fma2(xv[k][r][i] * f2(sq[r]), wv[i], bv[i]);
+      if (row0 + r < rows) store_f2<TY, W>(y + (row0 + r) * ld_y + c, o);
     }
   }
 }
@@ -659,27 +661,6 @@ int cfb_layernorm_fwd(const void* x, int x_type, long long ld_x, const void* w, 
     using TX = typename decltype(tx)::type;
 #define CFB_FWD(NW, NV, R) return launch_fwd<TY, TX, NW, NV, R>(a, st)
     if (W == 8) {
-      static const int var = getenv("CFB_LN") ? atoi(getenv("CFB_LN")) : 0;
-      if (var == 1) {
-        if (H <= 1024) CFB_FWD(1, 4, 1);
-        if (H <= 2048) CFB_FWD(1, 8, 1);
-        if (H <= 4096) CFB_FWD(2, 8, 1);
-      }
-      if (var == 2) {
-        if (H <= 1024) CFB_FWD(1, 4, 2);
-        if (H <= 2048) CFB_FWD(2, 4, 1);
-        if (H <= 4096) CFB_FWD(4, 4, 1);
-      }
-      if (var == 3) {
-        if (H <= 1024) CFB_FWD(1, 4, 1);
-        if (H <= 2048) CFB_FWD(2, 4, 2);
-        if (H <= 4096) CFB_FWD(4, 4, 2);
-      }
-      if (var == 4) {
-        if (H <= 1024) CFB_FWD(2, 2, 2);
-        if (H <= 2048) CFB_FWD(4, 2, 1);
-        if (H <= 4096) CFB_FWD(8, 2, 1);
-      }
       if (rows >= 148 * 8 && sizeof(TX) == 2) {  // several rows a team pay with blocks enough
         if (H <= 256) CFB_FWD(1, 1, 4);
         if (H <= 512) CFB_FWD(1, 2, 2);

@@ -127,7 +127,8 @@ __device__ __forceinline__ void with_act(int act, F&& f) {
 // ---------------------------------------------------------------- the product
 struct LinearArgs {
   int M, N, K;
-  int a_mn, b_mn;   // operands [K, M], [K, N] in memory instead of [M, K], [N, K]
+  int a_mn, b_mn;   // operands [K, M], [K, N] in memory instead of [M, K], [N, K] (as template
+                    // arguments they made the forward slower: 260 us for 254)
   int a_3d, b_3d;   // ... whose tiles one copy brings: {64 columns, k, groups of 64 columns}
   uint32_t idesc;   // instruction descriptor: shape, types and layouts
   int full;         // units below this are whole tiles, the others pieces of the tiles behind them
@@ -756,6 +757,326 @@ __global__ void __launch_bounds__(kLinearThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- few tiles
+// Issued by lane 0 through a predicate inside, in code that the whole warp runs: the addresses and
+// descriptors are then the warp's.  In a branch of lane 0, where they are moved to uniform registers for
+// every instruction, a block of four products took 665 clocks, 513 so.  (The kernel of many tiles, whose
+// products take as long, gained nothing: 262 us for 254.)
+__device__ __forceinline__ void mma_lane0(int lane, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.eq.s32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lane)
+      : "memory");
+}
+// Arrives on `bar` when the products issued before are done.
+__device__ __forceinline__ void commit_lane0(int lane, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.eq.s32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(lane)
+      : "memory");
+}
+
+// One tile of 128 x 128 to a cluster of up to eight CTAs, each with a part of k: an SM takes in about
+// 64 bytes of operands a clock, so that a few tiles with a long k leave most of the machine idle (16 x
+// 8192 by 2048 x 8192: 45 us with a CTA pair for each 256 columns).  Every CTA puts its sums into its
+// shared memory; behind a cluster barrier each finishes 128 / splits rows, adding the parts in order
+// (the same bits on every run), with accesses to global memory along the rows.
+//
+// Of rows of A and B that do not exist only the ones up to a multiple of eight are copied; what the
+// products make of the rest of a stage is never read.
+struct SplitShape {
+  static constexpr int BM = 128, BN = 128, BK = 64;
+  static constexpr int A_BYTES = BM * BK * 2, STAGE_BYTES = A_BYTES + BN * BK * 2;
+  static constexpr int STAGES = 6;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/;
+  static constexpr int ROW = BN + 4;  // floats between rows of the sums
+};
+constexpr int kSplitThreads = 320;  // producer, issuer, eight epilogue warps
+
+template <typename T, int KIND>
+__global__ void __launch_bounds__(kSplitThreads, 1)
+    linear_split_kernel(const __grid_constant__ CUtensorMap tmA,
+                        const __grid_constant__ CUtensorMap tmB, const LinearArgs p, int splits,
+                        int a_rows, int b_rows) {
+  using S = SplitShape;
+  constexpr bool A_MN = KIND == kLinearWgrad, B_MN = KIND != kLinearFwd;
+  // wgrad: an accumulator for every 1024 rows, up to four (see kSegment)
+  constexpr int kAccumulators = KIND == kLinearWgrad ? 4 : 1;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE_BYTES);
+  uint64_t* empty = full + S::STAGES;
+  uint64_t* done = empty + S::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = warp_id(), lane = lane_id();
+  const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int tile = blockIdx.x / splits;
+  const int num_n = (p.N + S::BN - 1) / S::BN;
+  const int m0 = tile / num_n * S::BM, n0 = tile % num_n * S::BN;
+  const int num_kb = (p.K + S::BK - 1) / S::BK;
+  const int kb0 = static_cast<int>(static_cast<long long>(rank) * num_kb / splits);
+  const int kb1 = static_cast<int>(static_cast<long long>(rank + 1) * num_kb / splits);
+  int per_acc = kSegment;  // blocks of k an accumulator takes
+  if (KIND != kLinearWgrad) per_acc = kb1 - kb0;
+  else if (kb1 - kb0 > kAccumulators * kSegment) per_acc = (kb1 - kb0 + kAccumulators - 1) / kAccumulators;
+  const uint32_t smem_base = smem_u32(smem);
+  const uint32_t bytes = (A_MN ? 2 * 8192 : a_rows * 128) + (B_MN ? 2 * 8192 : b_rows * 128);
+  const auto fill = [&](int kb) {  // the copies of block kb0 + kb
+    const int stage = kb % S::STAGES, k0 = (kb0 + kb) * S::BK;
+    const uint32_t bar = smem_u32(&full[stage]);
+    const uint32_t sa = smem_base + stage * S::STAGE_BYTES, sb = sa + S::A_BYTES;
+    mbar_arrive_expect_tx(bar, bytes);
+    if constexpr (A_MN) {
+      tma_load_2d(sa, &tmA, bar, m0, k0);
+      tma_load_2d(sa + 8192, &tmA, bar, m0 + 64, k0);
+    } else {
+      tma_load_2d(sa, &tmA, bar, k0, m0);
+    }
+    if constexpr (B_MN) {
+      tma_load_2d(sb, &tmB, bar, n0, k0);
+      tma_load_2d(sb + 8192, &tmB, bar, n0 + 64, k0);
+    } else {
+      tma_load_2d(sb, &tmB, bar, k0, n0);
+    }
+  };
+
+  const int blocks = kb1 - kb0, ahead = min(blocks, S::STAGES);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(done), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    after_previous();  // (an operand that was laid out anew)
+    for (int kb = 0; kb < ahead; ++kb) fill(kb);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), S::BN * kAccumulators);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  after_previous();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      int kb = ahead;
+      for (; kb < blocks; ++kb) {
+        ok = mbar_wait(smem_u32(&empty[kb % S::STAGES]), ((kb / S::STAGES) & 1) ^ 1, abort_flag,
+                       p.err, kErrWaitProducer);
+        if (!ok) break;
+        fill(kb);
+      }
+      if (!ok) tma_drain_ring(full, S::STAGES, kb);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t a_step = A_MN ? 2048 : 32, a_lbo = A_MN ? 8192 : 16;
+    constexpr uint32_t b_step = B_MN ? 2048 : 32, b_lbo = B_MN ? 8192 : 16;
+    int stage = 0, in_acc = 0;
+    uint32_t phase = 0, d = tmem_base;
+    bool ready = false;
+    for (int kb = 0; kb < blocks; ++kb) {
+      if (!ready && !mbar_wait(smem_u32(&full[stage]), phase, abort_flag, p.err, kErrWaitMma)) break;
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t sa = smem_base + stage * S::STAGE_BYTES, sb = sa + S::A_BYTES;
+#pragma unroll
+      for (int k = 0; k < S::BK / 16; ++k)
+        mma_lane0(lane, d, sdesc_sw128(sa + k * a_step, a_lbo, 1024),
+                     sdesc_sw128(sb + k * b_step, b_lbo, 1024), p.idesc, in_acc != 0 || k != 0);
+      const uint32_t freed = smem_u32(&empty[stage]);
+      if (++stage == S::STAGES) {
+        stage = 0;
+        phase ^= 1;
+      }
+      ready = kb + 1 < blocks && mbar_try_wait(smem_u32(&full[stage]), phase);
+      commit_lane0(lane, freed);
+      if (++in_acc == per_acc) {
+        in_acc = 0;
+        d += S::BN;
+      }
+    }
+    commit_lane0(lane, smem_u32(done));
+    __syncwarp();
+  }
+  // All products are done (waited for by everyone: the stages become the place of the sums, and TMEM
+  // is given up).
+  volatile int never = 0;
+  const bool ok = mbar_wait_idle(smem_u32(done), 0, &never, p.err, kErrWaitEpilogue) && !*abort_flag;
+  tc_fence_after();
+  float* sums = reinterpret_cast<float*>(smem);
+  if (warp >= 2 && ok) {
+    const int q = warp & 3, c0 = (warp - 2) / 4 * 64;
+    const uint32_t from = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c0;
+    uint32_t r[2][32];
+    CFB_TMEM_LD32(from, r[0]);
+    CFB_TMEM_LD32(from + 32, r[1]);
+    tmem_ld_wait();
+    for (int a = 1; a * per_acc < blocks; ++a) {  // (wgrad's other accumulators)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t more[32];
+        CFB_TMEM_LD32(from + a * S::BN + h * 32, more);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          r[h][i] = __float_as_uint(__uint_as_float(r[h][i]) + __uint_as_float(more[i]));
+      }
+    }
+    float* row = sums + (q * 32 + lane) * S::ROW + c0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        reinterpret_cast<uint4*>(row + h * 32)[i] =
+            make_uint4(r[h][4 * i], r[h][4 * i + 1], r[h][4 * i + 2], r[h][4 * i + 3]);
+  }
+  tc_fence_before();
+  if (splits > 1) cluster_sync(); else __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem_base, S::BN * kAccumulators);
+  }
+
+  if (warp >= 2 && ok) {
+    // The rows are dealt to the CTAs and their warps one by one, four to a turn, whose arithmetic runs
+    // together.  A lane has four neighbouring columns, or, where rows do not start on 16 bytes and at
+    // the last columns, every 32nd, which keeps the warp's accesses together.
+    const int rows = min(S::BM, p.M - m0);
+    constexpr int U = 4;
+    const auto finish = [&](auto act_tag, auto vec_tag) {
+      constexpr int ACT = decltype(act_tag)::act;
+      constexpr bool VEC = decltype(vec_tag)::value;
+      const int c = VEC ? lane * 4 : lane, col = n0 + c;
+      constexpr int kStep = VEC ? 1 : 32;
+      const int n = p.N - col;  // columns from the lane's first
+      const auto get = [&](const auto* from, float* f) {
+        if constexpr (VEC) load_f32<typename std::remove_const<typename std::remove_pointer<decltype(from)>::type>::type, 4>(from, f);
+        else
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = i * kStep < n ? to_f32(from[i * kStep]) : 0.f;
+      };
+      float bias[4] = {0.f, 0.f, 0.f, 0.f};
+      if (KIND == kLinearFwd && p.bias)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i * kStep < n) bias[i] = to_f32(static_cast<const T*>(p.bias)[col + i * kStep]);
+      for (int r0 = rank + (warp - 2) * splits; r0 < rows; r0 += 8 * U * splits) {
+        F2 v[U][2], other[U][2];
+        bool known[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + 8 * u * splits;
+          const long long row = m0 + r;
+          float f[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
+          known[u] = false;
+          if (r < rows && n > 0) {
+            if (KIND == kLinearFwd && p.R) get(static_cast<const T*>(p.R) + row * p.ldr + col, g);
+            if (KIND == kLinearDgrad) {
+              const long long src = p.z_rows ? p.z_rows[row] : row;
+              known[u] = index_in(src, p.n_z, p.err);  // (if not: recorded, and a zero row)
+              if (known[u]) get(static_cast<const T*>(p.Z) + src * p.ldz + col, g);
+            }
+            if (KIND == kLinearWgrad && p.add)
+              get(static_cast<const float*>(p.D) + row * p.ldd + col, g);
+            const float* mine = sums + r * S::ROW + c;
+            if (splits == 1) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) f[i] = mine[i * kStep];
+            } else {
+              float q[8][4];
+#pragma unroll
+              for (int s = 0; s < 8; ++s) {
+                if (s >= splits) continue;
+                const uint32_t at = mapa_shared(smem_u32(mine), s);
+                if constexpr (VEC) {
+                  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                               : "=f"(q[s][0]), "=f"(q[s][1]), "=f"(q[s][2]), "=f"(q[s][3])
+                               : "r"(at)
+                               : "memory");
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                 : "=f"(q[s][i])
+                                 : "r"(at + i * kStep * 4)
+                                 : "memory");
+                }
+              }
+#pragma unroll
+              for (int s = 0; s < 8; ++s)
+                if (s < splits)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) f[i] += q[s][i];
+            }
+          }
+          v[u][0] = f2(f[0], f[1]);
+          v[u][1] = f2(f[2], f[3]);
+          other[u][0] = f2(g[0], g[1]);
+          other[u][1] = f2(g[2], g[3]);
+        }
+        const auto put = [&](auto* base, long long ld) {
+          using O = typename std::remove_pointer<decltype(base)>::type;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int r = r0 + 8 * u * splits;
+            if (r >= rows || n <= 0) continue;
+            const float2 a = halves(v[u][0]), b = halves(v[u][1]);
+            const float f[4] = {a.x, a.y, b.x, b.y};
+            O* to = base + static_cast<long long>(m0 + r) * ld + col;
+            if constexpr (VEC) store_f32<O, 4>(to, f);
+            else
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (i * kStep < n) to[i * kStep] = from_f32<O>(f[i]);
+          }
+        };
+        if constexpr (KIND == kLinearFwd) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            v[u][0] = v[u][0] + f2(bias[0], bias[1]);
+            v[u][1] = v[u][1] + f2(bias[2], bias[3]);
+          }
+          if (p.Z) put(static_cast<T*>(p.Z), p.ldz);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if constexpr (KIND == kLinearDgrad)
+              v[u][i] = known[u] ? v[u][i] * act_slope<ACT>(other[u][i]) : f2(0.f);
+            else
+              v[u][i] = act_of<ACT>(v[u][i]) + other[u][i];
+          }
+        if constexpr (KIND == kLinearWgrad) put(static_cast<float*>(p.D), p.ldd);
+        else put(static_cast<T*>(p.D), p.ldd);
+      }
+    };
+    const bool vec = p.vec != kRowsAny && (n0 + S::BN <= p.N || p.N % 4 == 0);
+    const auto either = [&](auto act_tag) {
+      if (vec) finish(act_tag, std::true_type());
+      else finish(act_tag, std::false_type());
+    };
+    if constexpr (KIND == kLinearWgrad) either(ActTag<kActNone>());
+    else with_act(p.act, either);
+  }
+  if (splits > 1) cluster_sync();  // no CTA leaves while its sums are read
+}
+
 // ---------------------------------------------------------------- layout and column sums
 // dst [rows, ld_dst] = src [rows, cols] (2-byte elements)
 __global__ void __launch_bounds__(256) relayout_kernel(const unsigned short* __restrict__ src,
@@ -879,30 +1200,110 @@ int launch_linear(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMa
   return 0;
 }
 
+// How many clusters of `splits` CTAs of the split kernel run at once: an SM takes one CTA, and a cluster
+// does not cross a group of SMs, so fewer than 148 / splits may fit (15 of eight).
+int split_clusters(int splits) {
+  static int known[4] = {};
+  const int at = splits == 8 ? 3 : splits == 4 ? 2 : 1;
+  if (known[at] == 0) {
+    auto* kernel = linear_split_kernel<__nv_bfloat16, kLinearFwd>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(148 / splits * splits);
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = SplitShape::SMEM_BYTES;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = splits;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             SplitShape::SMEM_BYTES) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known[at] = n;
+  }
+  return known[at];
+}
+
+template <typename T, int KIND>
+int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, const LinearArgs& a, int splits,
+                 int a_rows, int b_rows, bool behind, cudaStream_t st) {
+  auto* kernel = linear_split_kernel<T, KIND>;
+  static bool allowed[kMaxDevices] = {};
+  const int dev = current_device();
+  if (dev < 0) return -3;
+  if (!allowed[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             SplitShape::SMEM_BYTES) != cudaSuccess) {
+      cudaGetLastError();
+      return -3;
+    }
+    allowed[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(((a.M + 127) / 128) * ((a.N + 127) / 128) * splits);
+  cfg.blockDim = dim3(kSplitThreads);
+  cfg.dynamicSmemBytes = SplitShape::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  if (splits > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (behind) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cfg.attrs = attr;
+  if (cudaLaunchKernelEx(&cfg, kernel, ta, tb, a, splits, a_rows, b_rows) != cudaSuccess) {
+    cudaGetLastError();
+    return -3;
+  }
+  ++cfb_row_launches();
+  return 0;
+}
+
 // How the output is cut: the tile (a 256 x 256 pair tile, or 128 x bn of one CTA), and the pieces that
 // the tiles of the pair's last wave are cut into.
 struct LinearPlan {
   int cg, bn;
   long long full;
   int pieces;
+  int splits;  // 0, or the parts of k of linear_split_kernel
 };
 // The least estimated time, in units of a pair tile: waves over the SMs times the time of a tile.  A
 // piece of half or a quarter of the columns takes 0.56 or 0.4 of a tile's time (the products of fewer
 // columns are bound by shared memory), the tiles of one CTA 0.73 (128 columns, half of the elements of
 // a CTA's share of a pair tile) and 0.5 (64 columns).
-LinearPlan plan_linear(long long M, long long N) {
+template <typename F>
+LinearPlan plan_linear(long long M, long long N, long long K, F&& clusters) {
+  // Where 128 x 128 tiles fill the SMs at most once, each is split over as many CTAs as that leaves,
+  // down to four blocks of 64 of k.
+  const long long small = ((M + 127) / 128) * ((N + 127) / 128);
+  if (small <= 148) {
+    int splits = 1;
+    while (splits < 8 && small <= clusters(splits * 2) && K >= 2 * splits * 256) splits *= 2;
+    return {1, 128, small, 1, splits};
+  }
   const auto waves = [](long long units, int slots) { return (units + slots - 1) / slots; };
   const long long pairs = ((M + 255) / 256) * ((N + 255) / 256);
   const long long full = pairs / 74 * 74, rest = pairs - full;
   double best = full / 74 + (rest > 0 ? 1.0 : 0.0);
-  LinearPlan plan = {2, 256, pairs, 1};
+  LinearPlan plan = {2, 256, pairs, 1, 0};
   const double times[] = {0.56, 0.4};
   for (int i = 0; i < 2 && rest > 0; ++i) {
     const int pieces = 2 << i;
     const double t = full / 74 + times[i] * waves(rest * pieces, 74);
     if (t < best) {
       best = t;
-      plan = {2, 256, full, pieces};
+      plan = {2, 256, full, pieces, 0};
     }
   }
   const double singles[] = {0.73, 0.5};
@@ -912,7 +1313,7 @@ LinearPlan plan_linear(long long M, long long N) {
     const double t = singles[i] * waves(tiles, 148);
     if (t < best) {
       best = t;
-      plan = {1, bn, tiles, 1};
+      plan = {1, bn, tiles, 1, 0};
     }
   }
   return plan;
@@ -1020,7 +1421,7 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
   if (rc) return rc;
   rc = lay_out(ob, work, st);
   if (rc) return rc;
-  const LinearPlan pl = plan_linear(p->M, p->N);
+  const LinearPlan pl = plan_linear(p->M, p->N, p->K, split_clusters);
   LinearArgs a = {};
   a.M = p->M;
   a.N = p->N;
@@ -1030,16 +1431,21 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
   a.idesc = idesc_bf16_f32(128 * pl.cg, pl.bn, a.a_mn, a.b_mn);
   if (p->type == kF16) a.idesc &= ~((1u << 7) | (1u << 10));  // f16 operands
   const int b_rows = pl.bn / pl.cg;
-  a.a_3d = a.a_mn && oa.cols % 64 == 0;  // (128 columns of a tile)
-  a.b_3d = a.b_mn && ob.cols % 64 == 0 && b_rows == 128;
+  // (rows of a K-major operand that a few-tile kernel copies: those there are, in eights)
+  const auto rows_of_box = [&](int rows, int box) {
+    return pl.splits && rows < box ? (rows + 7) / 8 * 8 : box;
+  };
+  const int box_a = rows_of_box(p->M, 128), box_b = rows_of_box(p->N, b_rows);
+  a.a_3d = a.a_mn && oa.cols % 64 == 0 && !pl.splits;  // (128 columns of a tile)
+  a.b_3d = a.b_mn && ob.cols % 64 == 0 && b_rows == 128 && !pl.splits;
   CUtensorMap ta, tb, tp;
   rc = a.a_3d   ? make_tmap_3d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 2)
        : a.a_mn ? make_tmap_2d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 64)
-                : make_tmap_2d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, 128);
+                : make_tmap_2d_bf16(&ta, oa.p, oa.rows, oa.cols, oa.ld, 64, box_a);
   if (rc) return rc * 100 - 1;
   rc = a.b_3d   ? make_tmap_3d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, 2)
        : a.b_mn ? make_tmap_2d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, 64)
-                : make_tmap_2d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, b_rows);
+                : make_tmap_2d_bf16(&tb, ob.p, ob.rows, ob.cols, ob.ld, 64, box_b);
   if (rc) return rc * 100 - 2;
   tp = tb;
   if (pl.pieces > 1 && (!a.b_mn || a.b_3d))
@@ -1066,6 +1472,14 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
            rows_of(bytes / 2, p->R, p->ldr, p->type) && rows_of(bytes / 2, p->Z, p->ldz, p->type);
   };
   a.vec = rows_on(32) ? kRows32 : rows_on(16) ? kRows16 : kRowsAny;
+#define CFB_SPLIT(T)                                                                              \
+  (p->kind == kLinearFwd                                                                         \
+       ? launch_split<T, kLinearFwd>(ta, tb, a, pl.splits, box_a, box_b, behind, st)             \
+   : p->kind == kLinearDgrad                                                                     \
+       ? launch_split<T, kLinearDgrad>(ta, tb, a, pl.splits, box_a, box_b, behind, st)           \
+       : launch_split<T, kLinearWgrad>(ta, tb, a, pl.splits, box_a, box_b, behind, st))
+  if (pl.splits) return p->type == kBF16 ? CFB_SPLIT(__nv_bfloat16) : CFB_SPLIT(__half);
+#undef CFB_SPLIT
 #define CFB_LINEAR(T)                                                                       \
   (p->kind == kLinearFwd     ? launch_plan<T, kLinearFwd>(pl, ta, tb, tp, a, behind, st)               \
    : p->kind == kLinearDgrad ? launch_plan<T, kLinearDgrad>(pl, ta, tb, tp, a, behind, st)             \
