@@ -880,3 +880,199 @@ def test_another_device_is_refused():
         fused.layernorm_fwd(x, w[0], None, EPS)
     with pytest.raises(ValueError):
         fused.distill_fwd(x, torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,N,K", [(20000, 256, 256), (16384, 300, 130), (9000, 5632, 1024),
+                                   (33000, 128, 128)])
+def test_wgrad_over_many_rows_keeps_fp32_accuracy(R, N, K):
+    """The products' own additions end after 1024 rows (2 * 1024 u of a segment's mass at most, for
+    more than 16384 rows to a block in proportion), the segments' sums are fp32."""
+    g = gen("cuda", R)
+    dy, x = rand(g, R, N, dtype=BF, shift=0.25), rand(g, R, K, dtype=BF, shift=0.25)
+    dw, db = torch.empty(N, K, device="cuda"), torch.empty(N, device="cuda")
+    runs = []
+    for _ in range(2):
+        gemm.linear_bias_wgrad(dy, x, dw, db, accumulate=False)
+        runs.append((dw.clone(), db.clone()))
+    assert torch.equal(runs[0][0], runs[1][0]) and torch.equal(runs[0][1], runs[1][1])
+    mass = dy.double().abs().t() @ x.double().abs()
+    close(dw, dy.double().t() @ x.double(), (2 * 1024 + R // 1024 + 2) * U * mass, "dw")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_distill_lists_with_strides(dev):
+    g, c = distill_case(dev, 20, 333, 6, BF, tail=True, tau=2.0)
+    want = fused.distill_fwd(**c)
+    wide = {}
+    for k in ("top_ids", "top_logits"):
+        buf = torch.full((20, 17), 5, dtype=c[k].dtype, device=dev)
+        buf[:, 3:9] = c[k]
+        wide[k] = buf[:, 3:9]
+    got = fused.distill_fwd(**{**c, **wide})
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    kw = dict(stats=want[3], lse=want[2], dkd=rand(g, 20), dce=rand(g, 20), labels=c["labels"],
+              temperature=2.0)
+    a = fused.distill_bwd(c["logits"], c["top_ids"], c["top_logits"], **kw)
+    assert torch.equal(fused.distill_bwd(c["logits"], wide["top_ids"], wide["top_logits"], **kw), a)
+
+
+# ---------------------------------------------------------------- together
+def student_step(s, rows):
+    """A block with layer norms and a biased MLP, its head, both losses, and the gradients over the
+    kept rows, as a training step calls them."""
+    kept_of = lambda t: fused.gather_rows(t, rows)  # noqa: E731
+    n1, m1, r1 = fused.layernorm_fwd(s["x"], s["g1"], s["b1"], EPS)
+    z = torch.empty(n1.shape[0], s["w1"].shape[0], dtype=n1.dtype, device=n1.device)
+    h = gemm.linear_act_fwd(n1, s["w1"], s["c1"], act="gelu_tanh", z=z)
+    y = gemm.linear_act_fwd(h, s["w2"], s["c2"], resid=s["x"])
+    n2, m2, r2 = fused.layernorm_fwd(y, s["g2"], s["b2"], EPS)
+    logits = gemm.linear_act_fwd(n2, s["head"])
+    kd, ce, lse, stats = fused.distill_fwd(logits, s["ids"], s["top"], 2.0, top_lse=s["top_lse"],
+                                           labels=s["labels"])
+    f32 = dict(dtype=F32, device=logits.device)
+    acc = {k: torch.zeros(s[k].shape, **f32) for k in ("head", "w1", "w2", "c1", "c2", "g1", "b1",
+                                                       "g2", "b2")}
+    dlogits = fused.distill_bwd(logits, s["ids"], s["top"], stats, s["dkd"], 2.0, labels=s["labels"],
+                                lse=lse, dce=s["dce"], rows=rows)
+    gemm.linear_bias_wgrad(dlogits, kept_of(n2), acc["head"])
+    dn2 = gemm.linear_dgrad(dlogits, s["head"])
+    dy = fused.layernorm_bwd(dn2, y, m2, r2, s["g2"], acc["g2"], acc["b2"], rows=rows)
+    gemm.linear_bias_wgrad(dy, kept_of(h), acc["w2"], acc["c2"])
+    dz = gemm.linear_act_dgrad(dy, s["w2"], z, "gelu_tanh", z_rows=rows)
+    gemm.linear_bias_wgrad(dz, kept_of(n1), acc["w1"], acc["c1"])
+    dn1 = gemm.linear_dgrad(dz, s["w1"])
+    dx = fused.layernorm_bwd(dn1, s["x"], m1, r1, s["g1"], acc["g1"], acc["b1"], rows=rows, dres=dy)
+    return {"kd": kd, "ce": ce, "dx": dx, **acc}
+
+
+def student_case(dev, T=96, R=50, H=64, F=128, V=160, K=8, seed=7):
+    g = gen(dev, seed)
+    w = lambda *shape, scale, shift=0.0: rand(g, *shape, dtype=BF, scale=scale, shift=shift)  # noqa: E731
+    s = {"x": w(T, H, scale=1.0), "w1": w(F, H, scale=H ** -0.5), "w2": w(H, F, scale=F ** -0.5),
+         "c1": w(F, scale=0.3), "c2": w(H, scale=0.3), "g1": w(H, scale=0.2, shift=1.0),
+         "g2": w(H, scale=0.2, shift=1.0), "b1": w(H, scale=0.2), "b2": w(H, scale=0.2),
+         "head": w(V, H, scale=2.0 * H ** -0.5)}
+    t = rand(g, T, V, scale=2.0)
+    s["top"], s["ids"] = t.topk(K, dim=1)
+    s["top_lse"] = (t.double() / 2.0).logsumexp(1).float()
+    s["labels"] = torch.randint(-1, V, (T,), generator=g, device=dev)
+    s["dkd"] = torch.rand(R, generator=g, device=dev)
+    s["dce"] = torch.rand(R, generator=g, device=dev)
+    return g, s, kept(g, T, R)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_step_of_a_student(dev):
+    """Twelve roundings of half a bf16 step lie on the longest way through the block, its head and
+    back, each of which moves a gradient by at most 2^-8 of its norm."""
+    _, s, rows = student_case(dev)
+    got = student_step(s, rows)
+    again = student_step(s, rows)
+    assert all(torch.equal(got[k], again[k]) for k in got)
+    leaf = {k: s[k].double().requires_grad_() for k in ("x", "w1", "w2", "c1", "c2", "g1", "b1", "g2",
+                                                        "b2", "head")}
+    n1 = ln64(leaf["x"], leaf["g1"], leaf["b1"])[0]
+    h = act64(n1 @ leaf["w1"].t() + leaf["c1"], "gelu_tanh")
+    y = h @ leaf["w2"].t() + leaf["c2"] + leaf["x"]
+    z = ln64(y, leaf["g2"], leaf["b2"])[0] @ leaf["head"].t()
+    kd, ce = distill64({"logits": z, "top_ids": s["ids"], "top_logits": s["top"], "temperature": 2.0,
+                        "top_lse": s["top_lse"], "labels": s["labels"]}, z)
+    at = rows.long()
+    # the gradient of what the kept rows' own losses say
+    ((kd[at] * s["dkd"].double()).sum() + (ce[at] * s["dce"].double()).sum()).backward()
+    want = {k: v.grad for k, v in leaf.items()}
+    want["dx"] = want.pop("x")[at]
+    for k, v in want.items():
+        err = float((got[k].double() - v).norm() / v.norm())
+        assert err < 12 * 2.0 ** -8, (k, err)
+    for k, v in (("kd", kd), ("ce", ce)):
+        assert float((got[k].double() - v.detach()).norm() / v.detach().norm()) < 5 * 2.0 ** -8
+
+
+@pytest.mark.gpu
+def test_student_captured_and_replayed_with_other_inputs():
+    cases = [student_case("cuda", seed=s, **k) for s, k in
+             ((1, {}), (2, dict(T=700, R=333, H=256, F=1024, V=2048, K=40)))]
+    for _, s, rows in cases:
+        student_step(s, rows)
+    torch.cuda.synchronize()
+    graphs = []
+    for _, s, rows in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = student_step(s, rows)
+        graphs.append((graph, res))
+    for turn in range(3):
+        for graph, _ in graphs:
+            graph.replay()
+        for (_, res), (_, s, rows) in zip(graphs, cases):
+            want = student_step(s, rows)
+            assert all(torch.equal(res[k], want[k]) for k in want)
+        for g, s, rows in cases:  # new values in the same places
+            for k in ("x", "w1", "c2", "g2", "head", "top"):
+                s[k].copy_(rand(g, *s[k].shape, scale=0.3 * (turn + 1)))
+            s["labels"].copy_(torch.randint(-1, 160, s["labels"].shape, generator=g, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_student_on_two_streams_at_once():
+    cases = [student_case("cuda", seed=s, T=500, R=222, H=128, F=512, V=1056, K=33) for s in (3, 4)]
+    want = [student_step(s, rows) for _, s, rows in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(5):
+        got = []
+        for st, (_, s, rows) in zip(streams, cases):
+            with torch.cuda.stream(st):
+                got.append(student_step(s, rows))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(a[k], b[k]) for k in b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["logits", "norm", "linear"])
+def test_offsets_past_32_bits(kind):
+    """More than 2^31 elements: the last rows against the same rows alone."""
+    g = gen("cuda", 9)
+    if kind == "logits":
+        T, V = 17000, 128256
+        z = torch.empty(T, V, dtype=BF, device="cuda")
+        z[-40:] = rand(g, 40, V, dtype=BF, scale=2.0)
+        z[:-40] = 0.0
+        t, ids = z[-40:].float().topk(6, dim=1)
+        top, all_ids = torch.zeros(T, 6, device="cuda"), torch.zeros(T, 6, dtype=torch.int32, device="cuda")
+        top[-40:], all_ids[-40:] = t, ids.int()
+        kd, _, _, stats = fused.distill_fwd(z, all_ids, top, 2.0)
+        want = fused.distill_fwd(z[-40:], ids.int(), t, 2.0)
+        # rows alone may be split over blocks, whose sums are joined in another order
+        assert torch.allclose(kd[-40:], want[0], rtol=1e-5, atol=1e-5)
+        d = torch.ones(T, device="cuda")
+        got = fused.distill_bwd(z, all_ids, top, stats, d, 2.0, out=z.clone())
+        alone = fused.distill_bwd(z[-40:], ids.int(), t, stats[-40:].contiguous(), d[:40], 2.0)
+        assert torch.equal(got[-40:], alone)
+    elif kind == "norm":
+        T, H = 530000, 4096
+        x = torch.zeros(T, H, dtype=BF, device="cuda")
+        x[-9:] = rand(g, 9, H, dtype=BF)
+        w = rand(g, H, dtype=BF)
+        y, mean, rstd = fused.layernorm_fwd(x, w, w, EPS)
+        assert torch.equal(y[-9:], fused.layernorm_fwd(x[-9:], w, w, EPS)[0])
+        rows = torch.arange(T - 9, T, dtype=torch.int32, device="cuda")
+        dy = rand(g, 9, H, dtype=BF)
+        dx = fused.layernorm_bwd(dy, x, mean, rstd, w, None, None, rows=rows)
+        assert torch.equal(dx, fused.layernorm_bwd(dy, x[-9:], mean[-9:], rstd[-9:], w, None, None))
+    else:
+        M, N, K = 70000, 32768, 64
+        x, w = rand(g, M, K, dtype=BF), rand(g, N, K, dtype=BF)
+        z = torch.empty(M, N, dtype=BF, device="cuda")
+        y = gemm.linear_act_fwd(x, w, act="relu", z=z)
+        want = x[-50:].double() @ w.double().t()
+        tol = 2 * (K + 2) * U * (x[-50:].double().abs() @ w.double().abs().t())
+        close(z[-50:], want, tol, "z")
+        close(y[-50:], want.clamp(min=0), tol, "y")
+        rows = torch.arange(M - 300, M, dtype=torch.int32, device="cuda")
+        dy, w2 = rand(g, 300, K, dtype=BF), rand(g, K, N, dtype=BF)
+        dz = gemm.linear_act_dgrad(dy, w2, z, "relu", z_rows=rows)
+        assert torch.equal(dz, gemm.linear_act_dgrad(dy, w2, z[-300:], "relu"))
