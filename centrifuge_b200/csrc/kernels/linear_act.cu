@@ -859,6 +859,10 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     after_previous();  // (an operand that was laid out anew)
     for (int kb = 0; kb < ahead; ++kb) fill(kb);
   }
+  if (threadIdx.x == 64) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), S::BN * kAccumulators);
     tmem_relinquish();
@@ -912,6 +916,51 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     commit_lane0(lane, smem_u32(done));
     __syncwarp();
   }
+  // What the first turn of the epilogue reads beside the products is on its way while they are formed.
+  constexpr int U = 8;  // rows of a warp's turn
+  const int rows = min(S::BM, p.M - m0);
+  const bool vec = p.vec != kRowsAny && (n0 + S::BN <= p.N || p.N % 4 == 0);
+  const int step = vec ? 1 : 32;  // between a lane's columns (see below)
+  const int c = vec ? lane * 4 : lane, col = n0 + c, n = p.N - col;
+  const auto get = [&](const auto* from, float* f) {
+    using E = typename std::remove_const<typename std::remove_pointer<decltype(from)>::type>::type;
+    if (vec) {
+      load_f32<E, 4>(from, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = 32 * i < n ? to_f32(from[32 * i]) : 0.f;
+    }
+  };
+  const bool reads = KIND == kLinearFwd ? p.R != nullptr : KIND == kLinearDgrad || p.add;
+  const auto beside = [&](int r0, float (*g)[4], bool* known) {
+    long long src[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + 8 * u * splits;
+      src[u] = m0 + r;
+      known[u] = r < rows && n > 0;
+      if (KIND == kLinearDgrad && known[u] && p.z_rows) src[u] = p.z_rows[src[u]];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      // (a row id outside z: recorded, and a zero row)
+      if (KIND == kLinearDgrad && known[u]) known[u] = index_in(src[u], p.n_z, p.err);
+      g[u][0] = g[u][1] = g[u][2] = g[u][3] = 0.f;
+      if (!known[u]) continue;
+      if constexpr (KIND == kLinearFwd) get(static_cast<const T*>(p.R) + src[u] * p.ldr + col, g[u]);
+      else if constexpr (KIND == kLinearDgrad) get(static_cast<const T*>(p.Z) + src[u] * p.ldz + col, g[u]);
+      else get(static_cast<const float*>(p.D) + src[u] * p.ldd + col, g[u]);
+    }
+  };
+  const int first = rank + (warp - 2) * splits;  // the warp's first row
+  float g[U][4], bias[4] = {0.f, 0.f, 0.f, 0.f};
+  bool known[U];
+  if (warp >= 2 && reads) beside(first, g, known);
+  if (warp >= 2 && KIND == kLinearFwd && p.bias) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i * step < n) bias[i] = to_f32(static_cast<const T*>(p.bias)[col + i * step]);
+  }
   // All products are done (waited for by everyone: the stages become the place of the sums, and TMEM
   // is given up).
   volatile int never = 0;
@@ -953,81 +1002,52 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   }
 
   if (warp >= 2 && ok) {
-    // The rows are dealt to the CTAs and their warps one by one, four to a turn, whose arithmetic runs
+    // The rows are dealt to the CTAs and their warps one by one, eight to a turn, whose arithmetic runs
     // together.  A lane has four neighbouring columns, or, where rows do not start on 16 bytes and at
     // the last columns, every 32nd, which keeps the warp's accesses together.
-    const int rows = min(S::BM, p.M - m0);
-    constexpr int U = 4;
     const auto finish = [&](auto act_tag, auto vec_tag) {
       constexpr int ACT = decltype(act_tag)::act;
       constexpr bool VEC = decltype(vec_tag)::value;
-      const int c = VEC ? lane * 4 : lane, col = n0 + c;
       constexpr int kStep = VEC ? 1 : 32;
-      const int n = p.N - col;  // columns from the lane's first
-      const auto get = [&](const auto* from, float* f) {
-        if constexpr (VEC) load_f32<typename std::remove_const<typename std::remove_pointer<decltype(from)>::type>::type, 4>(from, f);
-        else
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[i] = i * kStep < n ? to_f32(from[i * kStep]) : 0.f;
-      };
-      float bias[4] = {0.f, 0.f, 0.f, 0.f};
-      if (KIND == kLinearFwd && p.bias)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i * kStep < n) bias[i] = to_f32(static_cast<const T*>(p.bias)[col + i * kStep]);
-      for (int r0 = rank + (warp - 2) * splits; r0 < rows; r0 += 8 * U * splits) {
-        F2 v[U][2], other[U][2];
-        bool known[U];
+      for (int r0 = first; r0 < rows; r0 += 8 * U * splits) {
+        if (reads && r0 != first) beside(r0, g, known);
+        F2 v[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int r = r0 + 8 * u * splits;
-          const long long row = m0 + r;
-          float f[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f};
-          known[u] = false;
+          float f[4] = {0.f, 0.f, 0.f, 0.f};
           if (r < rows && n > 0) {
-            if (KIND == kLinearFwd && p.R) get(static_cast<const T*>(p.R) + row * p.ldr + col, g);
-            if (KIND == kLinearDgrad) {
-              const long long src = p.z_rows ? p.z_rows[row] : row;
-              known[u] = index_in(src, p.n_z, p.err);  // (if not: recorded, and a zero row)
-              if (known[u]) get(static_cast<const T*>(p.Z) + src * p.ldz + col, g);
-            }
-            if (KIND == kLinearWgrad && p.add)
-              get(static_cast<const float*>(p.D) + row * p.ldd + col, g);
             const float* mine = sums + r * S::ROW + c;
             if (splits == 1) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) f[i] = mine[i * kStep];
             } else {
-              float q[8][4];
+              for (int s = 0; s < splits; s += 2) {  // (splits is even)
+                float q[2][4];
 #pragma unroll
-              for (int s = 0; s < 8; ++s) {
-                if (s >= splits) continue;
-                const uint32_t at = mapa_shared(smem_u32(mine), s);
-                if constexpr (VEC) {
-                  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                               : "=f"(q[s][0]), "=f"(q[s][1]), "=f"(q[s][2]), "=f"(q[s][3])
-                               : "r"(at)
-                               : "memory");
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];"
-                                 : "=f"(q[s][i])
-                                 : "r"(at + i * kStep * 4)
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t at = mapa_shared(smem_u32(mine), s + h);
+                  if constexpr (VEC) {
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                 : "=f"(q[h][0]), "=f"(q[h][1]), "=f"(q[h][2]), "=f"(q[h][3])
+                                 : "r"(at)
                                  : "memory");
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                      asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                                   : "=f"(q[h][i])
+                                   : "r"(at + i * kStep * 4)
+                                   : "memory");
+                  }
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = f[i] + q[0][i] + q[1][i];
               }
-#pragma unroll
-              for (int s = 0; s < 8; ++s)
-                if (s < splits)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) f[i] += q[s][i];
             }
           }
           v[u][0] = f2(f[0], f[1]);
           v[u][1] = f2(f[2], f[3]);
-          other[u][0] = f2(g[0], g[1]);
-          other[u][1] = f2(g[2], g[3]);
         }
         const auto put = [&](auto* base, long long ld) {
           using O = typename std::remove_pointer<decltype(base)>::type;
@@ -1054,19 +1074,23 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
           if (p.Z) put(static_cast<T*>(p.Z), p.ldz);
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if constexpr (KIND == kLinearDgrad)
-              v[u][i] = known[u] ? v[u][i] * act_slope<ACT>(other[u][i]) : f2(0.f);
-            else
-              v[u][i] = act_of<ACT>(v[u][i]) + other[u][i];
+        for (int u = 0; u < U; ++u) {
+          if constexpr (KIND == kLinearDgrad) {
+            v[u][0] = known[u] ? v[u][0] * act_slope<ACT>(f2(g[u][0], g[u][1])) : f2(0.f);
+            v[u][1] = known[u] ? v[u][1] * act_slope<ACT>(f2(g[u][2], g[u][3])) : f2(0.f);
+          } else {
+            v[u][0] = act_of<ACT>(v[u][0]);
+            v[u][1] = act_of<ACT>(v[u][1]);
+            if (reads) {
+              v[u][0] = v[u][0] + f2(g[u][0], g[u][1]);
+              v[u][1] = v[u][1] + f2(g[u][2], g[u][3]);
+            }
           }
+        }
         if constexpr (KIND == kLinearWgrad) put(static_cast<float*>(p.D), p.ldd);
         else put(static_cast<T*>(p.D), p.ldd);
       }
     };
-    const bool vec = p.vec != kRowsAny && (n0 + S::BN <= p.N || p.N % 4 == 0);
     const auto either = [&](auto act_tag) {
       if (vec) finish(act_tag, std::true_type());
       else finish(act_tag, std::false_type());
@@ -1078,30 +1102,36 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 }
 
 // ---------------------------------------------------------------- layout and column sums
-// dst [rows, ld_dst] = src [rows, cols] (2-byte elements)
-__global__ void __launch_bounds__(256) relayout_kernel(const unsigned short* __restrict__ src,
-                                                       long long ld, int cols,
-                                                       unsigned short* __restrict__ dst,
-                                                       long long ld_dst, int rows) {
+// dst [rows, ld_dst] = src [rows, cols] in elements of E (one or two of 2 bytes).
+template <typename E>
+__global__ void __launch_bounds__(256) relayout_kernel(const E* __restrict__ src, long long ld, int cols,
+                                                       E* __restrict__ dst, long long ld_dst, int rows) {
   let_next_start();
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const unsigned short* s = src + r * ld;
-    unsigned short* d = dst + r * ld_dst;
-    for (int c = blockIdx.x * 256 + threadIdx.x; c < cols; c += gridDim.x * 256) d[c] = s[c];
+  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
+    const E* s = src + r * ld;
+    E* d = dst + r * ld_dst;
+    for (int c0 = threadIdx.x; c0 < cols; c0 += 8 * 256) {
+      E v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i * 256 < cols) v[i] = s[c0 + i * 256];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i * 256 < cols) d[c0 + i * 256] = v[i];
+    }
   }
 }
 
 // sum[c] (+)= the sum of column c of dy [rows, cols], in a fixed order.  A cluster of eight blocks
-// has a slab of columns, each thread W of them in every 256th (W = 8) row; the first block adds the
-// eight blocks' sums.  Bound by memory.
-template <typename T, int W>
+// has a slab of LANES * W columns, each thread W of them; the first block adds the eight blocks' sums.
+// Bound by memory: 8192 x 5632 bf16 in 15 us.
+template <typename T, int W, int LANES>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ dy, long long ld,
                                                          int rows, int cols,
                                                          float* __restrict__ sum, int add) {
-  constexpr int LANES = W == 8 ? 8 : 32;      // threads across a slab
-  constexpr int GROUPS = 256 / LANES;         // rows of a block at a time
+  constexpr int GROUPS = 256 / LANES;  // rows of a block at a time
   constexpr int SLAB = LANES * W;
-  __shared__ float part[GROUPS][SLAB + 1];
+  __shared__ float part[8][SLAB];  // each warp's sums
   __shared__ float total[SLAB];
   let_next_start();
   const uint32_t rank = cluster_ctarank();
@@ -1119,11 +1149,16 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ d
     }
   }
 #pragma unroll
-  for (int i = 0; i < W; ++i) part[rg][lane * W + i] = s[i];
+  for (int i = 0; i < W; ++i) {
+#pragma unroll
+    for (int o = LANES; o < 32; o *= 2) s[i] += __shfl_xor_sync(0xffffffffu, s[i], o);
+    if (lane_id() < LANES) part[warp_id()][lane * W + i] = s[i];
+  }
   __syncthreads();
   if (threadIdx.x < SLAB) {
     float t = 0.f;
-    for (int g = 0; g < GROUPS; ++g) t += part[g][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < 8; ++w) t += part[w][threadIdx.x];
     total[threadIdx.x] = t;
   }
   cluster_sync();
@@ -1350,12 +1385,15 @@ Operand operand_b(const CfbLinear& p) {
 int lay_out(Operand& o, uint8_t*& work, cudaStream_t st) {
   if (o.direct()) return 0;
   const long long bytes = o.packed_bytes();
-  unsigned short* dst = reinterpret_cast<unsigned short*>(work);
-  const int x = (o.cols + 1023) / 1024;
-  relayout_kernel<<<dim3(x < 64 ? x : 64, o.rows < 65535 ? o.rows : 65535), 256, 0, st>>>(
-      static_cast<const unsigned short*>(o.p), o.ld, o.cols, dst, o.packed_ld(), o.rows);
+  const int grid = o.rows < 148 * 16 ? o.rows : 148 * 16;
+  if (reinterpret_cast<uintptr_t>(o.p) % 4 == 0 && o.ld % 2 == 0 && o.cols % 2 == 0)
+    relayout_kernel<<<grid, 256, 0, st>>>(static_cast<const uint32_t*>(o.p), o.ld / 2, o.cols / 2,
+                                          reinterpret_cast<uint32_t*>(work), o.packed_ld() / 2, o.rows);
+  else
+    relayout_kernel<<<grid, 256, 0, st>>>(static_cast<const unsigned short*>(o.p), o.ld, o.cols,
+                                          reinterpret_cast<unsigned short*>(work), o.packed_ld(), o.rows);
+  o.p = work;
   work += bytes;
-  o.p = dst;
   o.ld = o.packed_ld();
   return launch_status();
 }
@@ -1363,8 +1401,10 @@ int lay_out(Operand& o, uint8_t*& work, cudaStream_t st) {
 template <typename T>
 int launch_column_sum(const CfbLinear& p, cudaStream_t st) {
   const bool wide = p.M % 8 == 0 && rows_of_8(p.A, p.lda, p.type);
+  // 64 columns to a slab, or 16 where that would leave SMs without a block
+  const int slab = !wide ? 32 : p.M >= 64 * 148 / 8 ? 64 : 16;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(8 * ((p.M + (wide ? 63 : 31)) / (wide ? 64 : 32)));
+  cfg.gridDim = dim3(8 * ((p.M + slab - 1) / slab));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -1373,12 +1413,12 @@ int launch_column_sum(const CfbLinear& p, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const T* dy = static_cast<const T*>(p.A);
-  const long long ld = p.lda;
-  const int rows = p.K, cols = p.M, add = p.add;
-  const cudaError_t e =
-      wide ? cudaLaunchKernelEx(&cfg, column_sum_kernel<T, 8>, dy, ld, rows, cols, p.dbias, add)
-           : cudaLaunchKernelEx(&cfg, column_sum_kernel<T, 1>, dy, ld, rows, cols, p.dbias, add);
+  const auto launch = [&](auto* kernel) {
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(p.A), p.lda, p.K, p.M, p.dbias, p.add);
+  };
+  const cudaError_t e = slab == 64   ? launch(column_sum_kernel<T, 8, 8>)
+                        : slab == 16 ? launch(column_sum_kernel<T, 8, 2>)
+                                     : launch(column_sum_kernel<T, 1, 32>);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return -3;
