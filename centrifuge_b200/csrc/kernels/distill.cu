@@ -560,25 +560,38 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
     index_in(ok ? 0 : -1, 1, p.err);
     if (CE && label >= p.V) index_in(label, p.V, p.err);
   }
-  int* sm_id = reinterpret_cast<int*>(dyn);  // -1: no entry
-  float* sm_p = reinterpret_cast<float*>(sm_id + K);
-  float* sm_g = sm_p + K;
+  int* sm_id = reinterpret_cast<int*>(dyn);           // -1: no entry
+  float* sm_p = reinterpret_cast<float*>(sm_id + K);  // the teacher's logits, then its shares
+  float* sm_g = sm_p + K;                             // the student's logits here, then the gradients
   int* table = reinterpret_cast<int*>(sm_g + K);
   const int slots = table_slots(K);
   const int entries = k != 0.f ? K : 0;
-  for (int i = lane; entries && i < slots; i += 32) table[i] = -1;
-  __syncwarp();
   const auto in_range = [&](long long v) { return v >= v0 && v < v0 + n; };
-  const bool labelled = g1 != 0.f;
-  float whole = 0.f;
-  bool twice = false, named = false;
+  for (int i = lane; entries && i < slots; i += 32) table[i] = -1;
   for (int j = lane; j < entries; j += 32) {
     const long long id = p.list.id(src, j);
     int at = -1;
-    float pj = 0.f;
     if (id >= 0 && index_in(id, p.V, p.err)) {
       at = static_cast<int>(id);
-      pj = static_cast<float>(exp(p.list.logit(src, j) * p.inv_temp64 - st.w));
+      sm_p[j] = p.list.logit(src, j);
+      if (in_range(at)) sm_g[j] = to_f32(z[at]);
+    }
+    sm_id[j] = at;
+  }
+  const bool labelled = CE && g1 != 0.f;
+  const bool label_here = labelled && in_range(label);
+  const float z_label = label_here ? to_f32(z[label]) : 0.f;
+  __syncthreads();
+
+  // While the others stream.  The differences of two probabilities are formed in 64 bits: where the
+  // student agrees with the teacher or the label, little is left of either.
+  float whole = 0.f;
+  bool twice = false, named = false;
+  for (int j = lane; j < entries; j += 32) {
+    const int at = sm_id[j];
+    float pj = 0.f;
+    if (at >= 0) {
+      pj = static_cast<float>(exp(sm_p[j] * p.inv_temp64 - st.w));
       unsigned slot = static_cast<unsigned>(at) * 2654435761u;
       for (;; ++slot) {  // (more slots than entries: it ends)
         const int old = atomicCAS(&table[slot & (slots - 1)], -1, at);
@@ -588,36 +601,36 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
     }
     named = named || (at >= 0 && at == label);
     whole += pj;
-    sm_id[j] = at;
     sm_p[j] = pj;
   }
   whole = warp_add(whole);
-  // what the teacher's terms add up to: one, but for a list of the whole vocabulary
-  if (st.y > -INFINITY) whole = fmaxf(whole, 1.f);
+  // What the teacher's terms add up to: one (without its lse: by its normaliser), or, for a list of the
+  // whole vocabulary, what the list's do.
+  if (st.y == st.x) whole = 1.f;
+  else if (st.y > -INFINITY) whole = fmaxf(whole, 1.f);
   named = __any_sync(0xffffffffu, named);
   twice = __any_sync(0xffffffffu, twice);
   __syncwarp();
+  const double lse1 = labelled ? lse[src] : 0.0;
   for (int j = lane; j < entries; j += 32) {
     const int at = sm_id[j];
     if (at < 0 || !in_range(at)) continue;
-    const float v = to_f32(z[at]);
+    const double v = sm_g[j];
     float share = sm_p[j];
     if (twice) {  // the same token's shares, summed in the list's order by each of its entries
       share = 0.f;
       for (int i = 0; i < K; ++i) share += sm_id[i] == at ? sm_p[i] : 0.f;
     }
-    float g = k * fmaf(whole, ex2(fmaf(v, c, -st.x * kL2e)), -share);
-    if (CE && labelled) g += g1 * (ex2(fmaf(v, kL2e, -ref1)) - (at == label ? 1.f : 0.f));
-    sm_g[j] = g;
+    double g = k * (whole * exp(v * p.inv_temp64 - st.x) - share);
+    if (labelled) g += g1 * (exp(v - lse1) - (at == label ? 1.0 : 0.0));
+    sm_g[j] = static_cast<float>(g);
   }
-  float label_grad = 0.f;
-  const bool label_alone = CE && labelled && !named && in_range(label);
-  if (label_alone) {
-    const float v = to_f32(z[label]);
-    label_grad = (spread ? gk * ex2(fmaf(v, c, -ref)) : 0.f) + g1 * (ex2(fmaf(v, kL2e, -ref1)) - 1.f);
-  }
-  __syncthreads();
-  __syncthreads();
+  const bool label_alone = label_here && !named;
+  const float label_grad =
+      label_alone ? static_cast<float>((spread ? gk * exp(z_label * p.inv_temp64 - st.y) : 0.0) +
+                                       g1 * (exp(z_label - lse1) - 1.0))
+                  : 0.f;
+  __syncthreads();  // the range is written
   for (int j = lane; j < entries; j += 32)
     if (sm_id[j] >= 0 && in_range(sm_id[j])) out[sm_id[j] - v0] = from_f32<T>(sm_g[j]);
   if (label_alone && lane == 0) out[label - v0] = from_f32<T>(label_grad);
