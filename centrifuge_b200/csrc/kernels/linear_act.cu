@@ -1442,7 +1442,8 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
     if (p->kind != kLinearWgrad) return -10;
     if (p->add) return 0;  // no rows: nothing to add
     if (p->dbias && cudaMemsetAsync(p->dbias, 0, 4ll * p->M, st) != cudaSuccess) return -3;
-    if (p->N > 0 && cudaMemset2DAsync(p->D, 4ll * p->ldd, 0, 4ll * p->N, p->M, st) != cudaSuccess)
+    const long long pitch = p->M == 1 ? p->N : p->ldd;  // (a single row's stride says nothing)
+    if (p->N > 0 && cudaMemset2DAsync(p->D, 4 * pitch, 0, 4ll * p->N, p->M, st) != cudaSuccess)
       return -3;
     return 0;
   }

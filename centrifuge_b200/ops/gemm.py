@@ -204,7 +204,8 @@ def linear_act_fwd(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor
     ``bias [N]`` is contiguous; any ``T``, ``N`` and ``K > 0``.  ``act``: one of :data:`ACTIVATIONS`
     (``gelu`` by the normal distribution, ``gelu_tanh`` by its approximation).  ``z [T, N]``, when
     given, receives the rounded ``x w^T + bias``, which :func:`linear_act_dgrad` needs.  ``out`` may
-    be ``resid`` itself; other overlaps are refused."""
+    be ``resid`` itself; other overlaps are refused.  CPU tensors may be fp32 too, as the definition
+    that the others are compared with."""
     code = _act_code("linear_act_fwd", act)
     if x.is_cuda:
         return kernels().linear_act_fwd(x, w, bias, code, resid, out, z)
@@ -275,7 +276,8 @@ def linear_bias_wgrad(dy: torch.Tensor, x: torch.Tensor, dw: torch.Tensor,
     """``dw (+)= dy^T x`` and ``dbias (+)= sum of the rows of dy`` (written without ``accumulate``),
     each summed in fp32 in a fixed order.  ``dy [R, N]`` and ``x [R, K]`` as in
     :func:`linear_act_fwd` (without rows nothing is added), ``dw [N, K]`` fp32 with any row stride,
-    ``dbias [N]`` contiguous fp32; what is written overlaps nothing else."""
+    ``dbias [N]`` contiguous fp32; what is written overlaps nothing else.  Sums below 1.2e-38 may count
+    as zero on the GPU."""
     if dy.is_cuda:
         kernels().linear_bias_wgrad(dy, x, dw, dbias, accumulate)
         return dw

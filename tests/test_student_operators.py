@@ -302,6 +302,21 @@ def test_linear_without_rows(dev):
     assert bool((db == 32.0).all())
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("rows", [0, 3])
+def test_single_output_row_has_no_stride(dev, rows):
+    """A weight gradient of one row, whose stride says nothing, with and without rows to sum."""
+    g = gen(dev, 5)
+    dy, x = rand(g, rows, 1, dtype=BF), rand(g, rows, 24, dtype=BF)
+    buf = torch.full((40,), 9.0, device=dev)
+    dw, db = buf.as_strided((1, 24), (1, 1), 8), torch.full((1,), 9.0, device=dev)
+    gemm.linear_bias_wgrad(dy, x, dw, db, accumulate=False)
+    want = dy.double().t() @ x.double()
+    close(dw, want, 2 * rows * U * (dy.double().abs().t() @ x.double().abs()), "dw")
+    close(db, dy.double().sum(0), rows * U * dy.double().abs().sum(0), "dbias")
+    assert bool((buf[:8] == 9.0).all()) and bool((buf[32:] == 9.0).all())
+
+
 # ---------------------------------------------------------------- layer norm
 def ln64(x, w, b):
     mean = x.mean(-1, keepdim=True)
