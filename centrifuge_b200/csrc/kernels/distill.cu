@@ -187,12 +187,18 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
   const int shift = 8 - head;  // bit of column i (from v0): i + shift, so a pack's bits are a byte
   const float c = p.inv_temp * kL2e;
 
+  constexpr int S = U * kThreads;  // packs of a step
   const auto load = [&](int first, Pack<T, 8>* k) {
+    if (first + S <= packs) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = first + u * kThreads + tid;
-      if (at < packs) k[u] = span.pack(at);
-      else set_ninf<T>(k[u]);
+      for (int u = 0; u < U; ++u) k[u] = span.pack(first + u * kThreads + tid);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int at = first + u * kThreads + tid;
+        if (at < packs) k[u] = span.pack(at);
+        else set_ninf<T>(k[u]);
+      }
     }
   };
   Pack<T, 8> now[U];
@@ -240,24 +246,21 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
     };
     if (tid < head) single(tid);
     if (tid < n - head - packs * 8) single(head + packs * 8 + tid);
-    for (int first = 0; first < packs; first += U * kThreads) {
-      Pack<T, 8> next[U];
-      load(first + U * kThreads, next);
+    const auto use = [&](int first, Pack<T, 8>* k) {
       if (REST) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int at = first + u * kThreads + tid;
-          const uint32_t b = at < packs ? byte[at + 1] : 0u;
-          if (b) mask_out<T>(now[u], b);
+        for (int u = 0; u < U; ++u) {  // (behind the last pack there is nothing left to mask)
+          const uint32_t b = byte[min(first + u * kThreads + tid + 1, packs)];
+          if (b) mask_out<T>(k[u], b);
         }
       }
-      s.raise(packs_max<T, U>(now), c);
+      s.raise(packs_max<T, U>(k), c);
       F2 a = f2(0.f), b1 = f2(0.f);
       const F2 cc = f2(c), nr = f2(-s.ref), cl = f2(kL2e), nr1 = f2(-s.ref1);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         F2 v[4];
-        unpack_f2<T, 8>(now[u], v);
+        unpack_f2<T, 8>(k[u], v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 x = halves(fma2(v[i], cc, nr));
@@ -269,10 +272,18 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
           }
           if (ONE == kOneSquare) b1 = fma2(e, e, b1);
         }
-        now[u] = next[u];
       }
       s.rest += sum2(a);
       if (ONE != kOneNone) s.one += sum2(b1);
+    };
+    constexpr int kUnroll = REST ? 1 : 2;  // two steps with masks spill registers (186 -> 216 us at tau = 1)
+#pragma unroll kUnroll
+    for (int first = 0; first < packs; first += S) {
+      Pack<T, 8> next[U];
+      load(first + S, next);
+      use(first, now);
+#pragma unroll
+      for (int u = 0; u < U; ++u) now[u] = next[u];
     }
   } else {
     for (int j = lane; j < K; j += 32) {
