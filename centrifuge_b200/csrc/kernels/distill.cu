@@ -29,8 +29,10 @@ namespace cfb {
 constexpr float kL2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
 // A row is streamed by four warps, seven such blocks to an SM: while some wait for their list or sums,
-// others stream (16384 x 32000 bf16 with tail and labels, tau = 2: 213 us; with eight warps and four
-// blocks 237, with two and twelve 212; the gradient of 8192 of its rows 181, 193 and 192 us).
+// others stream.  Of 16384 x 32000 bf16 logits with tail and labels at tau = 2 (161 us at the measured
+// copy rate) the forward takes 197 us, without tail 167; the gradient of 8192 rows (161 us) 174.  When
+// the shape was chosen these were 213 and 181; with eight warps and four blocks an SM 237 and 193,
+// with two and twelve 212 and 192, with six blocks of four (more registers) 210 and 185.
 constexpr int kThreads = 128;          // the streaming warps'
 constexpr int kBlock = kThreads + 32;  // ... and the lister's
 constexpr int kBlocksPerSm = 7;

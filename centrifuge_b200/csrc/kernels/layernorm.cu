@@ -16,7 +16,9 @@ namespace cfb {
 // A team of up to NW warps (a block; with NW = 1 each of a block's four warps is a team) holds R
 // rows: a thread has the same NV groups of eight columns of each, so that the weights are unpacked
 // once and the rows share the exchanges of their sums.  Short blocks, each of which first asks the
-// L2 cache for the rows of the block that will follow it on its SM.
+// L2 cache for the rows of the block that will follow it on its SM.  16384 x 2048 bf16: 27 us, 0.76 of
+// the measured copy rate; one row a team, four rows, eight or two warps, other columns a thread: 28 to
+// 79 us.  Above 4096 columns a row takes 16 or 32 warps, which wait together (8192: 0.55 of the rate).
 template <typename TY, typename TX, int NW, int NV, int R>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_kernel(
     const TX* __restrict__ x, long long ld_x, const TY* __restrict__ w, const TY* __restrict__ b,
@@ -109,7 +111,8 @@ __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_kernel(
   }
 }
 
-// Rows of other widths and alignments: one row a team, a pair of columns at a time.
+// Rows of other widths and alignments: one row a team, a pair of columns at a time (16384 x 2050 bf16:
+// 61 us), or, where rows start anywhere, a column (2049: 87 us).
 template <typename TY, typename TX, int W, int NW, int NV>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_pairs_kernel(
     const TX* __restrict__ x, long long ld_x, const TY* __restrict__ w, const TY* __restrict__ b,
@@ -217,6 +220,8 @@ __device__ __forceinline__ void pair_sums(float& a, float& b, float* slot, int t
 // loads of the next rows run while a row waits for its sums.  A row's stage is free again once every
 // thread has its columns in registers, which the barrier of the row's sums tells.  The weights lie
 // in shared memory in fp32, in two planes of the four low and the four high columns of each group.
+// 8190 x 4096 with an fp32 stream: 79 us with the join, 0.9 of the measured copy rate; 8192 x 2048 bf16
+// 34 us, 0.6: a row is short against the two exchanges of its sums, and the registers hold two blocks.
 template <typename TY, typename TX, int NW, int NV>
 __global__ void __launch_bounds__(NW < 4 ? 128 : NW * 32, NW < 4 ? 4 : NW <= 16 ? 16 / NW : 1)
     layernorm_bwd_ring_kernel(const LnBwd a, int stages) {

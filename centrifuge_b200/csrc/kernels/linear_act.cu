@@ -9,7 +9,11 @@
 // writes what is inside.  An operand whose rows do not start on 16 bytes is first laid out in a
 // workspace with rows that do.
 //
-// Bound by the tensor cores at a training step's sizes, by latency at small ones.
+// Bound by the tensor cores at a training step's sizes, by latency at small ones.  16384 x 2048 x 5632
+// bf16 (228 us at the measured rate of library products): 254 us without an activation, 277 with gelu
+// and z, in bursts of eight calls; the clock falls from 1.9 to 1.6 GHz meanwhile, and in a longer loop
+// the power limit makes the last 338.  Of 8192 of its rows (114 us): dgrad 152, wgrad 153 and with dbias
+// 168, whose sums are a pass of their own (dealt to the epilogue's warps they cost 22 us).
 #include "row_types.cuh"
 
 #include <cudaTypedefs.h>
@@ -783,7 +787,7 @@ __device__ __forceinline__ void commit_lane0(int lane, uint32_t bar) {
 
 // One tile of 128 x 128 to a cluster of up to eight CTAs, each with a part of k: an SM takes in about
 // 64 bytes of operands a clock, so that a few tiles with a long k leave most of the machine idle (16 x
-// 8192 by 2048 x 8192: 45 us with a CTA pair for each 256 columns).  Every CTA puts its sums into its
+// 8192 by 2048 x 8192: 45 us with a CTA pair for each 256 columns, 15 so).  Every CTA puts its sums into its
 // shared memory; behind a cluster barrier each finishes 128 / splits rows, adding the parts in order
 // (the same bits on every run), with accesses to global memory along the rows.
 //
