@@ -809,6 +809,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
                         int a_rows, int b_rows) {
   using S = SplitShape;
   constexpr bool A_MN = KIND == kLinearWgrad, B_MN = KIND != kLinearFwd;
+  if (KIND == kLinearWgrad) let_next_start();  // the column sums
   // wgrad: an accumulator for every 1024 rows, up to four (see kSegment)
   constexpr int kAccumulators = KIND == kLinearWgrad ? 4 : 1;
   extern __shared__ uint8_t smem_raw[];
@@ -1128,7 +1129,10 @@ __global__ void __launch_bounds__(256) relayout_kernel(const E* __restrict__ src
 
 // sum[c] (+)= the sum of column c of dy [rows, cols], in a fixed order.  A cluster of eight blocks
 // has a slab of LANES * W columns, each thread W of them; the first block adds the eight blocks' sums.
-// Bound by memory: 8192 x 5632 bf16 in 15 us.
+// Bound by memory: 8192 x 5632 bf16 in 15 us.  It is launched behind a product of few tiles and may
+// start as soon as that has, on the SMs that it leaves idle (16384 rows, 256 x 256: 17.1 us for 20.9);
+// but before one of many, which then finds much of dy in the L2 cache (8192 rows, 2048 x 5632: 168 us
+// for 180).
 template <typename T, int W, int LANES>
 __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ dy, long long ld,
                                                          int rows, int cols,
@@ -1180,6 +1184,7 @@ __global__ void __launch_bounds__(256) column_sum_kernel(const T* __restrict__ d
     sum[col] = (add ? sum[col] : 0.f) + t;
   }
   cluster_sync();  // no block leaves while its sums are read
+  after_previous();  // (behind a product: what follows the call has to wait for both)
 }
 
 }  // namespace cfb
@@ -1403,7 +1408,7 @@ int lay_out(Operand& o, uint8_t*& work, cudaStream_t st) {
 }
 
 template <typename T>
-int launch_column_sum(const CfbLinear& p, cudaStream_t st) {
+int launch_column_sum(const CfbLinear& p, bool behind, cudaStream_t st) {
   const bool wide = p.M % 8 == 0 && rows_of_8(p.A, p.lda, p.type);
   // 64 columns to a slab, or 16 where that would leave SMs without a block
   const int slab = !wide ? 32 : p.M >= 64 * 148 / 8 ? 64 : 16;
@@ -1411,12 +1416,14 @@ int launch_column_sum(const CfbLinear& p, cudaStream_t st) {
   cfg.gridDim = dim3(8 * ((p.M + slab - 1) / slab));
   cfg.blockDim = dim3(256);
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 8;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 8;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = behind ? 2 : 1;
   const auto launch = [&](auto* kernel) {
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(p.A), p.lda, p.K, p.M, p.dbias, p.add);
   };
@@ -1451,22 +1458,26 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
       return -3;
     return 0;
   }
-  bool behind = false;  // the product follows a kernel of the same call
-  if (p->kind == kLinearWgrad && p->dbias) {
-    const int rc = p->type == kBF16 ? launch_column_sum<__nv_bfloat16>(*p, st)
-                                    : launch_column_sum<__half>(*p, st);
-    if (rc || p->N == 0) return rc;
-    behind = true;
-  }
+  const auto column_sum = [&](bool behind) {
+    return p->type == kBF16 ? launch_column_sum<__nv_bfloat16>(*p, behind, st)
+                            : launch_column_sum<__half>(*p, behind, st);
+  };
+  if (p->N == 0) return column_sum(false);
   if (((p->M + 127LL) / 128) * ((p->N + 63LL) / 64) >= (1LL << 31)) return -11;
   Operand oa = operand_a(*p), ob = operand_b(*p);
-  behind = behind || !oa.direct() || !ob.direct();
+  const LinearPlan pl = plan_linear(p->M, p->N, p->K, split_clusters);
+  const bool sums = p->kind == kLinearWgrad && p->dbias;
+  if (sums && !pl.splits) {
+    const int rc = column_sum(false);
+    if (rc) return rc;
+  }
+  // whether the product follows a kernel of the same call
+  const bool behind = (sums && !pl.splits) || !oa.direct() || !ob.direct();
   uint8_t* work = static_cast<uint8_t*>(p->work);
   int rc = lay_out(oa, work, st);
   if (rc) return rc;
   rc = lay_out(ob, work, st);
   if (rc) return rc;
-  const LinearPlan pl = plan_linear(p->M, p->N, p->K, split_clusters);
   LinearArgs a = {};
   a.M = p->M;
   a.N = p->N;
@@ -1523,12 +1534,13 @@ int cfb_linear(const CfbLinear* p, cudaStream_t st) {
    : p->kind == kLinearDgrad                                                                     \
        ? launch_split<T, kLinearDgrad>(ta, tb, a, pl.splits, box_a, box_b, behind, st)           \
        : launch_split<T, kLinearWgrad>(ta, tb, a, pl.splits, box_a, box_b, behind, st))
-  if (pl.splits) return p->type == kBF16 ? CFB_SPLIT(__nv_bfloat16) : CFB_SPLIT(__half);
-#undef CFB_SPLIT
 #define CFB_LINEAR(T)                                                                       \
   (p->kind == kLinearFwd     ? launch_plan<T, kLinearFwd>(pl, ta, tb, tp, a, behind, st)               \
    : p->kind == kLinearDgrad ? launch_plan<T, kLinearDgrad>(pl, ta, tb, tp, a, behind, st)             \
                              : launch_plan<T, kLinearWgrad>(pl, ta, tb, tp, a, behind, st))
-  return p->type == kBF16 ? CFB_LINEAR(__nv_bfloat16) : CFB_LINEAR(__half);
+  if (pl.splits) rc = p->type == kBF16 ? CFB_SPLIT(__nv_bfloat16) : CFB_SPLIT(__half);
+  else rc = p->type == kBF16 ? CFB_LINEAR(__nv_bfloat16) : CFB_LINEAR(__half);
+#undef CFB_SPLIT
 #undef CFB_LINEAR
+  return rc == 0 && sums && pl.splits ? column_sum(true) : rc;
 }

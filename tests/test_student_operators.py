@@ -317,6 +317,40 @@ def test_single_output_row_has_no_stride(dev, rows):
     assert bool((buf[:8] == 9.0).all()) and bool((buf[32:] == 9.0).all())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,N,K", [(4096, 64, 64), (2000, 512, 256), (70, 136, 2100), (600, 2048, 2304)])
+def test_weight_gradients_in_a_row(R, N, K):
+    """Small integers, whose sums are exact: every call adds its whole product and column sums before
+    what follows it on the stream reads them, eagerly and in a graph."""
+    g = gen("cuda", 6)
+    dy = torch.randint(-2, 3, (R, N), generator=g, device="cuda").to(BF)
+    x = torch.randint(-2, 3, (R, K), generator=g, device="cuda").to(BF)
+    want_w, want_b = (dy.double().t() @ x.double()).float(), dy.double().sum(0).float()
+    dw, db = torch.zeros(N, K, device="cuda"), torch.zeros(N, device="cuda")
+    seen = [(torch.empty_like(dw), torch.empty_like(db)) for _ in range(8)]
+
+    def steps():
+        for w, b in seen:
+            gemm.linear_bias_wgrad(dy, x, dw, db)
+            w.copy_(dw)
+            b.copy_(db)
+
+    def check():
+        for i, (w, b) in enumerate(seen):
+            assert torch.equal(w, (i + 1) * want_w) and torch.equal(b, (i + 1) * want_b)
+            w.zero_(), b.zero_()
+        dw.zero_(), db.zero_()
+
+    steps()
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps()
+    for _ in range(3):
+        graph.replay()
+        check()
+
+
 # ---------------------------------------------------------------- layer norm
 def ln64(x, w, b):
     mean = x.mean(-1, keepdim=True)
