@@ -922,7 +922,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     __syncwarp();
   }
   // What the first turn of the epilogue reads beside the products is on its way while they are formed.
-  constexpr int U = 8;  // rows of a warp's turn
+  constexpr int U = 4;  // rows of a warp's turn (eight: 16 x 8192 x 2048 15.7 us for 15.0; two: dgrad slower)
   const int rows = min(S::BM, p.M - m0);
   const bool vec = p.vec != kRowsAny && (n0 + S::BN <= p.N || p.N % 4 == 0);
   const int step = vec ? 1 : 32;  // between a lane's columns (see below)
@@ -1007,7 +1007,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   }
 
   if (warp >= 2 && ok) {
-    // The rows are dealt to the CTAs and their warps one by one, eight to a turn, whose arithmetic runs
+    // The rows are dealt to the CTAs and their warps one by one, four to a turn, whose arithmetic runs
     // together.  A lane has four neighbouring columns, or, where rows do not start on 16 bytes and at
     // the last columns, every 32nd, which keeps the warp's accesses together.
     const auto finish = [&](auto act_tag, auto vec_tag) {
