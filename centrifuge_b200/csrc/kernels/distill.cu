@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
   constexpr int kWarps = kThreads / 32 + 1;
   extern __shared__ uint32_t dyn[];
   __shared__ float red[kWarps][4];
-  __shared__ float joined[4];  // this block's max, rest, listed, one
+  __shared__ float joined[5];  // this block's sums of the rest and of the list, behind their maxima, and one
   const int K = p.list.K, tid = threadIdx.x, lane = lane_id();
   const bool lister = tid >= kThreads;
   float* sm_t = reinterpret_cast<float*>(dyn);
@@ -373,31 +373,39 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
   }
   __syncthreads();
   if (!lister && splits == 1) return;
-  // Lane b: warp b's sums, or block b's, relative to the largest maximum of all `n` of them.
-  float top, ref, ref1, rest_sum, list_sum, one_sum;
-  const auto join = [&](float bm, float br, float bl, float bo) {
-    top = bm;
+  // Lane b: warp b's sums, or block b's.  The rest's sum and the list's keep a maximum each: relative
+  // to the other's, one that is 87 logits (times the temperature) below would be lost, and with it all
+  // that is to be said of the rest.
+  float rest_top, list_top, rest_sum, list_sum, one_sum;
+  const auto join = [&](float rest_max, float r, float list_max, float l, float o) {
+    const auto most = [](float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    ref = top == -INFINITY ? 0.f : __fmul_rn(top, c);
-    ref1 = top == -INFINITY ? 0.f : __fmul_rn(top, kL2e);
-    const float f = bm == -INFINITY ? 1.f : ex2(__fmul_rn(bm, c) - ref);  // (sums of nothing are zero)
-    const float f1 = bm == -INFINITY ? 1.f : ex2(__fmul_rn(bm, kL2e) - ref1);
-    rest_sum = warp_add(br * f);
-    list_sum = warp_add(bl * f);
-    one_sum = warp_add(bo * f1);
+      for (int i = 16; i > 0; i >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, i));
+      return v;
+    };
+    const auto moved = [](float sum, float from, float to, float scale) {
+      return from == to ? sum : sum * ex2(__fmul_rn(from, scale) - __fmul_rn(to, scale));
+    };
+    rest_top = most(rest_max);
+    list_top = REST ? most(list_max) : -INFINITY;
+    rest_sum = warp_add(moved(r, rest_max, rest_top, c));
+    list_sum = REST ? warp_add(moved(l, list_max, list_top, c)) : 0.f;
+    one_sum = ONE == kOneNone ? 0.f
+                              : warp_add(moved(o, fmaxf(rest_max, list_max), fmaxf(rest_top, list_top), kL2e));
   };
   if (lister) {
-    const bool in = lane < kWarps;
-    join(in ? red[lane][0] : -INFINITY, in ? red[lane][1] : 0.f, in ? red[lane][2] : 0.f,
-         in ? red[lane][3] : 0.f);
+    const bool streamed = lane < kWarps - 1, own_list = REST && lane == kWarps - 1;
+    join(streamed ? red[lane][0] : -INFINITY, streamed ? red[lane][1] : 0.f,
+         own_list ? red[lane][0] : -INFINITY, own_list ? red[lane][2] : 0.f,
+         lane < kWarps ? red[lane][3] : 0.f);
   }
   if (splits > 1) {
     if (lister && lane == 0) {
-      joined[0] = top;
+      joined[0] = rest_top;
       joined[1] = rest_sum;
-      joined[2] = list_sum;
-      joined[3] = one_sum;
+      joined[2] = list_top;
+      joined[3] = list_sum;
+      joined[4] = one_sum;
     }
     cluster_sync();
     if (lister && rank == 0) {
@@ -410,17 +418,33 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
                      : "memory");
         return v;
       };
-      join(peer(0, -INFINITY), peer(1, 0.f), peer(2, 0.f), peer(3, 0.f));
+      join(peer(0, -INFINITY), peer(1, 0.f), peer(2, -INFINITY), peer(3, 0.f), peer(4, 0.f));
     }
   }
   if (lister && rank == 0) {
-    // the logarithms of the whole, of the rest's part of it, and of the labels' sum, a lane each
-    const double whole = static_cast<double>(rest_sum) + list_sum;
-    const double part = REST ? rest_sum / whole : 1.0;
-    const double logs = log(lane == 0 ? whole : lane == 1 ? part : static_cast<double>(one_sum));
-    const double log_all = ref * kLn2 + __shfl_sync(0xffffffffu, logs, 0);
-    const double log_q = REST ? __shfl_sync(0xffffffffu, logs, 1) : 0.0;
-    const double log_one = ref1 * kLn2 + __shfl_sync(0xffffffffu, logs, 2);
+    // The larger of the rest's and the list's part, and the other's share of it, which may be far below
+    // fp32's range; then four logarithms, a lane each: of the whole (relative to the larger part's
+    // maximum), of the whole by the larger part, of the labels' sum, of the sums' quotient.
+    const bool list_high = REST && list_top > rest_top;
+    const float high_top = fmaxf(rest_top, list_top);
+    const double high_ref = high_top == -INFINITY ? 0.0 : __fmul_rn(high_top, c);
+    const double gap = REST ? __fmul_rn(list_high ? rest_top : list_top, c) - high_ref : 0.0;
+    const double high = list_high ? list_sum : rest_sum, low = list_high ? rest_sum : list_sum;
+    const double quotient = !REST || low == 0.0 ? 0.0 : low / high;
+    const double less = REST ? quotient * exp2(gap) : 0.0, more = 1.0 + less;
+    const double logs = log(lane == 0   ? high * more
+                            : lane == 1 ? more
+                            : lane == 2 ? static_cast<double>(one_sum)
+                                        : quotient);
+    const double log_all = high_ref * kLn2 + __shfl_sync(0xffffffffu, logs, 0);
+    const double part = (list_high ? less : 1.0) / more;  // the rest's share, and its logarithm
+    double log_q = 0.0;
+    if (REST) {
+      const double log_more = __shfl_sync(0xffffffffu, logs, 1);
+      log_q = (list_high ? gap * kLn2 + __shfl_sync(0xffffffffu, logs, 3) : 0.0) - log_more;
+    }
+    const double log_one = (high_top == -INFINITY ? 0.0 : __fmul_rn(high_top, kL2e)) * kLn2 +
+                           __shfl_sync(0xffffffffu, logs, 2);
     if (lane == 0) {
       double loss = any ? own + share * log_all : 0.0;
       double coef = REST || any ? 1.0 : 0.0;

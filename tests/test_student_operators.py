@@ -705,6 +705,72 @@ def test_distill_bwd_in_place(dev, V, dtype):
     assert torch.equal(fused.distill_bwd(**args, out=c["logits"]), want)
 
 
+def far_case(dev, T, V, K, dtype, gap, tau, labels, high="list"):
+    """The listed tokens and the others `gap` apart in the student's logits; the teacher leaves the
+    others 0.23.  Half of the labels are listed, some are ignored."""
+    g = gen(dev, V + K + int(gap))
+    z = rand(g, T, V)
+    ids = torch.rand(T, V, generator=g, device=dev).argsort(1)[:, :K].int()
+    z.scatter_add_(1, ids.long(), torch.full((T, K), gap if high == "list" else -gap, device=dev))
+    z = z.to(dtype)
+    p = torch.softmax(rand(g, T, K), 1) * 0.77
+    c = {"logits": z, "top_ids": ids, "top_logits": p.log() * tau, "temperature": tau,
+         "top_lse": torch.zeros(T, device=dev), "labels": None}
+    if labels:
+        lab = torch.randint(0, V, (T,), generator=g, device=dev)
+        lab[::2] = ids[::2, -1].long()
+        lab[T // 2] = -1
+        c["labels"] = lab
+    return g, c
+
+
+def distill_far_check(g, c, err):
+    """Both losses and their gradient against 64 bits, each exponential within `err` of its size."""
+    T, V = c["logits"].shape
+    tau, dev = c["temperature"], c["logits"].device
+    kd, ce, lse, stats = fused.distill_fwd(**c)
+    z = c["logits"].double().requires_grad_()
+    want_kd, want_ce = distill64(c, z)
+    close(kd, want_kd.detach(), 3 * log_error(c["logits"], tau), "kd")
+    dkd = rand(g, T)
+    args = {k: c[k] for k in ("logits", "top_ids", "top_logits", "temperature", "labels")}
+    total, soft, dce = (want_kd * dkd.double()).sum(), 0.0, None
+    if ce is not None:
+        close(ce, want_ce.detach(), 2 * log_error(c["logits"], 1.0), "ce")
+        dce = rand(g, T)
+        total = total + (want_ce * dce.double()).sum()
+        soft = dce.double().masked_fill(c["labels"] < 0, 0.0).abs()[:, None]
+        soft = soft * (torch.softmax(z.detach(), 1) + 2 * U)
+    got = fused.distill_bwd(**args, stats=stats, lse=lse, dkd=dkd, dce=dce)
+    want = torch.autograd.grad(total, z)[0]
+    x = z.detach() / tau
+    inside = torch.zeros(T, V, dtype=torch.bool, device=dev).scatter_(1, c["top_ids"].long(), True)
+    p = torch.exp(c["top_logits"].double() / tau)
+    named = torch.zeros(T, V, dtype=F64, device=dev).scatter_add_(1, c["top_ids"].long(), p)
+    q = torch.softmax(x, 1)
+    share = torch.softmax(x.masked_fill(inside, -math.inf), 1)
+    part = q.masked_fill(inside, 0.0).sum(1, keepdim=True)
+    k = dkd.double().abs()[:, None] / tau
+    mass = k * (q + named + share * (part + 0.23)) + 2 * soft
+    # an exponential below 2^-126 counts as zero: the weights k (part - 0.23) and dce multiply one each
+    weights = k if dce is None else k + dce.double().abs()[:, None]
+    close(got, want, err * mass + 2.0 ** -126 * weights, "dlogits")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,V,K,dtype,labels", [
+    (5, 64, 2, F32, True), (9, 515, 7, BF, False), (4, 20000, 33, F32, False), (3, 40000, 5, BF, True),
+    (1100, 300, 4, HF, True)])
+@pytest.mark.parametrize("high", ["list", "rest"])
+@pytest.mark.parametrize("gap,tau", [(60.0, 1.0), (90.0, 1.0), (200.0, 1.0), (9.5, 0.1), (60.0, 0.1),
+                                     (200.0, 0.1), (150.0, 2.0)])
+def test_distill_far_apart(dev, T, V, K, dtype, labels, high, gap, tau):
+    """The student gives one side of the list next to nothing, less than fp32 holds: its logarithm
+    is still there, and so is the gradient."""
+    g, c = far_case(dev, T, V, K, dtype, gap, tau, labels, high)
+    distill_far_check(g, c, (4 * log_error(c["logits"], min(tau, 1.0)) + 2.0 ** -21)[:, None])
+
+
 def test_distill_definition_against_torch():
     """Without the teacher's tail the gradient is that of torch's divergence to a dense teacher."""
     g, c = distill_case("cpu", 5, 40, 40, F32, tail=False, labels=False, tau=2.0, seed=1)
