@@ -28,6 +28,16 @@ namespace cfb {
 
 constexpr float kL2e = 1.4426950408889634f;
 constexpr double kLn2 = 0.69314718055994530942;
+// From here on fp32 has no digits behind the point, and the logarithm of a sum does not say by how much
+// it differs from its largest term: a rest that lies so far below the list counts as none, and an
+// exponential relative to such a logarithm as zero.  Ordinary logits stay far below; masks do not.
+constexpr float kNoDigits = 8388608.f;  // 2^23
+// The lowest binary exponent: finite logits below it (masks by the type's lowest value, whose product
+// with the temperature may overflow) count as being there.
+constexpr float kLowest = -1073741824.f;  // -2^30
+__device__ __forceinline__ float exponent(float z, float scale) {
+  return fmaxf(__fmul_rn(z, scale), kLowest);  // rounded, as all that uses it
+}
 // A row is streamed by four warps, seven such blocks to an SM: while some wait for their list or sums,
 // others stream.  Of 16384 x 32000 bf16 logits with tail and labels at tau = 2 (161 us at the measured
 // copy rate) the forward takes 197 us, without tail 167; the gradient of 8192 rows (161 us) 174.  When
@@ -75,25 +85,38 @@ struct DistillArgs {
   int* err;
 };
 
+// How exp(z) comes beside exp(z / tau): not wanted or the same; an exponential of its own; the square
+// of the other (tau = 2), which halves the exponentials of a kernel that they would bind.
+enum { kOneNone = 0, kOneOwn = 1, kOneSquare = 2 };
+
 // The running sums of one thread: of exp2(z c - ref) over the tokens outside the list (or over all),
-// over the listed ones, and of exp2(z log2 e - ref1) over all.
+// over the listed ones, and of exp2(z log2 e - ref1) (or of the squares of the others) over all.
+template <int ONE>
 struct Sums {
-  float max = -INFINITY, ref = 0.f, ref1 = 0.f;
+  float max = -INFINITY, ref = kLowest, ref1 = kLowest;
   float rest = 0.f, listed = 0.f, one = 0.f;
   // moves the references to a new maximum
   __device__ __forceinline__ void raise(float m, float c) {
     if (!(m > max)) return;
-    const float r = __fmul_rn(m, c), r1 = __fmul_rn(m, kL2e);  // rounded, as all that uses them
-    const float f = max == -INFINITY ? 0.f : ex2(ref - r);
-    const float f1 = max == -INFINITY ? 0.f : ex2(ref1 - r1);
+    max = m;
+    const float r = exponent(m, c), f = ex2(ref - r);
     rest *= f;
     listed *= f;
-    one *= f1;
-    max = m;
     ref = r;
-    ref1 = r1;
+    if (ONE == kOneOwn) {
+      const float r1 = exponent(m, kL2e);
+      one *= ex2(ref1 - r1);
+      ref1 = r1;
+    }
+    if (ONE == kOneSquare) one *= f * f;
   }
 };
+
+// A listed logit's or the label's binary exponent, in 64 bits.
+__device__ __forceinline__ double listed_exponent(float z, float scale) {
+  const double x = static_cast<double>(z) * scale;
+  return x < kLowest && z > -INFINITY ? kLowest : x;
+}
 
 // Eight logits as they lie in memory: -inf in all places, or in those whose bits are set; the largest.
 __device__ __forceinline__ uint32_t ninf2(__nv_bfloat16) { return 0xff80ff80u; }
@@ -156,10 +179,6 @@ struct Span {
   __device__ __forceinline__ int tail() const { return head + packs * 8; }
   __device__ __forceinline__ Pack<T, 8> pack(int i) const { return load_pack<T, 8>(z + head + i * 8); }
 };
-
-// How exp(z) comes beside exp(z / tau): not wanted or the same; an exponential of its own; the square
-// of the other (tau = 2), which halves the exponentials of a kernel that they would bind.
-enum { kOneNone = 0, kOneOwn = 1, kOneSquare = 2 };
 
 // A row to a block (or, split over its columns, to a cluster of up to eight): four warps stream the
 // logits, a fifth reads the list, marks its tokens in a bit mask in shared memory for the others, and
@@ -229,7 +248,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
   }
   if (REST) __syncthreads();
 
-  Sums s;
+  Sums<ONE> s;
   // the teacher's part of the divergence, its shares' sum and normaliser (rank 0's lister)
   double own = 0.0, share = 0.0, norm = 0.0, left = 0.0, log_left = 0.0;
   bool any = false, label_in = false;
@@ -300,8 +319,10 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
         if (!(flags[j] & 2)) continue;
         const float v = sm_z[j];
         s.raise(v, c);
-        s.listed += ex2(fmaf(v, c, -s.ref));
-        if (ONE != kOneNone) s.one += ex2(fmaf(v, kL2e, -s.ref1));
+        const float e = ex2(fmaf(v, c, -s.ref));
+        s.listed += e;
+        if (ONE == kOneOwn) s.one += ex2(fmaf(v, kL2e, -s.ref1));
+        if (ONE == kOneSquare) s.one = fmaf(e, e, s.one);
       }
     }
     if (rank == 0) {
@@ -340,7 +361,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
           const double log_p = sm_t[j] * inv_temp - norm;
           const double pj = exp(log_p);
           share += pj;
-          if (!(pj == 0.0)) own += pj * (log_p - static_cast<double>(sm_z[j]) * c * kLn2);
+          if (!(pj == 0.0)) own += pj * (log_p - listed_exponent(sm_z[j], c) * kLn2);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -373,31 +394,41 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
   }
   __syncthreads();
   if (!lister && splits == 1) return;
-  // Lane b: warp b's sums, or block b's.  The rest's sum and the list's keep a maximum each: relative
-  // to the other's, one that is 87 logits (times the temperature) below would be lost, and with it all
-  // that is to be said of the rest.
+  // The rest's sum and the list's keep a maximum each: relative to the other's, one that is 87 logits
+  // (times the temperature) below would be lost, and with it all that is to be said of the rest.
+  // Lane b: warp b's sums, or block b's, each relative to the largest maximum of them.
   float rest_top, list_top, rest_sum, list_sum, one_sum;
-  const auto join = [&](float rest_max, float r, float list_max, float l, float o) {
-    const auto most = [](float v) {
+  const auto most = [](float v) {
 #pragma unroll
-      for (int i = 16; i > 0; i >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, i));
-      return v;
-    };
-    const auto moved = [](float sum, float from, float to, float scale) {
-      return from == to ? sum : sum * ex2(__fmul_rn(from, scale) - __fmul_rn(to, scale));
-    };
-    rest_top = most(rest_max);
-    list_top = REST ? most(list_max) : -INFINITY;
-    rest_sum = warp_add(moved(r, rest_max, rest_top, c));
-    list_sum = REST ? warp_add(moved(l, list_max, list_top, c)) : 0.f;
-    one_sum = ONE == kOneNone ? 0.f
-                              : warp_add(moved(o, fmaxf(rest_max, list_max), fmaxf(rest_top, list_top), kL2e));
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+  };
+  const auto moved = [](float sum, float from, float to, float scale) {
+    return sum * ex2(exponent(from, scale) - exponent(to, scale));
   };
   if (lister) {
-    const bool streamed = lane < kWarps - 1, own_list = REST && lane == kWarps - 1;
-    join(streamed ? red[lane][0] : -INFINITY, streamed ? red[lane][1] : 0.f,
-         own_list ? red[lane][0] : -INFINITY, own_list ? red[lane][2] : 0.f,
-         lane < kWarps ? red[lane][3] : 0.f);
+    const bool in = lane < kWarps, list_lane = REST && lane == kWarps - 1;
+    const float bm = in ? red[lane][0] : -INFINITY, rm = list_lane ? -INFINITY : bm;
+    rest_top = most(rm);
+    rest_sum = warp_add(moved(in ? red[lane][1] : 0.f, rm, rest_top, c));
+    list_top = REST ? red[kWarps - 1][0] : -INFINITY;
+    list_sum = REST ? red[kWarps - 1][2] : 0.f;
+    const float top = fmaxf(rest_top, list_top);
+    one_sum = ONE == kOneNone ? 0.f : warp_add(moved(in ? red[lane][3] : 0.f, bm, top, kL2e));
+    // nothing but masks (and -inf): they count one each
+    const auto masks = [](float top, float scale) { return top > -INFINITY && __fmul_rn(top, scale) < kLowest; };
+    if (masks(top, fmaxf(c, kL2e))) {
+      int all = 0, listed = 0;
+      for (int i = lane; i < n; i += 32) all += to_f32(mine[i]) > -INFINITY;
+      for (int j = lane; REST && j < K; j += 32) listed += (flags[j] & 2) && sm_z[j] > -INFINITY;
+      all = __reduce_add_sync(0xffffffffu, all);
+      listed = __reduce_add_sync(0xffffffffu, listed);
+      if (masks(top, c)) {
+        rest_sum = all - listed;
+        list_sum = listed;
+      }
+      if (masks(top, kL2e)) one_sum = all;
+    }
   }
   if (splits > 1) {
     if (lister && lane == 0) {
@@ -418,52 +449,48 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
                      : "memory");
         return v;
       };
-      join(peer(0, -INFINITY), peer(1, 0.f), peer(2, -INFINITY), peer(3, 0.f), peer(4, 0.f));
+      const float rm = peer(0, -INFINITY), lm = peer(2, -INFINITY);
+      rest_top = most(rm);
+      rest_sum = warp_add(moved(peer(1, 0.f), rm, rest_top, c));
+      if (REST) {
+        list_top = most(lm);
+        list_sum = warp_add(moved(peer(3, 0.f), lm, list_top, c));
+      }
+      one_sum = warp_add(moved(peer(4, 0.f), fmaxf(rm, lm), fmaxf(rest_top, list_top), kL2e));
     }
   }
   if (lister && rank == 0) {
-    // The larger of the rest's and the list's part, and the other's share of it, which may be far below
-    // fp32's range; then four logarithms, a lane each: of the whole (relative to the larger part's
-    // maximum), of the whole by the larger part, of the labels' sum, of the sums' quotient.
-    const bool list_high = REST && list_top > rest_top;
-    const float high_top = fmaxf(rest_top, list_top);
-    const double high_ref = high_top == -INFINITY ? 0.0 : __fmul_rn(high_top, c);
-    const double gap = REST ? __fmul_rn(list_high ? rest_top : list_top, c) - high_ref : 0.0;
-    const double high = list_high ? list_sum : rest_sum, low = list_high ? rest_sum : list_sum;
-    const double quotient = !REST || low == 0.0 ? 0.0 : low / high;
-    const double less = REST ? quotient * exp2(gap) : 0.0, more = 1.0 + less;
-    const double logs = log(lane == 0   ? high * more
-                            : lane == 1 ? more
-                            : lane == 2 ? static_cast<double>(one_sum)
-                                        : quotient);
-    const double log_all = high_ref * kLn2 + __shfl_sync(0xffffffffu, logs, 0);
-    const double part = (list_high ? less : 1.0) / more;  // the rest's share, and its logarithm
-    double log_q = 0.0;
-    if (REST) {
-      const double log_more = __shfl_sync(0xffffffffu, logs, 1);
-      log_q = (list_high ? gap * kLn2 + __shfl_sync(0xffffffffu, logs, 3) : 0.0) - log_more;
-    }
-    const double log_one = (high_top == -INFINITY ? 0.0 : __fmul_rn(high_top, kL2e)) * kLn2 +
-                           __shfl_sync(0xffffffffu, logs, 2);
+    // the logarithms of the whole, of the rest's sum, and of the labels' sum, a lane each
+    const float top = fmaxf(rest_top, list_top);
+    const float ref = exponent(top, c), rest_ref = exponent(rest_top, c);
+    const float rest_part = REST ? rest_sum * ex2(rest_ref - ref) : rest_sum;
+    const double whole = REST ? rest_part + static_cast<double>(list_sum * ex2(exponent(list_top, c) - ref))
+                              : static_cast<double>(rest_part);
+    const double logs = log(lane == 0 ? whole : static_cast<double>(lane == 1 ? rest_sum : one_sum));
+    const double log_all = ref * kLn2 + __shfl_sync(0xffffffffu, logs, 0);
+    const double log_rest = REST ? rest_ref * kLn2 + __shfl_sync(0xffffffffu, logs, 1) : log_all;
+    const double log_one = exponent(top, kL2e) * kLn2 + __shfl_sync(0xffffffffu, logs, 2);
     if (lane == 0) {
       double loss = any ? own + share * log_all : 0.0;
       double coef = REST || any ? 1.0 : 0.0;
+      bool some = true;
       if (REST) {
-        const bool some = rest_sum != 0.f;  // tokens outside the list, not all of them at -inf
-        if (some && !(left == 0.0)) loss += left * (log_left - log_q);
-        coef = some ? (share > 1.0 ? share : 1.0) * part - left : 0.0;
+        // tokens outside the list, not all of them at -inf or masked (a NaN among them stays one)
+        some = rest_sum != 0.f && !(rest_sum > 0.f && (rest_ref - ref) * kLn2 < -kNoDigits);
+        if (some && !(left == 0.0)) loss += left * (log_left - (log_rest - log_all));
+        coef = some ? (share > 1.0 ? share : 1.0) * (rest_part / whole) - left : 0.0;
       }
       kd[row] = static_cast<float>(loss);
       float4 o;
       o.x = static_cast<float>(log_all);
-      o.y = static_cast<float>(log_all + log_q);
+      o.y = some ? static_cast<float>(log_rest) : -INFINITY;
       o.z = static_cast<float>(coef);
       o.w = static_cast<float>(norm);
       reinterpret_cast<float4*>(stats)[row] = o;
       if (p.labels) {
         const double full = ONE == kOneNone ? log_all : log_one;
         lse[row] = static_cast<float>(full);
-        ce[row] = label_in ? static_cast<float>(full - static_cast<double>(z_label) * kL2e * kLn2) : 0.f;
+        ce[row] = label_in ? static_cast<float>(full - listed_exponent(z_label, kL2e) * kLn2) : 0.f;
       }
     }
   }
@@ -473,6 +500,10 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
 __device__ __forceinline__ F2 exp_of(F2 v, float scale, float off) {
   const float2 x = halves(fma2(v, f2(scale), f2(-off)));
   return f2(ex2(x.x), ex2(x.y));
+}
+// What exponentials relative to a logarithm count from; a far one leaves none of them.
+__device__ __forceinline__ float reference(float log_sum) {
+  return fabsf(log_sum) >= kNoDigits ? 3e38f : log_sum * kL2e;
 }
 // Slots of the table in which the lister finds a token that is named twice.
 __host__ __device__ inline int table_slots(int K) {
@@ -530,10 +561,10 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
   if (k != 0.f) st = reinterpret_cast<const float4*>(stats)[src];
   const float gk = k * st.z;
-  const bool spread = gk != 0.f;  // also a NaN
+  const bool spread = gk != 0.f && !(CE == kCeSame && fabsf(st.y) >= kNoDigits);  // also a NaN
   const float c = p.inv_temp * kL2e;
-  const float ref = spread ? st.y * kL2e : 0.f;
-  const float ref1 = CE && g1 != 0.f ? lse[src] * kL2e : 0.f;
+  const float ref = spread ? reference(st.y) : 0.f;
+  const float ref1 = CE && g1 != 0.f ? reference(lse[src]) : 0.f;
 
   if (!lister) {
     const auto stream = [&](auto&& value) {
@@ -648,7 +679,8 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
   named = __any_sync(0xffffffffu, named);
   twice = __any_sync(0xffffffffu, twice);
   __syncwarp();
-  const double lse1 = labelled ? lse[src] : 0.0;
+  const auto from = [](float log_sum) -> double { return fabsf(log_sum) >= kNoDigits ? INFINITY : log_sum; };
+  const double from_all = from(st.x), from1 = labelled ? from(lse[src]) : 0.0;
   for (int j = lane; j < entries; j += 32) {
     const int at = sm_id[j];
     if (at < 0 || !in_range(at)) continue;
@@ -658,14 +690,14 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
       share = 0.f;
       for (int i = 0; i < K; ++i) share += sm_id[i] == at ? sm_p[i] : 0.f;
     }
-    double g = k * (whole * exp(v * p.inv_temp64 - st.x) - share);
-    if (labelled) g += g1 * (exp(v - lse1) - (at == label ? 1.0 : 0.0));
+    double g = k * (whole * exp(v * p.inv_temp64 - from_all) - share);
+    if (labelled) g += g1 * (exp(v - from1) - (at == label ? 1.0 : 0.0));
     sm_g[j] = static_cast<float>(g);
   }
   const bool label_alone = label_here && !named;
   const float label_grad =
-      label_alone ? static_cast<float>((spread ? gk * exp(z_label * p.inv_temp64 - st.y) : 0.0) +
-                                       g1 * (exp(z_label - lse1) - 1.0))
+      label_alone ? static_cast<float>((spread ? gk * exp(z_label * p.inv_temp64 - from(st.y)) : 0.0) +
+                                       g1 * (exp(z_label - from1) - 1.0))
                   : 0.f;
   __syncthreads();  // the range is written
   for (int j = lane; j < entries; j += 32)

@@ -493,12 +493,17 @@ def distill_fwd(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: torch.T
       ``kd = sum p (log p - log q)``; an empty list, or one of ``-inf`` alone, gives 0.
     * ``top_lse [T]`` (fp32) is ``log sum exp`` of *all* the teacher's logits ``/ tau``; then
       ``p = exp(top_logits / tau - top_lse)``, and what is left of 1 is compared with the student's
-      share of all tokens outside the list (where the student gives them any).
+      share of all tokens outside the list (where the student gives them any: one whose logarithm is
+      2^23 or more below the list's, as of masked logits, counts as none).
 
     ``kd`` is not scaled by ``tau^2``.  With ``labels`` (int64 ``[T]``; negative: ignored, 0), ``ce``
     and ``lse`` are those of :func:`ce_fwd`, without them ``None``.  ``stats`` (fp32 ``[T, 4]``:
     ``log sum exp(logits / tau)``, the same of the tokens outside the list, their share less the
     teacher's, and the teacher's normaliser) is what :func:`distill_bwd` needs.
+
+    Logits may be masked by ``-inf`` or by their type's lowest value: a finite logit (for kd: over
+    ``tau``) below ``-2^30 log 2`` counts as being there, so that a row of such masks alone is a uniform
+    distribution.
 
     Logits and ``top_logits`` are bf16, fp16 or fp32 with any row stride and alignment, ``V`` up to
     1048576, ``K`` up to 1024.  On the GPU an id or label outside the vocabulary records an error in
@@ -526,7 +531,9 @@ def distill_bwd(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: torch.T
     all when ``None``), rounded once: what both losses give, in one pass.
 
     ``dkd [R]`` and ``dce [R]`` are fp32; ``labels``, ``lse`` (of the forward) and ``dce`` go
-    together.  A weight of zero adds nothing, whatever the row holds.  ``out [R, V]`` has the type of
+    together.  A weight of zero adds nothing, whatever the row holds.  Relative to a logarithm of 2^23 or
+    more in size (a row of masks alone) exponentials count as zero, since fp32 statistics do not hold
+    its digits.  ``out [R, V]`` has the type of
     the logits and any row stride, and may be the logits themselves without ``rows``; other overlaps
     are refused.  On the GPU a row id outside the logits records an error in the status block and
     gives a zero row; on the CPU it raises ``IndexError``."""

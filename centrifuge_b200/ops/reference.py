@@ -117,12 +117,23 @@ def linear_act_dgrad(dy, w, z, act):
     return (dy.float() @ w.float()) * activation_grad(z.float(), act)
 
 
+# From here on fp32 has no digits behind the point: a rest of the vocabulary that lies so far below the
+# list counts as none, and an exponential relative to such a logarithm of a sum as zero.
+NO_DIGITS = 2.0 ** 23
+# Finite logits below this (masks by the type's lowest value) count as being there.
+LOWEST = -2.0 ** 30 * math.log(2.0)
+
+
+def _with_masks(x):
+    return torch.where((x < LOWEST) & (x > -math.inf), torch.full_like(x, LOWEST), x)
+
+
 def distill(logits, top_ids, top_logits, temperature, top_lse=None, labels=None):
     """Divergence of the student from a teacher's top logits and the labels' cross entropy (fp64):
     ``(kd, ce, lse, stats)``; entries with a negative id are left out."""
     z, ids = logits.double(), top_ids.long()
     ok, inf = ids >= 0, float("inf")
-    x = z / temperature
+    x = _with_masks(z / temperature)
     lse = torch.logsumexp(x, -1)
     t = (top_logits.double() / temperature).masked_fill(~ok, -inf)
     norm = torch.logsumexp(t, -1) if top_lse is None else top_lse.double()
@@ -134,7 +145,9 @@ def distill(logits, top_ids, top_logits, temperature, top_lse=None, labels=None)
     base, coef = lse, (~none).double()
     if top_lse is not None:
         others = torch.cat([x, x[:, :1]], -1).scatter(-1, ids.masked_fill(~ok, x.shape[-1]), -inf)
-        base = torch.logsumexp(others[:, :-1], -1)
+        others = others[:, :-1]
+        gap = others.amax(-1) - x.amax(-1)
+        base = torch.logsumexp(others, -1).masked_fill(gap < -NO_DIGITS, -inf)
         share = p.sum(-1)
         left = (1.0 - share).clamp(min=0.0)
         rest = (base - lse).masked_fill(base == -inf, -inf)
@@ -143,9 +156,14 @@ def distill(logits, top_ids, top_logits, temperature, top_lse=None, labels=None)
     stats = torch.stack([lse, base, coef, norm], -1)
     if labels is None:
         return kd, None, None, stats
+    z = _with_masks(z)
     full = torch.logsumexp(z, -1)
     ce = full - z.gather(-1, labels.clamp(min=0).unsqueeze(-1)).squeeze(-1)
     return kd, ce.masked_fill(labels < 0, 0.0), full, stats
+
+
+def _exp_from(x, log_sum):
+    return torch.exp(x - log_sum).masked_fill(log_sum.abs() >= NO_DIGITS, 0.0)
 
 
 def distill_bwd(logits, top_ids, top_logits, stats, dkd, temperature, labels=None, lse=None,
@@ -157,19 +175,19 @@ def distill_bwd(logits, top_ids, top_logits, stats, dkd, temperature, labels=Non
     k = (dkd.double() / temperature).unsqueeze(-1)
     x = z / temperature
     spread = k * st[:, 2:3]
-    g = (torch.exp(x - st[:, 1:2]) * spread).masked_fill(spread == 0, 0.0)
+    g = (_exp_from(x, st[:, 1:2]) * spread).masked_fill(spread == 0, 0.0)
     t = (top_logits.double() / temperature).masked_fill(~ok, -inf)
     p = torch.exp(t - st[:, 3:4]).masked_fill(~ok, 0.0)
     g = torch.cat([g, g[:, :1]], -1)
     at = ids.masked_fill(~ok, V)
-    q = torch.exp(x.gather(-1, ids.clamp(min=0)) - st[:, 0:1])
+    q = _exp_from(x.gather(-1, ids.clamp(min=0)), st[:, 0:1])
     whole = p.sum(-1, keepdim=True)  # what the teacher's terms add up to: one, but for a list of all
     whole = torch.where(st[:, 1:2] == -inf, whole, whole.clamp(min=1.0))
     g.scatter_(-1, at, k * q * whole).scatter_add_(-1, at, -k * p)
     g = g[:, :V].masked_fill((k == 0), 0.0)
     if labels is not None:
         w = dce.double().masked_fill(labels < 0, 0.0).unsqueeze(-1)
-        soft = torch.exp(z - lse.double().unsqueeze(-1))
+        soft = _exp_from(z, lse.double().unsqueeze(-1))
         soft.scatter_add_(-1, labels.clamp(min=0).unsqueeze(-1), -torch.ones_like(w))
         g = g + (w * soft).masked_fill(w == 0, 0.0)
     return g

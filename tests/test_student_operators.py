@@ -771,6 +771,64 @@ def test_distill_far_apart(dev, T, V, K, dtype, labels, high, gap, tau):
     distill_far_check(g, c, (4 * log_error(c["logits"], min(tau, 1.0)) + 2.0 ** -21)[:, None])
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("T,V,kept_cols", [
+    (4, 1000, 992), (4, 1003, 1002), (3, 40000, 28000), (2, 64, 8), (1100, 300, 100)])
+@pytest.mark.parametrize("tau,tail", [(1.0, True), (2.0, True), (0.7, True), (1.0, False), (0.5, False)])
+def test_distill_logits_masked_by_the_lowest_value(dev, dtype, T, V, kept_cols, tau, tail):
+    """A mask by the type's lowest value, whose product with the temperature may overflow, is one by
+    -inf: in some columns, and where the list is all that is left of the vocabulary."""
+    if dtype == HF:  # (-65504 is a logit like any other: the list may not be all that is left)
+        kept_cols = max(kept_cols, 40)
+    g = gen(dev, V + T)
+    z = rand(g, T, V, dtype=dtype)
+    K = min(kept_cols, 8)
+    ids = torch.rand(T, kept_cols, generator=g, device=dev).argsort(1)[:, :K]
+    lab = torch.randint(0, kept_cols, (T,), generator=g, device=dev)
+    top = rand(g, T, K)
+    lse = (top / tau).logsumexp(1) + 0.2 if tail else None
+    dkd, dce = rand(g, T), rand(g, T)
+    outs = []
+    for low in (-math.inf, torch.finfo(dtype).min):
+        z[:, kept_cols:] = low
+        kd, ce, s, stats = fused.distill_fwd(z, ids, top, tau, top_lse=lse, labels=lab)
+        outs.append((kd, ce, s, stats, fused.distill_bwd(z, ids, top, stats, dkd, tau, labels=lab,
+                                                         lse=s, dce=dce)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert all(bool(t.isfinite().all()) for t in outs[0][:3] + outs[0][4:])
+    c = {"logits": z[:, :kept_cols], "top_ids": ids, "top_logits": top, "temperature": tau,
+         "top_lse": lse, "labels": lab}
+    want_kd, want_ce = distill64(c)
+    close(kd, want_kd, 3 * log_error(c["logits"], tau), "kd")
+    close(ce, want_ce, 2 * log_error(c["logits"], 1.0), "ce")
+    assert not outs[0][4][:, kept_cols:].any()
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("low", [None, -1e4, -1e9, -1e30])
+@pytest.mark.parametrize("T,V,tau,tail", [(3, 200, 1.0, True), (2, 20000, 2.0, True), (5, 515, 0.7, False),
+                                          (4, 1000, 0.5, True)])
+def test_distill_rows_of_which_nothing_is_left(dev, dtype, low, T, V, tau, tail):
+    """All logits at the value of a mask: what is left is a uniform distribution."""
+    low = torch.finfo(dtype).min if low is None or dtype == HF else low
+    g = gen(dev, V)
+    z = torch.full((T, V), low, dtype=dtype, device=dev)
+    ids, lab = torch.arange(6, device=dev).repeat(T, 1), torch.full((T,), 3, device=dev)
+    top = rand(g, T, 6)
+    lse = (top / tau).logsumexp(1) + 0.2 if tail else None
+    kd, ce, s, stats = fused.distill_fwd(z, ids, top, tau, top_lse=lse, labels=lab)
+    c = {"logits": z * 0, "top_ids": ids, "top_logits": top, "temperature": tau, "top_lse": lse,
+         "labels": lab}
+    want_kd, want_ce = distill64(c)
+    close(kd, want_kd, 3 * log_error(c["logits"], tau), "kd")
+    close(ce, want_ce, 2 * log_error(c["logits"], 1.0), "ce")
+    assert bool(s.isfinite().all()) and bool(stats.isfinite().all())
+    got = fused.distill_bwd(z, ids, top, stats, rand(g, T), tau, labels=lab, lse=s, dce=rand(g, T))
+    assert bool(got.isfinite().all()) and bool(got.abs().max() < 20 / tau)
+
+
 def test_distill_definition_against_torch():
     """Without the teacher's tail the gradient is that of torch's divergence to a dense teacher."""
     g, c = distill_case("cpu", 5, 40, 40, F32, tail=False, labels=False, tau=2.0, seed=1)
