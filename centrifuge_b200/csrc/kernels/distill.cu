@@ -633,7 +633,8 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
   float* sm_g = sm_p + K;                             // the student's logits here, then the gradients
   int* table = reinterpret_cast<int*>(sm_g + K);
   const int slots = table_slots(K);
-  const int entries = k != 0.f ? K : 0;
+  // (a list without the teacher's lse and without a share says nothing)
+  const int entries = k != 0.f && !(st.w == -INFINITY && st.z == 0.f) ? K : 0;
   const auto in_range = [&](long long v) { return v >= v0 && v < v0 + n; };
   for (int i = lane; entries && i < slots; i += 32) table[i] = -1;
   for (int j = lane; j < entries; j += 32) {

@@ -173,6 +173,7 @@ def distill_bwd(logits, top_ids, top_logits, stats, dkd, temperature, labels=Non
     V, inf = z.shape[-1], float("inf")
     ok = ids >= 0
     k = (dkd.double() / temperature).unsqueeze(-1)
+    k = k.masked_fill((st[:, 3:4] == -inf) & (st[:, 2:3] == 0), 0.0)  # a list without a share
     x = z / temperature
     spread = k * st[:, 2:3]
     g = (_exp_from(x, st[:, 1:2]) * spread).masked_fill(spread == 0, 0.0)

@@ -829,6 +829,34 @@ def test_distill_rows_of_which_nothing_is_left(dev, dtype, low, T, V, tau, tail)
     assert bool(got.isfinite().all()) and bool(got.abs().max() < 20 / tau)
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,V,K", [(4, 64, 2), (5, 1003, 1), (3, 40000, 33), (1100, 300, 6)])
+@pytest.mark.parametrize("tau,labels", [(1.0, False), (1.0, True), (2.0, True), (0.7, False)])
+def test_distill_lists_without_a_share(dev, T, V, K, tau, labels):
+    """A list of nothing but -inf is an empty one: no divergence, and no gradient but the labels'."""
+    g = gen(dev, V)
+    z, ids = rand(g, T, V), torch.rand(T, V, generator=g, device=dev).argsort(1)[:, :K]
+    top = torch.full((T, K), -math.inf, device=dev)
+    top[0] = rand(g, K)
+    lab = ids[:, -1].clone() if labels else None
+    if labels:
+        lab[::2] = (ids[::2, 0] + 1) % V
+    dkd, dce = rand(g, T), rand(g, T) if labels else None
+    grads = []
+    for where in (ids, torch.where(top > -math.inf, ids, torch.full_like(ids, -1))):
+        kd, _, lse, stats = fused.distill_fwd(z, where, top, tau, labels=lab)
+        assert not kd[1:].any() and bool(kd[0] > 0)
+        grads.append(fused.distill_bwd(z, where, top, stats, dkd, tau, labels=lab, lse=lse, dce=dce))
+    # (of a listed label the exponential is formed in 64 bits)
+    close(grads[0], grads[1].double(), 2.0 ** -20 * grads[1].double().abs(), "as without entries")
+    alone = fused.distill_bwd(z, ids, top, stats, torch.zeros_like(dkd), tau, labels=lab, lse=lse, dce=dce)
+    assert torch.equal(grads[0][1:], alone[1:]) and bool(grads[0][0].any())
+    top[1, 0] = math.nan
+    kd, _, lse, stats = fused.distill_fwd(z, ids, top, tau, labels=lab)
+    got = fused.distill_bwd(z, ids, top, stats, dkd, tau, labels=lab, lse=lse, dce=dce)
+    assert bool(kd[1].isnan()) and bool(got[1].isnan().any())
+
+
 def test_distill_definition_against_torch():
     """Without the teacher's tail the gradient is that of torch's divergence to a dense teacher."""
     g, c = distill_case("cpu", 5, 40, 40, F32, tail=False, labels=False, tau=2.0, seed=1)
