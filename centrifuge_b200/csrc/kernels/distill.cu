@@ -14,7 +14,8 @@
 //
 // Beside it ce = lse(z) - z_label, dce/dz = softmax(z) - onehot.  The other tokens' sum is formed
 // over them alone (the whole minus the listed would lose it), a row's statistics are
-//   stats = (log sum exp(z / tau), the same of the tokens outside the list, q_rest - left, norm)
+//   stats = (log sum exp(z / tau), the same of the tokens outside the list, q_rest - left (times what
+//            makes up for the rounding of a far logarithm before it), norm)
 // (without the teacher's lse: (lse, lse, 1, norm)), so that the gradient reads each logit once and
 // takes one exponential for either loss.
 //
@@ -112,6 +113,10 @@ struct Sums {
   }
 };
 
+// What the gradient's exponentials relative to a logarithm count from; a far one leaves none of them.
+__device__ __forceinline__ float reference(float log_sum) {
+  return fabsf(log_sum) >= kNoDigits ? 3e38f : log_sum * kL2e;
+}
 // A listed logit's or the label's binary exponent, in 64 bits.
 __device__ __forceinline__ double listed_exponent(float z, float scale) {
   const double x = static_cast<double>(z) * scale;
@@ -484,6 +489,12 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
       float4 o;
       o.x = static_cast<float>(log_all);
       o.y = some ? static_cast<float>(log_rest) : -INFINITY;
+      if (REST && some && fabsf(o.y) > 128.f) {
+        // What multiplies the exponentials relative to this logarithm makes up for its rounding, and for
+        // that of the gradient's binary exponents: 1e-5 of them at 128, as much as theirs at 1e6.
+        const double t = reference(o.y) * kLn2 - log_rest;
+        coef *= fabs(t) < 0.002 ? 1.0 + t + 0.5 * t * t : fabs(t) < 2.0 ? exp(t) : 1.0;
+      }
       o.z = static_cast<float>(coef);
       o.w = static_cast<float>(norm);
       reinterpret_cast<float4*>(stats)[row] = o;
@@ -500,10 +511,6 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
 __device__ __forceinline__ F2 exp_of(F2 v, float scale, float off) {
   const float2 x = halves(fma2(v, f2(scale), f2(-off)));
   return f2(ex2(x.x), ex2(x.y));
-}
-// What exponentials relative to a logarithm count from; a far one leaves none of them.
-__device__ __forceinline__ float reference(float log_sum) {
-  return fabsf(log_sum) >= kNoDigits ? 3e38f : log_sum * kL2e;
 }
 // Slots of the table in which the lister finds a token that is named twice.
 __host__ __device__ inline int table_slots(int K) {
@@ -697,7 +704,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_bwd_kernel(
   }
   const bool label_alone = label_here && !named;
   const float label_grad =
-      label_alone ? static_cast<float>((spread ? gk * exp(z_label * p.inv_temp64 - from(st.y)) : 0.0) +
+      label_alone ? static_cast<float>((spread ? gk * exp2(static_cast<double>(z_label) * c - ref) : 0.0) +
                                        g1 * (exp(z_label - from1) - 1.0))
                   : 0.f;
   __syncthreads();  // the range is written

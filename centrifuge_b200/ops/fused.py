@@ -499,7 +499,8 @@ def distill_fwd(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: torch.T
     ``kd`` is not scaled by ``tau^2``.  With ``labels`` (int64 ``[T]``; negative: ignored, 0), ``ce``
     and ``lse`` are those of :func:`ce_fwd`, without them ``None``.  ``stats`` (fp32 ``[T, 4]``:
     ``log sum exp(logits / tau)``, the same of the tokens outside the list, their share less the
-    teacher's, and the teacher's normaliser) is what :func:`distill_bwd` needs.
+    teacher's (times what makes up for the rounding of a large value before it), and the teacher's
+    normaliser) is what :func:`distill_bwd` needs.
 
     Logits may be masked by ``-inf`` or by their type's lowest value: a finite logit (for kd: over
     ``tau``) below ``-2^30 log 2`` counts as being there, so that a row of such masks alone is a uniform

@@ -152,7 +152,9 @@ def distill(logits, top_ids, top_logits, temperature, top_lse=None, labels=None)
         left = (1.0 - share).clamp(min=0.0)
         rest = (base - lse).masked_fill(base == -inf, -inf)
         kd = kd + (left * (left.log() - rest)).masked_fill((left == 0) | (base == -inf), 0.0)
-        coef = (share.clamp(min=1.0) * rest.exp() - left).masked_fill(base == -inf, 0.0)
+        rounded = base.float().double()  # as a statistic, and what makes up for it
+        coef = (share.clamp(min=1.0) * rest.exp() - left) * (rounded - base).clamp(-2.0, 2.0).exp()
+        coef, base = coef.masked_fill(base == -inf, 0.0), rounded
     stats = torch.stack([lse, base, coef, norm], -1)
     if labels is None:
         return kd, None, None, stats

@@ -772,6 +772,35 @@ def test_distill_far_apart(dev, T, V, K, dtype, labels, high, gap, tau):
 
 
 @pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T,V,K", [(5, 300, 3), (3, 20000, 33)])
+@pytest.mark.parametrize("gap,tau", [(200.0, 0.1), (1e4, 1.0), (1e4, 2.0), (3e5, 0.7), (4e6, 1.0)])
+@pytest.mark.parametrize("labels", [False, True])
+def test_distill_gradient_of_a_far_rest(dev, T, V, K, gap, tau, labels):
+    """The gradient of the tokens outside the list does not depend on how far they all lie below it,
+    although an fp32 logarithm of their sum has ever fewer digits."""
+    g, c = far_case(dev, T, V, K, F32, gap, tau, labels)
+    c["logits"] -= gap  # the list near zero, the others far below
+    _, _, lse, stats = fused.distill_fwd(**c)
+    dkd, dce = rand(g, T), rand(g, T) if labels else None
+    args = {k: c[k] for k in ("logits", "top_ids", "top_logits", "temperature", "labels")}
+    got = fused.distill_bwd(**args, stats=stats, lse=lse, dkd=dkd, dce=dce)
+    x = c["logits"].double() / tau
+    out = torch.zeros(T, V, dtype=torch.bool, device=dev).scatter_(1, c["top_ids"].long(), True)
+    left = (1 - torch.exp(c["top_logits"].double() / tau).sum(1, keepdim=True))
+    share = torch.softmax(x.masked_fill(out, -math.inf), 1)
+    want = -dkd.double()[:, None] / tau * left * share
+    if labels:
+        at = torch.arange(T, device=dev)[c["labels"] >= 0], c["labels"][c["labels"] >= 0]
+        want[at] -= dce.double()[c["labels"] >= 0]
+    # the sum (2^-22 of each exponential, a chain of 200 additions) and the exponential (the same, its
+    # argument rounded at up to 150), the differences of the logits times the rounded temperature, five
+    # roundings of factors
+    spread = (x.masked_fill(out, -math.inf).amax(1) - x.masked_fill(out, math.inf).amin(1))[:, None]
+    tol = (2.0 ** -21 + (64 + 200 + 150 + 5 + 3 * spread) * U) * want.abs() + 2.0 ** -126 * dkd.abs()[:, None]
+    close(got.masked_fill(out, 0.0), want.masked_fill(out, 0.0), tol, "dlogits")
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 @pytest.mark.parametrize("T,V,kept_cols", [
     (4, 1000, 992), (4, 1003, 1002), (3, 40000, 28000), (2, 64, 8), (1100, 300, 100)])
