@@ -173,7 +173,8 @@ struct TileShape {
 constexpr int kLinearThreads = 384, kEpilogueWarp = 4;
 constexpr int kFewRegisters = 56, kManyRegisters = 224;
 // wgrad: the tensor cores' additions lose 1.1e-9 of the result for each further row (8192 rows:
-// 9.1e-6), so that their sum ends after 1024 rows and is added to fp32 sums in registers.
+// 9.1e-6; of one sign, twice that), so that their sum ends after 1024 rows and is added to fp32 sums in
+// registers.
 constexpr int kSegment = 16;  // blocks of 64 rows
 
 // The m-blocks of a group of 16 take turns, so that their rows and the columns at hand stay in L2.
@@ -810,7 +811,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   using S = SplitShape;
   constexpr bool A_MN = KIND == kLinearWgrad, B_MN = KIND != kLinearFwd;
   if (KIND == kLinearWgrad) let_next_start();  // the column sums
-  // wgrad: an accumulator for every 1024 rows, up to four (see kSegment)
+  // wgrad: four accumulators, of which each takes 1024 rows at a time (see kSegment), while the epilogue
+  // adds the others' to its registers
   constexpr int kAccumulators = KIND == kLinearWgrad ? 4 : 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -818,7 +820,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE_BYTES);
   uint64_t* empty = full + S::STAGES;
   uint64_t* done = empty + S::STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* acc_full = done + 1;
+  uint64_t* acc_empty = acc_full + kAccumulators;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAccumulators);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = warp_id(), lane = lane_id();
   const int rank = splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -828,9 +832,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   const int num_kb = (p.K + S::BK - 1) / S::BK;
   const int kb0 = static_cast<int>(static_cast<long long>(rank) * num_kb / splits);
   const int kb1 = static_cast<int>(static_cast<long long>(rank + 1) * num_kb / splits);
-  int per_acc = kSegment;  // blocks of k an accumulator takes
-  if (KIND != kLinearWgrad) per_acc = kb1 - kb0;
-  else if (kb1 - kb0 > kAccumulators * kSegment) per_acc = (kb1 - kb0 + kAccumulators - 1) / kAccumulators;
+  // segments of k, each with an accumulator for as long as it takes
+  const int segments = KIND == kLinearWgrad ? (kb1 - kb0 + kSegment - 1) / kSegment : 1;
   const uint32_t smem_base = smem_u32(smem);
   const uint32_t bytes = (A_MN ? 2 * 8192 : a_rows * 128) + (B_MN ? 2 * 8192 : b_rows * 128);
   const auto fill = [&](int kb) {  // the copies of block kb0 + kb
@@ -868,6 +871,11 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmB);
   }
+  if (KIND == kLinearWgrad && warp == 3 && lane < kAccumulators) {
+    mbar_init(smem_u32(&acc_full[lane]), 1);
+    mbar_init(smem_u32(&acc_empty[lane]), 8);  // the epilogue warps
+    fence_mbar_init();
+  }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), S::BN * kAccumulators);
     tmem_relinquish();
@@ -894,29 +902,38 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   } else if (warp == 1) {
     constexpr uint32_t a_step = A_MN ? 2048 : 32, a_lbo = A_MN ? 8192 : 16;
     constexpr uint32_t b_step = B_MN ? 2048 : 32, b_lbo = B_MN ? 8192 : 16;
-    int stage = 0, in_acc = 0;
-    uint32_t phase = 0, d = tmem_base;
-    bool ready = false;
-    for (int kb = 0; kb < blocks; ++kb) {
-      if (!ready && !mbar_wait(smem_u32(&full[stage]), phase, abort_flag, p.err, kErrWaitMma)) break;
-      __syncwarp();
-      tc_fence_after();
-      const uint32_t sa = smem_base + stage * S::STAGE_BYTES, sb = sa + S::A_BYTES;
+    int stage = 0, kb = 0;
+    uint32_t phase = 0;
+    bool ready = false, ok = true;
+    for (int segment = 0; kb < blocks && ok; ++segment) {
+      const int accumulator = segment % kAccumulators;
+      if (KIND == kLinearWgrad && segment >= kAccumulators &&
+          !mbar_wait(smem_u32(&acc_empty[accumulator]), (segment / kAccumulators & 1) ^ 1, abort_flag, p.err,
+                     kErrWaitMma))
+        break;
+      const uint32_t d = tmem_base + accumulator * S::BN;
+      const int end = KIND == kLinearWgrad ? min(blocks, kb + kSegment) : blocks;
+      for (bool first = true; kb < end; ++kb, first = false) {
+        if (!ready && !mbar_wait(smem_u32(&full[stage]), phase, abort_flag, p.err, kErrWaitMma)) {
+          ok = false;
+          break;
+        }
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t sa = smem_base + stage * S::STAGE_BYTES, sb = sa + S::A_BYTES;
 #pragma unroll
-      for (int k = 0; k < S::BK / 16; ++k)
-        mma_lane0(lane, d, sdesc_sw128(sa + k * a_step, a_lbo, 1024),
-                     sdesc_sw128(sb + k * b_step, b_lbo, 1024), p.idesc, in_acc != 0 || k != 0);
-      const uint32_t freed = smem_u32(&empty[stage]);
-      if (++stage == S::STAGES) {
-        stage = 0;
-        phase ^= 1;
+        for (int k = 0; k < S::BK / 16; ++k)
+          mma_lane0(lane, d, sdesc_sw128(sa + k * a_step, a_lbo, 1024),
+                    sdesc_sw128(sb + k * b_step, b_lbo, 1024), p.idesc, !first || k != 0);
+        const uint32_t freed = smem_u32(&empty[stage]);
+        if (++stage == S::STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+        ready = kb + 1 < blocks && mbar_try_wait(smem_u32(&full[stage]), phase);
+        commit_lane0(lane, freed);
       }
-      ready = kb + 1 < blocks && mbar_try_wait(smem_u32(&full[stage]), phase);
-      commit_lane0(lane, freed);
-      if (++in_acc == per_acc) {
-        in_acc = 0;
-        d += S::BN;
-      }
+      if (KIND == kLinearWgrad && ok && kb < blocks) commit_lane0(lane, smem_u32(&acc_full[accumulator]));
     }
     commit_lane0(lane, smem_u32(done));
     __syncwarp();
@@ -966,6 +983,34 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     for (int i = 0; i < 4; ++i)
       if (i * step < n) bias[i] = to_f32(static_cast<const T*>(p.bias)[col + i * step]);
   }
+  const int q = warp & 3, c0 = (warp - 2) / 4 * 64;  // (of the epilogue warps)
+  const uint32_t from = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c0;
+  constexpr int kHeld = KIND == kLinearWgrad ? 2 : 0;
+  float v[kHeld + 1][32];  // wgrad: the sums of the segments before the last
+#pragma unroll
+  for (int h = 0; h < kHeld; ++h)
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[h][i] = 0.f;
+  if (KIND == kLinearWgrad && warp >= 2) {
+    for (int segment = 0; segment + 1 < segments; ++segment) {
+      const int a = segment % kAccumulators;
+      if (!mbar_wait_idle(smem_u32(&acc_full[a]), segment / kAccumulators & 1, abort_flag, p.err,
+                          kErrWaitEpilogue))
+        break;
+      tc_fence_after();
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h) {
+        uint32_t r[32];
+        CFB_TMEM_LD32(from + a * S::BN + h * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[h][i] += __uint_as_float(r[i]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&acc_empty[a]));
+    }
+  }
   // All products are done (waited for by everyone: the stages become the place of the sums, and TMEM
   // is given up).
   volatile int never = 0;
@@ -973,30 +1018,23 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   tc_fence_after();
   float* sums = reinterpret_cast<float*>(smem);
   if (warp >= 2 && ok) {
-    const int q = warp & 3, c0 = (warp - 2) / 4 * 64;
-    const uint32_t from = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + c0;
+    const uint32_t last = from + (segments - 1) % kAccumulators * S::BN;
     uint32_t r[2][32];
-    CFB_TMEM_LD32(from, r[0]);
-    CFB_TMEM_LD32(from + 32, r[1]);
+    CFB_TMEM_LD32(last, r[0]);
+    CFB_TMEM_LD32(last + 32, r[1]);
     tmem_ld_wait();
-    for (int a = 1; a * per_acc < blocks; ++a) {  // (wgrad's other accumulators)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t more[32];
-        CFB_TMEM_LD32(from + a * S::BN + h * 32, more);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          r[h][i] = __float_as_uint(__uint_as_float(r[h][i]) + __uint_as_float(more[i]));
-      }
-    }
     float* row = sums + (q * 32 + lane) * S::ROW + c0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      if (h < kHeld) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[h][i] = __float_as_uint(v[h < kHeld ? h : 0][i] + __uint_as_float(r[h][i]));
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         reinterpret_cast<uint4*>(row + h * 32)[i] =
             make_uint4(r[h][4 * i], r[h][4 * i + 1], r[h][4 * i + 2], r[h][4 * i + 3]);
+    }
   }
   tc_fence_before();
   if (splits > 1) cluster_sync(); else __syncthreads();

@@ -1130,6 +1130,29 @@ def test_wgrad_over_many_rows_keeps_fp32_accuracy(R, N, K):
     close(dw, dy.double().t() @ x.double(), (2 * 1024 + R // 1024 + 2) * U * mass, "dw")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,N,K", [
+    (16384, 1280, 1280), (16385, 1500, 1500), (65536, 1500, 1500), (131072, 1280, 1280), (100000, 256, 250),
+    (9217, 128, 64), (5000, 200, 1200), (4096, 1500, 1500), (65536, 640, 512), (40000, 5632, 1024)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_wgrad_error_does_not_grow_with_the_rows(R, N, K, dtype):
+    """Products of one sign, whose errors add up: an instruction adds those of 16 rows to a sum of at
+    most 1024 rows and may drop a step (2 u) of it, the sums of 1024 rows are added in fp32."""
+    g = gen("cuda", R + N)
+    dy, x = rand(g, R, N, dtype=dtype).abs(), rand(g, R, K, dtype=dtype).abs()
+    dw = rand(g, N, K).abs()
+    before = dw.clone()
+    gemm.linear_bias_wgrad(dy, x, dw)
+    cols = torch.randperm(N, generator=g, device="cuda")[:96]
+    want = torch.zeros(len(cols), K, dtype=F64, device="cuda")
+    for i in range(0, R, 1 << 14):
+        want += dy[i:i + (1 << 14), cols].double().t() @ x[i:i + (1 << 14)].double()
+    close(dw[cols], want + before[cols].double(), (2 * 64 + R // 1024 + 4) * U * (want + before[cols]), "dw")
+    again = before.clone()
+    gemm.linear_bias_wgrad(dy, x, again)
+    assert torch.equal(dw, again)
+
+
 @pytest.mark.parametrize("dev", CPU_GPU)
 def test_distill_lists_with_strides(dev):
     g, c = distill_case(dev, 20, 333, 6, BF, tail=True, tau=2.0)
