@@ -654,7 +654,13 @@ int launch_ring(const LnBwd& b, cudaStream_t st) {
 int cfb_layernorm_fwd(const void* x, int x_type, long long ld_x, const void* w, const void* b,
                       int type, float eps, void* y, long long ld_y, float* mean, float* rstd,
                       int rows, int H, cudaStream_t st) {
-  if (rows == 0 || H == 0) return 0;
+  if (rows == 0) return 0;
+  if (H == 0) {  // the mean of nothing: all bits set are a NaN
+    return cudaMemsetAsync(mean, 0xff, 4ll * rows, st) == cudaSuccess &&
+                   cudaMemsetAsync(rstd, 0xff, 4ll * rows, st) == cudaSuccess
+               ? 0
+               : -3;
+  }
   if (H > kLayerNormMaxH) return -11;
   const LnFwd a = {x, ld_x, w, b, eps, y, ld_y, mean, rstd, rows, H};
   const int W = widest([&](int n) {

@@ -494,6 +494,20 @@ def test_layernorm_odd_rows(dev):
     assert fused.layernorm_fwd(x[:, :0], w[:0], b[:0], EPS)[0].shape == (40, 0)
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("T", [1, 40, 1000])
+def test_layernorm_statistics_without_columns(dev, T):
+    """The mean of nothing is NaN, on both devices."""
+    w = torch.ones(0, device=dev)
+    old = [torch.full((T,), 7.0, device=dev) for _ in range(4)]  # (memory that the call may be given)
+    del old
+    y, mean, rstd = fused.layernorm_fwd(torch.ones(T, 0, device=dev), w, w, EPS)
+    assert y.shape == (T, 0) and mean.shape == rstd.shape == (T,)
+    assert bool(mean.isnan().all()) and bool(rstd.isnan().all())
+    dw = torch.ones(0, device=dev)
+    assert fused.layernorm_bwd(y, y, mean, rstd, w, dw, None, accumulate=False).shape == (T, 0)
+
+
 # ---------------------------------------------------------------- distillation
 def distill_case(dev, T, V, K, dtype, top_dtype=F32, tail=True, labels=True, tau=1.0, pad=0, skew=0,
                  ids64=False, seed=0):
