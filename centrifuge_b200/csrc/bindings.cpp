@@ -9,7 +9,6 @@
 #include <torch/extension.h>
 
 #include <algorithm>
-#include <cmath>
 #include <initializer_list>
 #include <string>
 #include <tuple>
@@ -1522,8 +1521,9 @@ CfbDistill distill_args(const char* what, const Tensor& logits, const Tensor& id
                     kDistillMaxTop);
   check_rows(ids, T, K, what, "top_ids");
   check_rows(top, T, K, what, "top_logits");
-  TORCH_CHECK_VALUE(temperature > 0 && std::isfinite(temperature), what, ": temperature = ",
-                    temperature, " is not positive");
+  // (its reciprocal is an fp32 factor; not a number fails, too)
+  TORCH_CHECK_VALUE(temperature >= kDistillLowTemperature && temperature <= kDistillHighTemperature, what,
+                    ": temperature = ", temperature, " is not from 2^-100 to 2^100");
   same_device(logits, ids, "top_ids");
   same_device(logits, top, "top_logits");
   same_device(logits, labels, "labels");

@@ -347,6 +347,7 @@ int cfb_layernorm_bwd(const void* dy, int type, long long ld_dy, const void* x, 
 
 // Distillation from a teacher's top logits beside the labels' cross entropy (formulas in distill.cu).
 constexpr int kDistillMaxTop = 1024, kDistillMaxVocab = 1 << 20;
+constexpr double kDistillLowTemperature = 0x1p-100, kDistillHighTemperature = 0x1p100;
 struct CfbDistill {
   int type, V, K;
   const void* z;  // logits

@@ -1113,6 +1113,23 @@ def test_refusals(dev, calls):
             pytest.fail(f"call {i} was not refused")
 
 
+@pytest.mark.parametrize("dev", CPU_GPU)
+def test_temperatures_beyond_fp32(dev):
+    """One whose reciprocal fp32 does not hold gave NaN on the GPU; large ones make a softmax uniform."""
+    z, ids, top = torch.zeros(3, 40, device=dev), torch.arange(4, device=dev).repeat(3, 1), torch.zeros(3, 4, device=dev)
+    z[:, 30:] = -math.inf
+    z[1, :20], z[2] = 2.0, z[2] - 3.0
+    kd, _, _, stats = fused.distill_fwd(z, ids, top, 2.0 ** 100)
+    close(kd, torch.full((3,), math.log(30 / 4), dtype=F64, device=dev), 1e-6, "kd")
+    args = (z, ids, top, stats, kd)
+    assert bool(fused.distill_bwd(*args, temperature=2.0 ** 100).isfinite().all())
+    for tau in (1e-46, 1e-39, 2.0 ** -101, 2.0 ** 101, 1e39, 1e46, 1e300):
+        with pytest.raises(ValueError):
+            fused.distill_fwd(z, ids, top, tau)
+        with pytest.raises(ValueError):
+            fused.distill_bwd(*args, temperature=tau)
+
+
 @pytest.mark.gpu
 def test_another_device_is_refused():
     x, w = torch.zeros(4, 16, dtype=BF, device="cuda"), torch.zeros(8, 16, dtype=BF)
