@@ -41,9 +41,12 @@ __device__ __forceinline__ float exponent(float z, float scale) {
 }
 // A row is streamed by four warps, seven such blocks to an SM: while some wait for their list or sums,
 // others stream.  Of 16384 x 32000 bf16 logits with tail and labels at tau = 2 (161 us at the measured
-// copy rate) the forward takes 197 us, without tail 167; the gradient of 8192 rows (161 us) 174.  When
-// the shape was chosen these were 213 and 181; with eight warps and four blocks an SM 237 and 193,
-// with two and twelve 212 and 192, with six blocks of four (more registers) 210 and 185.
+// copy rate) the forward takes 198 us in bursts of eight calls, and 215 to 223 in a loop, whose power
+// takes the clock from 1.97 to 1.64 GHz, since it is bound by issue slots; without tail and labels 177
+// and 189; the gradient of 8192 rows (161 us) 177 in both.  When the shape was chosen the first and the
+// last were 213 and 181; with eight warps and four blocks an SM 237 and 193, with two and twelve 212 and
+// 192, with six blocks of four (more registers) 210 and 185.  At the 56 registers of seven blocks the
+// fp32 gradients spill 56 to 152 bytes, and forwards with an exponential of their own up to 88.
 constexpr int kThreads = 128;          // the streaming warps'
 constexpr int kBlock = kThreads + 32;  // ... and the lister's
 constexpr int kBlocksPerSm = 7;
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(kBlock, kBlocksPerSm) distill_fwd_kernel(
       o.y = some ? static_cast<float>(log_rest) : -INFINITY;
       if (REST && some && fabsf(o.y) > 128.f) {
         // What multiplies the exponentials relative to this logarithm makes up for its rounding, and for
-        // that of the gradient's binary exponents: 1e-5 of them at 128, as much as theirs at 1e6.
+        // that of the gradient's binary exponents: 1e-5 of each term at 128, 7e-2 at 1e6.
         const double t = reference(o.y) * kLn2 - log_rest;
         coef *= fabs(t) < 0.002 ? 1.0 + t + 0.5 * t * t : fabs(t) < 2.0 ? exp(t) : 1.0;
       }

@@ -18,7 +18,9 @@ namespace cfb {
 // once and the rows share the exchanges of their sums.  Short blocks, each of which first asks the
 // L2 cache for the rows of the block that will follow it on its SM.  16384 x 2048 bf16: 27 us, 0.76 of
 // the measured copy rate; one row a team, four rows, eight or two warps, other columns a thread: 28 to
-// 79 us.  Above 4096 columns a row takes 16 or 32 warps, which wait together (8192: 0.55 of the rate).
+// 79 us.  Above 4096 columns a 16-bit row takes 16 warps, and above 8192 any row 32, which wait together
+// (4096 x 8192 bf16: 37 us, 0.56 of the rate); up to 8192 an fp32 row takes eight (45 to 48 us, 0.86 or
+// more).
 template <typename TY, typename TX, int NW, int NV, int R>
 __global__ void __launch_bounds__(NW == 1 ? 128 : NW * 32) layernorm_fwd_kernel(
     const TX* __restrict__ x, long long ld_x, const TY* __restrict__ w, const TY* __restrict__ b,

@@ -361,7 +361,7 @@ __device__ __forceinline__ void chunk_out_f32(uint8_t* buf, const float* v, floa
   if (vec == kRows32 && cols >= 32) {
     float* d = dst + lane * ld;
     if (lane >= rows) return;
-    if (add) {  // each element once: the same bits as a load, an addition and a store
+    if (add) {  // each element once: the same bits as a load, an addition and a store but below 1.2e-38
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(d + 4 * j),
